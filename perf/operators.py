@@ -301,7 +301,7 @@ def _decode(code, low):
 
 def _encode(x, scale, low, u):
     t = _times(x, -scale)
-    e = torch.clamp_min(torch.frexp(t).exponent - 1, low)
+    e = torch.where(t > 0, torch.clamp_min(torch.frexp(t).exponent - 1, low), low)
     return ((e - low) * 8 + torch.floor(_times(t, 3 - e) + u)).to(torch.int64)
 
 
