@@ -14,7 +14,7 @@ import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libcrystalframer_hip.so")
-ABI_VERSION = 14
+ABI_VERSION = 15
 
 CFH_WINDOW_REFERENCE = 0
 CFH_WINDOW_WIDE = 1
@@ -88,6 +88,33 @@ class CfhAdamWJob(ctypes.Structure):
                 ("exp_avg_sq", ctypes.c_void_p), ("n", ctypes.c_int64)]
 
 
+FLOAT32, BFLOAT16, FLOAT16 = 0, 1, 2        # CFH_FLOAT32, CFH_BFLOAT16, CFH_FLOAT16
+ELEMENT_TYPES = {torch.float32: FLOAT32, torch.bfloat16: BFLOAT16, torch.float16: FLOAT16}
+NORM_KINDS = {None: 0, "layer": 1, "rms": 2}          # CFH_NORM_NONE, CFH_NORM_LAYER, CFH_NORM_RMS
+MOMENT_BLOCK = 64       # elements that share a scale in 8-bit moments, and what every tensor's moments are aligned to
+
+
+class CfhParamJob(ctypes.Structure):
+    """Mirror of ``cfh_param_job`` in include/crystalframer_hip.h."""
+    _fields_ = [("param", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("n", ctypes.c_int64), ("first", ctypes.c_int64),
+                ("dtype", ctypes.c_int32), ("reserved0", ctypes.c_int32)]
+
+
+class CfhMoments(ctypes.Structure):
+    """Mirror of ``cfh_moments`` in include/crystalframer_hip.h."""
+    _fields_ = [("exp_avg", ctypes.c_void_p), ("exp_avg_sq", ctypes.c_void_p), ("exp_avg_scale", ctypes.c_void_p),
+                ("exp_avg_sq_scale", ctypes.c_void_p), ("size", ctypes.c_int64), ("bits", ctypes.c_int32),
+                ("reserved0", ctypes.c_int32)]
+
+
+class CfhResidualNorm(ctypes.Structure):
+    """Mirror of ``cfh_residual_norm`` in include/crystalframer_hip.h."""
+    _fields_ = ([(n, ctypes.c_int32) for n in ("struct_size", "dtype", "weight_dtype", "norm", "block_norm", "joined")]
+                + [(n, ctypes.c_float) for n in ("eps", "block_eps", "residual_scale", "block_scale")]
+                + [(n, ctypes.c_int64) for n in ("rows", "dim", "gate_rows", "x_stride", "block_stride")]
+                + [(n, ctypes.c_void_p) for n in ("x", "block", "gate", "weight", "bias", "block_weight", "block_bias")])
+
+
 class CfhModelLayer(ctypes.Structure):
     """Mirror of ``cfh_model_layer`` in include/crystalframer_hip.h."""
     _fields_ = ([("core", CfhParams)]
@@ -135,7 +162,9 @@ EXPORTS = ("cfh_abi_version", "cfh_last_error", "cfh_workspace_bytes", "cfh_fram
            "cfh_fused_core_workspace_bytes", "cfh_fused_core_hist_words", "cfh_fused_core_forward",
            "cfh_fused_core_backward", "cfh_adamw_step_batch",
            "cfh_fused_core_weight_gradients_workspace_bytes", "cfh_fused_core_weight_gradients",
-           "cfh_model_sizes", "cfh_model_forward", "cfh_model_backward")
+           "cfh_model_sizes", "cfh_model_forward", "cfh_model_backward",
+           "cfh_adamw_step_moments", "cfh_adamw_moments", "cfh_grad_norm_workspace_bytes", "cfh_grad_norm",
+           "cfh_residual_norm_forward", "cfh_residual_norm_backward_workspace_bytes", "cfh_residual_norm_backward")
 
 _lib = None
 _lock = threading.Lock()
@@ -253,6 +282,21 @@ def load():
         lib.cfh_second_stream_get.argtypes = [ctypes.POINTER(_P)]
         lib.cfh_second_stream_join.restype = ctypes.c_int
         lib.cfh_second_stream_join.argtypes = [_P]
+        _D = ctypes.c_double
+        lib.cfh_adamw_step_moments.restype = ctypes.c_int
+        lib.cfh_adamw_step_moments.argtypes = [_P, _I32, _P, _D, _D, _D, _D, _D, _P, _P, _P, _P]
+        lib.cfh_adamw_moments.restype = ctypes.c_int
+        lib.cfh_adamw_moments.argtypes = [_P] * 4
+        lib.cfh_grad_norm_workspace_bytes.restype = ctypes.c_size_t
+        lib.cfh_grad_norm_workspace_bytes.argtypes = [_P, _I32]
+        lib.cfh_grad_norm.restype = ctypes.c_int
+        lib.cfh_grad_norm.argtypes = [_P, _I32, _D, _P, _P, ctypes.c_size_t, _P]
+        lib.cfh_residual_norm_forward.restype = ctypes.c_int
+        lib.cfh_residual_norm_forward.argtypes = [_P] * 5
+        lib.cfh_residual_norm_backward_workspace_bytes.restype = ctypes.c_size_t
+        lib.cfh_residual_norm_backward_workspace_bytes.argtypes = [_P]
+        lib.cfh_residual_norm_backward.restype = ctypes.c_int
+        lib.cfh_residual_norm_backward.argtypes = [_P] * 12 + [ctypes.c_size_t, _P]
         if lib.cfh_abi_version() != ABI_VERSION:
             raise RuntimeError(f"ABI version {lib.cfh_abi_version()} of {LIB_PATH} != {ABI_VERSION}")
         _lib = lib

@@ -6,6 +6,7 @@ instantiation compiled once by hipcc into ``libcrystalframer_hip.so`` next to th
 """
 from __future__ import annotations
 
+import concurrent.futures
 import os
 import shutil
 import subprocess
@@ -18,8 +19,10 @@ LIB_NAME = "libcrystalframer_hip.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 HOST_PATH = os.path.join(HERE, "_host.so")
 
+LIB_SOURCES = ("crystalframer_hip", "training_ops")
+
 HIPCC_FLAGS = [
-    "-O3", "--offload-arch=gfx950", "-std=c++17", "-shared", "-fPIC",
+    "-O3", "--offload-arch=gfx950", "-std=c++17", "-fPIC",
     # packed FP32 instructions are kept out of the generated code
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]
@@ -32,18 +35,32 @@ def hipcc_path() -> str:
     raise RuntimeError("hipcc not found (looked on PATH and in /opt/rocm/bin)")
 
 
-def build_library(verbose: bool = True) -> str:
-    """Compile csrc/crystalframer_hip.hip -> libcrystalframer_hip.so (always recompiles)."""
-    src = os.path.join(CSRC, "crystalframer_hip.hip")
-    tmp = LIB_PATH + ".tmp"
-    # CFH_EXTRA_HIPCC_FLAGS: extra flags for diagnostics builds (e.g. -DCFH_PHASE_TIMING)
-    extra = os.environ.get("CFH_EXTRA_HIPCC_FLAGS", "").split()
-    cmd = [hipcc_path(), *HIPCC_FLAGS, *extra, "-o", tmp, src]
+def _run(cmd, verbose):
     if verbose:
         print("[crystalframer_amd] " + " ".join(cmd), flush=True)
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        sys.stderr.write(res.stdout + res.stderr)
+    return subprocess.run(cmd, capture_output=True, text=True)
+
+
+def build_library(verbose: bool = True) -> str:
+    """Compile the sources of csrc -> libcrystalframer_hip.so (always recompiles), side by side, and link them."""
+    # CFH_EXTRA_HIPCC_FLAGS: extra flags for diagnostics builds (e.g. -DCFH_PHASE_TIMING)
+    extra = os.environ.get("CFH_EXTRA_HIPCC_FLAGS", "").split()
+    tmp = LIB_PATH + ".tmp"
+    objects = [os.path.join(HERE, name + ".o") for name in LIB_SOURCES]
+    cmds = [[hipcc_path(), *HIPCC_FLAGS, *extra, "-c", "-o", obj, os.path.join(CSRC, name + ".hip")]
+            for name, obj in zip(LIB_SOURCES, objects)]
+    try:
+        with concurrent.futures.ThreadPoolExecutor(len(cmds)) as pool:
+            failed = [res for res in pool.map(lambda cmd: _run(cmd, verbose), cmds) if res.returncode != 0]
+        if not failed:
+            res = _run([hipcc_path(), "--offload-arch=gfx950", "-shared", "-fPIC", "-o", tmp, *objects], verbose)
+            failed = [res] if res.returncode != 0 else []
+    finally:
+        for obj in objects:
+            if os.path.exists(obj):
+                os.remove(obj)
+    if failed:
+        sys.stderr.write("".join(res.stdout + res.stderr for res in failed))
         raise RuntimeError("hipcc failed building " + LIB_NAME)
     os.replace(tmp, LIB_PATH)
     return LIB_PATH

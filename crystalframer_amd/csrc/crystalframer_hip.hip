@@ -30,18 +30,29 @@
 #include "bridge_infer.hpp"
 #include "adamw.hpp"
 #include "model_tail.hpp"
+#include "host_error.hpp"
 
 namespace {
-
 thread_local char g_err[512] = "";
+}
 
-int fail(int code, const char* fmt, ...) {
+int cfh::fail(int code, const char* fmt, ...) {
     va_list ap;
     va_start(ap, fmt);
     vsnprintf(g_err, sizeof(g_err), fmt, ap);
     va_end(ap);
     return code;
 }
+
+int cfh::finish_launch(const char* what) {
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return fail(CFH_ELAUNCH, "%s: %s", what, hipGetErrorString(e));
+    return CFH_OK;
+}
+
+namespace {
+
+using cfh::fail;
 
 constexpr int MAX_HEADS = 64;
 constexpr size_t QUEUE_OFFSET = 512;           // workspace header: 256 reserved bytes, 32 uint64 statistics, then the work queues
@@ -269,11 +280,7 @@ void fill_common(cfh::KernelArgs& A, const cfh_params* p, const float* a_ih, con
     A.bc = basis_consts(p);
 }
 
-int finish_launch(const char* what) {
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return fail(CFH_ELAUNCH, "%s: %s", what, hipGetErrorString(e));
-    return CFH_OK;
-}
+using cfh::finish_launch;
 
 // Wavefronts that are resident at once for this kernel on the current device.  Work is dealt to
 // wavefronts statically, so launching more than fit would run them in a second wave of blocks and

@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define CFH_ABI_VERSION 14
+#define CFH_ABI_VERSION 15
 
 enum {
     CFH_OK = 0,
@@ -510,6 +510,110 @@ typedef struct cfh_adamw_job {
 } cfh_adamw_job;
 int cfh_adamw_step_batch(const cfh_adamw_job* jobs, int32_t njobs, float lr, float beta1, float beta2, float eps,
                          float weight_decay, uint64_t* step_dev, void* stream);
+
+/* Element types of the entry points that take more than float32. */
+enum { CFH_FLOAT32 = 0, CFH_BFLOAT16 = 1, CFH_FLOAT16 = 2 };
+
+/*
+ * One AdamW step for tensors of several types, with moments in 32 or in 8 bits and gradients that may be clipped by
+ * their common norm: the rule of cfh_adamw_step_batch with c g in the place of g,
+ *     c = min(1, max_norm / (|g| + 1e-6)),  |g| the norm over all tensors (cfh_grad_norm; c = 1 without it).
+ * A tensor is contiguous with n elements of `dtype`, its gradient likewise; its moments are the elements
+ * first ... first + n - 1 of the flat moments of `state`; first is a multiple of 64.  The arithmetic is in 32 bits (the
+ * parameter is rounded to its type at the end), that of 8-bit moments in 64, every product and sum by itself, until they are
+ * rounded:
+ *   bits = 32   exp_avg, exp_avg_sq float32; the scales are not used.
+ *   bits = 8    64 consecutive elements (the last of a tensor: fewer) share a scale 2^(s - 127), s a byte at index
+ *               element / 64.  exp_avg: e4m3 (OCP), the largest finite magnitude of the 64 scaled into [128, 256); what is
+ *               not finite becomes NaN.  exp_avg_sq: no sign, 5 exponent bits E, 3 mantissa bits M, value (8 + M) 2^(E - 33),
+ *               M 2^-32 for E = 0, the largest scaled into [1, 2); 255 stands for what 32 bits do not hold; what is not
+ *               zero does not become zero.  Both are rounded to one of the two codes around them with the odds of their
+ *               distance: floor(x / step + (2 k + 1) / 2^17), k the low (exp_avg) or high (exp_avg_sq) half of the 32-bit hash
+ *                   x = e * 0x9E3779B1 + key;  x ^= x >> 16;  x *= 0xBB67AE85;  x ^= x >> 15,
+ *               e the element (modulo 2^32) and key = t * 0x6A09E667; key ^= key >> 15; key *= 0x9E3779B1;
+ *               key ^= key >> 16, t the number of the step.
+ * `step_dev` counts as in cfh_adamw_step_batch; `scratch` (16 floats, device) belongs to the call until it has run on the
+ * stream.  `clip` (NULL: no clipping) points to the two floats that cfh_grad_norm left on the device.
+ */
+typedef struct cfh_param_job {
+    void* param;             /* not read by cfh_grad_norm                                         */
+    const void* grad;
+    int64_t n;
+    int64_t first;
+    int32_t dtype;
+    int32_t reserved0;
+} cfh_param_job;
+typedef struct cfh_moments {
+    void* exp_avg;
+    void* exp_avg_sq;
+    uint8_t* exp_avg_scale;
+    uint8_t* exp_avg_sq_scale;
+    int64_t size;            /* elements of the flat moments                                      */
+    int32_t bits;            /* 8 or 32                                                           */
+    int32_t reserved0;
+} cfh_moments;
+int cfh_adamw_step_moments(const cfh_param_job* jobs, int32_t njobs, const cfh_moments* state, double lr, double beta1,
+                           double beta2, double eps, double weight_decay, const float* clip, uint64_t* step_dev,
+                           float* scratch, void* stream);
+
+/* The float32 values that 8-bit moments stand for: exp_avg, exp_avg_sq (state->size elements each). */
+int cfh_adamw_moments(const cfh_moments* state, float* exp_avg, float* exp_avg_sq, void* stream);
+
+/*
+ * out[0] = |g| over the gradients of all jobs (summed in 64 bits, in a fixed order), out[1] = the factor
+ * min(1, max_norm / (|g| + 1e-6)); a norm that is no number gives a factor that is none.
+ */
+size_t cfh_grad_norm_workspace_bytes(const cfh_param_job* jobs, int32_t njobs);
+int cfh_grad_norm(const cfh_param_job* jobs, int32_t njobs, double max_norm, float* out, void* workspace,
+                  size_t workspace_bytes, void* stream);
+
+/*
+ * Residual stream and block output joined and normed, forward and backward, for the norms before and after the blocks of
+ * a transformer:
+ *     a = N_b(block)  (or block),     h = residual_scale x + block_scale gate a,     y = N(h)
+ * for `rows` rows of `dim` elements (1 ... 16384); N, N_b: layer norm ((h - mean) / sqrt(var + eps) w + b), root-mean-square
+ * norm (h / sqrt(mean h^2 + eps) w + b) or none.  block NULL: h = residual_scale x.  gate: gate_rows rows of dim elements, each
+ * for rows / gate_rows rows after one another (1: per channel; rows: per element; 0: no gate).  x, block, gate and the
+ * outputs have the type `dtype`, weights and biases (each may be NULL: 1 and 0) `weight_dtype`, equal to dtype or float32.
+ * Statistics and sums are in 32 bits, everything is rounded once where it is written.  x and block have their own row strides
+ * (in elements); everything else is contiguous.  Replaces torch.nn.LayerNorm and the additions around it
+ * (models/indexed_latticeformer_encoder.py:848-877).
+ *   forward    h, y: may be NULL; stats (rows, 4) float32: what the backward pass needs, may be NULL.
+ *   backward   gh, gy: gradients of h and y, either may be NULL (zero).  dx, dblock, dgate, dweight, dbias, dblock_weight,
+ *              dblock_bias: NULL where they are not wanted; dblock may be dx where both are the same (equal scales, no gate, no
+ *              block norm).  joined != 0: `x` holds h, as the forward pass wrote it in float32, and block is not read
+ *              (no gate, no block norm).  Column sums are added in a fixed order.
+ */
+enum { CFH_NORM_NONE = 0, CFH_NORM_LAYER = 1, CFH_NORM_RMS = 2 };
+typedef struct cfh_residual_norm {
+    int32_t struct_size;     /* = sizeof(cfh_residual_norm)                                       */
+    int32_t dtype;
+    int32_t weight_dtype;
+    int32_t norm;
+    int32_t block_norm;
+    int32_t joined;          /* backward only                                                     */
+    float eps;
+    float block_eps;
+    float residual_scale;
+    float block_scale;
+    int64_t rows;
+    int64_t dim;
+    int64_t gate_rows;
+    int64_t x_stride;
+    int64_t block_stride;
+    const void* x;
+    const void* block;
+    const void* gate;
+    const void* weight;
+    const void* bias;
+    const void* block_weight;
+    const void* block_bias;
+} cfh_residual_norm;
+int cfh_residual_norm_forward(const cfh_residual_norm* args, void* h, void* y, float* stats, void* stream);
+size_t cfh_residual_norm_backward_workspace_bytes(const cfh_residual_norm* args);
+int cfh_residual_norm_backward(const cfh_residual_norm* args, const float* stats, const void* gh, const void* gy, void* dx,
+                               void* dblock, void* dgate, void* dweight, void* dbias, void* dblock_weight, void* dblock_bias,
+                               void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Projections with few rows (one per crystal: the head after pooling), where the general GEMM runs on
