@@ -19,7 +19,7 @@ LIB_NAME = "libcrystalframer_hip.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 HOST_PATH = os.path.join(HERE, "_host.so")
 
-LIB_SOURCES = ("crystalframer_hip", "training_ops")
+LIB_SOURCES = ("crystalframer_hip", "training_ops", "residual_norm_f32", "residual_norm_bf16", "residual_norm_f16")
 
 HIPCC_FLAGS = [
     "-O3", "--offload-arch=gfx950", "-std=c++17", "-fPIC",

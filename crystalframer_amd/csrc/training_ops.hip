@@ -9,7 +9,7 @@
 
 #include "adamw_moments.hpp"
 #include "host_error.hpp"
-#include "residual_norm.hpp"
+#include "residual_norm_args.hpp"
 
 namespace {
 
@@ -185,14 +185,15 @@ int cfh_residual_norm_forward(const cfh_residual_norm* a, void* h, void* y, floa
     const cfh::ResidualNorm A = device_args(a);
     with_type(a->dtype, [&](auto t) {
         using T = decltype(t);
-        hipLaunchKernelGGL(cfh::residual_norm_forward_kernel<T>, dim3((unsigned)a->rows), dim3(256), 0, (hipStream_t)stream, A, (T*)h, (T*)y, stats);
+        cfh::residual_norm_forward<T>(A, (T*)h, (T*)y, stats, (hipStream_t)stream);
     });
     return finish_launch("residual_norm_forward");
 }
 
 size_t cfh_residual_norm_backward_workspace_bytes(const cfh_residual_norm* a) {
     if (check_norm(a, true)) return 0;
-    return (size_t)(a->rows > 0 ? a->rows : 1) * 4 * sizeof(float);
+    const cfh::NormPlan P = cfh::norm_plan(a->rows, a->dim, a->dtype == CFH_FLOAT32 ? 4 : 8, a->gate_rows);
+    return (P.column_floats + P.gate_floats + 4) * sizeof(float);
 }
 
 int cfh_residual_norm_backward(const cfh_residual_norm* a, const float* stats, const void* gh, const void* gy, void* dx, void* dblock,
@@ -212,12 +213,11 @@ int cfh_residual_norm_backward(const cfh_residual_norm* a, const float* stats, c
                     cfh_residual_norm_backward_workspace_bytes(a));
     cfh::ResidualNorm A = device_args(a);
     if (a->joined) A.in_scale = 1.0f;
-    const cfh::NormGrads G{stats, gh, gy, dx, dblock, dgate, dweight, dbias, dblock_weight, dblock_bias, reinterpret_cast<float*>(workspace)};
+    cfh::NormGrads G{};
+    G.stats = stats; G.gh = gh; G.gy = gy; G.dx = dx; G.df = dblock == dx ? nullptr : dblock; G.dgate = dgate;
+    G.dw = dweight; G.db = dbias; G.dwf = dblock_weight; G.dbf = dblock_bias;
     with_type(a->dtype, [&](auto t) {
-        using T = decltype(t);
-        if (a->rows > 0)
-            hipLaunchKernelGGL(cfh::residual_norm_row_grad_kernel<T>, dim3((unsigned)a->rows), dim3(256), 0, (hipStream_t)stream, A, G);
-        hipLaunchKernelGGL(cfh::residual_norm_column_grad_kernel<T>, dim3((unsigned)((a->dim + 63) / 64), 5), dim3(256), 0, (hipStream_t)stream, A, G);
+        cfh::residual_norm_backward<decltype(t)>(A, G, a->gate_rows, reinterpret_cast<float*>(workspace), (hipStream_t)stream);
     });
     return finish_launch("residual_norm_backward");
 }
