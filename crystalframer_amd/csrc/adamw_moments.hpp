@@ -7,15 +7,17 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "element_types.hpp"
 
 namespace cfh {
 
 constexpr int MOMENT_BLOCK = 64;          // elements that share a scale
 constexpr int PARAM_MAX_JOBS = 88;        // tensors per launch (kernel arguments: 4 KB)
-constexpr int ADAMW_CHUNK = 256;          // elements per workgroup of 256 threads
+constexpr int ADAMW_CHUNK = 2048;         // elements per workgroup of 256 threads
 constexpr int GRAD_NORM_CHUNK = 4096;     // elements per turn of a workgroup of 256 threads
-constexpr int GRAD_NORM_BLOCKS = 1024;    // workgroups per launch at most
+constexpr int GRAD_NORM_BLOCKS = 2048;    // workgroups per launch at most
 
 struct ParamJob {
     void* p;
@@ -77,23 +79,24 @@ __device__ __forceinline__ uint32_t moment_hash(uint32_t element, uint32_t key) 
     return x ^ (x >> 15);
 }
 
+// (The hardware's root and reciprocal: each within one unit of the last place of what is a thousandth of the parameter.)
 __device__ __forceinline__ float adamw_update(float p, float m, float v, const AdamWStep& S, float eps) {
-    return p * S.decay - S.step_size * (m / (sqrtf(v) * S.inv_sqrt_bc2 + eps));
+    const float root = __builtin_amdgcn_sqrtf(v) * S.inv_sqrt_bc2 + eps;
+    return p * S.decay - S.step_size * (m * __builtin_amdgcn_rcpf(root));
 }
 
 // An 8-bit code without its sign is a double's exponent and mantissa cut to three bits: its bits, moved under the high word's
 // exponent field, are the value times 2^bias, denormals included, and back it is one shift.  bias: 1016 (exp_avg, e4m3: the
 // smallest normal value 2^-6 has exponent field 1) and 993 (exp_avg_sq: 2^-29).
 constexpr int M_BIAS = 1016, V_BIAS = 993, M_TOP = 7, V_TOP = 0;
+constexpr uint32_t HIGH_INF = 0x7ff00000u, HIGH_2_128 = 0x47f00000u;      // high words: no number from here on; 2^128
 
+__device__ __forceinline__ uint32_t high_word(double x) { return (uint32_t)__double2hiint(x); }
 __device__ __forceinline__ double code_value(uint32_t code, int bias) {
     return ldexp(__hiloint2double((int)(code << 17), 0), bias);
 }
-// floor(x / step + (2 k + 1) / 2^17) as a code; x >= 0, k in 16 bits
-__device__ __forceinline__ uint32_t code_of(double x, int bias, uint32_t k) {
-    return ((uint32_t)__double2hiint(ldexp(x, -bias)) + 2u * k + 1u) >> 17;
-}
-__device__ __forceinline__ bool finite_double(double x) { return (__double2hiint(x) & 0x7ff00000) != 0x7ff00000; }
+// floor(x / step + (2 k + 1) / 2^17) as a code; x >= 0, odd = 2 k + 1 in 17 bits
+__device__ __forceinline__ uint32_t code_of(double x, int bias, uint32_t odd) { return (high_word(ldexp(x, -bias)) + odd) >> 17; }
 
 // The scale byte of a block whose largest magnitude has this high word (0: none): the largest then lies in [2^top, 2^(top + 1)).
 __device__ __forceinline__ int scale_byte(uint32_t high, int top) {
@@ -108,57 +111,128 @@ __device__ __forceinline__ double moment_mix(double b, double x, double y) {
     return b * x + y;
 }
 
+// Largest over the LANES (8 or 16) neighbouring lanes of a block.
+template <int LANES>
+__device__ __forceinline__ uint32_t block_max(uint32_t x) {
+    auto other = [&](auto ctrl) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, 0xf, 0xf, false); };
+    x = max(x, other(std::integral_constant<int, 0xB1>()));       // quad_perm [1,0,3,2], [2,3,0,1], half_mirror, mirror
+    x = max(x, other(std::integral_constant<int, 0x4E>()));
+    x = max(x, other(std::integral_constant<int, 0x141>()));
+    if constexpr (LANES == 16) x = max(x, other(std::integral_constant<int, 0x140>()));
+    return x;
+}
+
+// `E` elements of a tensor from `i` on (fewer at its end, none behind it), of which a lane takes care: a block of 64 lies in 64 / E lanes.
+template <typename T, int E>
+__device__ __forceinline__ void load_elements(T (&o)[E], const T* from, uint32_t i, uint32_t n) {
+    if (i + E <= n) __builtin_memcpy(o, from + i, sizeof(o));
+    else {
+#pragma unroll
+        for (int j = 0; j < E; j++) o[j] = i + j < n ? from[i + j] : T{};
+    }
+}
+template <typename T, int E>
+__device__ __forceinline__ void store_elements(T* to, const T (&o)[E], uint32_t i, uint32_t n) {
+    if (i + E <= n) __builtin_memcpy(to + i, o, sizeof(o));
+    else {
+#pragma unroll
+        for (int j = 0; j < E; j++)
+            if (i + j < n) to[i + j] = o[j];
+    }
+}
+
+template <typename T, int E>
+__device__ __forceinline__ void moments32(const ParamJob& J, uint32_t i, const T (&g)[E], T (&p)[E], const Moments& W, const AdamWStep& S,
+                                          const AdamWRates& R) {
+    float* const pm = reinterpret_cast<float*>(W.m) + J.first;
+    float* const pv = reinterpret_cast<float*>(W.v) + J.first;
+    const float b1 = (float)R.beta1, a1 = (float)(1.0 - R.beta1), b2 = (float)R.beta2, a2 = (float)(1.0 - R.beta2);
+    float m[E], v[E];
+    load_elements(m, pm, i, J.n);
+    load_elements(v, pv, i, J.n);
+#pragma unroll
+    for (int j = 0; j < E; j++) {
+        const float c = to_float(g[j]) * S.clip;
+        m[j] = b1 * m[j] + a1 * c;
+        v[j] = b2 * v[j] + a2 * c * c;
+        p[j] = from_float<T>(adamw_update(to_float(p[j]), m[j], v[j], S, R.eps));
+    }
+    store_elements(pm, m, i, J.n);
+    store_elements(pv, v, i, J.n);
+}
+
+template <typename T, int E>
+__device__ __forceinline__ void moments8(const ParamJob& J, uint32_t i, const T (&g)[E], T (&p)[E], const Moments& W, const AdamWStep& S,
+                                         const AdamWRates& R) {
+    uint8_t* const pm = reinterpret_cast<uint8_t*>(W.m) + J.first;
+    uint8_t* const pv = reinterpret_cast<uint8_t*>(W.v) + J.first;
+    uint8_t* const ps = W.m_scale + J.first / MOMENT_BLOCK;
+    uint8_t* const pt = W.v_scale + J.first / MOMENT_BLOCK;
+    uint8_t cm[E], cv[E];
+    load_elements(cm, pm, i, J.n);
+    load_elements(cv, pv, i, J.n);
+    const int sm0 = i < J.n ? M_BIAS - 127 + (int)ps[i / MOMENT_BLOCK] : 0, sv0 = i < J.n ? V_BIAS - 127 + (int)pt[i / MOMENT_BLOCK] : 0;
+    double m[E], v[E];
+    bool odd = false;
+    uint32_t hm = 0, hv = 0;
+#pragma unroll
+    for (int j = 0; j < E; j++) {
+        const double c = (double)to_float(g[j]) * (double)S.clip;
+        double a = code_value(cm[j] & 127u, sm0), b = code_value(cv[j], sv0);
+        a = __hiloint2double((int)(high_word(a) | (uint32_t)(cm[j] & 128u) << 24), __double2loint(a));
+        if ((cm[j] & 127u) == 127u) a = __longlong_as_double(0x7ff8000000000000LL);
+        if (cv[j] == 255u) b = __longlong_as_double(0x7ff0000000000000LL);
+        m[j] = moment_mix(R.beta1, a, (1.0 - R.beta1) * c);
+        v[j] = moment_mix(R.beta2, b, (1.0 - R.beta2) * c * c);
+        hm = max(hm, high_word(m[j]) & 0x7fffffffu);
+        hv = max(hv, high_word(v[j]));
+    }
+    odd = __any(hm >= HIGH_INF || hv >= HIGH_2_128);
+    if (odd) {            // what 32 bits do not hold stays out of the scale
+        hm = hv = 0;
+#pragma unroll
+        for (int j = 0; j < E; j++) {
+            const uint32_t a = high_word(m[j]) & 0x7fffffffu, b = high_word(v[j]);
+            hm = a < HIGH_INF ? max(hm, a) : hm;
+            hv = b < HIGH_2_128 ? max(hv, b) : hv;
+        }
+    }
+    const int sm = scale_byte(block_max<MOMENT_BLOCK / E>(hm), M_TOP), sv = scale_byte(block_max<MOMENT_BLOCK / E>(hv), V_TOP);
+#pragma unroll
+    for (int j = 0; j < E; j++) {
+        const uint32_t h = moment_hash((uint32_t)J.first + i + j, S.key);
+        uint32_t a = code_of(fabs(m[j]), M_BIAS - 127 + sm, (h << 1 & 0x1ffffu) | 1u);
+        uint32_t b = code_of(v[j], V_BIAS - 127 + sv, h >> 15 | 1u);
+        b = max(b, v[j] > 0.0 ? 1u : 0u);
+        if (odd) {
+            if ((high_word(m[j]) & 0x7fffffffu) >= HIGH_INF) a = 127u;
+            if (high_word(v[j]) >= HIGH_2_128) b = 255u;
+        }
+        cm[j] = (uint8_t)(a | (high_word(m[j]) >> 24 & 128u));
+        cv[j] = (uint8_t)b;
+        p[j] = from_float<T>(adamw_update(to_float(p[j]), (float)m[j], (float)v[j], S, R.eps));
+    }
+    store_elements(pm, cm, i, J.n);
+    store_elements(pv, cv, i, J.n);
+    if (i < J.n && i % MOMENT_BLOCK == 0) {
+        ps[i / MOMENT_BLOCK] = (uint8_t)sm;
+        pt[i / MOMENT_BLOCK] = (uint8_t)sv;
+    }
+}
+
 template <typename T, int BITS>
-__device__ void adamw_chunk(const ParamJob& J, uint32_t base, const Moments& W, const AdamWStep& S, const AdamWRates& R) {
-    const uint32_t i = base + threadIdx.x;
-    const bool live = i < J.n;
-    const uint64_t e = J.first + i;
-    T* const p = reinterpret_cast<T*>(J.p) + i;
-    const float g = live ? to_float(reinterpret_cast<const T*>(J.g)[i]) : 0.0f;
-    if constexpr (BITS == 32) {
-        if (!live) return;
-        float* const pm = reinterpret_cast<float*>(W.m) + e;
-        float* const pv = reinterpret_cast<float*>(W.v) + e;
-        const float c = g * S.clip;
-        const float m = (float)R.beta1 * *pm + (float)(1.0 - R.beta1) * c;
-        const float v = (float)R.beta2 * *pv + (float)(1.0 - R.beta2) * c * c;
-        *pm = m;
-        *pv = v;
-        *p = from_float<T>(adamw_update(to_float(*p), m, v, S, R.eps));
-    } else {
-        uint8_t* const pm = reinterpret_cast<uint8_t*>(W.m) + e;
-        uint8_t* const pv = reinterpret_cast<uint8_t*>(W.v) + e;
-        double m = 0.0, v = 0.0;
-        if (live) {
-            const uint32_t cm = *pm, cv = *pv;
-            const double c = (double)g * (double)S.clip;
-            m = code_value(cm & 127u, M_BIAS + (int)W.m_scale[e / MOMENT_BLOCK] - 127);
-            if ((cm & 127u) == 127u) m = __longlong_as_double(0x7ff8000000000000LL);
-            if (cm & 128u) m = -m;
-            v = code_value(cv, V_BIAS + (int)W.v_scale[e / MOMENT_BLOCK] - 127);
-            if (cv == 255u) v = __longlong_as_double(0x7ff0000000000000LL);
-            m = moment_mix(R.beta1, m, (1.0 - R.beta1) * c);
-            v = moment_mix(R.beta2, v, (1.0 - R.beta2) * c * c);
-        }
-        const bool fm = finite_double(m), fv = fabs(v) < 0x1p128;
-        uint32_t hm = fm ? (uint32_t)__double2hiint(m) & 0x7fffffffu : 0u, hv = fv ? (uint32_t)__double2hiint(v) : 0u;
-        for (int d = 1; d < 64; d *= 2) {
-            hm = max(hm, (uint32_t)__shfl_xor((int)hm, d));
-            hv = max(hv, (uint32_t)__shfl_xor((int)hv, d));
-        }
-        if (!live) return;
-        const int sm = scale_byte(hm, M_TOP), sv = scale_byte(hv, V_TOP);
-        const uint32_t h = moment_hash((uint32_t)e, S.key);
-        uint32_t cm = fm ? code_of(fabs(m), M_BIAS + sm - 127, h & 0xffffu) : 127u;
-        uint32_t cv = fv ? code_of(v, V_BIAS + sv - 127, h >> 16) : 255u;
-        if (cv == 0u && v > 0.0) cv = 1u;
-        *pm = (uint8_t)(cm | ((uint32_t)__double2hiint(m) >> 31 << 7));
-        *pv = (uint8_t)cv;
-        if (i % MOMENT_BLOCK == 0) {
-            W.m_scale[e / MOMENT_BLOCK] = (uint8_t)sm;
-            W.v_scale[e / MOMENT_BLOCK] = (uint8_t)sv;
-        }
-        *p = from_float<T>(adamw_update(to_float(*p), (float)m, (float)v, S, R.eps));
+__device__ __forceinline__ void adamw_chunk(const ParamJob& J, uint32_t base, const Moments& W, const AdamWStep* step, const AdamWRates& R) {
+    constexpr int E = 16 / (int)sizeof(T);
+    T* const pp = reinterpret_cast<T*>(J.p);
+    const AdamWStep S = *step;
+    for (int k = 0; k < ADAMW_CHUNK / (256 * E); k++) {
+        const uint32_t i = base + ((uint32_t)k * 256 + threadIdx.x) * E;
+        T g[E], p[E];
+        load_elements(g, reinterpret_cast<const T*>(J.g), i, J.n);
+        load_elements(p, pp, i, J.n);
+        if constexpr (BITS == 32) moments32(J, i, g, p, W, S, R);
+        else moments8(J, i, g, p, W, S, R);
+        store_elements(pp, p, i, J.n);
     }
 }
 
@@ -167,19 +241,33 @@ __global__ __launch_bounds__(256) void adamw_moments_kernel(const ParamJobs T, c
                                                             const AdamWRates R) {
     const ParamJob& J = job_of(T, blockIdx.x);
     const uint32_t base = (blockIdx.x - J.chunk0) * ADAMW_CHUNK;
-    const AdamWStep S = *step;
-    if (J.dtype == TYPE_F32) adamw_chunk<float, BITS>(J, base, W, S, R);
-    else if (J.dtype == TYPE_BF16) adamw_chunk<bf16, BITS>(J, base, W, S, R);
-    else adamw_chunk<f16, BITS>(J, base, W, S, R);
+    if (J.dtype == TYPE_F32) adamw_chunk<float, BITS>(J, base, W, step, R);
+    else if (J.dtype == TYPE_BF16) adamw_chunk<bf16, BITS>(J, base, W, step, R);
+    else adamw_chunk<f16, BITS>(J, base, W, step, R);
 }
 
+// Four elements per lane: 8 bytes read, 32 written.  In 32 bits the codes' bits, moved under a float's exponent field, are the values
+// times 2^-120 and 2^-97.
 __global__ __launch_bounds__(256) void moment_values_kernel(const Moments W, uint64_t size, float* m, float* v) {
-    const uint64_t e = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    const uint64_t e = ((uint64_t)blockIdx.x * 256 + threadIdx.x) * 4;
     if (e >= size) return;
-    const uint32_t cm = reinterpret_cast<const uint8_t*>(W.m)[e], cv = reinterpret_cast<const uint8_t*>(W.v)[e];
-    const float a = (float)code_value(cm & 127u, M_BIAS + (int)W.m_scale[e / MOMENT_BLOCK] - 127);
-    m[e] = copysignf((cm & 127u) == 127u ? __int_as_float(0x7fc00000) : a, cm & 128u ? -1.0f : 1.0f);
-    v[e] = cv == 255u ? __int_as_float(0x7f800000) : (float)code_value(cv, V_BIAS + (int)W.v_scale[e / MOMENT_BLOCK] - 127);
+    const uint8_t* const pm = reinterpret_cast<const uint8_t*>(W.m) + e;
+    const uint8_t* const pv = reinterpret_cast<const uint8_t*>(W.v) + e;
+    const uint32_t n = size - e < 4 ? (uint32_t)(size - e) : 4u;
+    uint8_t cm[4], cv[4];
+    load_elements(cm, pm, 0, n);
+    load_elements(cv, pv, 0, n);
+    const int sm = 120 - 127 + (int)W.m_scale[e / MOMENT_BLOCK], sv = 97 - 127 + (int)W.v_scale[e / MOMENT_BLOCK];
+    float a[4], b[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const uint32_t c = cm[j] & 127u;
+        a[j] = c == 127u ? __int_as_float(0x7fc00000) : ldexpf(__int_as_float((int)(c << 20)), sm);
+        a[j] = copysignf(a[j], cm[j] & 128u ? -1.0f : 1.0f);
+        b[j] = cv[j] == 255u ? __int_as_float(0x7f800000) : ldexpf(__int_as_float((int)((uint32_t)cv[j] << 20)), sv);
+    }
+    store_elements(m + e, a, 0, n);
+    store_elements(v + e, b, 0, n);
 }
 
 // ------------------------------------------------------------------------------------------------- norm of the gradients
@@ -193,12 +281,18 @@ __device__ __forceinline__ double block_sum(double x) {
 
 template <typename T>
 __device__ double square_sum(const ParamJob& J, uint32_t base) {
-    const T* const g = reinterpret_cast<const T*>(J.g);
+    constexpr int E = 16 / (int)sizeof(T), TURNS = GRAD_NORM_CHUNK / (256 * E);
+    T g[TURNS][E];
+#pragma unroll
+    for (int k = 0; k < TURNS; k++) load_elements(g[k], reinterpret_cast<const T*>(J.g), base + (k * 256 + threadIdx.x) * E, J.n);
     double s = 0.0;
-    for (uint32_t i = base + threadIdx.x; i < min(base + (uint32_t)GRAD_NORM_CHUNK, J.n); i += 256) {
-        const double x = (double)to_float(g[i]);
-        s = fma(x, x, s);
-    }
+#pragma unroll
+    for (int k = 0; k < TURNS; k++)
+#pragma unroll
+        for (int j = 0; j < E; j++) {
+            const double x = (double)to_float(g[k][j]);
+            s = fma(x, x, s);
+        }
     return s;
 }
 
