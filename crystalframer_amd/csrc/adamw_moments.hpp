@@ -73,8 +73,8 @@ __global__ void adamw_begin_kernel(AdamWStep* out, unsigned long long* step, dou
     out->key = k ^ (k >> 16);
 }
 
-__device__ __forceinline__ uint32_t moment_hash(uint32_t element, uint32_t key) {
-    uint32_t x = element * 0x9E3779B1u + key;
+// of element * 0x9E3779B1 + key
+__device__ __forceinline__ uint32_t moment_hash(uint32_t x) {
     x = (x ^ (x >> 16)) * 0xBB67AE85u;
     return x ^ (x >> 15);
 }
@@ -92,11 +92,19 @@ constexpr int M_BIAS = 1016, V_BIAS = 993, M_TOP = 7, V_TOP = 0;
 constexpr uint32_t HIGH_INF = 0x7ff00000u, HIGH_2_128 = 0x47f00000u;      // high words: no number from here on; 2^128
 
 __device__ __forceinline__ uint32_t high_word(double x) { return (uint32_t)__double2hiint(x); }
-__device__ __forceinline__ double code_value(uint32_t code, int bias) {
-    return ldexp(__hiloint2double((int)(code << 17), 0), bias);
+// The value of byte j of a word of codes; with the sign in its top bit for exp_avg.
+__device__ __forceinline__ double m_value(uint32_t word, int j, int scale) {
+    const int high = (((int)(word << (24 - 8 * j)) >> 24) << 17) & (int)0x80FE0000u;
+    return ldexp(__hiloint2double(high, 0), scale);
+}
+__device__ __forceinline__ double v_value(uint32_t word, int j, int scale) {
+    return ldexp(__hiloint2double((int)((word >> 8 * j & 255u) << 17), 0), scale);
 }
 // floor(x / step + (2 k + 1) / 2^17) as a code; x >= 0, odd = 2 k + 1 in 17 bits
-__device__ __forceinline__ uint32_t code_of(double x, int bias, uint32_t odd) { return (high_word(ldexp(x, -bias)) + odd) >> 17; }
+__device__ __forceinline__ uint32_t code_of(double x, int scale, uint32_t odd) { return (high_word(ldexp(x, scale)) + odd) >> 17; }
+// Whether a word of codes holds one that is no number (exp_avg) or more than 32 bits hold (exp_avg_sq).
+__device__ __forceinline__ bool m_odd(uint32_t w) { return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0; }
+__device__ __forceinline__ bool v_odd(uint32_t w) { return (((w & 0x7f7f7f7fu) + 0x01010101u) & w & 0x80808080u) != 0; }
 
 // The scale byte of a block whose largest magnitude has this high word (0: none): the largest then lies in [2^top, 2^(top + 1)).
 __device__ __forceinline__ int scale_byte(uint32_t high, int top) {
@@ -122,34 +130,48 @@ __device__ __forceinline__ uint32_t block_max(uint32_t x) {
     return x;
 }
 
-// `E` elements of a tensor from `i` on (fewer at its end, none behind it), of which a lane takes care: a block of 64 lies in 64 / E lanes.
-template <typename T, int E>
+// `E` elements of a tensor from `i` on, of which a lane takes care: a block of 64 lies in 64 / E lanes.  WHOLE: all of them are there;
+// else there may be fewer, or none.
+template <bool WHOLE, typename T, int E>
 __device__ __forceinline__ void load_elements(T (&o)[E], const T* from, uint32_t i, uint32_t n) {
-    if (i + E <= n) __builtin_memcpy(o, from + i, sizeof(o));
+    if (WHOLE || i + E <= n) __builtin_memcpy(o, from + i, sizeof(o));
     else {
 #pragma unroll
         for (int j = 0; j < E; j++) o[j] = i + j < n ? from[i + j] : T{};
     }
 }
-template <typename T, int E>
+template <bool WHOLE, typename T, int E>
 __device__ __forceinline__ void store_elements(T* to, const T (&o)[E], uint32_t i, uint32_t n) {
-    if (i + E <= n) __builtin_memcpy(to + i, o, sizeof(o));
+    if (WHOLE || i + E <= n) __builtin_memcpy(to + i, o, sizeof(o));
     else {
 #pragma unroll
         for (int j = 0; j < E; j++)
             if (i + j < n) to[i + j] = o[j];
     }
 }
+// E codes as words
+template <bool WHOLE, int E>
+__device__ __forceinline__ void load_codes(uint32_t (&w)[E / 4], const uint8_t* from, uint32_t i, uint32_t n) {
+    uint8_t c[E];
+    load_elements<WHOLE>(c, from, i, n);
+    __builtin_memcpy(w, c, E);
+}
+template <bool WHOLE, int E>
+__device__ __forceinline__ void store_codes(uint8_t* to, const uint32_t (&w)[E / 4], uint32_t i, uint32_t n) {
+    uint8_t c[E];
+    __builtin_memcpy(c, w, E);
+    store_elements<WHOLE>(to, c, i, n);
+}
 
-template <typename T, int E>
+template <bool WHOLE, typename T, int E>
 __device__ __forceinline__ void moments32(const ParamJob& J, uint32_t i, const T (&g)[E], T (&p)[E], const Moments& W, const AdamWStep& S,
                                           const AdamWRates& R) {
     float* const pm = reinterpret_cast<float*>(W.m) + J.first;
     float* const pv = reinterpret_cast<float*>(W.v) + J.first;
     const float b1 = (float)R.beta1, a1 = (float)(1.0 - R.beta1), b2 = (float)R.beta2, a2 = (float)(1.0 - R.beta2);
     float m[E], v[E];
-    load_elements(m, pm, i, J.n);
-    load_elements(v, pv, i, J.n);
+    load_elements<WHOLE>(m, pm, i, J.n);
+    load_elements<WHOLE>(v, pv, i, J.n);
 #pragma unroll
     for (int j = 0; j < E; j++) {
         const float c = to_float(g[j]) * S.clip;
@@ -157,33 +179,47 @@ __device__ __forceinline__ void moments32(const ParamJob& J, uint32_t i, const T
         v[j] = b2 * v[j] + a2 * c * c;
         p[j] = from_float<T>(adamw_update(to_float(p[j]), m[j], v[j], S, R.eps));
     }
-    store_elements(pm, m, i, J.n);
-    store_elements(pv, v, i, J.n);
+    store_elements<WHOLE>(pm, m, i, J.n);
+    store_elements<WHOLE>(pv, v, i, J.n);
 }
 
-template <typename T, int E>
+// Some 60 vector instructions per element, which the 16 bytes of a float32 parameter hide and the 10 of one in 16 bits nearly do;
+// what 32 bits do not hold is looked for in words of four codes and in the largest of a lane, and dealt with on a path of its own.
+template <bool WHOLE, typename T, int E>
 __device__ __forceinline__ void moments8(const ParamJob& J, uint32_t i, const T (&g)[E], T (&p)[E], const Moments& W, const AdamWStep& S,
                                          const AdamWRates& R) {
     uint8_t* const pm = reinterpret_cast<uint8_t*>(W.m) + J.first;
     uint8_t* const pv = reinterpret_cast<uint8_t*>(W.v) + J.first;
     uint8_t* const ps = W.m_scale + J.first / MOMENT_BLOCK;
     uint8_t* const pt = W.v_scale + J.first / MOMENT_BLOCK;
-    uint8_t cm[E], cv[E];
-    load_elements(cm, pm, i, J.n);
-    load_elements(cv, pv, i, J.n);
-    const int sm0 = i < J.n ? M_BIAS - 127 + (int)ps[i / MOMENT_BLOCK] : 0, sv0 = i < J.n ? V_BIAS - 127 + (int)pt[i / MOMENT_BLOCK] : 0;
+    uint32_t cm[E / 4], cv[E / 4];
+    load_codes<WHOLE, E>(cm, pm, i, J.n);
+    load_codes<WHOLE, E>(cv, pv, i, J.n);
+    const bool some = WHOLE || i < J.n;
+    const int sm0 = some ? M_BIAS - 127 + (int)ps[i / MOMENT_BLOCK] : 0, sv0 = some ? V_BIAS - 127 + (int)pt[i / MOMENT_BLOCK] : 0;
+    const double a1 = 1.0 - R.beta1, a2 = 1.0 - R.beta2;
     double m[E], v[E];
     bool odd = false;
+#pragma unroll
+    for (int k = 0; k < E / 4; k++) odd = odd || m_odd(cm[k]) || v_odd(cv[k]);
+#pragma unroll
+    for (int j = 0; j < E; j++) {
+        m[j] = m_value(cm[j / 4], j % 4, sm0);
+        v[j] = v_value(cv[j / 4], j % 4, sv0);
+    }
+    if (__any(odd)) {
+#pragma unroll
+        for (int j = 0; j < E; j++) {
+            if ((cm[j / 4] >> 8 * (j % 4) & 127u) == 127u) m[j] = __longlong_as_double(0x7ff8000000000000LL);
+            if ((cv[j / 4] >> 8 * (j % 4) & 255u) == 255u) v[j] = __longlong_as_double(0x7ff0000000000000LL);
+        }
+    }
     uint32_t hm = 0, hv = 0;
 #pragma unroll
     for (int j = 0; j < E; j++) {
         const double c = (double)to_float(g[j]) * (double)S.clip;
-        double a = code_value(cm[j] & 127u, sm0), b = code_value(cv[j], sv0);
-        a = __hiloint2double((int)(high_word(a) | (uint32_t)(cm[j] & 128u) << 24), __double2loint(a));
-        if ((cm[j] & 127u) == 127u) a = __longlong_as_double(0x7ff8000000000000LL);
-        if (cv[j] == 255u) b = __longlong_as_double(0x7ff0000000000000LL);
-        m[j] = moment_mix(R.beta1, a, (1.0 - R.beta1) * c);
-        v[j] = moment_mix(R.beta2, b, (1.0 - R.beta2) * c * c);
+        m[j] = moment_mix(R.beta1, m[j], a1 * c);
+        v[j] = moment_mix(R.beta2, v[j], a2 * c * c);
         hm = max(hm, high_word(m[j]) & 0x7fffffffu);
         hv = max(hv, high_word(v[j]));
     }
@@ -198,29 +234,32 @@ __device__ __forceinline__ void moments8(const ParamJob& J, uint32_t i, const T 
         }
     }
     const int sm = scale_byte(block_max<MOMENT_BLOCK / E>(hm), M_TOP), sv = scale_byte(block_max<MOMENT_BLOCK / E>(hv), V_TOP);
+    const uint32_t x0 = ((uint32_t)J.first + i) * 0x9E3779B1u + S.key;
+#pragma unroll
+    for (int k = 0; k < E / 4; k++) cm[k] = cv[k] = 0;
 #pragma unroll
     for (int j = 0; j < E; j++) {
-        const uint32_t h = moment_hash((uint32_t)J.first + i + j, S.key);
-        uint32_t a = code_of(fabs(m[j]), M_BIAS - 127 + sm, (h << 1 & 0x1ffffu) | 1u);
-        uint32_t b = code_of(v[j], V_BIAS - 127 + sv, h >> 15 | 1u);
-        b = max(b, v[j] > 0.0 ? 1u : 0u);
+        const uint32_t h = moment_hash(x0 + (uint32_t)j * 0x9E3779B1u);
+        uint32_t a = code_of(fabs(m[j]), -(M_BIAS - 127 + sm), (h << 1 & 0x1ffffu) | 1u);
+        uint32_t b = code_of(v[j], -(V_BIAS - 127 + sv), h >> 15 | 1u);
+        b = max(b, min(high_word(v[j]), 1u));          // (no double that comes up here is below 2^-1022)
         if (odd) {
             if ((high_word(m[j]) & 0x7fffffffu) >= HIGH_INF) a = 127u;
             if (high_word(v[j]) >= HIGH_2_128) b = 255u;
         }
-        cm[j] = (uint8_t)(a | (high_word(m[j]) >> 24 & 128u));
-        cv[j] = (uint8_t)b;
+        cm[j / 4] |= ((high_word(m[j]) >> 24 & 128u) | a) << 8 * (j % 4);
+        cv[j / 4] |= b << 8 * (j % 4);
         p[j] = from_float<T>(adamw_update(to_float(p[j]), (float)m[j], (float)v[j], S, R.eps));
     }
-    store_elements(pm, cm, i, J.n);
-    store_elements(pv, cv, i, J.n);
-    if (i < J.n && i % MOMENT_BLOCK == 0) {
+    store_codes<WHOLE, E>(pm, cm, i, J.n);
+    store_codes<WHOLE, E>(pv, cv, i, J.n);
+    if (some && i % MOMENT_BLOCK == 0) {
         ps[i / MOMENT_BLOCK] = (uint8_t)sm;
         pt[i / MOMENT_BLOCK] = (uint8_t)sv;
     }
 }
 
-template <typename T, int BITS>
+template <typename T, int BITS, bool WHOLE>
 __device__ __forceinline__ void adamw_chunk(const ParamJob& J, uint32_t base, const Moments& W, const AdamWStep* step, const AdamWRates& R) {
     constexpr int E = 16 / (int)sizeof(T);
     T* const pp = reinterpret_cast<T*>(J.p);
@@ -228,11 +267,11 @@ __device__ __forceinline__ void adamw_chunk(const ParamJob& J, uint32_t base, co
     for (int k = 0; k < ADAMW_CHUNK / (256 * E); k++) {
         const uint32_t i = base + ((uint32_t)k * 256 + threadIdx.x) * E;
         T g[E], p[E];
-        load_elements(g, reinterpret_cast<const T*>(J.g), i, J.n);
-        load_elements(p, pp, i, J.n);
-        if constexpr (BITS == 32) moments32(J, i, g, p, W, S, R);
-        else moments8(J, i, g, p, W, S, R);
-        store_elements(pp, p, i, J.n);
+        load_elements<WHOLE>(g, reinterpret_cast<const T*>(J.g), i, J.n);
+        load_elements<WHOLE>(p, pp, i, J.n);
+        if constexpr (BITS == 32) moments32<WHOLE>(J, i, g, p, W, S, R);
+        else moments8<WHOLE>(J, i, g, p, W, S, R);
+        store_elements<WHOLE>(pp, p, i, J.n);
     }
 }
 
@@ -241,9 +280,14 @@ __global__ __launch_bounds__(256) void adamw_moments_kernel(const ParamJobs T, c
                                                             const AdamWRates R) {
     const ParamJob& J = job_of(T, blockIdx.x);
     const uint32_t base = (blockIdx.x - J.chunk0) * ADAMW_CHUNK;
-    if (J.dtype == TYPE_F32) adamw_chunk<float, BITS>(J, base, W, step, R);
-    else if (J.dtype == TYPE_BF16) adamw_chunk<bf16, BITS>(J, base, W, step, R);
-    else adamw_chunk<f16, BITS>(J, base, W, step, R);
+    auto run = [&](auto t) {
+        using E = decltype(t);
+        if (base + ADAMW_CHUNK <= J.n) adamw_chunk<E, BITS, true>(J, base, W, step, R);
+        else adamw_chunk<E, BITS, false>(J, base, W, step, R);
+    };
+    if (J.dtype == TYPE_F32) run(float());
+    else if (J.dtype == TYPE_BF16) run(bf16());
+    else run(f16());
 }
 
 // Four elements per lane: 8 bytes read, 32 written.  In 32 bits the codes' bits, moved under a float's exponent field, are the values
@@ -255,8 +299,8 @@ __global__ __launch_bounds__(256) void moment_values_kernel(const Moments W, uin
     const uint8_t* const pv = reinterpret_cast<const uint8_t*>(W.v) + e;
     const uint32_t n = size - e < 4 ? (uint32_t)(size - e) : 4u;
     uint8_t cm[4], cv[4];
-    load_elements(cm, pm, 0, n);
-    load_elements(cv, pv, 0, n);
+    load_elements<false>(cm, pm, 0, n);
+    load_elements<false>(cv, pv, 0, n);
     const int sm = 120 - 127 + (int)W.m_scale[e / MOMENT_BLOCK], sv = 97 - 127 + (int)W.v_scale[e / MOMENT_BLOCK];
     float a[4], b[4];
 #pragma unroll
@@ -266,8 +310,8 @@ __global__ __launch_bounds__(256) void moment_values_kernel(const Moments W, uin
         a[j] = copysignf(a[j], cm[j] & 128u ? -1.0f : 1.0f);
         b[j] = cv[j] == 255u ? __int_as_float(0x7f800000) : ldexpf(__int_as_float((int)((uint32_t)cv[j] << 20)), sv);
     }
-    store_elements(m + e, a, 0, n);
-    store_elements(v + e, b, 0, n);
+    store_elements<false>(m + e, a, 0, n);
+    store_elements<false>(v + e, b, 0, n);
 }
 
 // ------------------------------------------------------------------------------------------------- norm of the gradients
@@ -284,7 +328,7 @@ __device__ double square_sum(const ParamJob& J, uint32_t base) {
     constexpr int E = 16 / (int)sizeof(T), TURNS = GRAD_NORM_CHUNK / (256 * E);
     T g[TURNS][E];
 #pragma unroll
-    for (int k = 0; k < TURNS; k++) load_elements(g[k], reinterpret_cast<const T*>(J.g), base + (k * 256 + threadIdx.x) * E, J.n);
+    for (int k = 0; k < TURNS; k++) load_elements<false>(g[k], reinterpret_cast<const T*>(J.g), base + (k * 256 + threadIdx.x) * E, J.n);
     double s = 0.0;
 #pragma unroll
     for (int k = 0; k < TURNS; k++)
