@@ -344,6 +344,29 @@ struct Updates {
         }
         return n;
     }
+    // The same for cfh_adamw_step_moments, whose tensors have types of their own and whose moments are given by their place.
+    int64_t fill_params(uintptr_t jobs) const {
+        cfh_param_job* const J = reinterpret_cast<cfh_param_job*>(jobs);
+        int64_t n = 0;
+        for (size_t i = 0; i < params.size(); i++) {
+            const at::Tensor& p = params[i];
+            const at::Tensor& g = p.grad();
+            if (!g.defined()) continue;
+            const at::ScalarType t = p.scalar_type();
+            if (offset[i] < 0 || g.layout() != at::kStrided || g.scalar_type() != t || !g.is_contiguous() || !p.is_contiguous() ||
+                p.numel() != numel[i] || g.numel() != numel[i] || p.device() != device || g.device() != device ||
+                !(t == at::kFloat || t == at::kBFloat16 || t == at::kHalf))
+                return -1;
+            cfh_param_job& j = J[n++];
+            j.param = p.data_ptr();
+            j.grad = g.data_ptr();
+            j.n = numel[i];
+            j.first = offset[i];
+            j.dtype = t == at::kFloat ? CFH_FLOAT32 : t == at::kBFloat16 ? CFH_BFLOAT16 : CFH_FLOAT16;
+            j.reserved0 = 0;
+        }
+        return n;
+    }
     // every .grad becomes None
     void drop() {
         for (auto& p : params) p.mutable_grad().reset();
@@ -374,5 +397,6 @@ PYBIND11_MODULE(_host, mod) {
         .def(py::init<std::vector<at::Tensor>, std::vector<int64_t>, std::vector<int64_t>, const at::Tensor&>())
         .def("of", &Updates::of)
         .def("fill", &Updates::fill)
+        .def("fill_params", &Updates::fill_params)
         .def("drop", &Updates::drop);
 }

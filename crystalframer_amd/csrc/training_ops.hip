@@ -58,6 +58,13 @@ void in_tables(const cfh_param_job* jobs, int32_t njobs, int64_t chunk, F launch
     if (T.njobs > 0) launch(T);
 }
 
+// Elements that a workgroup of the norm takes at a time: the larger count once there are two such turns for each compute unit.
+int64_t norm_chunk(const cfh_param_job* jobs, int32_t njobs) {
+    int64_t n = 0;
+    for (int32_t j = 0; j < njobs; j++) n += jobs[j].n;
+    return n < 512LL * cfh::GRAD_NORM_CHUNK ? cfh::GRAD_NORM_FEW : cfh::GRAD_NORM_CHUNK;
+}
+
 int check_moments(const char* what, const cfh_moments* s) {
     if (!s) return fail(CFH_EINVAL, "%s: state must not be NULL", what);
     if (s->bits != 8 && s->bits != 32) return fail(CFH_EINVAL, "%s: moments in %d bits: 8 or 32", what, (int)s->bits);
@@ -144,7 +151,8 @@ int cfh_adamw_moments(const cfh_moments* state, float* exp_avg, float* exp_avg_s
     if (state->size == 0) return CFH_OK;
     if (!exp_avg || !exp_avg_sq) return fail(CFH_EINVAL, "adamw_moments: exp_avg and exp_avg_sq must not be NULL");
     const cfh::Moments W{state->exp_avg, state->exp_avg_sq, state->exp_avg_scale, state->exp_avg_sq_scale};
-    hipLaunchKernelGGL(cfh::moment_values_kernel, dim3((unsigned)((state->size + 1023) / 1024)), dim3(256), 0, (hipStream_t)stream, W,
+    hipLaunchKernelGGL(cfh::moment_values_kernel, dim3((unsigned)((state->size + cfh::VALUES_CHUNK - 1) / cfh::VALUES_CHUNK)), dim3(256), 0,
+                       (hipStream_t)stream, W,
                        (uint64_t)state->size, exp_avg, exp_avg_sq);
     return finish_launch("adamw_moments");
 }
@@ -152,7 +160,7 @@ int cfh_adamw_moments(const cfh_moments* state, float* exp_avg, float* exp_avg_s
 size_t cfh_grad_norm_workspace_bytes(const cfh_param_job* jobs, int32_t njobs) {
     if (check_jobs("grad_norm", jobs, njobs, false)) return 0;
     size_t n = 1;
-    in_tables(jobs, njobs, cfh::GRAD_NORM_CHUNK, [&](const cfh::ParamJobs& T) { n += T.chunks < cfh::GRAD_NORM_BLOCKS ? T.chunks : cfh::GRAD_NORM_BLOCKS; });
+    in_tables(jobs, njobs, norm_chunk(jobs, njobs), [&](const cfh::ParamJobs& T) { n += T.chunks < cfh::GRAD_NORM_BLOCKS ? T.chunks : cfh::GRAD_NORM_BLOCKS; });
     return n * sizeof(double);
 }
 
@@ -167,9 +175,12 @@ int cfh_grad_norm(const cfh_param_job* jobs, int32_t njobs, double max_norm, flo
     hipStream_t st = (hipStream_t)stream;
     double* const partial = reinterpret_cast<double*>(workspace);
     int count = 0;
-    in_tables(jobs, njobs, cfh::GRAD_NORM_CHUNK, [&](const cfh::ParamJobs& T) {
+    const int64_t chunk = norm_chunk(jobs, njobs);
+    in_tables(jobs, njobs, chunk, [&](const cfh::ParamJobs& T) {
         const int blocks = T.chunks < cfh::GRAD_NORM_BLOCKS ? (int)T.chunks : cfh::GRAD_NORM_BLOCKS;
-        hipLaunchKernelGGL(cfh::grad_norm_kernel, dim3(blocks), dim3(256), 0, st, T, partial + count);
+        if (chunk == cfh::GRAD_NORM_FEW)
+            hipLaunchKernelGGL(cfh::grad_norm_kernel<cfh::GRAD_NORM_FEW>, dim3(blocks), dim3(256), 0, st, T, partial + count);
+        else hipLaunchKernelGGL(cfh::grad_norm_kernel<cfh::GRAD_NORM_CHUNK>, dim3(blocks), dim3(256), 0, st, T, partial + count);
         count += blocks;
     });
     hipLaunchKernelGGL(cfh::grad_norm_end_kernel, dim3(1), dim3(256), 0, st, partial, count, max_norm, out);

@@ -191,7 +191,12 @@ class AdamW(torch.optim.Optimizer):
         """The step of groups of any type, with moments in 32 or 8 bits; the gradients' common norm first if they are clipped."""
         filled = []
         for group, st, plan in work:
-            jobs, n, keep = self._fill_moments(plan)
+            jobs = plan.get("param_jobs")
+            if jobs is None:
+                jobs = plan["param_jobs"] = (_lib.CfhParamJob * max(len(plan["params"]), 1))()
+            n, keep = plan["native"].fill_params(ctypes.addressof(jobs)), None
+            if n < 0:
+                n, keep = self._fill_moments(plan, jobs)      # a gradient that has to be looked at
             if n:
                 filled.append((group, st, plan, jobs, n, keep))
         clip = None
@@ -232,9 +237,9 @@ class AdamW(torch.optim.Optimizer):
         return out
 
     @staticmethod
-    def _fill_moments(plan):
-        """The job table of ``cfh_adamw_step_moments``: (jobs, how many, gradients made contiguous here)."""
-        jobs, n, keep = (_lib.CfhParamJob * max(len(plan["params"]), 1))(), 0, None
+    def _fill_moments(plan, jobs):
+        """The job table of ``cfh_adamw_step_moments`` parameter by parameter: (jobs, gradients made contiguous here)."""
+        n, keep = 0, None
         for p, off, count in zip(plan["params"], plan["offs"], plan["counts"]):
             g = p.grad
             if g is None:
@@ -248,7 +253,7 @@ class AdamW(torch.optim.Optimizer):
             j = jobs[n]
             j.param, j.grad, j.n, j.first, j.dtype = p.data_ptr(), g.data_ptr(), count, off, _lib.ELEMENT_TYPES[p.dtype]
             n += 1
-        return jobs, n, keep
+        return n, keep
 
     @staticmethod
     def _gradient(p, g, off, count, device):
