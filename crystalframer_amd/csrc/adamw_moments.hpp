@@ -292,45 +292,31 @@ __global__ __launch_bounds__(256) void adamw_moments_kernel(const ParamJobs T, c
     else run(f16());
 }
 
-// Four elements per lane and turn: 8 bytes read, 32 written; the turns' loads are all on their way before the first store.  In 32 bits
-// the codes' bits, moved under a float's exponent field, are the values times 2^-120 and 2^-97.  Stores that leave the caches to
-// others: 151 M elements 423 -> 328 us.
-constexpr int VALUES_TURNS = 4, VALUES_CHUNK = 256 * 4 * VALUES_TURNS;
+// Four elements of one of the moments (blockIdx.y) per lane, nothing of it left in the caches: bound by HBM's writes.  In 32 bits the
+// codes' bits, moved under a float's exponent field, are the values times 2^-120 and 2^-97.
+constexpr int VALUES_CHUNK = 256 * 4;
 __global__ __launch_bounds__(256) void moment_values_kernel(const Moments W, uint64_t size, float* m, float* v) {
     typedef float f4 __attribute__((ext_vector_type(4)));
-    const uint64_t e0 = (uint64_t)blockIdx.x * VALUES_CHUNK;
-    const uint32_t n = size - e0 < VALUES_CHUNK ? (uint32_t)(size - e0) : VALUES_CHUNK;
-    const uint8_t* const pm = reinterpret_cast<const uint8_t*>(W.m) + e0;
-    const uint8_t* const pv = reinterpret_cast<const uint8_t*>(W.v) + e0;
-    uint32_t cm[VALUES_TURNS][1], cv[VALUES_TURNS][1];
-    int sm[VALUES_TURNS], sv[VALUES_TURNS];
+    const bool first = blockIdx.y == 0;
+    const uint64_t e = (uint64_t)blockIdx.x * VALUES_CHUNK + threadIdx.x * 4;
+    if (e >= size) return;
+    const uint8_t* const codes = reinterpret_cast<const uint8_t*>(first ? W.m : W.v) + e;
+    float* const out = (first ? m : v) + e;
+    const uint32_t n = size - e < 4 ? (uint32_t)(size - e) : 4u;
+    uint32_t w[1];
+    if (n == 4) w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(codes));
+    else load_codes<false, 4>(w, codes, 0, n);
+    const int scale = (first ? 120 - 127 : 97 - 127) + (int)(first ? W.m_scale : W.v_scale)[e / MOMENT_BLOCK];
+    const uint32_t field = first ? 127u : 255u, none = first ? 0x7fc00000u : 0x7f800000u, sign = first ? 0x80000000u : 0u;
+    float a[4];
 #pragma unroll
-    for (int k = 0; k < VALUES_TURNS; k++) {
-        const uint32_t i = ((uint32_t)k * 256 + threadIdx.x) * 4;
-        load_codes<false, 4>(cm[k], pm, i, n);
-        load_codes<false, 4>(cv[k], pv, i, n);
-        sm[k] = i < n ? 120 - 127 + (int)W.m_scale[(e0 + i) / MOMENT_BLOCK] : 0;
-        sv[k] = i < n ? 97 - 127 + (int)W.v_scale[(e0 + i) / MOMENT_BLOCK] : 0;
+    for (int j = 0; j < 4; j++) {
+        const uint32_t c = w[0] >> 8 * j & field;
+        const uint32_t bits = c == field ? none : (uint32_t)__float_as_int(ldexpf(__int_as_float((int)(c << 20)), scale));
+        a[j] = __int_as_float((int)(bits | (w[0] << (24 - 8 * j) & sign)));
     }
-#pragma unroll
-    for (int k = 0; k < VALUES_TURNS; k++) {
-        const uint32_t i = ((uint32_t)k * 256 + threadIdx.x) * 4;
-        float a[4], b[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const uint32_t c = cm[k][0] >> 8 * j & 127u, d = cv[k][0] >> 8 * j & 255u;
-            a[j] = c == 127u ? __int_as_float(0x7fc00000) : ldexpf(__int_as_float((int)(c << 20)), sm[k]);
-            a[j] = __int_as_float(__float_as_int(a[j]) | (int)(cm[k][0] << (24 - 8 * j) & 0x80000000u));
-            b[j] = d == 255u ? __int_as_float(0x7f800000) : ldexpf(__int_as_float((int)(d << 20)), sv[k]);
-        }
-        if (i + 4 <= n) {
-            __builtin_nontemporal_store(f4{a[0], a[1], a[2], a[3]}, reinterpret_cast<f4*>(m + e0 + i));
-            __builtin_nontemporal_store(f4{b[0], b[1], b[2], b[3]}, reinterpret_cast<f4*>(v + e0 + i));
-        } else {
-            store_elements<false>(m + e0, a, i, n);
-            store_elements<false>(v + e0, b, i, n);
-        }
-    }
+    if (n == 4 && ((uintptr_t)out & 15) == 0) __builtin_nontemporal_store(f4{a[0], a[1], a[2], a[3]}, reinterpret_cast<f4*>(out));
+    else store_elements<false>(out, a, 0, n);
 }
 
 // ------------------------------------------------------------------------------------------------- norm of the gradients

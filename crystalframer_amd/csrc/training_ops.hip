@@ -151,7 +151,7 @@ int cfh_adamw_moments(const cfh_moments* state, float* exp_avg, float* exp_avg_s
     if (state->size == 0) return CFH_OK;
     if (!exp_avg || !exp_avg_sq) return fail(CFH_EINVAL, "adamw_moments: exp_avg and exp_avg_sq must not be NULL");
     const cfh::Moments W{state->exp_avg, state->exp_avg_sq, state->exp_avg_scale, state->exp_avg_sq_scale};
-    hipLaunchKernelGGL(cfh::moment_values_kernel, dim3((unsigned)((state->size + cfh::VALUES_CHUNK - 1) / cfh::VALUES_CHUNK)), dim3(256), 0,
+    hipLaunchKernelGGL(cfh::moment_values_kernel, dim3((unsigned)((state->size + cfh::VALUES_CHUNK - 1) / cfh::VALUES_CHUNK), 2), dim3(256), 0,
                        (hipStream_t)stream, W,
                        (uint64_t)state->size, exp_avg, exp_avg_sq);
     return finish_launch("adamw_moments");
