@@ -18,6 +18,7 @@ constexpr int PARAM_MAX_JOBS = 88;        // tensors per launch (kernel argument
 constexpr int ADAMW_CHUNK = 2048;         // elements per workgroup of 256 threads
 constexpr int GRAD_NORM_CHUNK = 8192;     // elements per turn of a workgroup of 256 threads: eight (four) loads under way per lane
 constexpr int GRAD_NORM_FEW = 2048;       // the same where there are not enough of those to go round
+constexpr int64_t GRAD_NORM_CACHED = 256LL << 20;      // bytes that the last cache holds
 constexpr int GRAD_NORM_BLOCKS = 2048;    // workgroups per launch at most
 
 struct ParamJob {
@@ -328,12 +329,28 @@ __device__ __forceinline__ double block_sum(double x) {
     return part[0] + part[1] + part[2] + part[3];
 }
 
-template <typename T, int CHUNK>
+// 16 bytes of a tensor that will not be looked at again soon.
+template <typename T, int E>
+__device__ __forceinline__ void stream_elements(T (&o)[E], const T* from, uint32_t i, uint32_t n) {
+    typedef uint32_t words4 __attribute__((ext_vector_type(4), aligned(4)));
+    typedef uint32_t words2 __attribute__((ext_vector_type(4), aligned(2)));
+    using V = std::conditional_t<sizeof(T) == 4, words4, words2>;
+    if (i + E <= n) {
+        const V x = __builtin_nontemporal_load(reinterpret_cast<const V*>(from + i));
+        __builtin_memcpy(o, &x, sizeof(o));
+    } else load_elements<false>(o, from, i, n);
+}
+
+template <typename T, int CHUNK, bool STREAM>
 __device__ __forceinline__ double square_sum(const ParamJob& J, uint32_t base) {
     constexpr int E = 16 / (int)sizeof(T), TURNS = CHUNK / (256 * E);
     T g[TURNS][E];
 #pragma unroll
-    for (int k = 0; k < TURNS; k++) load_elements<false>(g[k], reinterpret_cast<const T*>(J.g), base + (k * 256 + threadIdx.x) * E, J.n);
+    for (int k = 0; k < TURNS; k++) {
+        const uint32_t i = base + (k * 256 + threadIdx.x) * E;
+        if constexpr (STREAM) stream_elements(g[k], reinterpret_cast<const T*>(J.g), i, J.n);
+        else load_elements<false>(g[k], reinterpret_cast<const T*>(J.g), i, J.n);
+    }
     double s = 0.0;
 #pragma unroll
     for (int k = 0; k < TURNS; k++)
@@ -345,14 +362,16 @@ __device__ __forceinline__ double square_sum(const ParamJob& J, uint32_t base) {
     return s;
 }
 
-template <int CHUNK>
+// STREAM: gradients that the last cache does not hold until the update reads them again go past it; 134 M float32 gradients, norm and
+// update 511 -> 460 us, 34 M (128 MiB) 120 -> 121, 34 M bfloat16 87 -> 91.
+template <int CHUNK, bool STREAM>
 __global__ __launch_bounds__(256) void grad_norm_kernel(const ParamJobs T, double* partial) {
     double s = 0.0;
     for (uint32_t c = blockIdx.x; c < T.chunks; c += gridDim.x) {
         const ParamJob& J = job_of(T, c);
         const uint32_t base = (c - J.chunk0) * CHUNK;
-        s += J.dtype == TYPE_F32 ? square_sum<float, CHUNK>(J, base) : J.dtype == TYPE_BF16 ? square_sum<bf16, CHUNK>(J, base)
-                                                                                            : square_sum<f16, CHUNK>(J, base);
+        s += J.dtype == TYPE_F32 ? square_sum<float, CHUNK, STREAM>(J, base)
+             : J.dtype == TYPE_BF16 ? square_sum<bf16, CHUNK, STREAM>(J, base) : square_sum<f16, CHUNK, STREAM>(J, base);
     }
     s = block_sum(s);
     if (threadIdx.x == 0) partial[blockIdx.x] = s;

@@ -176,11 +176,14 @@ int cfh_grad_norm(const cfh_param_job* jobs, int32_t njobs, double max_norm, flo
     double* const partial = reinterpret_cast<double*>(workspace);
     int count = 0;
     const int64_t chunk = norm_chunk(jobs, njobs);
+    int64_t bytes = 0;
+    for (int32_t j = 0; j < njobs; j++) bytes += jobs[j].n * (jobs[j].dtype == CFH_FLOAT32 ? 4 : 2);
     in_tables(jobs, njobs, chunk, [&](const cfh::ParamJobs& T) {
         const int blocks = T.chunks < cfh::GRAD_NORM_BLOCKS ? (int)T.chunks : cfh::GRAD_NORM_BLOCKS;
-        if (chunk == cfh::GRAD_NORM_FEW)
-            hipLaunchKernelGGL(cfh::grad_norm_kernel<cfh::GRAD_NORM_FEW>, dim3(blocks), dim3(256), 0, st, T, partial + count);
-        else hipLaunchKernelGGL(cfh::grad_norm_kernel<cfh::GRAD_NORM_CHUNK>, dim3(blocks), dim3(256), 0, st, T, partial + count);
+        const auto kernel = chunk == cfh::GRAD_NORM_FEW ? cfh::grad_norm_kernel<cfh::GRAD_NORM_FEW, false>
+                            : bytes < cfh::GRAD_NORM_CACHED ? cfh::grad_norm_kernel<cfh::GRAD_NORM_CHUNK, false>
+                                                            : cfh::grad_norm_kernel<cfh::GRAD_NORM_CHUNK, true>;
+        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, st, T, partial + count);
         count += blocks;
     });
     hipLaunchKernelGGL(cfh::grad_norm_end_kernel, dim3(1), dim3(256), 0, st, partial, count, max_norm, out);
