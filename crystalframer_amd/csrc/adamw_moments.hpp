@@ -16,9 +16,9 @@ namespace cfh {
 constexpr int MOMENT_BLOCK = 64;          // elements that share a scale
 constexpr int PARAM_MAX_JOBS = 88;        // tensors per launch (kernel arguments: 4 KB)
 constexpr int ADAMW_CHUNK = 2048;         // elements per workgroup of 256 threads
+constexpr int64_t CACHED_BYTES = 256LL << 20;      // that the last cache holds
 constexpr int GRAD_NORM_CHUNK = 8192;     // elements per turn of a workgroup of 256 threads: eight (four) loads under way per lane
 constexpr int GRAD_NORM_FEW = 2048;       // the same where there are not enough of those to go round
-constexpr int64_t GRAD_NORM_CACHED = 256LL << 20;      // bytes that the last cache holds
 constexpr int GRAD_NORM_BLOCKS = 2048;    // workgroups per launch at most
 
 struct ParamJob {
@@ -133,48 +133,75 @@ __device__ __forceinline__ uint32_t block_max(uint32_t x) {
     return x;
 }
 
-// `E` elements of a tensor from `i` on, of which a lane takes care: a block of 64 lies in 64 / E lanes.  WHOLE: all of them are there;
-// else there may be fewer, or none.
-template <bool WHOLE, typename T, int E>
+// Words of a lane's 4 to 32 bytes at an address of ALIGN bytes, for accesses past the caches.
+template <int BYTES, int ALIGN>
+struct Words;
+#define CFH_WORDS(bytes, alignment) \
+    template <> struct Words<bytes, alignment> { typedef uint32_t type __attribute__((ext_vector_type(bytes / 4), aligned(alignment))); };
+CFH_WORDS(16, 4)
+CFH_WORDS(16, 2)
+CFH_WORDS(32, 4)
+CFH_WORDS(8, 1)
+#undef CFH_WORDS
+template <> struct Words<4, 1> { typedef uint32_t type __attribute__((aligned(1))); };
+
+// How a chunk is gone through.  WHOLE: all its elements are there; else a lane may find fewer, or none.  STREAM: past the caches.
+template <bool WHOLE_, bool STREAM_>
+struct Way {
+    static constexpr bool WHOLE = WHOLE_, STREAM = STREAM_;
+};
+// `E` elements of a tensor from `i` on, of which a lane takes care: a block of 64 lies in 64 / E lanes.
+template <typename WAY, typename T, int E>
 __device__ __forceinline__ void load_elements(T (&o)[E], const T* from, uint32_t i, uint32_t n) {
-    if (WHOLE || i + E <= n) __builtin_memcpy(o, from + i, sizeof(o));
-    else {
+    if (WAY::WHOLE || i + E <= n) {
+        if constexpr (WAY::STREAM) {
+            using V = typename Words<sizeof(o), alignof(T)>::type;
+            const V x = __builtin_nontemporal_load(reinterpret_cast<const V*>(from + i));
+            __builtin_memcpy(o, &x, sizeof(o));
+        } else __builtin_memcpy(o, from + i, sizeof(o));
+    } else {
 #pragma unroll
         for (int j = 0; j < E; j++) o[j] = i + j < n ? from[i + j] : T{};
     }
 }
-template <bool WHOLE, typename T, int E>
+template <typename WAY, typename T, int E>
 __device__ __forceinline__ void store_elements(T* to, const T (&o)[E], uint32_t i, uint32_t n) {
-    if (WHOLE || i + E <= n) __builtin_memcpy(to + i, o, sizeof(o));
-    else {
+    if (WAY::WHOLE || i + E <= n) {
+        if constexpr (WAY::STREAM) {
+            using V = typename Words<sizeof(o), alignof(T)>::type;
+            V x;
+            __builtin_memcpy(&x, o, sizeof(o));
+            __builtin_nontemporal_store(x, reinterpret_cast<V*>(to + i));
+        } else __builtin_memcpy(to + i, o, sizeof(o));
+    } else {
 #pragma unroll
         for (int j = 0; j < E; j++)
             if (i + j < n) to[i + j] = o[j];
     }
 }
 // E codes as words
-template <bool WHOLE, int E>
+template <typename WAY, int E>
 __device__ __forceinline__ void load_codes(uint32_t (&w)[E / 4], const uint8_t* from, uint32_t i, uint32_t n) {
     uint8_t c[E];
-    load_elements<WHOLE>(c, from, i, n);
+    load_elements<WAY>(c, from, i, n);
     __builtin_memcpy(w, c, E);
 }
-template <bool WHOLE, int E>
+template <typename WAY, int E>
 __device__ __forceinline__ void store_codes(uint8_t* to, const uint32_t (&w)[E / 4], uint32_t i, uint32_t n) {
     uint8_t c[E];
     __builtin_memcpy(c, w, E);
-    store_elements<WHOLE>(to, c, i, n);
+    store_elements<WAY>(to, c, i, n);
 }
 
-template <bool WHOLE, typename T, int E>
+template <typename WAY, typename T, int E>
 __device__ __forceinline__ void moments32(const ParamJob& J, uint32_t i, const T (&g)[E], T (&p)[E], const Moments& W, const AdamWStep& S,
                                           const AdamWRates& R) {
     float* const pm = reinterpret_cast<float*>(W.m) + J.first;
     float* const pv = reinterpret_cast<float*>(W.v) + J.first;
     const float b1 = (float)R.beta1, a1 = (float)(1.0 - R.beta1), b2 = (float)R.beta2, a2 = (float)(1.0 - R.beta2);
     float m[E], v[E];
-    load_elements<WHOLE>(m, pm, i, J.n);
-    load_elements<WHOLE>(v, pv, i, J.n);
+    load_elements<WAY>(m, pm, i, J.n);
+    load_elements<WAY>(v, pv, i, J.n);
 #pragma unroll
     for (int j = 0; j < E; j++) {
         const float c = to_float(g[j]) * S.clip;
@@ -182,13 +209,13 @@ __device__ __forceinline__ void moments32(const ParamJob& J, uint32_t i, const T
         v[j] = b2 * v[j] + a2 * c * c;
         p[j] = from_float<T>(adamw_update(to_float(p[j]), m[j], v[j], S, R.eps));
     }
-    store_elements<WHOLE>(pm, m, i, J.n);
-    store_elements<WHOLE>(pv, v, i, J.n);
+    store_elements<WAY>(pm, m, i, J.n);
+    store_elements<WAY>(pv, v, i, J.n);
 }
 
 // Some 60 vector instructions per element, which the 16 bytes of a float32 parameter hide and the 10 of one in 16 bits nearly do;
 // what 32 bits do not hold is looked for in words of four codes and in the largest of a lane, and dealt with on a path of its own.
-template <bool WHOLE, typename T, int E>
+template <typename WAY, typename T, int E>
 __device__ __forceinline__ void moments8(const ParamJob& J, uint32_t i, const T (&g)[E], T (&p)[E], const Moments& W, const AdamWStep& S,
                                          const AdamWRates& R) {
     uint8_t* const pm = reinterpret_cast<uint8_t*>(W.m) + J.first;
@@ -196,9 +223,9 @@ __device__ __forceinline__ void moments8(const ParamJob& J, uint32_t i, const T 
     uint8_t* const ps = W.m_scale + J.first / MOMENT_BLOCK;
     uint8_t* const pt = W.v_scale + J.first / MOMENT_BLOCK;
     uint32_t cm[E / 4], cv[E / 4];
-    load_codes<WHOLE, E>(cm, pm, i, J.n);
-    load_codes<WHOLE, E>(cv, pv, i, J.n);
-    const bool some = WHOLE || i < J.n;
+    load_codes<WAY, E>(cm, pm, i, J.n);
+    load_codes<WAY, E>(cv, pv, i, J.n);
+    const bool some = WAY::WHOLE || i < J.n;
     const int sm0 = some ? M_BIAS - 127 + (int)ps[i / MOMENT_BLOCK] : 0, sv0 = some ? V_BIAS - 127 + (int)pt[i / MOMENT_BLOCK] : 0;
     const double a1 = 1.0 - R.beta1, a2 = 1.0 - R.beta2;
     double m[E], v[E];
@@ -254,15 +281,15 @@ __device__ __forceinline__ void moments8(const ParamJob& J, uint32_t i, const T 
         cv[j / 4] |= b << 8 * (j % 4);
         p[j] = from_float<T>(adamw_update(to_float(p[j]), (float)m[j], (float)v[j], S, R.eps));
     }
-    store_codes<WHOLE, E>(pm, cm, i, J.n);
-    store_codes<WHOLE, E>(pv, cv, i, J.n);
+    store_codes<WAY, E>(pm, cm, i, J.n);
+    store_codes<WAY, E>(pv, cv, i, J.n);
     if (some && i % MOMENT_BLOCK == 0) {
         ps[i / MOMENT_BLOCK] = (uint8_t)sm;
         pt[i / MOMENT_BLOCK] = (uint8_t)sv;
     }
 }
 
-template <typename T, int BITS, bool WHOLE>
+template <typename T, int BITS, typename WAY>
 __device__ __forceinline__ void adamw_chunk(const ParamJob& J, uint32_t base, const Moments& W, const AdamWStep* step, const AdamWRates& R) {
     constexpr int E = 16 / (int)sizeof(T);
     T* const pp = reinterpret_cast<T*>(J.p);
@@ -270,23 +297,25 @@ __device__ __forceinline__ void adamw_chunk(const ParamJob& J, uint32_t base, co
     for (int k = 0; k < ADAMW_CHUNK / (256 * E); k++) {
         const uint32_t i = base + ((uint32_t)k * 256 + threadIdx.x) * E;
         T g[E], p[E];
-        load_elements<WHOLE>(g, reinterpret_cast<const T*>(J.g), i, J.n);
-        load_elements<WHOLE>(p, pp, i, J.n);
-        if constexpr (BITS == 32) moments32<WHOLE>(J, i, g, p, W, S, R);
-        else moments8<WHOLE>(J, i, g, p, W, S, R);
-        store_elements<WHOLE>(pp, p, i, J.n);
+        load_elements<WAY>(g, reinterpret_cast<const T*>(J.g), i, J.n);
+        load_elements<WAY>(p, pp, i, J.n);
+        if constexpr (BITS == 32) moments32<WAY>(J, i, g, p, W, S, R);
+        else moments8<WAY>(J, i, g, p, W, S, R);
+        store_elements<WAY>(pp, p, i, J.n);
     }
 }
 
-template <int BITS>
+// STREAM: tensors and moments that the last cache does not hold from one step to the next go past it (151 M float32 parameters, 8 bits
+// 430 -> 420 us, 32 bits 764 -> 746); smaller ones stay for who reads them next (25 M bfloat16: the values of the moments 48 -> 36).
+template <int BITS, bool STREAM>
 __global__ __launch_bounds__(256) void adamw_moments_kernel(const ParamJobs T, const Moments W, const AdamWStep* step,
                                                             const AdamWRates R) {
     const ParamJob& J = job_of(T, blockIdx.x);
     const uint32_t base = (blockIdx.x - J.chunk0) * ADAMW_CHUNK;
     auto run = [&](auto t) {
         using E = decltype(t);
-        if (base + ADAMW_CHUNK <= J.n) adamw_chunk<E, BITS, true>(J, base, W, step, R);
-        else adamw_chunk<E, BITS, false>(J, base, W, step, R);
+        if (base + ADAMW_CHUNK <= J.n) adamw_chunk<E, BITS, Way<true, STREAM>>(J, base, W, step, R);
+        else adamw_chunk<E, BITS, Way<false, STREAM>>(J, base, W, step, R);
     };
     if (J.dtype == TYPE_F32) run(float());
     else if (J.dtype == TYPE_BF16) run(bf16());
@@ -306,7 +335,7 @@ __global__ __launch_bounds__(256) void moment_values_kernel(const Moments W, uin
     const uint32_t n = size - e < 4 ? (uint32_t)(size - e) : 4u;
     uint32_t w[1];
     if (n == 4) w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(codes));
-    else load_codes<false, 4>(w, codes, 0, n);
+    else load_codes<Way<false, false>, 4>(w, codes, 0, n);
     const int scale = (first ? 120 - 127 : 97 - 127) + (int)(first ? W.m_scale : W.v_scale)[e / MOMENT_BLOCK];
     const uint32_t field = first ? 127u : 255u, none = first ? 0x7fc00000u : 0x7f800000u, sign = first ? 0x80000000u : 0u;
     float a[4];
@@ -317,7 +346,7 @@ __global__ __launch_bounds__(256) void moment_values_kernel(const Moments W, uin
         a[j] = __int_as_float((int)(bits | (w[0] << (24 - 8 * j) & sign)));
     }
     if (n == 4 && ((uintptr_t)out & 15) == 0) __builtin_nontemporal_store(f4{a[0], a[1], a[2], a[3]}, reinterpret_cast<f4*>(out));
-    else store_elements<false>(out, a, 0, n);
+    else store_elements<Way<false, false>>(out, a, 0, n);
 }
 
 // ------------------------------------------------------------------------------------------------- norm of the gradients
@@ -329,28 +358,13 @@ __device__ __forceinline__ double block_sum(double x) {
     return part[0] + part[1] + part[2] + part[3];
 }
 
-// 16 bytes of a tensor that will not be looked at again soon.
-template <typename T, int E>
-__device__ __forceinline__ void stream_elements(T (&o)[E], const T* from, uint32_t i, uint32_t n) {
-    typedef uint32_t words4 __attribute__((ext_vector_type(4), aligned(4)));
-    typedef uint32_t words2 __attribute__((ext_vector_type(4), aligned(2)));
-    using V = std::conditional_t<sizeof(T) == 4, words4, words2>;
-    if (i + E <= n) {
-        const V x = __builtin_nontemporal_load(reinterpret_cast<const V*>(from + i));
-        __builtin_memcpy(o, &x, sizeof(o));
-    } else load_elements<false>(o, from, i, n);
-}
-
 template <typename T, int CHUNK, bool STREAM>
 __device__ __forceinline__ double square_sum(const ParamJob& J, uint32_t base) {
     constexpr int E = 16 / (int)sizeof(T), TURNS = CHUNK / (256 * E);
     T g[TURNS][E];
 #pragma unroll
-    for (int k = 0; k < TURNS; k++) {
-        const uint32_t i = base + (k * 256 + threadIdx.x) * E;
-        if constexpr (STREAM) stream_elements(g[k], reinterpret_cast<const T*>(J.g), i, J.n);
-        else load_elements<false>(g[k], reinterpret_cast<const T*>(J.g), i, J.n);
-    }
+    for (int k = 0; k < TURNS; k++)
+        load_elements<Way<false, STREAM>>(g[k], reinterpret_cast<const T*>(J.g), base + (k * 256 + threadIdx.x) * E, J.n);
     double s = 0.0;
 #pragma unroll
     for (int k = 0; k < TURNS; k++)

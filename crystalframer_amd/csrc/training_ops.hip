@@ -65,6 +65,13 @@ int64_t norm_chunk(const cfh_param_job* jobs, int32_t njobs) {
     return n < 512LL * cfh::GRAD_NORM_CHUNK ? cfh::GRAD_NORM_FEW : cfh::GRAD_NORM_CHUNK;
 }
 
+// Bytes of the tensors' elements.
+int64_t tensor_bytes(const cfh_param_job* jobs, int32_t njobs) {
+    int64_t bytes = 0;
+    for (int32_t j = 0; j < njobs; j++) bytes += jobs[j].n * (jobs[j].dtype == CFH_FLOAT32 ? 4 : 2);
+    return bytes;
+}
+
 int check_moments(const char* what, const cfh_moments* s) {
     if (!s) return fail(CFH_EINVAL, "%s: state must not be NULL", what);
     if (s->bits != 8 && s->bits != 32) return fail(CFH_EINVAL, "%s: moments in %d bits: 8 or 32", what, (int)s->bits);
@@ -135,11 +142,13 @@ int cfh_adamw_step_moments(const cfh_param_job* jobs, int32_t njobs, const cfh_m
     const cfh::Moments W{state->exp_avg, state->exp_avg_sq, state->exp_avg_scale, state->exp_avg_sq_scale};
     cfh::AdamWStep* const S = reinterpret_cast<cfh::AdamWStep*>(scratch);
     const cfh::AdamWRates R{beta1, beta2, (float)eps};
+    const bool past = 2 * tensor_bytes(jobs, njobs) + state->size * (state->bits / 4) >= 2 * cfh::CACHED_BYTES;
     hipLaunchKernelGGL(cfh::adamw_begin_kernel, dim3(1), dim3(1), 0, st, S, reinterpret_cast<unsigned long long*>(step_dev), lr, beta1, beta2,
                        weight_decay, clip);
     in_tables(jobs, njobs, cfh::ADAMW_CHUNK, [&](const cfh::ParamJobs& T) {
-        if (state->bits == 8) hipLaunchKernelGGL(cfh::adamw_moments_kernel<8>, dim3(T.chunks), dim3(256), 0, st, T, W, S, R);
-        else hipLaunchKernelGGL(cfh::adamw_moments_kernel<32>, dim3(T.chunks), dim3(256), 0, st, T, W, S, R);
+        const auto kernel = state->bits == 8 ? (past ? cfh::adamw_moments_kernel<8, true> : cfh::adamw_moments_kernel<8, false>)
+                                             : (past ? cfh::adamw_moments_kernel<32, true> : cfh::adamw_moments_kernel<32, false>);
+        hipLaunchKernelGGL(kernel, dim3(T.chunks), dim3(256), 0, st, T, W, S, R);
     });
     return finish_launch("adamw_step_moments");
 }
@@ -176,12 +185,11 @@ int cfh_grad_norm(const cfh_param_job* jobs, int32_t njobs, double max_norm, flo
     double* const partial = reinterpret_cast<double*>(workspace);
     int count = 0;
     const int64_t chunk = norm_chunk(jobs, njobs);
-    int64_t bytes = 0;
-    for (int32_t j = 0; j < njobs; j++) bytes += jobs[j].n * (jobs[j].dtype == CFH_FLOAT32 ? 4 : 2);
+    const int64_t bytes = tensor_bytes(jobs, njobs);
     in_tables(jobs, njobs, chunk, [&](const cfh::ParamJobs& T) {
         const int blocks = T.chunks < cfh::GRAD_NORM_BLOCKS ? (int)T.chunks : cfh::GRAD_NORM_BLOCKS;
         const auto kernel = chunk == cfh::GRAD_NORM_FEW ? cfh::grad_norm_kernel<cfh::GRAD_NORM_FEW, false>
-                            : bytes < cfh::GRAD_NORM_CACHED ? cfh::grad_norm_kernel<cfh::GRAD_NORM_CHUNK, false>
+                            : bytes < cfh::CACHED_BYTES ? cfh::grad_norm_kernel<cfh::GRAD_NORM_CHUNK, false>
                                                             : cfh::grad_norm_kernel<cfh::GRAD_NORM_CHUNK, true>;
         hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, st, T, partial + count);
         count += blocks;
