@@ -3,7 +3,7 @@
 //     dx = s_x dh;  da = s_f gate dh;  dgate = sum s_f a dh;  df = N_b's backward of da;  dw = sum gy xhat;  db = sum gy
 //
 // Both passes are bound by HBM: some 20 operations per element and way against 2 to 4 bytes for each of 3 to 7 arrays.  A row
-// is held in the registers of a team of 16, 64, 256 or 1024 lanes, 16 bytes of each array per lane and turn, so that every
+// is held in the registers of a team of lanes, from a quarter of a wavefront to 16 of them, 16 bytes of each array per lane, so that every
 // array is read once and the statistics (mean first, then the squares of what is left) need no second pass over memory.
 // Rows need not be aligned to more than their elements: gfx950 takes 16-byte accesses at any address.
 #pragma once
@@ -24,51 +24,65 @@ struct Vec {
     T e[N];
 };
 
-// Sum over the LANES lanes of a team; every lane gets it.  Teams of more than a wavefront are whole workgroups; two halves of `part`
-// in turn, so that one barrier per sum is enough.
+// Sum over the lanes of a team; every lane gets it.  LANES 16, 32 or 64: a part of a wavefront, in DPP and lane swaps; 0: the whole
+// workgroup, through two halves of `part` in turn, so that one barrier per sum is enough.
 template <int LANES>
 struct TeamSum {
+    static constexpr int MOST = 16;                     // wavefronts of a workgroup
+    static constexpr int WORDS = LANES == 0 ? 4 * MOST : 1;
     float* part;
     int phase = 0;
     __device__ __forceinline__ explicit TeamSum(float* p) : part(p) {}
-    static constexpr int WAVES = LANES > 64 ? LANES / 64 : 1;
-    static constexpr int WORDS = LANES > 64 ? 4 * WAVES : 1;
+    __device__ __forceinline__ static float lanes(float a) {
+        if constexpr (LANES == 16) return row_sum(a);
+        if constexpr (LANES == 32) {
+            float p, q;
+            swap16(row_sum(a), p, q);
+            return p + q;
+        }
+        return wave_sum(a);
+    }
     __device__ __forceinline__ void operator()(float& a, float& b) {
-        if constexpr (LANES == 16) { a = row_sum(a); b = row_sum(b); return; }
-        a = wave_sum(a);
-        b = wave_sum(b);
-        if constexpr (LANES > 64) {
-            float* const p = part + phase * 2 * WAVES;
+        a = lanes(a);
+        b = lanes(b);
+        if constexpr (LANES == 0) {
+            float* const p = part + phase * 2 * MOST;
             phase ^= 1;
-            if ((threadIdx.x & 63) == 0) { p[threadIdx.x >> 6] = a; p[WAVES + (threadIdx.x >> 6)] = b; }
+            const int waves = (int)blockDim.x >> 6;
+            if ((threadIdx.x & 63) == 0) { p[threadIdx.x >> 6] = a; p[MOST + (threadIdx.x >> 6)] = b; }
             __syncthreads();
             a = 0.0f;
             b = 0.0f;
-            for (int k = 0; k < WAVES; k++) { a += p[k]; b += p[WAVES + k]; }
+            for (int k = 0; k < waves; k++) { a += p[k]; b += p[MOST + k]; }
         }
     }
     __device__ __forceinline__ float operator()(float a) {
-        if constexpr (LANES == 16) return row_sum(a);
-        a = wave_sum(a);
-        if constexpr (LANES > 64) {
-            float* const p = part + phase * 2 * WAVES;
+        a = lanes(a);
+        if constexpr (LANES == 0) {
+            float* const p = part + phase * 2 * MOST;
             phase ^= 1;
+            const int waves = (int)blockDim.x >> 6;
             if ((threadIdx.x & 63) == 0) p[threadIdx.x >> 6] = a;
             __syncthreads();
             a = 0.0f;
-            for (int k = 0; k < WAVES; k++) a += p[k];
+            for (int k = 0; k < waves; k++) a += p[k];
         }
         return a;
     }
 };
 
-// A lane's part of a row: VPT pieces of 16 bytes, LANES * 16 bytes apart.
+// A lane's part of a row: VPT pieces of 16 bytes, a team's width apart.
 template <typename T, int LANES, int VPT>
 struct Share {
-    static constexpr int E = Vec<T>::N, N = VPT * E, CAP = LANES * N;
+    static constexpr int E = Vec<T>::N, N = VPT * E, CAP = LANES * N, TEAMS = LANES ? 256 / LANES : 1;
     struct Raw { Vec<T> v[VPT]; };
-    int lane, dim;
-    __device__ __forceinline__ int col(int k) const { return (k * LANES + lane) * E; }
+    int lane, dim, width;
+    __device__ __forceinline__ explicit Share(int dim_) : dim(dim_) {
+        width = LANES ? LANES : (int)blockDim.x;
+        lane = LANES ? (int)threadIdx.x % (LANES ? LANES : 1) : (int)threadIdx.x;
+    }
+    __device__ __forceinline__ static int team() { return LANES ? (int)threadIdx.x / (LANES ? LANES : 1) : 0; }
+    __device__ __forceinline__ int col(int k) const { return (k * width + lane) * E; }
     __device__ __forceinline__ bool live(int i) const { return col(i / E) + i % E < dim; }
     __device__ __forceinline__ void load(Raw& r, const T* row) const {
 #pragma unroll
@@ -84,9 +98,22 @@ struct Share {
     // weights: of the type of the rows or float32; `none` where there are none, 0 behind the last
     __device__ __forceinline__ void weights(float (&o)[N], const void* w, bool f32, float none) const {
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            const int c = col(i / E) + i % E;
-            o[i] = c >= dim ? 0.0f : !w ? none : f32 ? reinterpret_cast<const float*>(w)[c] : to_float(reinterpret_cast<const T*>(w)[c]);
+        for (int k = 0; k < VPT; k++) {
+            const int c = col(k);
+            if (w && c + E <= dim) {
+                if (f32) __builtin_memcpy(o + k * E, reinterpret_cast<const float*>(w) + c, E * sizeof(float));
+                else {
+                    Vec<T> v;
+                    __builtin_memcpy(&v, reinterpret_cast<const T*>(w) + c, 16);
+#pragma unroll
+                    for (int j = 0; j < E; j++) o[k * E + j] = to_float(v.e[j]);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < E; j++)
+                    o[k * E + j] = c + j >= dim ? 0.0f : !w ? none : f32 ? reinterpret_cast<const float*>(w)[c + j]
+                                                                         : to_float(reinterpret_cast<const T*>(w)[c + j]);
+            }
         }
     }
     __device__ __forceinline__ void store(T* row, const float (&o)[N]) const {
@@ -128,13 +155,13 @@ __device__ __forceinline__ void row_stats(const S& sh, const float (&v)[S::N], i
 }
 
 template <typename T, int LANES, int VPT, bool BN>
-__global__ __launch_bounds__(LANES > 256 ? LANES : 256) void residual_norm_forward_kernel(const ResidualNorm A, T* h_out, T* y_out,
+__global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_forward_kernel(const ResidualNorm A, T* h_out, T* y_out,
                                                                                           float* stats) {
     using S = Share<T, LANES, VPT>;
-    constexpr int N = S::N, TEAMS = LANES > 256 ? 1 : 256 / LANES;
+    constexpr int N = S::N, TEAMS = S::TEAMS;
     __shared__ float part[TeamSum<LANES>::WORDS];
     TeamSum<LANES> sum(part);
-    const S sh{(int)threadIdx.x % LANES, A.dim};
+    const S sh(A.dim);
     float w[N], b[N], wf[BN ? N : 1], bf[BN ? N : 1];
     if (y_out) {
         sh.weights(w, A.w, A.w_float, 1.0f);
@@ -144,7 +171,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void residual_norm_forwa
         sh.weights(wf, A.wf, A.w_float, 1.0f);
         sh.weights(bf, A.bf, A.w_float, 0.0f);
     }
-    for (int64_t row = (int64_t)blockIdx.x * TEAMS + threadIdx.x / LANES; row < A.rows; row += (int64_t)gridDim.x * TEAMS) {
+    for (int64_t row = (int64_t)blockIdx.x * TEAMS + S::team(); row < A.rows; row += (int64_t)gridDim.x * TEAMS) {
         typename S::Raw rx, rf, rg;
         sh.load(rx, reinterpret_cast<const T*>(A.x) + row * A.xs);
         if (A.f) sh.load(rf, reinterpret_cast<const T*>(A.f) + row * A.fs);
@@ -184,29 +211,27 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void residual_norm_forwa
 // Sums over rows are kept per lane, for its columns, while a workgroup goes through its strips, then added over its teams and
 // written down per workgroup (or strip, for the gate); a second launch adds these in a fixed order.
 // GATE: 0 none, 1 a row for several rows (its gradient is a column sum), 2 one for each row.
-template <typename T, int LANES, int VPT, bool BN, int GATE>
-__global__ __launch_bounds__(LANES > 256 ? LANES : 256) void residual_norm_backward_kernel(const ResidualNorm A, const NormGrads G) {
+// BIAS: the block's norm has a bias, or the gradient of a bias is wanted.
+template <typename T, int LANES, int VPT, bool BN, int GATE, bool BIAS>
+__global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_backward_kernel(const ResidualNorm A, const NormGrads G) {
     using S = Share<T, LANES, VPT>;
-    constexpr int N = S::N, TEAMS = LANES > 256 ? 1 : 256 / LANES;
+    constexpr int N = S::N, TEAMS = S::TEAMS;
     __shared__ float part[TeamSum<LANES>::WORDS];
     __shared__ float cols[TEAMS > 1 ? TEAMS * S::CAP : 1];
     TeamSum<LANES> sum(part);
-    const int team = (int)threadIdx.x / LANES;
-    const S sh{(int)threadIdx.x % LANES, A.dim};
+    const int team = S::team();
+    const S sh(A.dim);
     const T* const gh = reinterpret_cast<const T*>(G.gh);
     const T* const gy = reinterpret_cast<const T*>(G.gy);
     const float inv = 1.0f / (float)A.dim;
-    float w[N], wf[BN ? N : 1], bf[BN ? N : 1], g[GATE ? N : 1];
-    float dw[N], db[N], dwf[BN ? N : 1], dbf[BN ? N : 1], dg[GATE == 1 ? N : 1];
-    sh.weights(w, A.w, A.w_float, 1.0f);
-    if constexpr (BN) {
-        sh.weights(wf, A.wf, A.w_float, 1.0f);
-        sh.weights(bf, A.bf, A.w_float, 0.0f);
+    float dw[N], db[BIAS ? N : 1], dwf[BN ? N : 1], dbf[BN && BIAS ? N : 1], dg[GATE == 1 ? N : 1];
 #pragma unroll
-        for (int i = 0; i < N; i++) dwf[i] = dbf[i] = 0.0f;
+    for (int i = 0; i < N; i++) {
+        dw[i] = 0.0f;
+        if constexpr (BIAS) db[i] = 0.0f;
+        if constexpr (BN) dwf[i] = 0.0f;
+        if constexpr (BN && BIAS) dbf[i] = 0.0f;
     }
-#pragma unroll
-    for (int i = 0; i < N; i++) dw[i] = db[i] = 0.0f;
 
     // the workgroup's sum of a column each: to float32 `sums`, or (NULL) rounded to `out`
     auto flush = [&](const float (&acc)[N], float* sums, void* out, bool f32) {
@@ -237,57 +262,62 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void residual_norm_backw
     for (int64_t strip = blockIdx.x; strip < G.strips; strip += gridDim.x) {
         const int64_t segment = strip / G.parts, sub = strip - segment * G.parts;
         const int64_t row0 = segment * span + span * sub / G.parts, row1 = segment * span + span * (sub + 1) / G.parts;
+        typename S::Raw rg;
         if constexpr (GATE == 1) {
-            typename S::Raw rg;
             sh.load(rg, reinterpret_cast<const T*>(A.gate) + segment * A.dim);
 #pragma unroll
-            for (int i = 0; i < N; i++) { g[i] = S::at(rg, i); dg[i] = 0.0f; }
+            for (int i = 0; i < N; i++) dg[i] = 0.0f;
         }
         for (int64_t row = row0 + team; row < row1; row += TEAMS) {
-            typename S::Raw rx, rf, rg, rgh, rgy;
+            typename S::Raw rx, rf, rgh, rgy;
             sh.load(rx, reinterpret_cast<const T*>(A.x) + row * A.xs);
             if (A.f) sh.load(rf, reinterpret_cast<const T*>(A.f) + row * A.fs);
             if constexpr (GATE == 2) sh.load(rg, reinterpret_cast<const T*>(A.gate) + row * A.dim);
             if (gh) sh.load(rgh, gh + row * A.dim);
             if (gy) sh.load(rgy, gy + row * A.dim);
             const float4 st = *reinterpret_cast<const float4*>(G.stats + 4 * row);
-            if constexpr (GATE == 2) {
-#pragma unroll
-                for (int i = 0; i < N; i++) g[i] = S::at(rg, i);
-            }
-            float a[BN || GATE ? N : 1], dh[N];
-            if constexpr (BN || GATE) {
-#pragma unroll
-                for (int i = 0; i < N; i++) {
-                    const float f = S::at(rf, i);
-                    a[i] = BN ? (f - st.x) * st.y : f;          // with a norm of the block: before its weight
-                }
-            }
-            auto block_out = [&](int i) { return BN ? fmaf(a[i], wf[i], bf[i]) : a[i]; };
-#pragma unroll
-            for (int i = 0; i < N; i++) dh[i] = gh ? S::at(rgh, i) : 0.0f;
+            // What the rows' own values give is computed again where it is needed a second time, and the weights are read again for every
+            // row, from the caches: kept in registers, they would halve the wavefronts.
+            float wf[BN ? N : 1], bf[BN && BIAS ? N : 1];
+            if constexpr (BN) sh.weights(wf, A.wf, A.w_float, 1.0f);
+            if constexpr (BN && BIAS) sh.weights(bf, A.bf, A.w_float, 0.0f);
+            auto gate = [&](int i) { return GATE ? S::at(rg, i) : 1.0f; };
+            auto ahat = [&](int i) { return (S::at(rf, i) - st.x) * st.y; };
+            auto block_out = [&](int i) {
+                if constexpr (BN && BIAS) return fmaf(ahat(i), wf[i], bf[i]);
+                else if constexpr (BN) return ahat(i) * wf[i];
+                else return S::at(rf, i);
+            };
+            float dh[N];
             if (gy) {
-                float s = 0.0f, t = 0.0f, xhat[N];
+                float w[N], xhat[N], s = 0.0f, t = 0.0f;
+                sh.weights(w, A.w, A.w_float, 1.0f);
 #pragma unroll
                 for (int i = 0; i < N; i++) {
                     float v = A.in_scale * S::at(rx, i);
-                    if constexpr (BN || GATE) v = fmaf(A.sf, GATE ? g[i] * block_out(i) : block_out(i), v);
-                    else if (A.f) v = fmaf(A.sf, S::at(rf, i), v);
+                    if (BN || GATE || A.f) v = fmaf(A.sf, GATE ? gate(i) * block_out(i) : block_out(i), v);
                     xhat[i] = (v - st.z) * st.w;
-                    const float e = S::at(rgy, i), u = e * w[i];
-                    s += u;
-                    t = fmaf(u, xhat[i], t);
+                    const float e = S::at(rgy, i);
                     dw[i] = fmaf(e, xhat[i], dw[i]);
-                    db[i] += e;
+                    if constexpr (BIAS) db[i] += e;
+                    dh[i] = e * w[i];
+                    s += dh[i];
+                    t = fmaf(dh[i], xhat[i], t);
                 }
                 sum(s, t);
                 s = A.norm == 1 ? s * inv : 0.0f;
                 t *= inv;
 #pragma unroll
-                for (int i = 0; i < N; i++) dh[i] = fmaf(st.w, S::at(rgy, i) * w[i] - s - xhat[i] * t, dh[i]);
+                for (int i = 0; i < N; i++) {
+                    const float v = dh[i] - s - xhat[i] * t;
+                    dh[i] = gh ? fmaf(st.w, v, S::at(rgh, i)) : st.w * v;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; i++) dh[i] = gh ? S::at(rgh, i) : 0.0f;
             }
-            float o[N];
             if (G.dx) {
+                float o[N];
 #pragma unroll
                 for (int i = 0; i < N; i++) o[i] = A.sx * dh[i];
                 sh.store(reinterpret_cast<T*>(G.dx) + row * A.dim, o);
@@ -298,28 +328,29 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void residual_norm_backw
             }
             if constexpr (GATE == 2) {
                 if (G.dgate) {
+                    float o[N];
 #pragma unroll
                     for (int i = 0; i < N; i++) o[i] = A.sf * block_out(i) * dh[i];
                     sh.store(reinterpret_cast<T*>(G.dgate) + row * A.dim, o);
                 }
             }
 #pragma unroll
-            for (int i = 0; i < N; i++) dh[i] *= GATE ? A.sf * g[i] : A.sf;
+            for (int i = 0; i < N; i++) dh[i] *= GATE ? A.sf * gate(i) : A.sf;
             if constexpr (BN) {
                 float s = 0.0f, t = 0.0f;
 #pragma unroll
                 for (int i = 0; i < N; i++) {
-                    const float u = dh[i] * wf[i];
+                    const float u = dh[i] * wf[i], v = ahat(i);
                     s += u;
-                    t = fmaf(u, a[i], t);
-                    dwf[i] = fmaf(dh[i], a[i], dwf[i]);
-                    dbf[i] += dh[i];
+                    t = fmaf(u, v, t);
+                    dwf[i] = fmaf(dh[i], v, dwf[i]);
+                    if constexpr (BIAS) dbf[i] += dh[i];
                 }
                 sum(s, t);
                 s = A.block_norm == 1 ? s * inv : 0.0f;
                 t *= inv;
 #pragma unroll
-                for (int i = 0; i < N; i++) dh[i] = st.y * (dh[i] * wf[i] - s - a[i] * t);
+                for (int i = 0; i < N; i++) dh[i] = st.y * (dh[i] * wf[i] - s - ahat(i) * t);
             }
             if (G.df) sh.store(reinterpret_cast<T*>(G.df) + row * A.dim, dh);
         }
@@ -329,9 +360,13 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void residual_norm_backw
     }
     auto column = [&](int k) { return G.column ? G.column + ((int64_t)k * gridDim.x + blockIdx.x) * A.dim : nullptr; };
     if (G.dw) flush(dw, column(0), G.dw, A.w_float);
-    if (G.db) flush(db, column(1), G.db, A.w_float);
+    if constexpr (BIAS) {
+        if (G.db) flush(db, column(1), G.db, A.w_float);
+    }
     if constexpr (BN) {
         if (G.dwf) flush(dwf, column(2), G.dwf, A.w_float);
+    }
+    if constexpr (BN && BIAS) {
         if (G.dbf) flush(dbf, column(3), G.dbf, A.w_float);
     }
 }
@@ -347,8 +382,17 @@ __global__ __launch_bounds__(256) void residual_norm_columns_kernel(const NormGr
     const int64_t count = k < 4 ? blocks : G.parts;
     const float* const src = k < 4 ? G.column + (int64_t)k * blocks * dim : G.gate_column + (int64_t)(k - 4) * G.parts * dim;
     float s = 0.0f;
-    if (c < dim)
-        for (int64_t r = lane; r < count; r += 16) s += src[r * dim + c];
+    if (c < dim) {
+        int64_t r = lane;
+        for (; r + 7 * 16 < count; r += 8 * 16) {          // eight loads under way
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] = src[(r + 16 * k) * dim + c];
+#pragma unroll
+            for (int k = 0; k < 8; k++) s += v[k];
+        }
+        for (; r < count; r += 16) s += src[r * dim + c];
+    }
     part[lane][threadIdx.x & 15] = s;
     __syncthreads();
     if (lane == 0 && c < dim) {
@@ -361,30 +405,28 @@ __global__ __launch_bounds__(256) void residual_norm_columns_kernel(const NormGr
 }
 
 // ------------------------------------------------------------------------------------------------- launches
-// Lanes of a team and pieces of 16 bytes per lane: the smallest that hold a row, up to 64 bytes of each array per lane.  16 lanes
-// for short rows, so that a wavefront is not half idle; a wavefront while its registers hold the row (sums without a barrier).
+// f(lanes of a team, pieces of 16 bytes per lane, threads of a workgroup): see norm_threads.
 template <typename T, typename F>
 void with_share(int64_t dim, F f) {
     constexpr int E = Vec<T>::N;
-    if (dim <= 16 * E) f(std::integral_constant<int, 16>(), std::integral_constant<int, 1>());
-    else if (dim <= 16 * E * 2) f(std::integral_constant<int, 16>(), std::integral_constant<int, 2>());
-    else if (dim <= 64 * E) f(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
-    else if (dim <= 64 * E * 2) f(std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
-    else if (dim <= 256 * E) f(std::integral_constant<int, 256>(), std::integral_constant<int, 1>());
-    else if (dim <= 256 * E * 2) f(std::integral_constant<int, 256>(), std::integral_constant<int, 2>());
-    else if (dim <= 256 * E * 4) f(std::integral_constant<int, 256>(), std::integral_constant<int, 4>());
-    else if (dim <= 1024 * E * 2) f(std::integral_constant<int, 1024>(), std::integral_constant<int, 2>());
-    else if constexpr (1024 * E * 2 < NORM_MAX_DIM) f(std::integral_constant<int, 1024>(), std::integral_constant<int, 4>());
+    const int threads = norm_threads(dim, E);
+    using std::integral_constant;
+    if (dim <= 16 * E) f(integral_constant<int, 16>(), integral_constant<int, 1>(), threads);
+    else if (dim <= 32 * E) f(integral_constant<int, 32>(), integral_constant<int, 1>(), threads);
+    else if (dim <= 64 * E) f(integral_constant<int, 64>(), integral_constant<int, 1>(), threads);
+    else if (dim <= 1024 * E) f(integral_constant<int, 0>(), integral_constant<int, 1>(), threads);
+    else if (dim <= 1024 * E * 2) f(integral_constant<int, 0>(), integral_constant<int, 2>(), threads);
+    else if constexpr (1024 * E * 2 < NORM_MAX_DIM) f(integral_constant<int, 0>(), integral_constant<int, 4>(), threads);
 }
 
 template <typename T>
 void residual_norm_forward(const ResidualNorm& A, T* h, T* y, float* stats, hipStream_t st) {
-    with_share<T>(A.dim, [&](auto lanes, auto vpt) {
-        constexpr int L = decltype(lanes)::value, V = decltype(vpt)::value, TEAMS = L > 256 ? 1 : 256 / L, THREADS = L > 256 ? L : 256;
-        const int64_t blocks = (A.rows + TEAMS - 1) / TEAMS, most = (int64_t)NORM_CUS * 8;
+    with_share<T>(A.dim, [&](auto lanes, auto vpt, int threads) {
+        constexpr int L = decltype(lanes)::value, V = decltype(vpt)::value, TEAMS = L ? 256 / L : 1;
+        const int64_t blocks = (A.rows + TEAMS - 1) / TEAMS, most = (int64_t)NORM_CUS * (2048 / threads);
         const dim3 grid((unsigned)(blocks < most ? blocks : most));
-        if (A.block_norm) hipLaunchKernelGGL((residual_norm_forward_kernel<T, L, V, true>), grid, dim3(THREADS), 0, st, A, h, y, stats);
-        else hipLaunchKernelGGL((residual_norm_forward_kernel<T, L, V, false>), grid, dim3(THREADS), 0, st, A, h, y, stats);
+        if (A.block_norm) hipLaunchKernelGGL((residual_norm_forward_kernel<T, L, V, true>), grid, dim3(threads), 0, st, A, h, y, stats);
+        else hipLaunchKernelGGL((residual_norm_forward_kernel<T, L, V, false>), grid, dim3(threads), 0, st, A, h, y, stats);
     });
 }
 
@@ -397,16 +439,20 @@ void residual_norm_backward(const ResidualNorm& A, NormGrads G, int64_t gate_row
     G.parts = P.parts;
     int blocks = P.blocks;
     if (A.rows > 0) {
-        with_share<T>(A.dim, [&](auto lanes, auto vpt) {
-            constexpr int L = decltype(lanes)::value, V = decltype(vpt)::value, THREADS = L > 256 ? L : 256;
-            auto launch = [&](auto bn, auto gate) {
-                hipLaunchKernelGGL((residual_norm_backward_kernel<T, L, V, decltype(bn)::value, decltype(gate)::value>), dim3((unsigned)blocks),
-                                   dim3(THREADS), 0, st, A, G);
+        with_share<T>(A.dim, [&](auto lanes, auto vpt, int threads) {
+            constexpr int L = decltype(lanes)::value, V = decltype(vpt)::value;
+            auto launch = [&](auto bn, auto gate, auto bias) {
+                hipLaunchKernelGGL((residual_norm_backward_kernel<T, L, V, decltype(bn)::value, decltype(gate)::value, decltype(bias)::value>),
+                                   dim3((unsigned)blocks), dim3(threads), 0, st, A, G);
+            };
+            auto biased = [&](auto bn, auto gate) {
+                if (G.db || G.dbf || A.bf) launch(bn, gate, std::true_type());
+                else launch(bn, gate, std::false_type());
             };
             auto gated = [&](auto bn) {
-                if (gate_rows == 0) launch(bn, std::integral_constant<int, 0>());
-                else if (P.gate_rows_shared) launch(bn, std::integral_constant<int, 1>());
-                else launch(bn, std::integral_constant<int, 2>());
+                if (gate_rows == 0) biased(bn, std::integral_constant<int, 0>());
+                else if (P.gate_rows_shared) biased(bn, std::integral_constant<int, 1>());
+                else biased(bn, std::integral_constant<int, 2>());
             };
             if (A.block_norm) gated(std::true_type());
             else gated(std::false_type());

@@ -28,25 +28,33 @@ struct NormGrads {
 constexpr int NORM_CUS = 256;
 
 struct NormPlan {
-    int lanes, teams, blocks, parts;
+    int teams, blocks, parts;
     int64_t segments, strips;
     bool gate_rows_shared;
     size_t column_floats, gate_floats;
 };
 
-inline int norm_lanes(int64_t dim, int elements) {
-    return dim <= 16 * elements * 2 ? 16 : dim <= 64 * elements * 2 ? 64 : dim <= 256 * elements * 4 ? 256 : 1024;
+// Threads of a workgroup: for rows of up to 64 pieces of 16 bytes 256, in teams of 16, 32 or 64 lanes with a piece each; else one team of as
+// many wavefronts as there are 64 pieces in a row, up to 16, where lanes take two or four.  A piece per lane is what leaves the backward
+// pass, with its column sums, registers for four wavefronts per SIMD.
+inline int norm_threads(int64_t dim, int elements) {
+    const int64_t pieces = (dim + elements - 1) / elements;
+    if (pieces <= 64) return 256;
+    return pieces >= 1024 ? 1024 : (int)((pieces + 63) / 64 * 64);
+}
+inline int norm_teams(int64_t dim, int elements) {
+    const int64_t pieces = (dim + elements - 1) / elements;
+    return pieces <= 16 ? 16 : pieces <= 32 ? 8 : pieces <= 64 ? 4 : 1;
 }
 
 // Strips of rows: as many as there are workgroups at once, but with four rows for each team of a workgroup where there are fewer, and
 // none across two rows of the gate.
 inline NormPlan norm_plan(int64_t rows, int64_t dim, int elements, int64_t gate_rows) {
     NormPlan P{};
-    P.lanes = norm_lanes(dim, elements);
-    P.teams = P.lanes > 256 ? 1 : 256 / P.lanes;
+    P.teams = norm_teams(dim, elements);
     P.gate_rows_shared = gate_rows > 0 && gate_rows < rows;
     P.segments = P.gate_rows_shared ? gate_rows : 1;
-    const int64_t target = P.lanes > 256 ? NORM_CUS : 2 * NORM_CUS, span = rows / P.segments;
+    const int64_t resident = 1024 / norm_threads(dim, elements), target = NORM_CUS * (resident < 1 ? 1 : resident), span = rows / P.segments;
     int64_t strips = rows / (4 * P.teams);
     strips = strips < 1 ? 1 : strips > target ? target : strips;
     int64_t parts = strips / P.segments;
