@@ -71,8 +71,9 @@ struct TeamSum {
     }
 };
 
-// A lane's part of a row: VPT pieces of 16 bytes, a team's width apart.
-template <typename T, int LANES, int VPT>
+// A lane's part of a row: VPT pieces of 16 bytes, a team's width apart.  TAIL: the pieces of a team reach over
+// the row's end; else they are the row, and nothing has to be looked at.
+template <typename T, int LANES, int VPT, bool TAIL>
 struct Share {
     static constexpr int E = Vec<T>::N, N = VPT * E, CAP = LANES * N, TEAMS = LANES ? 256 / LANES : 1;
     struct Raw { Vec<T> v[VPT]; };
@@ -83,36 +84,81 @@ struct Share {
     }
     __device__ __forceinline__ static int team() { return LANES ? (int)threadIdx.x / (LANES ? LANES : 1) : 0; }
     __device__ __forceinline__ int col(int k) const { return (k * width + lane) * E; }
-    __device__ __forceinline__ bool live(int i) const { return col(i / E) + i % E < dim; }
+    __device__ __forceinline__ bool live(int i) const { return !TAIL || col(i / E) + i % E < dim; }
+    // What lies behind the row's end is not read.  TAIL: a piece that reaches over it, or lies behind it, is read from the last 16 bytes of
+    // the row and moved into place by trim(), so that no load waits behind a branch.  (Rows shorter than a piece: element by element.)
     __device__ __forceinline__ void load(Raw& r, const T* row) const {
+        if (!TAIL) {
+#pragma unroll
+            for (int k = 0; k < VPT; k++) __builtin_memcpy(&r.v[k], row + col(k), 16);
+        } else if (dim >= E) {
+#pragma unroll
+            for (int k = 0; k < VPT; k++) __builtin_memcpy(&r.v[k], row + min(col(k), dim - E), 16);
+        } else {
+#pragma unroll
+            for (int k = 0; k < VPT; k++)
+#pragma unroll
+                for (int j = 0; j < E; j++) r.v[k].e[j] = col(k) + j < dim ? row[col(k) + j] : (T)0.0f;
+        }
+    }
+    __device__ __forceinline__ void trim(Raw& r) const {
+        if (!TAIL) return;
 #pragma unroll
         for (int k = 0; k < VPT; k++) {
-            const int c = col(k);
-            if (c + E <= dim) __builtin_memcpy(&r.v[k], row + c, 16);
-            else {
-#pragma unroll
-                for (int j = 0; j < E; j++) r.v[k].e[j] = c + j < dim ? row[c + j] : (T)0.0f;
+            const int over = col(k) + E - dim;
+            if (over > 0 && dim >= E) {
+                uint64_t w[2];
+                __builtin_memcpy(w, &r.v[k], 16);
+                const int bits = over * 8 * (int)sizeof(T);
+                if (bits >= 64) {
+                    w[0] = bits >= 128 ? 0 : w[1] >> (bits - 64);
+                    w[1] = 0;
+                } else {
+                    w[0] = w[0] >> bits | w[1] << (64 - bits);
+                    w[1] >>= bits;
+                }
+                __builtin_memcpy(&r.v[k], w, 16);
             }
         }
     }
     // weights: of the type of the rows or float32; `none` where there are none, 0 behind the last
     __device__ __forceinline__ void weights(float (&o)[N], const void* w, bool f32, float none) const {
+        if (!w || (TAIL && dim < E)) {
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const int c = col(i / E) + i % E;
+                o[i] = !live(i) ? 0.0f : !w ? none : f32 ? reinterpret_cast<const float*>(w)[c] : to_float(reinterpret_cast<const T*>(w)[c]);
+            }
+            return;
+        }
+        if (sizeof(T) < 4 && !f32) {
+            Raw r;
+            load(r, reinterpret_cast<const T*>(w));
+            trim(r);
+#pragma unroll
+            for (int i = 0; i < N; i++) o[i] = at(r, i);
+            return;
+        }
 #pragma unroll
         for (int k = 0; k < VPT; k++) {
-            const int c = col(k);
-            if (w && c + E <= dim) {
-                if (f32) __builtin_memcpy(o + k * E, reinterpret_cast<const float*>(w) + c, E * sizeof(float));
-                else {
-                    Vec<T> v;
-                    __builtin_memcpy(&v, reinterpret_cast<const T*>(w) + c, 16);
+            if (!TAIL) {
+                __builtin_memcpy(o + k * E, reinterpret_cast<const float*>(w) + col(k), E * sizeof(float));
+                continue;
+            }
+            __builtin_memcpy(o + k * E, reinterpret_cast<const float*>(w) + min(col(k), dim - E), E * sizeof(float));
+            const int over = col(k) + E - dim;
+            if (over > 0) {
 #pragma unroll
-                    for (int j = 0; j < E; j++) o[k * E + j] = to_float(v.e[j]);
+                for (int d = E / 2; d > 0; d /= 2)
+#pragma unroll
+                    for (int j = 0; j < E; j++) {
+                        const float v = j + d < E ? o[k * E + (j + d) % E] : 0.0f;
+                        o[k * E + j] = over & d ? v : o[k * E + j];
+                    }
+                if (over >= E) {
+#pragma unroll
+                    for (int j = 0; j < E; j++) o[k * E + j] = 0.0f;
                 }
-            } else {
-#pragma unroll
-                for (int j = 0; j < E; j++)
-                    o[k * E + j] = c + j >= dim ? 0.0f : !w ? none : f32 ? reinterpret_cast<const float*>(w)[c + j]
-                                                                         : to_float(reinterpret_cast<const T*>(w)[c + j]);
             }
         }
     }
@@ -123,8 +169,8 @@ struct Share {
             Vec<T> v;
 #pragma unroll
             for (int j = 0; j < E; j++) v.e[j] = from_float<T>(o[k * E + j]);
-            if (c + E <= dim) __builtin_memcpy(row + c, &v, 16);
-            else {
+            if (!TAIL || c + E <= dim) __builtin_memcpy(row + c, &v, 16);
+            else if (TAIL) {
 #pragma unroll
                 for (int j = 0; j < E; j++)
                     if (c + j < dim) row[c + j] = v.e[j];
@@ -154,10 +200,10 @@ __device__ __forceinline__ void row_stats(const S& sh, const float (&v)[S::N], i
     r = 1.0f / sqrtf(sum(s) * inv + eps);
 }
 
-template <typename T, int LANES, int VPT, bool BN>
+template <typename T, int LANES, int VPT, bool TAIL, bool BN>
 __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_forward_kernel(const ResidualNorm A, T* h_out, T* y_out,
                                                                                           float* stats) {
-    using S = Share<T, LANES, VPT>;
+    using S = Share<T, LANES, VPT, TAIL>;
     constexpr int N = S::N, TEAMS = S::TEAMS;
     __shared__ float part[TeamSum<LANES>::WORDS];
     TeamSum<LANES> sum(part);
@@ -176,6 +222,9 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_forward_kern
         sh.load(rx, reinterpret_cast<const T*>(A.x) + row * A.xs);
         if (A.f) sh.load(rf, reinterpret_cast<const T*>(A.f) + row * A.fs);
         if (A.gate) sh.load(rg, reinterpret_cast<const T*>(A.gate) + row / A.gate_span * A.dim);
+        sh.trim(rx);
+        if (A.f) sh.trim(rf);
+        if (A.gate) sh.trim(rg);
         float h[N], st[4] = {0.0f, 1.0f, 0.0f, 1.0f};
         if (A.f) {
 #pragma unroll
@@ -212,9 +261,9 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_forward_kern
 // written down per workgroup (or strip, for the gate); a second launch adds these in a fixed order.
 // GATE: 0 none, 1 a row for several rows (its gradient is a column sum), 2 one for each row.
 // BIAS: the block's norm has a bias, or the gradient of a bias is wanted.
-template <typename T, int LANES, int VPT, bool BN, int GATE, bool BIAS>
+template <typename T, int LANES, int VPT, bool TAIL, bool BN, int GATE, bool BIAS>
 __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_backward_kernel(const ResidualNorm A, const NormGrads G) {
-    using S = Share<T, LANES, VPT>;
+    using S = Share<T, LANES, VPT, TAIL>;
     constexpr int N = S::N, TEAMS = S::TEAMS;
     __shared__ float part[TeamSum<LANES>::WORDS];
     __shared__ float cols[TEAMS > 1 ? TEAMS * S::CAP : 1];
@@ -265,6 +314,7 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_backward_ker
         typename S::Raw rg;
         if constexpr (GATE == 1) {
             sh.load(rg, reinterpret_cast<const T*>(A.gate) + segment * A.dim);
+            sh.trim(rg);
 #pragma unroll
             for (int i = 0; i < N; i++) dg[i] = 0.0f;
         }
@@ -276,6 +326,11 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_backward_ker
             if (gh) sh.load(rgh, gh + row * A.dim);
             if (gy) sh.load(rgy, gy + row * A.dim);
             const float4 st = *reinterpret_cast<const float4*>(G.stats + 4 * row);
+            sh.trim(rx);
+            if (A.f) sh.trim(rf);
+            if constexpr (GATE == 2) sh.trim(rg);
+            if (gh) sh.trim(rgh);
+            if (gy) sh.trim(rgy);
             // What the rows' own values give is computed again where it is needed a second time, and the weights are read again for every
             // row, from the caches: kept in registers, they would halve the wavefronts.
             float wf[BN ? N : 1], bf[BN && BIAS ? N : 1];
@@ -405,28 +460,34 @@ __global__ __launch_bounds__(256) void residual_norm_columns_kernel(const NormGr
 }
 
 // ------------------------------------------------------------------------------------------------- launches
-// f(lanes of a team, pieces of 16 bytes per lane, threads of a workgroup): see norm_threads.
+// f(lanes of a team, pieces of 16 bytes per lane, whether they reach over a row's end, threads of a workgroup): see norm_threads.
 template <typename T, typename F>
 void with_share(int64_t dim, F f) {
     constexpr int E = Vec<T>::N;
     const int threads = norm_threads(dim, E);
     using std::integral_constant;
-    if (dim <= 16 * E) f(integral_constant<int, 16>(), integral_constant<int, 1>(), threads);
-    else if (dim <= 32 * E) f(integral_constant<int, 32>(), integral_constant<int, 1>(), threads);
-    else if (dim <= 64 * E) f(integral_constant<int, 64>(), integral_constant<int, 1>(), threads);
-    else if (dim <= 1024 * E) f(integral_constant<int, 0>(), integral_constant<int, 1>(), threads);
-    else if (dim <= 1024 * E * 2) f(integral_constant<int, 0>(), integral_constant<int, 2>(), threads);
-    else if constexpr (1024 * E * 2 < NORM_MAX_DIM) f(integral_constant<int, 0>(), integral_constant<int, 4>(), threads);
+    auto share = [&](auto lanes, auto vpt) {
+        const int64_t whole = (int64_t)(decltype(lanes)::value ? decltype(lanes)::value : threads) * decltype(vpt)::value * E;
+        if (dim == whole) f(lanes, vpt, std::false_type(), threads);
+        else f(lanes, vpt, std::true_type(), threads);
+    };
+    if (dim <= 16 * E) share(integral_constant<int, 16>(), integral_constant<int, 1>());
+    else if (dim <= 32 * E) share(integral_constant<int, 32>(), integral_constant<int, 1>());
+    else if (dim <= 64 * E) share(integral_constant<int, 64>(), integral_constant<int, 1>());
+    else if (dim <= 1024 * E) share(integral_constant<int, 0>(), integral_constant<int, 1>());
+    else if (dim <= 1024 * E * 2) share(integral_constant<int, 0>(), integral_constant<int, 2>());
+    else if constexpr (1024 * E * 2 < NORM_MAX_DIM) share(integral_constant<int, 0>(), integral_constant<int, 4>());
 }
 
 template <typename T>
 void residual_norm_forward(const ResidualNorm& A, T* h, T* y, float* stats, hipStream_t st) {
-    with_share<T>(A.dim, [&](auto lanes, auto vpt, int threads) {
+    with_share<T>(A.dim, [&](auto lanes, auto vpt, auto tail, int threads) {
         constexpr int L = decltype(lanes)::value, V = decltype(vpt)::value, TEAMS = L ? 256 / L : 1;
+        constexpr bool TAIL = decltype(tail)::value;
         const int64_t blocks = (A.rows + TEAMS - 1) / TEAMS, most = (int64_t)NORM_CUS * (2048 / threads);
         const dim3 grid((unsigned)(blocks < most ? blocks : most));
-        if (A.block_norm) hipLaunchKernelGGL((residual_norm_forward_kernel<T, L, V, true>), grid, dim3(threads), 0, st, A, h, y, stats);
-        else hipLaunchKernelGGL((residual_norm_forward_kernel<T, L, V, false>), grid, dim3(threads), 0, st, A, h, y, stats);
+        if (A.block_norm) hipLaunchKernelGGL((residual_norm_forward_kernel<T, L, V, TAIL, true>), grid, dim3(threads), 0, st, A, h, y, stats);
+        else hipLaunchKernelGGL((residual_norm_forward_kernel<T, L, V, TAIL, false>), grid, dim3(threads), 0, st, A, h, y, stats);
     });
 }
 
@@ -439,10 +500,11 @@ void residual_norm_backward(const ResidualNorm& A, NormGrads G, int64_t gate_row
     G.parts = P.parts;
     int blocks = P.blocks;
     if (A.rows > 0) {
-        with_share<T>(A.dim, [&](auto lanes, auto vpt, int threads) {
+        with_share<T>(A.dim, [&](auto lanes, auto vpt, auto tail, int threads) {
             constexpr int L = decltype(lanes)::value, V = decltype(vpt)::value;
+            constexpr bool TAIL = decltype(tail)::value;
             auto launch = [&](auto bn, auto gate, auto bias) {
-                hipLaunchKernelGGL((residual_norm_backward_kernel<T, L, V, decltype(bn)::value, decltype(gate)::value, decltype(bias)::value>),
+                hipLaunchKernelGGL((residual_norm_backward_kernel<T, L, V, TAIL, decltype(bn)::value, decltype(gate)::value, decltype(bias)::value>),
                                    dim3((unsigned)blocks), dim3(threads), 0, st, A, G);
             };
             auto biased = [&](auto bn, auto gate) {

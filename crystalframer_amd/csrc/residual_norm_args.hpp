@@ -47,7 +47,7 @@ inline int norm_teams(int64_t dim, int elements) {
     return pieces <= 16 ? 16 : pieces <= 32 ? 8 : pieces <= 64 ? 4 : 1;
 }
 
-// Strips of rows: as many as there are workgroups at once, but with four rows for each team of a workgroup where there are fewer, and
+// Strips of rows: as many as there are workgroups at once, but with two rows for each team of a workgroup where there are fewer, and
 // none across two rows of the gate.
 inline NormPlan norm_plan(int64_t rows, int64_t dim, int elements, int64_t gate_rows) {
     NormPlan P{};
@@ -55,7 +55,7 @@ inline NormPlan norm_plan(int64_t rows, int64_t dim, int elements, int64_t gate_
     P.gate_rows_shared = gate_rows > 0 && gate_rows < rows;
     P.segments = P.gate_rows_shared ? gate_rows : 1;
     const int64_t resident = 1024 / norm_threads(dim, elements), target = NORM_CUS * (resident < 1 ? 1 : resident), span = rows / P.segments;
-    int64_t strips = rows / (4 * P.teams);
+    int64_t strips = rows / (2 * P.teams);
     strips = strips < 1 ? 1 : strips > target ? target : strips;
     int64_t parts = strips / P.segments;
     if (parts < 1) parts = 1;

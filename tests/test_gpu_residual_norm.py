@@ -115,7 +115,7 @@ def _compare(shape, dtype, wtype=None, norm="layer", block_norm=None, gate=None,
 
 
 SIZES = [(1, 1), (3, 2), (5, 3), (1, 17), (2, 63), (7, 64), (65, 65), (13, 127), (300, 128), (33, 129), (4, 255), (70, 256), (9, 511),
-         (17, 513), (6, 1000), (5, 1001), (3, 1024), (3, 2047), (2, 2049), (5, 4096), (2, 4100), (1, 8192), (3, 8200), (2, 12345), (2, 16384)]
+         (17, 513), (6, 1000), (5, 1001), (3, 1024), (3, 2047), (2, 2049), (5, 4096), (2, 4100), (1, 8192), (3, 8200), (2, 12288), (2, 12345), (2, 16384)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
