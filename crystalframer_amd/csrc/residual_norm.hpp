@@ -180,27 +180,33 @@ struct Share {
     __device__ __forceinline__ static float at(const Raw& r, int i) { return to_float(r.v[i / E].e[i % E]); }
 };
 
-// Mean (layer norm; else 0) and one over the deviation of a team's row.
-template <int LANES, typename S>
+// Mean (layer norm; else 0) and one over the deviation of a team's row.  CENTRE: there may be layer norms.
+template <bool CENTRE, int LANES, typename S>
 __device__ __forceinline__ void row_stats(const S& sh, const float (&v)[S::N], int kind, float eps, TeamSum<LANES>& sum, float& mean, float& r) {
     const float inv = 1.0f / (float)sh.dim;
     mean = 0.0f;
     float s = 0.0f;
-    if (kind == 1) {
+    if constexpr (!CENTRE) {
 #pragma unroll
-        for (int i = 0; i < S::N; i++) s += v[i];
-        mean = sum(s) * inv;
-    }
-    s = 0.0f;
+        for (int i = 0; i < S::N; i++) s = fmaf(v[i], v[i], s);          // (behind the row's end it is zero)
+    } else {
+        if (kind == 1) {
 #pragma unroll
-    for (int i = 0; i < S::N; i++) {
-        const float d = sh.live(i) ? v[i] - mean : 0.0f;
-        s = fmaf(d, d, s);
+            for (int i = 0; i < S::N; i++) s += v[i];
+            mean = sum(s) * inv;
+        }
+        s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < S::N; i++) {
+            const float d = sh.live(i) ? v[i] - mean : 0.0f;
+            s = fmaf(d, d, s);
+        }
     }
     r = 1.0f / sqrtf(sum(s) * inv + eps);
 }
 
-template <typename T, int LANES, int VPT, bool TAIL, bool BN>
+// GENERAL: some norm is a layer norm or has a bias; else root-mean-square norms with weights alone.
+template <typename T, int LANES, int VPT, bool TAIL, bool BN, bool GENERAL>
 __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_forward_kernel(const ResidualNorm A, T* h_out, T* y_out,
                                                                                           float* stats) {
     using S = Share<T, LANES, VPT, TAIL>;
@@ -208,15 +214,13 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_forward_kern
     __shared__ float part[TeamSum<LANES>::WORDS];
     TeamSum<LANES> sum(part);
     const S sh(A.dim);
-    float w[N], b[N], wf[BN ? N : 1], bf[BN ? N : 1];
-    if (y_out) {
-        sh.weights(w, A.w, A.w_float, 1.0f);
-        sh.weights(b, A.b, A.w_float, 0.0f);
+    float w[N], b[GENERAL ? N : 1], wf[BN ? N : 1], bf[BN && GENERAL ? N : 1];
+    if (y_out) sh.weights(w, A.w, A.w_float, 1.0f);
+    if constexpr (GENERAL) {
+        if (y_out) sh.weights(b, A.b, A.w_float, 0.0f);
     }
-    if constexpr (BN) {
-        sh.weights(wf, A.wf, A.w_float, 1.0f);
-        sh.weights(bf, A.bf, A.w_float, 0.0f);
-    }
+    if constexpr (BN) sh.weights(wf, A.wf, A.w_float, 1.0f);
+    if constexpr (BN && GENERAL) sh.weights(bf, A.bf, A.w_float, 0.0f);
     for (int64_t row = (int64_t)blockIdx.x * TEAMS + S::team(); row < A.rows; row += (int64_t)gridDim.x * TEAMS) {
         typename S::Raw rx, rf, rg;
         sh.load(rx, reinterpret_cast<const T*>(A.x) + row * A.xs);
@@ -230,9 +234,9 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_forward_kern
 #pragma unroll
             for (int i = 0; i < N; i++) h[i] = S::at(rf, i);
             if constexpr (BN) {
-                row_stats<LANES, S>(sh, h, A.block_norm, A.block_eps, sum, st[0], st[1]);
+                row_stats<GENERAL, LANES, S>(sh, h, A.block_norm, A.block_eps, sum, st[0], st[1]);
 #pragma unroll
-                for (int i = 0; i < N; i++) h[i] = fmaf((h[i] - st[0]) * st[1], wf[i], bf[i]);
+                for (int i = 0; i < N; i++) h[i] = GENERAL ? fmaf((h[i] - st[0]) * st[1], wf[i], bf[i]) : h[i] * st[1] * wf[i];
             }
             if (A.gate) {
 #pragma unroll
@@ -246,10 +250,10 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_forward_kern
         }
         if (h_out) sh.store(h_out + row * A.dim, h);
         if (A.norm) {
-            row_stats<LANES, S>(sh, h, A.norm, A.eps, sum, st[2], st[3]);
+            row_stats<GENERAL, LANES, S>(sh, h, A.norm, A.eps, sum, st[2], st[3]);
             if (y_out) {
 #pragma unroll
-                for (int i = 0; i < N; i++) h[i] = fmaf((h[i] - st[2]) * st[3], w[i], b[i]);
+                for (int i = 0; i < N; i++) h[i] = GENERAL ? fmaf((h[i] - st[2]) * st[3], w[i], b[i]) : h[i] * st[3] * w[i];
                 sh.store(y_out + row * A.dim, h);
             }
         }
@@ -260,8 +264,8 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_forward_kern
 // Sums over rows are kept per lane, for its columns, while a workgroup goes through its strips, then added over its teams and
 // written down per workgroup (or strip, for the gate); a second launch adds these in a fixed order.
 // GATE: 0 none, 1 a row for several rows (its gradient is a column sum), 2 one for each row.
-// BIAS: the block's norm has a bias, or the gradient of a bias is wanted.
-template <typename T, int LANES, int VPT, bool TAIL, bool BN, int GATE, bool BIAS>
+// GENERAL as above, or the gradient of a bias is wanted.
+template <typename T, int LANES, int VPT, bool TAIL, bool BN, int GATE, bool GENERAL>
 __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_backward_kernel(const ResidualNorm A, const NormGrads G) {
     using S = Share<T, LANES, VPT, TAIL>;
     constexpr int N = S::N, TEAMS = S::TEAMS;
@@ -273,13 +277,13 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_backward_ker
     const T* const gh = reinterpret_cast<const T*>(G.gh);
     const T* const gy = reinterpret_cast<const T*>(G.gy);
     const float inv = 1.0f / (float)A.dim;
-    float dw[N], db[BIAS ? N : 1], dwf[BN ? N : 1], dbf[BN && BIAS ? N : 1], dg[GATE == 1 ? N : 1];
+    float dw[N], db[GENERAL ? N : 1], dwf[BN ? N : 1], dbf[BN && GENERAL ? N : 1], dg[GATE == 1 ? N : 1];
 #pragma unroll
     for (int i = 0; i < N; i++) {
         dw[i] = 0.0f;
-        if constexpr (BIAS) db[i] = 0.0f;
+        if constexpr (GENERAL) db[i] = 0.0f;
         if constexpr (BN) dwf[i] = 0.0f;
-        if constexpr (BN && BIAS) dbf[i] = 0.0f;
+        if constexpr (BN && GENERAL) dbf[i] = 0.0f;
     }
 
     // the workgroup's sum of a column each: to float32 `sums`, or (NULL) rounded to `out`
@@ -333,13 +337,14 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_backward_ker
             if (gy) sh.trim(rgy);
             // What the rows' own values give is computed again where it is needed a second time, and the weights are read again for every
             // row, from the caches: kept in registers, they would halve the wavefronts.
-            float wf[BN ? N : 1], bf[BN && BIAS ? N : 1];
+            float wf[BN ? N : 1], bf[BN && GENERAL ? N : 1];
             if constexpr (BN) sh.weights(wf, A.wf, A.w_float, 1.0f);
-            if constexpr (BN && BIAS) sh.weights(bf, A.bf, A.w_float, 0.0f);
+            if constexpr (BN && GENERAL) sh.weights(bf, A.bf, A.w_float, 0.0f);
             auto gate = [&](int i) { return GATE ? S::at(rg, i) : 1.0f; };
-            auto ahat = [&](int i) { return (S::at(rf, i) - st.x) * st.y; };
+            const float off_a = -st.x * st.y, off_h = -st.z * st.w;
+            auto ahat = [&](int i) { return GENERAL ? fmaf(S::at(rf, i), st.y, off_a) : S::at(rf, i) * st.y; };
             auto block_out = [&](int i) {
-                if constexpr (BN && BIAS) return fmaf(ahat(i), wf[i], bf[i]);
+                if constexpr (BN && GENERAL) return fmaf(ahat(i), wf[i], bf[i]);
                 else if constexpr (BN) return ahat(i) * wf[i];
                 else return S::at(rf, i);
             };
@@ -351,20 +356,22 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_backward_ker
                 for (int i = 0; i < N; i++) {
                     float v = A.in_scale * S::at(rx, i);
                     if (BN || GATE || A.f) v = fmaf(A.sf, GATE ? gate(i) * block_out(i) : block_out(i), v);
-                    xhat[i] = (v - st.z) * st.w;
+                    xhat[i] = GENERAL ? fmaf(v, st.w, off_h) : v * st.w;
                     const float e = S::at(rgy, i);
                     dw[i] = fmaf(e, xhat[i], dw[i]);
-                    if constexpr (BIAS) db[i] += e;
+                    if constexpr (GENERAL) db[i] += e;
                     dh[i] = e * w[i];
-                    s += dh[i];
+                    if constexpr (GENERAL) s += dh[i];
                     t = fmaf(dh[i], xhat[i], t);
                 }
-                sum(s, t);
-                s = A.norm == 1 ? s * inv : 0.0f;
+                if constexpr (GENERAL) {
+                    sum(s, t);
+                    s = A.norm == 1 ? s * inv : 0.0f;
+                } else t = sum(t);
                 t *= inv;
 #pragma unroll
                 for (int i = 0; i < N; i++) {
-                    const float v = dh[i] - s - xhat[i] * t;
+                    const float v = fmaf(-xhat[i], t, GENERAL ? dh[i] - s : dh[i]);
                     dh[i] = gh ? fmaf(st.w, v, S::at(rgh, i)) : st.w * v;
                 }
             } else {
@@ -396,16 +403,18 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_backward_ker
 #pragma unroll
                 for (int i = 0; i < N; i++) {
                     const float u = dh[i] * wf[i], v = ahat(i);
-                    s += u;
+                    if constexpr (GENERAL) s += u;
                     t = fmaf(u, v, t);
                     dwf[i] = fmaf(dh[i], v, dwf[i]);
-                    if constexpr (BIAS) dbf[i] += dh[i];
+                    if constexpr (GENERAL) dbf[i] += dh[i];
                 }
-                sum(s, t);
-                s = A.block_norm == 1 ? s * inv : 0.0f;
+                if constexpr (GENERAL) {
+                    sum(s, t);
+                    s = A.block_norm == 1 ? s * inv : 0.0f;
+                } else t = sum(t);
                 t *= inv;
 #pragma unroll
-                for (int i = 0; i < N; i++) dh[i] = st.y * (dh[i] * wf[i] - s - ahat(i) * t);
+                for (int i = 0; i < N; i++) dh[i] = st.y * fmaf(dh[i], wf[i], fmaf(-ahat(i), t, -s));
             }
             if (G.df) sh.store(reinterpret_cast<T*>(G.df) + row * A.dim, dh);
         }
@@ -415,13 +424,13 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_backward_ker
     }
     auto column = [&](int k) { return G.column ? G.column + ((int64_t)k * gridDim.x + blockIdx.x) * A.dim : nullptr; };
     if (G.dw) flush(dw, column(0), G.dw, A.w_float);
-    if constexpr (BIAS) {
+    if constexpr (GENERAL) {
         if (G.db) flush(db, column(1), G.db, A.w_float);
     }
     if constexpr (BN) {
         if (G.dwf) flush(dwf, column(2), G.dwf, A.w_float);
     }
-    if constexpr (BN && BIAS) {
+    if constexpr (BN && GENERAL) {
         if (G.dbf) flush(dbf, column(3), G.dbf, A.w_float);
     }
 }
@@ -486,8 +495,16 @@ void residual_norm_forward(const ResidualNorm& A, T* h, T* y, float* stats, hipS
         constexpr bool TAIL = decltype(tail)::value;
         const int64_t blocks = (A.rows + TEAMS - 1) / TEAMS, most = (int64_t)NORM_CUS * (2048 / threads);
         const dim3 grid((unsigned)(blocks < most ? blocks : most));
-        if (A.block_norm) hipLaunchKernelGGL((residual_norm_forward_kernel<T, L, V, TAIL, true>), grid, dim3(threads), 0, st, A, h, y, stats);
-        else hipLaunchKernelGGL((residual_norm_forward_kernel<T, L, V, TAIL, false>), grid, dim3(threads), 0, st, A, h, y, stats);
+        auto launch = [&](auto bn, auto general) {
+            hipLaunchKernelGGL((residual_norm_forward_kernel<T, L, V, TAIL, decltype(bn)::value, decltype(general)::value>), grid, dim3(threads), 0, st, A,
+                               h, y, stats);
+        };
+        auto kind_of = [&](auto bn) {
+            if (A.norm == 1 || A.block_norm == 1 || A.b || A.bf) launch(bn, std::true_type());
+            else launch(bn, std::false_type());
+        };
+        if (A.block_norm) kind_of(std::true_type());
+        else kind_of(std::false_type());
     });
 }
 
@@ -507,14 +524,15 @@ void residual_norm_backward(const ResidualNorm& A, NormGrads G, int64_t gate_row
                 hipLaunchKernelGGL((residual_norm_backward_kernel<T, L, V, TAIL, decltype(bn)::value, decltype(gate)::value, decltype(bias)::value>),
                                    dim3((unsigned)blocks), dim3(threads), 0, st, A, G);
             };
-            auto biased = [&](auto bn, auto gate) {
-                if (G.db || G.dbf || A.bf) launch(bn, gate, std::true_type());
+            const bool general = A.norm == 1 || A.block_norm == 1 || A.bf || G.db || G.dbf;
+            auto kind_of = [&](auto bn, auto gate) {
+                if (general) launch(bn, gate, std::true_type());
                 else launch(bn, gate, std::false_type());
             };
             auto gated = [&](auto bn) {
-                if (gate_rows == 0) biased(bn, std::integral_constant<int, 0>());
-                else if (P.gate_rows_shared) biased(bn, std::integral_constant<int, 1>());
-                else biased(bn, std::integral_constant<int, 2>());
+                if (gate_rows == 0) kind_of(bn, std::integral_constant<int, 0>());
+                else if (P.gate_rows_shared) kind_of(bn, std::integral_constant<int, 1>());
+                else kind_of(bn, std::integral_constant<int, 2>());
             };
             if (A.block_norm) gated(std::true_type());
             else gated(std::false_type());
