@@ -343,6 +343,8 @@ def load_host():
             raise RuntimeError(f"ABI version {mod.abi} of crystalframer_amd/_host.so != {ABI_VERSION}")
         addr = lambda f: ctypes.cast(f, ctypes.c_void_p).value
         mod.bind(addr(lib.cfh_model_sizes), addr(lib.cfh_model_forward), addr(lib.cfh_model_backward), addr(lib.cfh_last_error))
+        mod.bind_norm(addr(lib.cfh_residual_norm_forward), addr(lib.cfh_residual_norm_backward_workspace_bytes),
+                      addr(lib.cfh_residual_norm_backward))
         _host = mod
     return _host
 

@@ -5,9 +5,13 @@
 // over, 190 us on the gradients' tensors and the bookkeeping of the autograd function and 100 us on the optimizer's job
 // table, per training step of the 4-layer model with its 65 parameters, as long as the GPU takes for a step on 13 crystals.
 //
+// The residual norms (norms.py) are here for the same reason: their launches take 3 to 10 us on the sizes of a crystal batch, and the
+// checks, the argument structure and the autograd function in Python took 140 us per forward and backward pass.
+//
 // The entry points are called through addresses that the Python side hands over: the module does not link the library.
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
@@ -303,6 +307,221 @@ int watchers() {
     return seen;
 }
 
+// ---- residual norms ------------------------------------------------------------------------------------------------------------
+struct NormLibrary {
+    int (*forward)(const cfh_residual_norm*, void*, void*, float*, void*) = nullptr;
+    size_t (*backward_bytes)(const cfh_residual_norm*) = nullptr;
+    int (*backward)(const cfh_residual_norm*, const float*, const void*, const void*, void*, void*, void*, void*, void*, void*, void*, void*,
+                    size_t, void*) = nullptr;
+} g_norm;
+
+constexpr int64_t NORM_MAX_DIM = 16384;
+enum { X, BLOCK, GATE, WEIGHT, BIAS, BLOCK_WEIGHT, BLOCK_BIAS, NORM_TENSORS };
+const char* const NORM_NAMES[NORM_TENSORS] = {"x", "block", "gate", "weight", "bias", "block_weight", "block_bias"};
+using NormTensors = std::array<at::Tensor, NORM_TENSORS>;
+
+struct NormSpec {
+    int norm, block_norm;
+    float eps, block_eps, residual_scale, block_scale;
+    bool keep;
+};
+
+int element_type(at::ScalarType t) {
+    return t == at::kFloat ? CFH_FLOAT32 : t == at::kBFloat16 ? CFH_BFLOAT16 : t == at::kHalf ? CFH_FLOAT16 : -1;
+}
+
+// How many rows the gate has: 1 (a factor per channel), one for as many rows of x after one another, or one for each.
+int64_t gate_rows(const at::Tensor& gate, const at::Tensor& x) {
+    const int64_t D = x.size(-1);
+    if (gate.dim() == 1 && gate.size(0) == D) return 1;
+    if (gate.dim() == x.dim() && gate.dim() > 0 && gate.size(-1) == D) {
+        int64_t k = 0, rows = 1;
+        while (k + 1 < gate.dim() && gate.size(k) == x.size(k)) rows *= gate.size(k++);
+        while (k + 1 < gate.dim() && gate.size(k) == 1) k++;
+        if (k + 1 == gate.dim()) return rows;
+    }
+    TORCH_CHECK_VALUE(false, "gate of shape ", gate.sizes(), " for x of shape ", x.sizes(), ": its last dimension must be that of x, and its "
+                      "leading dimensions none, or those of x up to some dimension and 1 from there on");
+}
+
+void check_norm(const NormTensors& t, const NormSpec& s) {
+    const at::Tensor& x = t[X];
+    for (const auto& u : t)
+        TORCH_CHECK(!u.defined() || u.is_cuda(), "crystalframer_amd operators run on a HIP device only (tensor on ", u.device(),
+                    "); there is no CPU path");
+    TORCH_CHECK_TYPE(element_type(x.scalar_type()) >= 0, "x of ", x.scalar_type(), ": float32, bfloat16 or float16");
+    TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= NORM_MAX_DIM, "x of shape ", x.sizes(), ": 1 to ", NORM_MAX_DIM, " channels");
+    TORCH_CHECK_VALUE(s.eps >= 0.0f && s.block_eps >= 0.0f, "eps and block_eps must not be negative");
+    TORCH_CHECK_VALUE(s.norm || s.keep, "norm None with keep_residual False: nothing is left to return");
+    TORCH_CHECK_VALUE(s.norm || !(t[WEIGHT].defined() || t[BIAS].defined()), "weight and bias belong to a norm");
+    TORCH_CHECK_VALUE(s.block_norm || !(t[BLOCK_WEIGHT].defined() || t[BLOCK_BIAS].defined()), "block_weight and block_bias belong to a block_norm");
+    TORCH_CHECK_VALUE(t[BLOCK].defined() || !(t[GATE].defined() || s.block_norm), "gate and block_norm belong to a block");
+    for (int k : {BLOCK, GATE})
+        TORCH_CHECK_TYPE(!t[k].defined() || t[k].scalar_type() == x.scalar_type(), NORM_NAMES[k], " of ", t[k].scalar_type(), ", x of ",
+                         x.scalar_type(), ": they must have one type");
+    TORCH_CHECK_VALUE(!t[BLOCK].defined() || t[BLOCK].sizes() == x.sizes(), "block of shape ", t[BLOCK].sizes(), ", x of shape ", x.sizes());
+    c10::optional<at::ScalarType> kind;
+    for (int k : {WEIGHT, BIAS, BLOCK_WEIGHT, BLOCK_BIAS}) {
+        if (!t[k].defined()) continue;
+        const at::ScalarType type = t[k].scalar_type();
+        TORCH_CHECK_VALUE(t[k].dim() == 1 && t[k].size(0) == x.size(-1), NORM_NAMES[k], " of shape ", t[k].sizes(), " for ", x.size(-1), " channels");
+        TORCH_CHECK_TYPE((type == x.scalar_type() || type == at::kFloat) && (!kind || *kind == type), NORM_NAMES[k], " of ", type,
+                         ": weights and biases have one type, that of x or float32");
+        kind = type;
+    }
+    for (const auto& u : t) TORCH_CHECK(!u.defined() || u.device() == x.device(), "the tensors are on different devices");
+    if (t[GATE].defined()) gate_rows(t[GATE], x);
+}
+
+// t as rows of its last dimension, `stride` elements apart: in place if they lie evenly and their elements next to each other.
+at::Tensor rows_of(const at::Tensor& t, int64_t& stride) {
+    stride = t.size(-1);
+    if (t.is_contiguous()) return t;
+    if (t.dim() == 2 && t.stride(1) == 1 && t.stride(0) >= t.size(1)) {
+        stride = t.stride(0);
+        return t;
+    }
+    return t.contiguous();
+}
+
+// The library's arguments; `t` becomes the tensors that they point to.
+cfh_residual_norm norm_args(NormTensors& t, const NormSpec& s) {
+    cfh_residual_norm a;
+    std::memset(&a, 0, sizeof(a));
+    a.struct_size = (int32_t)sizeof(a);
+    a.dtype = a.weight_dtype = element_type(t[X].scalar_type());
+    a.norm = s.norm; a.block_norm = s.block_norm;
+    a.eps = s.eps; a.block_eps = s.block_eps; a.residual_scale = s.residual_scale; a.block_scale = s.block_scale;
+    a.dim = t[X].size(-1);
+    a.rows = t[X].numel() / a.dim;
+    if (t[GATE].defined()) a.gate_rows = gate_rows(t[GATE], t[X]);
+    t[X] = rows_of(t[X], a.x_stride);
+    if (t[BLOCK].defined()) t[BLOCK] = rows_of(t[BLOCK], a.block_stride);
+    for (int k = GATE; k < NORM_TENSORS; k++) {
+        if (!t[k].defined()) continue;
+        t[k] = t[k].contiguous();
+        if (k >= WEIGHT) a.weight_dtype = element_type(t[k].scalar_type());
+    }
+    auto p = [&](int k) { return t[k].defined() ? t[k].data_ptr() : nullptr; };
+    a.x = p(X); a.block = p(BLOCK); a.gate = p(GATE); a.weight = p(WEIGHT); a.bias = p(BIAS); a.block_weight = p(BLOCK_WEIGHT);
+    a.block_bias = p(BLOCK_BIAS);
+    return a;
+}
+void* raw_stream(const at::Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+
+struct ResidualNormBackward : public torch::autograd::Node {
+    NormSpec spec;
+    bool joined = false;                       // `saved[X]` is h (the last of the outputs that are kept for this)
+    std::vector<int64_t> shape;
+    std::array<torch::autograd::SavedVariable, NORM_TENSORS> saved;
+    at::Tensor stats;
+    bool released = false;
+
+    std::string name() const override { return "ResidualNormHIPBackward"; }
+    void release_variables() override {
+        released = true;
+        for (auto& s : saved) s.reset_data();
+        stats.reset();
+    }
+    torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+        TORCH_CHECK(!released, "Trying to backward through a residual norm a second time: make the first pass with retain_graph=True");
+        torch::autograd::variable_list out(NORM_TENSORS);
+        at::Tensor gh = spec.keep ? grads[0] : at::Tensor(), gy = spec.norm ? grads[spec.keep ? 1 : 0] : at::Tensor();
+        if (!gh.defined() && !gy.defined()) return out;
+        NormTensors t;
+        for (int k = 0; k < NORM_TENSORS; k++) {
+            t[k] = saved[k].unpack(shared_from_this());
+            if (t[k].defined()) t[k] = t[k].detach();
+        }
+        c10::DeviceGuard guard(t[X].device());
+        const bool differentiable = at::GradMode::is_enabled();
+        {
+            at::AutoDispatchBelowADInplaceOrView below;
+            const auto options = t[X].options();
+            for (int k = GATE; k < NORM_TENSORS; k++)
+                if (t[k].defined() && task_should_compute_output(k)) out[k] = at::empty(t[k].sizes(), t[k].options());
+            cfh_residual_norm a = norm_args(t, spec);
+            a.joined = joined ? 1 : 0;
+            const bool same = !t[GATE].defined() && !spec.block_norm && spec.residual_scale == spec.block_scale;
+            if (task_should_compute_output(X)) out[X] = at::empty(shape, options);
+            if (task_should_compute_output(BLOCK)) out[BLOCK] = same && out[X].defined() ? out[X] : at::empty(shape, options);
+            if (a.rows == 0) {
+                for (int k = GATE; k < NORM_TENSORS; k++)
+                    if (out[k].defined()) out[k].zero_();
+            } else {
+                if (gh.defined()) gh = gh.detach().contiguous();
+                if (gy.defined()) gy = gy.detach().contiguous();
+                // (scratch of its own for every call: two captured passes never share it)
+                const at::Tensor scratch = bytes(g_norm.backward_bytes(&a), t[X].device());
+                auto p = [](const at::Tensor& u) { return u.defined() ? u.data_ptr() : nullptr; };
+                check(g_norm.backward(&a, stats.data_ptr<float>(), p(gh), p(gy), p(out[X]), p(out[BLOCK]), p(out[GATE]), p(out[WEIGHT]), p(out[BIAS]),
+                                      p(out[BLOCK_WEIGHT]), p(out[BLOCK_BIAS]), scratch.data_ptr(), (size_t)scratch.numel(), raw_stream(t[X])),
+                      "cfh_residual_norm_backward");
+            }
+        }
+        if (differentiable) {                  // a gradient of this gradient would be wrong without a word
+            auto error = std::make_shared<torch::autograd::DelayedError>(
+                "the gradients of a residual norm are not differentiable", (int64_t)out.size());
+            torch::autograd::variable_list given = out;
+            for (auto& g : given)
+                if (g.defined()) g = g.detach().requires_grad_(true);
+            given = (*error)(std::move(given));
+            for (size_t k = 0; k < out.size(); k++)
+                if (out[k].defined()) out[k] = given[k];
+        }
+        return out;
+    }
+};
+
+py::object residual_norm(const at::Tensor& x, const c10::optional<at::Tensor>& block, const c10::optional<at::Tensor>& gate,
+                         const c10::optional<at::Tensor>& weight, const c10::optional<at::Tensor>& bias,
+                         const c10::optional<at::Tensor>& block_weight, const c10::optional<at::Tensor>& block_bias, int norm, double eps,
+                         int block_norm, double block_eps, double residual_scale, double block_scale, bool keep) {
+    auto given = [](const c10::optional<at::Tensor>& t) { return t ? *t : at::Tensor(); };
+    const NormTensors inputs = {x, given(block), given(gate), given(weight), given(bias), given(block_weight), given(block_bias)};
+    const NormSpec s{norm, block_norm, (float)eps, (float)block_eps, (float)residual_scale, (float)block_scale, keep};
+    check_norm(inputs, s);
+    TORCH_CHECK(!(watchers() & WATCHED), "a residual norm is one call of the library: it cannot be traced or transformed");
+    bool train = false;
+    if (at::GradMode::is_enabled())
+        for (const auto& t : inputs) train = train || (t.defined() && t.requires_grad());
+    c10::DeviceGuard guard(x.device());
+    NormTensors t = inputs;
+    at::Tensor h, y, stats;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const cfh_residual_norm a = norm_args(t, s);
+        if (keep) h = at::empty(x.sizes(), x.options());
+        if (norm) y = at::empty(x.sizes(), x.options());
+        if (train) stats = at::empty({a.rows, 4}, x.options().dtype(at::kFloat));
+        check(g_norm.forward(&a, keep ? h.data_ptr() : nullptr, norm ? y.data_ptr() : nullptr, train ? stats.data_ptr<float>() : nullptr, raw_stream(x)),
+              "cfh_residual_norm_forward");
+    }
+    if (train) {
+        auto node = std::shared_ptr<ResidualNormBackward>(new ResidualNormBackward(), torch::autograd::deleteNode);
+        node->spec = s;
+        node->shape = x.sizes().vec();
+        node->stats = std::move(stats);
+        torch::autograd::edge_list edges;
+        for (const auto& u : inputs)
+            edges.push_back(u.defined() && u.requires_grad() ? torch::autograd::impl::gradient_edge(u) : torch::autograd::Edge());
+        node->set_next_edges(std::move(edges));
+        if (keep) torch::autograd::set_history(h, node);
+        if (norm) torch::autograd::set_history(y, node);
+        // In float32 h is what the norm saw: where it is there anyway, and nothing else needs the block's output, it is kept instead of x
+        // and block.  16 bits hold it rounded: the backward pass puts it together again.
+        node->joined = keep && x.scalar_type() == at::kFloat && !inputs[GATE].defined() && !block_norm;
+        for (int k = 0; k < NORM_TENSORS; k++) {
+            if (!inputs[k].defined() || (k == BLOCK && node->joined)) continue;
+            if (k == X && node->joined) node->saved[k] = torch::autograd::SavedVariable(h, true);
+            else node->saved[k] = torch::autograd::SavedVariable(inputs[k], false);
+        }
+    }
+    if (!norm) return py::cast(h);
+    if (!keep) return py::cast(y);
+    return py::make_tuple(py::cast(h), py::cast(y));
+}
+
 // Addresses of an optimizer's launch: fills the jobs of the parameters that have a gradient.  Returns how many, or -1 when a
 // gradient is one that the Python side has to look at (not contiguous, sparse, another type) or does not fit the moments:
 // the kernel goes over as many words of parameter, gradient and moments as the parameter had when these were made.
@@ -382,6 +601,13 @@ PYBIND11_MODULE(_host, mod) {
         g_lib.backward = reinterpret_cast<decltype(g_lib.backward)>(backward);
         g_lib.last_error = reinterpret_cast<decltype(g_lib.last_error)>(last_error);
     });
+    mod.def("bind_norm", [](uintptr_t forward, uintptr_t backward_bytes, uintptr_t backward) {
+        g_norm.forward = reinterpret_cast<decltype(g_norm.forward)>(forward);
+        g_norm.backward_bytes = reinterpret_cast<decltype(g_norm.backward_bytes)>(backward_bytes);
+        g_norm.backward = reinterpret_cast<decltype(g_norm.backward)>(backward);
+    });
+    mod.def("residual_norm", &residual_norm);
+    mod.def("gate_rows", &gate_rows);
     mod.attr("abi") = CFH_ABI_VERSION;
     mod.attr("WATCHED") = (int)WATCHED;
     mod.attr("FUNCTION_MODE") = (int)FUNCTION_MODE;

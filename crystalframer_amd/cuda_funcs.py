@@ -16,7 +16,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .norms import ResidualNormHIP, residual_norm  # noqa: F401
+from .norms import residual_norm  # noqa: F401
 
 CUPY_AVAILABLE = True   # name kept from the reference: "the native path is usable"
 
