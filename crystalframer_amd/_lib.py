@@ -107,6 +107,12 @@ class CfhMoments(ctypes.Structure):
                 ("reserved0", ctypes.c_int32)]
 
 
+class CfhGradClip(ctypes.Structure):
+    """Mirror of ``cfh_grad_clip`` in include/crystalframer_hip.h."""
+    _fields_ = [("sums", ctypes.c_void_p), ("count", ctypes.c_int32), ("reserved0", ctypes.c_int32), ("max_norm", ctypes.c_double),
+                ("out", ctypes.c_void_p)]
+
+
 class CfhResidualNorm(ctypes.Structure):
     """Mirror of ``cfh_residual_norm`` in include/crystalframer_hip.h."""
     _fields_ = ([(n, ctypes.c_int32) for n in ("struct_size", "dtype", "weight_dtype", "norm", "block_norm", "joined")]
@@ -163,7 +169,7 @@ EXPORTS = ("cfh_abi_version", "cfh_last_error", "cfh_workspace_bytes", "cfh_fram
            "cfh_fused_core_backward", "cfh_adamw_step_batch",
            "cfh_fused_core_weight_gradients_workspace_bytes", "cfh_fused_core_weight_gradients",
            "cfh_model_sizes", "cfh_model_forward", "cfh_model_backward",
-           "cfh_adamw_step_moments", "cfh_adamw_moments", "cfh_grad_norm_workspace_bytes", "cfh_grad_norm",
+           "cfh_adamw_step_moments", "cfh_adamw_moments", "cfh_grad_square_sums_count", "cfh_grad_square_sums",
            "cfh_residual_norm_forward", "cfh_residual_norm_backward_workspace_bytes", "cfh_residual_norm_backward")
 
 _lib = None
@@ -287,10 +293,10 @@ def load():
         lib.cfh_adamw_step_moments.argtypes = [_P, _I32, _P, _D, _D, _D, _D, _D, _P, _P, _P, _P]
         lib.cfh_adamw_moments.restype = ctypes.c_int
         lib.cfh_adamw_moments.argtypes = [_P] * 4
-        lib.cfh_grad_norm_workspace_bytes.restype = ctypes.c_size_t
-        lib.cfh_grad_norm_workspace_bytes.argtypes = [_P, _I32]
-        lib.cfh_grad_norm.restype = ctypes.c_int
-        lib.cfh_grad_norm.argtypes = [_P, _I32, _D, _P, _P, ctypes.c_size_t, _P]
+        lib.cfh_grad_square_sums_count.restype = _I32
+        lib.cfh_grad_square_sums_count.argtypes = [_P, _I32]
+        lib.cfh_grad_square_sums.restype = ctypes.c_int
+        lib.cfh_grad_square_sums.argtypes = [_P, _I32, _P, _I32, _P]
         lib.cfh_residual_norm_forward.restype = ctypes.c_int
         lib.cfh_residual_norm_forward.argtypes = [_P] * 5
         lib.cfh_residual_norm_backward_workspace_bytes.restype = ctypes.c_size_t

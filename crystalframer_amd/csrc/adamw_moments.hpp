@@ -16,6 +16,7 @@ namespace cfh {
 constexpr int MOMENT_BLOCK = 64;          // elements that share a scale
 constexpr int PARAM_MAX_JOBS = 88;        // tensors per launch (kernel arguments: 4 KB)
 constexpr int ADAMW_CHUNK = 2048;         // elements per workgroup of 256 threads
+constexpr int ADAMW_FEW = 1024;           // the same where there are not enough of those to go round
 constexpr int64_t CACHED_BYTES = 256LL << 20;      // that the last cache holds
 constexpr int GRAD_NORM_CHUNK = 8192;     // elements per turn of a workgroup of 256 threads: eight (four) loads under way per lane
 constexpr int GRAD_NORM_FEW = 2048;       // the same where there are not enough of those to go round
@@ -61,19 +62,49 @@ __device__ __forceinline__ const ParamJob& job_of(const ParamJobs& T, uint32_t c
     return T.job[__popcll(__builtin_amdgcn_ballot_w64(a)) + __popcll(__builtin_amdgcn_ballot_w64(b)) - 1];
 }
 
-__global__ void adamw_begin_kernel(AdamWStep* out, unsigned long long* step, double lr, double beta1, double beta2, double wd,
-                                   const float* clip) {
-    const unsigned long long t = *step + 1ULL;
-    *step = t;
-    // 1 - beta^t by expm1: for beta close to 1 and the first steps the difference cancels
-    const double bc1 = -expm1((double)t * log(beta1)), bc2 = -expm1((double)t * log(beta2));
-    out->step_size = (float)(lr / bc1);
-    out->inv_sqrt_bc2 = (float)(1.0 / sqrt(bc2));
-    out->decay = (float)(1.0 - lr * wd);
-    out->clip = clip ? clip[1] : 1.0f;
-    uint32_t k = (uint32_t)t * 0x6A09E667u;
-    k = (k ^ (k >> 15)) * 0x9E3779B1u;
-    out->key = k ^ (k >> 16);
+__device__ __forceinline__ double block_sum(double x) {
+    __shared__ double part[4];
+    for (int d = 32; d > 0; d /= 2) x += __shfl_xor(x, d);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
+    __syncthreads();
+    return part[0] + part[1] + part[2] + part[3];
+}
+
+struct GradClip {
+    const double* sums;
+    int count;
+    double max_norm;
+    float* out;               // NULL: no clipping
+};
+
+// One workgroup: the norm by all its threads, what depends on the number of the step by one of another wavefront meanwhile.
+__global__ __launch_bounds__(256) void adamw_begin_kernel(AdamWStep* out, unsigned long long* step, double lr, double beta1, double beta2,
+                                                          double wd, const GradClip C) {
+    if (threadIdx.x == 64) {
+        const unsigned long long t = *step + 1ULL;
+        *step = t;
+        // 1 - beta^t by expm1: for beta close to 1 and the first steps the difference cancels
+        const double bc1 = -expm1((double)t * log(beta1)), bc2 = -expm1((double)t * log(beta2));
+        out->step_size = (float)(lr / bc1);
+        out->inv_sqrt_bc2 = (float)(1.0 / sqrt(bc2));
+        out->decay = (float)(1.0 - lr * wd);
+        uint32_t k = (uint32_t)t * 0x6A09E667u;
+        k = (k ^ (k >> 15)) * 0x9E3779B1u;
+        out->key = k ^ (k >> 16);
+    }
+    float factor = 1.0f;
+    if (C.out) {
+        double s = 0.0;
+        for (int i = threadIdx.x; i < C.count; i += 256) s += C.sums[i];
+        s = sqrt(block_sum(s));
+        const double c = C.max_norm / (s + 1e-6);
+        factor = c >= 1.0 ? 1.0f : (float)c;
+        if (threadIdx.x == 0) {
+            C.out[0] = (float)s;
+            C.out[1] = factor;
+        }
+    }
+    if (threadIdx.x == 0) out->clip = factor;
 }
 
 // of element * 0x9E3779B1 + key
@@ -142,6 +173,7 @@ CFH_WORDS(16, 4)
 CFH_WORDS(16, 2)
 CFH_WORDS(32, 4)
 CFH_WORDS(8, 1)
+CFH_WORDS(8, 2)
 #undef CFH_WORDS
 template <> struct Words<4, 1> { typedef uint32_t type __attribute__((aligned(1))); };
 
@@ -289,12 +321,12 @@ __device__ __forceinline__ void moments8(const ParamJob& J, uint32_t i, const T 
     }
 }
 
-template <typename T, int BITS, typename WAY>
+template <typename T, int BITS, int CHUNK, typename WAY>
 __device__ __forceinline__ void adamw_chunk(const ParamJob& J, uint32_t base, const Moments& W, const AdamWStep* step, const AdamWRates& R) {
-    constexpr int E = 16 / (int)sizeof(T);
+    constexpr int E = 16 / (int)sizeof(T) < CHUNK / 256 ? 16 / (int)sizeof(T) : CHUNK / 256;
     T* const pp = reinterpret_cast<T*>(J.p);
     const AdamWStep S = *step;
-    for (int k = 0; k < ADAMW_CHUNK / (256 * E); k++) {
+    for (int k = 0; k < CHUNK / (256 * E); k++) {
         const uint32_t i = base + ((uint32_t)k * 256 + threadIdx.x) * E;
         T g[E], p[E];
         load_elements<WAY>(g, reinterpret_cast<const T*>(J.g), i, J.n);
@@ -307,15 +339,15 @@ __device__ __forceinline__ void adamw_chunk(const ParamJob& J, uint32_t base, co
 
 // STREAM: tensors and moments that the last cache does not hold from one step to the next go past it (151 M float32 parameters, 8 bits
 // 430 -> 420 us, 32 bits 764 -> 746); smaller ones stay for who reads them next (25 M bfloat16: the values of the moments 48 -> 36).
-template <int BITS, bool STREAM>
+template <int BITS, int CHUNK, bool STREAM>
 __global__ __launch_bounds__(256) void adamw_moments_kernel(const ParamJobs T, const Moments W, const AdamWStep* step,
                                                             const AdamWRates R) {
     const ParamJob& J = job_of(T, blockIdx.x);
-    const uint32_t base = (blockIdx.x - J.chunk0) * ADAMW_CHUNK;
+    const uint32_t base = (blockIdx.x - J.chunk0) * CHUNK;
     auto run = [&](auto t) {
         using E = decltype(t);
-        if (base + ADAMW_CHUNK <= J.n) adamw_chunk<E, BITS, Way<true, STREAM>>(J, base, W, step, R);
-        else adamw_chunk<E, BITS, Way<false, STREAM>>(J, base, W, step, R);
+        if (base + CHUNK <= J.n) adamw_chunk<E, BITS, CHUNK, Way<true, STREAM>>(J, base, W, step, R);
+        else adamw_chunk<E, BITS, CHUNK, Way<false, STREAM>>(J, base, W, step, R);
     };
     if (J.dtype == TYPE_F32) run(float());
     else if (J.dtype == TYPE_BF16) run(bf16());
@@ -350,13 +382,6 @@ __global__ __launch_bounds__(256) void moment_values_kernel(const Moments W, uin
 }
 
 // ------------------------------------------------------------------------------------------------- norm of the gradients
-__device__ __forceinline__ double block_sum(double x) {
-    __shared__ double part[4];
-    for (int d = 32; d > 0; d /= 2) x += __shfl_xor(x, d);
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
-    __syncthreads();
-    return part[0] + part[1] + part[2] + part[3];
-}
 
 template <typename T, int CHUNK, bool STREAM>
 __device__ __forceinline__ double square_sum(const ParamJob& J, uint32_t base) {
@@ -379,7 +404,7 @@ __device__ __forceinline__ double square_sum(const ParamJob& J, uint32_t base) {
 // STREAM: gradients that the last cache does not hold until the update reads them again go past it; 134 M float32 gradients, norm and
 // update 511 -> 460 us, 34 M (128 MiB) 120 -> 121, 34 M bfloat16 87 -> 91.
 template <int CHUNK, bool STREAM>
-__global__ __launch_bounds__(256) void grad_norm_kernel(const ParamJobs T, double* partial) {
+__global__ __launch_bounds__(256) void grad_square_kernel(const ParamJobs T, double* partial) {
     double s = 0.0;
     for (uint32_t c = blockIdx.x; c < T.chunks; c += gridDim.x) {
         const ParamJob& J = job_of(T, c);
@@ -389,17 +414,6 @@ __global__ __launch_bounds__(256) void grad_norm_kernel(const ParamJobs T, doubl
     }
     s = block_sum(s);
     if (threadIdx.x == 0) partial[blockIdx.x] = s;
-}
-
-__global__ __launch_bounds__(256) void grad_norm_end_kernel(const double* partial, int count, double max_norm, float* out) {
-    double s = 0.0;
-    for (int i = threadIdx.x; i < count; i += 256) s += partial[i];
-    s = sqrt(block_sum(s));
-    if (threadIdx.x == 0) {
-        const double c = max_norm / (s + 1e-6);
-        out[0] = (float)s;
-        out[1] = c >= 1.0 ? 1.0f : (float)c;
-    }
 }
 
 }  // namespace cfh

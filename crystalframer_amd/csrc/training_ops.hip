@@ -58,11 +58,15 @@ void in_tables(const cfh_param_job* jobs, int32_t njobs, int64_t chunk, F launch
     if (T.njobs > 0) launch(T);
 }
 
-// Elements that a workgroup of the norm takes at a time: the larger count once there are two such turns for each compute unit.
-int64_t norm_chunk(const cfh_param_job* jobs, int32_t njobs) {
+int64_t elements(const cfh_param_job* jobs, int32_t njobs) {
     int64_t n = 0;
     for (int32_t j = 0; j < njobs; j++) n += jobs[j].n;
-    return n < 512LL * cfh::GRAD_NORM_CHUNK ? cfh::GRAD_NORM_FEW : cfh::GRAD_NORM_CHUNK;
+    return n;
+}
+
+// Elements that a workgroup of the norm takes at a time: the larger count once there are two such turns for each compute unit.
+int64_t norm_chunk(const cfh_param_job* jobs, int32_t njobs) {
+    return elements(jobs, njobs) < 512LL * cfh::GRAD_NORM_CHUNK ? cfh::GRAD_NORM_FEW : cfh::GRAD_NORM_CHUNK;
 }
 
 // Bytes of the tensors' elements.
@@ -128,7 +132,7 @@ void with_type(int dtype, F f) {
 extern "C" {
 
 int cfh_adamw_step_moments(const cfh_param_job* jobs, int32_t njobs, const cfh_moments* state, double lr, double beta1, double beta2,
-                           double eps, double weight_decay, const float* clip, uint64_t* step_dev, float* scratch, void* stream) {
+                           double eps, double weight_decay, const cfh_grad_clip* clip, uint64_t* step_dev, float* scratch, void* stream) {
     int rc = check_jobs("adamw", jobs, njobs, true);
     if (rc || (rc = check_moments("adamw", state))) return rc;
     if (!step_dev || !scratch) return fail(CFH_EINVAL, "adamw: step_dev and scratch must not be NULL");
@@ -138,16 +142,24 @@ int cfh_adamw_step_moments(const cfh_param_job* jobs, int32_t njobs, const cfh_m
         if (jobs[j].first < 0 || jobs[j].first % cfh::MOMENT_BLOCK || jobs[j].first > state->size - jobs[j].n)
             return fail(CFH_EINVAL, "adamw: job %d: elements %lld ... of %lld moments (a multiple of %d)", (int)j, (long long)jobs[j].first,
                         (long long)state->size, cfh::MOMENT_BLOCK);
+    if (clip && (!clip->out || clip->count < 0 || (clip->count > 0 && !clip->sums) || !(clip->max_norm >= 0.0)))
+        return fail(CFH_EINVAL, "adamw: clip: max_norm = %g must not be negative, sums and out not NULL", clip->max_norm);
     hipStream_t st = (hipStream_t)stream;
     const cfh::Moments W{state->exp_avg, state->exp_avg_sq, state->exp_avg_scale, state->exp_avg_sq_scale};
     cfh::AdamWStep* const S = reinterpret_cast<cfh::AdamWStep*>(scratch);
     const cfh::AdamWRates R{beta1, beta2, (float)eps};
     const bool past = 2 * tensor_bytes(jobs, njobs) + state->size * (state->bits / 4) >= 2 * cfh::CACHED_BYTES;
-    hipLaunchKernelGGL(cfh::adamw_begin_kernel, dim3(1), dim3(1), 0, st, S, reinterpret_cast<unsigned long long*>(step_dev), lr, beta1, beta2,
-                       weight_decay, clip);
-    in_tables(jobs, njobs, cfh::ADAMW_CHUNK, [&](const cfh::ParamJobs& T) {
-        const auto kernel = state->bits == 8 ? (past ? cfh::adamw_moments_kernel<8, true> : cfh::adamw_moments_kernel<8, false>)
-                                             : (past ? cfh::adamw_moments_kernel<32, true> : cfh::adamw_moments_kernel<32, false>);
+    cfh::GradClip C{};
+    if (clip) C = {clip->sums, clip->count, clip->max_norm, clip->out};
+    hipLaunchKernelGGL(cfh::adamw_begin_kernel, dim3(1), dim3(256), 0, st, S, reinterpret_cast<unsigned long long*>(step_dev), lr, beta1, beta2,
+                       weight_decay, C);
+    const bool few = elements(jobs, njobs) < 512LL * cfh::ADAMW_CHUNK;
+    in_tables(jobs, njobs, few ? cfh::ADAMW_FEW : cfh::ADAMW_CHUNK, [&](const cfh::ParamJobs& T) {
+        using cfh::adamw_moments_kernel;
+        const auto kernel = state->bits == 8 ? (few ? adamw_moments_kernel<8, cfh::ADAMW_FEW, false>
+                                                : past ? adamw_moments_kernel<8, cfh::ADAMW_CHUNK, true> : adamw_moments_kernel<8, cfh::ADAMW_CHUNK, false>)
+                                             : (few ? adamw_moments_kernel<32, cfh::ADAMW_FEW, false>
+                                                : past ? adamw_moments_kernel<32, cfh::ADAMW_CHUNK, true> : adamw_moments_kernel<32, cfh::ADAMW_CHUNK, false>);
         hipLaunchKernelGGL(kernel, dim3(T.chunks), dim3(256), 0, st, T, W, S, R);
     });
     return finish_launch("adamw_step_moments");
@@ -166,36 +178,31 @@ int cfh_adamw_moments(const cfh_moments* state, float* exp_avg, float* exp_avg_s
     return finish_launch("adamw_moments");
 }
 
-size_t cfh_grad_norm_workspace_bytes(const cfh_param_job* jobs, int32_t njobs) {
-    if (check_jobs("grad_norm", jobs, njobs, false)) return 0;
-    size_t n = 1;
+int32_t cfh_grad_square_sums_count(const cfh_param_job* jobs, int32_t njobs) {
+    int rc = check_jobs("grad_square_sums", jobs, njobs, false);
+    if (rc) return rc;
+    int64_t n = 0;
     in_tables(jobs, njobs, norm_chunk(jobs, njobs), [&](const cfh::ParamJobs& T) { n += T.chunks < cfh::GRAD_NORM_BLOCKS ? T.chunks : cfh::GRAD_NORM_BLOCKS; });
-    return n * sizeof(double);
+    if (n > 0x7fffffff) return fail(CFH_EINVAL, "grad_square_sums: too many tensors");
+    return (int32_t)n;
 }
 
-int cfh_grad_norm(const cfh_param_job* jobs, int32_t njobs, double max_norm, float* out, void* workspace, size_t workspace_bytes,
-                  void* stream) {
-    int rc = check_jobs("grad_norm", jobs, njobs, false);
-    if (rc) return rc;
-    if (!out) return fail(CFH_EINVAL, "grad_norm: out must not be NULL");
-    if (!(max_norm >= 0.0)) return fail(CFH_EINVAL, "grad_norm: max_norm = %g must not be negative", max_norm);
-    if (!workspace || ((uintptr_t)workspace & 7) || workspace_bytes < cfh_grad_norm_workspace_bytes(jobs, njobs))
-        return fail(CFH_EWORKSPACE, "grad_norm: workspace of %zu bytes, aligned to 8, is missing", cfh_grad_norm_workspace_bytes(jobs, njobs));
+int cfh_grad_square_sums(const cfh_param_job* jobs, int32_t njobs, double* sums, int32_t count, void* stream) {
+    const int32_t need = cfh_grad_square_sums_count(jobs, njobs);
+    if (need < 0) return need;
+    if (count != need || (need > 0 && !sums) || ((uintptr_t)sums & 7))
+        return fail(CFH_EINVAL, "grad_square_sums: %d sums, aligned to 8 bytes, have to be there", (int)need);
     hipStream_t st = (hipStream_t)stream;
-    double* const partial = reinterpret_cast<double*>(workspace);
-    int count = 0;
-    const int64_t chunk = norm_chunk(jobs, njobs);
-    const int64_t bytes = tensor_bytes(jobs, njobs);
+    const int64_t chunk = norm_chunk(jobs, njobs), bytes = tensor_bytes(jobs, njobs);
     in_tables(jobs, njobs, chunk, [&](const cfh::ParamJobs& T) {
         const int blocks = T.chunks < cfh::GRAD_NORM_BLOCKS ? (int)T.chunks : cfh::GRAD_NORM_BLOCKS;
-        const auto kernel = chunk == cfh::GRAD_NORM_FEW ? cfh::grad_norm_kernel<cfh::GRAD_NORM_FEW, false>
-                            : bytes < cfh::CACHED_BYTES ? cfh::grad_norm_kernel<cfh::GRAD_NORM_CHUNK, false>
-                                                            : cfh::grad_norm_kernel<cfh::GRAD_NORM_CHUNK, true>;
-        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, st, T, partial + count);
-        count += blocks;
+        const auto kernel = chunk == cfh::GRAD_NORM_FEW ? cfh::grad_square_kernel<cfh::GRAD_NORM_FEW, false>
+                            : bytes < cfh::CACHED_BYTES ? cfh::grad_square_kernel<cfh::GRAD_NORM_CHUNK, false>
+                                                        : cfh::grad_square_kernel<cfh::GRAD_NORM_CHUNK, true>;
+        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, st, T, sums);
+        sums += blocks;
     });
-    hipLaunchKernelGGL(cfh::grad_norm_end_kernel, dim3(1), dim3(256), 0, st, partial, count, max_norm, out);
-    return finish_launch("grad_norm");
+    return finish_launch("grad_square_sums");
 }
 
 int cfh_residual_norm_forward(const cfh_residual_norm* a, void* h, void* y, float* stats, void* stream) {

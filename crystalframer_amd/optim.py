@@ -137,7 +137,7 @@ class AdamW(torch.optim.Optimizer):
             m, v = st["exp_avg"], st["exp_avg_sq"]
             if st["bits"] == 8:
                 dev, state = m.device, self._moments_struct(st)
-                m, v = torch.empty((2, m.numel()), dtype=torch.float32, device=dev)
+                m, v = (torch.empty(m.numel(), dtype=torch.float32, device=dev) for _ in range(2))
                 with torch.cuda.device(dev):
                     rc = lib.cfh_adamw_moments(ctypes.byref(state), m.data_ptr(), v.data_ptr(), _lib.raw_stream(dev))
                 _lib.check(rc, "cfh_adamw_moments")
@@ -210,12 +210,12 @@ class AdamW(torch.optim.Optimizer):
             with torch.cuda.device(dev):
                 rc = lib.cfh_adamw_step_moments(
                     jobs, n, ctypes.byref(state), float(group["lr"]), float(b1), float(b2), float(group["eps"]),
-                    float(group["weight_decay"]), None if clip is None else clip.data_ptr(), st["step"].data_ptr(),
+                    float(group["weight_decay"]), None if clip is None else ctypes.byref(clip), st["step"].data_ptr(),
                     st["scratch"].data_ptr(), _lib.raw_stream(dev))
             _lib.check(rc, "cfh_adamw_step_moments")
 
     def _clip(self, lib, filled):
-        """(norm, factor) of the gradients of all groups, on the device."""
+        """The sums of squares of the gradients of all groups are on their way: what the steps need of them."""
         dev = filled[0][2]["device"]
         if any(plan["device"] != dev for _, _, plan, *_ in filled):
             raise RuntimeError("max_grad_norm needs the parameters of all groups on one device")
@@ -226,15 +226,19 @@ class AdamW(torch.optim.Optimizer):
             for *_, part, n, _ in filled:
                 ctypes.memmove(ctypes.addressof(jobs) + at * ctypes.sizeof(_lib.CfhParamJob), part, n * ctypes.sizeof(_lib.CfhParamJob))
                 at += n
-        out = torch.empty(2, dtype=torch.float32, device=dev)
-        # (scratch of its own for every step: two captured steps never share it)
-        scratch = torch.empty(lib.cfh_grad_norm_workspace_bytes(jobs, total), dtype=torch.uint8, device=dev)
+        clip = _lib.CfhGradClip()
+        clip.count = lib.cfh_grad_square_sums_count(jobs, total)
+        if clip.count < 0:
+            _lib.check(clip.count, "cfh_grad_square_sums_count")
+        # the norm (a double's place: the factor comes behind it), then the sums; memory of its own for every step, so that two captured
+        # steps never share it
+        memory = torch.empty(clip.count + 1, dtype=torch.float64, device=dev)
+        clip.out, clip.sums, clip.max_norm = memory.data_ptr(), memory.data_ptr() + 8, float(self.max_grad_norm)
         with torch.cuda.device(dev):
-            rc = lib.cfh_grad_norm(jobs, total, float(self.max_grad_norm), out.data_ptr(), scratch.data_ptr(), scratch.numel(),
-                                   _lib.raw_stream(dev))
-        _lib.check(rc, "cfh_grad_norm")
-        self.grad_norm = out[0]
-        return out
+            rc = lib.cfh_grad_square_sums(jobs, total, clip.sums, clip.count, _lib.raw_stream(dev))
+        _lib.check(rc, "cfh_grad_square_sums")
+        self.grad_norm = memory.view(torch.float32)[0]
+        return clip
 
     @staticmethod
     def _fill_moments(plan, jobs):

@@ -517,7 +517,8 @@ enum { CFH_FLOAT32 = 0, CFH_BFLOAT16 = 1, CFH_FLOAT16 = 2 };
 /*
  * One AdamW step for tensors of several types, with moments in 32 or in 8 bits and gradients that may be clipped by
  * their common norm: the rule of cfh_adamw_step_batch with c g in the place of g,
- *     c = min(1, max_norm / (|g| + 1e-6)),  |g| the norm over all tensors (cfh_grad_norm; c = 1 without it).
+ *     c = min(1, max_norm / (|g| + 1e-6)),  |g| the norm over the tensors that `clip` speaks of (NULL: c = 1); a norm that is no
+ * number makes every update one that is none.
  * A tensor is contiguous with n elements of `dtype`, its gradient likewise; its moments are the elements
  * first ... first + n - 1 of the flat moments of `state`; first is a multiple of 64.  The arithmetic is in 32 bits (the
  * parameter is rounded to its type at the end), that of 8-bit moments in 64, every product and sum by itself, until they are
@@ -533,10 +534,10 @@ enum { CFH_FLOAT32 = 0, CFH_BFLOAT16 = 1, CFH_FLOAT16 = 2 };
  *               e the element (modulo 2^32) and key = t * 0x6A09E667; key ^= key >> 15; key *= 0x9E3779B1;
  *               key ^= key >> 16, t the number of the step.
  * `step_dev` counts as in cfh_adamw_step_batch; `scratch` (16 floats, device) belongs to the call until it has run on the
- * stream.  `clip` (NULL: no clipping) points to the two floats that cfh_grad_norm left on the device.
+ * stream.
  */
 typedef struct cfh_param_job {
-    void* param;             /* not read by cfh_grad_norm                                         */
+    void* param;             /* not read by cfh_grad_square_sums                                  */
     const void* grad;
     int64_t n;
     int64_t first;
@@ -552,20 +553,26 @@ typedef struct cfh_moments {
     int32_t bits;            /* 8 or 32                                                           */
     int32_t reserved0;
 } cfh_moments;
+typedef struct cfh_grad_clip {
+    const double* sums;      /* device: what cfh_grad_square_sums left, for one group of tensors or for several */
+    int32_t count;
+    int32_t reserved0;
+    double max_norm;
+    float* out;              /* device: |g| and c are written here                                */
+} cfh_grad_clip;
 int cfh_adamw_step_moments(const cfh_param_job* jobs, int32_t njobs, const cfh_moments* state, double lr, double beta1,
-                           double beta2, double eps, double weight_decay, const float* clip, uint64_t* step_dev,
+                           double beta2, double eps, double weight_decay, const cfh_grad_clip* clip, uint64_t* step_dev,
                            float* scratch, void* stream);
 
 /* The float32 values that 8-bit moments stand for: exp_avg, exp_avg_sq (state->size elements each). */
 int cfh_adamw_moments(const cfh_moments* state, float* exp_avg, float* exp_avg_sq, void* stream);
 
 /*
- * out[0] = |g| over the gradients of all jobs (summed in 64 bits, in a fixed order), out[1] = the factor
- * min(1, max_norm / (|g| + 1e-6)); a norm that is no number gives a factor that is none.
+ * Sums of squares of the gradients of all jobs, in 64 bits and a fixed order: as many doubles as cfh_grad_square_sums_count says (a
+ * negative CFH_E* code where the jobs are refused), whose sum is |g|^2.
  */
-size_t cfh_grad_norm_workspace_bytes(const cfh_param_job* jobs, int32_t njobs);
-int cfh_grad_norm(const cfh_param_job* jobs, int32_t njobs, double max_norm, float* out, void* workspace,
-                  size_t workspace_bytes, void* stream);
+int32_t cfh_grad_square_sums_count(const cfh_param_job* jobs, int32_t njobs);
+int cfh_grad_square_sums(const cfh_param_job* jobs, int32_t njobs, double* sums, int32_t count, void* stream);
 
 /*
  * Residual stream and block output joined and normed, forward and backward, for the norms before and after the blocks of

@@ -83,15 +83,21 @@ def test_adamw_arguments(job, state, rates, word):
     assert rc < 0 and word in lib.cfh_last_error()
 
 
-def test_grad_norm_and_moments_arguments():
+def test_sums_of_squares_clipping_and_values_of_moments():
     lib = _lib.load()
     jobs = _job()
-    need = lib.cfh_grad_norm_workspace_bytes(jobs, 1)
-    assert need >= 8
-    for args in ((None, 1, 1.0, A, A, need), (jobs, -1, 1.0, A, A, need), (jobs, 1, -1.0, A, A, need), (jobs, 1, float("nan"), A, A, need),
-                 (jobs, 1, 1.0, None, A, need), (jobs, 1, 1.0, A, None, need), (jobs, 1, 1.0, A, A, need - 1), (jobs, 1, 1.0, A, A + 4, need)):
-        assert lib.cfh_grad_norm(*args, None) < 0
-    assert lib.cfh_grad_norm_workspace_bytes(_job(dtype=7), 1) == 0
+    need = lib.cfh_grad_square_sums_count(jobs, 1)
+    assert need == 1 and lib.cfh_grad_square_sums_count(_job(n=0), 1) == 0 and lib.cfh_grad_square_sums_count(None, 0) == 0
+    for args in ((None, 1, A, need), (jobs, -1, A, need), (jobs, 1, None, need), (jobs, 1, A, need - 1), (jobs, 1, A, need + 1), (jobs, 1, A + 4, need)):
+        assert lib.cfh_grad_square_sums(*args, None) < 0
+    assert lib.cfh_grad_square_sums_count(_job(dtype=7), 1) < 0
+    for change in (dict(out=None), dict(sums=None), dict(count=-1), dict(max_norm=-1.0), dict(max_norm=float("nan"))):
+        clip = _lib.CfhGradClip()
+        clip.sums, clip.count, clip.max_norm, clip.out = A, 1, 1.0, A
+        for k, v in change.items():
+            setattr(clip, k, v)
+        rc = lib.cfh_adamw_step_moments(jobs, 1, ctypes.byref(_state()), 1e-3, 0.9, 0.99, 1e-8, 0.0, ctypes.byref(clip), A, A, None)
+        assert rc < 0 and b"clip" in lib.cfh_last_error()
     for state, m in ((_state(bits=32), A), (_state(exp_avg=None), A), (_state(), None)):
         assert lib.cfh_adamw_moments(ctypes.byref(state), m, A, None) < 0
     assert lib.cfh_adamw_moments(None, A, A, None) < 0
@@ -99,6 +105,7 @@ def test_grad_norm_and_moments_arguments():
 
 def test_structures_match_the_header():
     assert ctypes.sizeof(_lib.CfhResidualNorm) == 136 and ctypes.sizeof(_lib.CfhParamJob) == 40 and ctypes.sizeof(_lib.CfhMoments) == 48
+    assert ctypes.sizeof(_lib.CfhGradClip) == 32
 
 
 def test_python_refuses_host_tensors_and_wrong_options():
