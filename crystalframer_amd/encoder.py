@@ -15,7 +15,7 @@ import torch.nn.functional as F
 from torch import Tensor, nn
 from torch.nn.init import constant_, xavier_uniform_
 
-from . import cuda_funcs, geometry
+from . import _lib, cuda_funcs, geometry, norms
 from .attention import CrystalformerMultiheadAttentionCUDA
 from .params import LatticeformerParams
 
@@ -23,6 +23,41 @@ from .params import LatticeformerParams
 # Between the attention cores of consecutive layers everything acts on single atoms: one launch per layer
 # (cuda_funcs.LayerBridgeHIP) when the layers have no layer norm, no active dropout and the ReLU activation.
 FUSED_LAYER_BRIDGE = True
+# Layers with layer norms: the residual addition and the norm behind it in one launch each way (cuda_funcs.residual_norm), to the
+# same values as the modules up to the rounding of float32 sums.  False: torch.nn.LayerNorm and the addition by themselves.
+FUSED_RESIDUAL_NORM = True
+
+
+def _norm_is_plain(norm: nn.Module, x: Tensor) -> bool:
+    """Nobody but the library has to see this norm: a layer norm over the channels of ``x`` as torch makes it, without hooks, a
+    forward of its own, autocast, tracing or modes."""
+    if not (FUSED_RESIDUAL_NORM and type(norm) is nn.LayerNorm and x.is_cuda and x.dtype in _lib.ELEMENT_TYPES
+            and norm.normalized_shape == (x.shape[-1],) and x.shape[-1] <= norms.MAX_DIM):
+        return False
+    own = norm.__dict__
+    if (norm._forward_hooks or norm._forward_pre_hooks or norm._backward_hooks or norm._backward_pre_hooks or "forward" in own
+            or own.get("_compiled_call_impl") is not None or torch.nn.modules.module._has_any_global_hook()):
+        return False
+    if any(t is not None and (t.dtype not in (x.dtype, torch.float32) or t.device != x.device) for t in (norm.weight, norm.bias)):
+        return False
+    host = _lib.load_host()
+    return not (host.watchers() & (host.WATCHED | host.FUNCTION_MODE) or torch.is_autocast_enabled("cuda")
+                or torch.autograd.forward_ad._current_level >= 0)
+
+
+def _normed(norm: nn.Module, x: Tensor) -> Tensor:
+    """``norm(x)``."""
+    if _norm_is_plain(norm, x):
+        return norms.residual_norm(x, None, norm.weight, norm.bias, eps=norm.eps, keep_residual=False)
+    return norm(x)
+
+
+def _normed_sum(norm: nn.Module, x: Tensor, block: Tensor, keep_sum: bool = False):
+    """``norm(x + block)``; with ``keep_sum`` (x + block, norm(x + block))."""
+    if block.dtype == x.dtype and block.shape == x.shape and block.is_cuda and _norm_is_plain(norm, x):
+        return norms.residual_norm(x, block, norm.weight, norm.bias, eps=norm.eps, keep_residual=keep_sum)
+    x = x + block
+    return (x, norm(x)) if keep_sum else norm(x)
 
 
 def _activation(name):
@@ -86,13 +121,13 @@ class CrystalformerEncoderLayerCUDA(nn.Module):
                 this_epoch: int = None) -> Tensor:
         x = src
         if self.norm_first:
-            x = x + self._sa_block(self.norm1(x), batch, edges, pos_ij, dist2_min, trans, kr_base, rvecs,
-                                   vcell, onehot, this_epoch)
-            x = x + self._ff_block(self.norm2(x))
+            x, normed = _normed_sum(self.norm2, x, self._sa_block(_normed(self.norm1, x), batch, edges, pos_ij, dist2_min, trans,
+                                                                  kr_base, rvecs, vcell, onehot, this_epoch), keep_sum=True)
+            x = x + self._ff_block(normed)
         else:
-            x = self.norm1(x + self._sa_block(x, batch, edges, pos_ij, dist2_min, trans, kr_base, rvecs,
-                                              vcell, onehot, this_epoch))
-            x = self.norm2(x + self._ff_block(x))
+            x = _normed_sum(self.norm1, x, self._sa_block(x, batch, edges, pos_ij, dist2_min, trans, kr_base, rvecs,
+                                                          vcell, onehot, this_epoch))
+            x = _normed_sum(self.norm2, x, self._ff_block(x))
         return x
 
 
@@ -186,5 +221,5 @@ class CrystalformerEncoderCUDA(nn.Module):
                 # rvecs: the lengths of the reciprocal vectors are all the layers use, computed once here
                 x = layer(x, batch, geo.edges, geo.rpos, None, trans, None, geo.rvlen, geo.vcell, onehot, this_epoch)
         if self.norm is not None:
-            x = self.norm(x)
+            x = _normed(self.norm, x)
         return x

@@ -14,6 +14,7 @@ import torch
 
 from . import _lib
 
+MAX_DIM = 16384        # channels (the native checks hold the same number)
 _native = None
 
 
@@ -35,6 +36,8 @@ def residual_norm(x: torch.Tensor, block: Optional[torch.Tensor] = None, weight:
     global _native
     if _native is None:
         _native = _lib.load_host().residual_norm
+    if torch.autograd.forward_ad._current_level >= 0:
+        raise RuntimeError("a residual norm has no forward-mode derivative")
     kinds = _lib.NORM_KINDS
     if norm not in kinds or block_norm not in kinds:
         raise ValueError(f"norm {norm!r}, block_norm {block_norm!r}: \"layer\", \"rms\" or None")
