@@ -18,6 +18,7 @@
 #include <torch/csrc/utils/pybind.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <ATen/ATen.h>
 #include <ATen/PythonTorchFunctionTLS.h>
@@ -409,6 +410,20 @@ cfh_residual_norm norm_args(NormTensors& t, const NormSpec& s) {
 }
 void* raw_stream(const at::Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
+// A gradient of a leaf that an eager graph still holds is accumulated on that graph's stream, which a backward pass under capture must
+// not wait for: that ends the process, so it is refused here, before anything is recorded.
+void check_capture(const NormTensors& t) {
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    const c10::Stream now = c10::hip::getCurrentHIPStream(t[X].device().index()).unwrap();
+    for (const auto& u : t) {
+        if (!u.defined() || !u.requires_grad() || !u.is_leaf()) continue;
+        const auto node = torch::autograd::impl::try_get_grad_accumulator(u);
+        const auto stream = node ? node->stream() : c10::nullopt;
+        TORCH_CHECK(!stream || *stream == now, "a residual norm is captured while a graph that was made on another stream still holds one of "
+                    "its parameters or inputs: let go of that graph's outputs (a loss, a prediction) first");
+    }
+}
+
 struct ResidualNormBackward : public torch::autograd::Node {
     NormSpec spec;
     bool joined = false;                       // `saved[X]` is h (the last of the outputs that are kept for this)
@@ -486,6 +501,7 @@ py::object residual_norm(const at::Tensor& x, const c10::optional<at::Tensor>& b
     if (at::GradMode::is_enabled())
         for (const auto& t : inputs) train = train || (t.defined() && t.requires_grad());
     c10::DeviceGuard guard(x.device());
+    if (train) check_capture(inputs);
     NormTensors t = inputs;
     at::Tensor h, y, stats;
     {

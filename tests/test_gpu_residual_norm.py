@@ -289,6 +289,27 @@ def test_equal_runs_give_equal_bits_and_graphs_replay_them():
             assert all(torch.equal(a, b) for a, b in zip(held, want)), k
 
 
+def test_capture_beside_an_eager_graph_of_the_same_leaves_is_refused():
+    from crystalframer_amd import cuda_funcs
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    x = torch.randn(7, 64, device="cuda")
+    loss = cuda_funcs.residual_norm(x, None, w, keep_residual=False).sum()           # kept
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="let go"):
+        with torch.cuda.graph(graph):
+            cuda_funcs.residual_norm(x, None, w, keep_residual=False)
+    del loss
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cuda_funcs.residual_norm(x, None, w, keep_residual=False).sum().backward()
+    for k in range(3):
+        w.grad.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = cuda_funcs.residual_norm(x, None, torch.ones(64, device="cuda"), keep_residual=False).sum(0)
+        assert (w.grad - want).abs().max() <= 64 * 2.0 ** -24 * 7 * 3, k
+
+
 def test_offsets_beyond_32_bits():
     from crystalframer_amd import cuda_funcs
     rows, dim = (1 << 31) // 16384 + 5, 16384
