@@ -110,7 +110,7 @@ class CfhMoments(ctypes.Structure):
 class CfhGradClip(ctypes.Structure):
     """Mirror of ``cfh_grad_clip`` in include/crystalframer_hip.h."""
     _fields_ = [("sums", ctypes.c_void_p), ("count", ctypes.c_int32), ("reserved0", ctypes.c_int32), ("max_norm", ctypes.c_double),
-                ("out", ctypes.c_void_p)]
+                ("norm", ctypes.c_void_p)]
 
 
 class CfhResidualNorm(ctypes.Structure):

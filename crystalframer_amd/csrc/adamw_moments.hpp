@@ -74,7 +74,7 @@ struct GradClip {
     const double* sums;
     int count;
     double max_norm;
-    float* out;               // NULL: no clipping
+    float* norm;              // NULL: no clipping
 };
 
 // One workgroup: the norm by all its threads, what depends on the number of the step by one of another wavefront meanwhile.
@@ -93,16 +93,13 @@ __global__ __launch_bounds__(256) void adamw_begin_kernel(AdamWStep* out, unsign
         out->key = k ^ (k >> 16);
     }
     float factor = 1.0f;
-    if (C.out) {
+    if (C.norm) {
         double s = 0.0;
         for (int i = threadIdx.x; i < C.count; i += 256) s += C.sums[i];
         s = sqrt(block_sum(s));
         const double c = C.max_norm / (s + 1e-6);
         factor = c >= 1.0 ? 1.0f : (float)c;
-        if (threadIdx.x == 0) {
-            C.out[0] = (float)s;
-            C.out[1] = factor;
-        }
+        if (threadIdx.x == 0) *C.norm = (float)s;
     }
     if (threadIdx.x == 0) out->clip = factor;
 }

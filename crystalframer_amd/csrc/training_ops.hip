@@ -142,15 +142,15 @@ int cfh_adamw_step_moments(const cfh_param_job* jobs, int32_t njobs, const cfh_m
         if (jobs[j].first < 0 || jobs[j].first % cfh::MOMENT_BLOCK || jobs[j].first > state->size - jobs[j].n)
             return fail(CFH_EINVAL, "adamw: job %d: elements %lld ... of %lld moments (a multiple of %d)", (int)j, (long long)jobs[j].first,
                         (long long)state->size, cfh::MOMENT_BLOCK);
-    if (clip && (!clip->out || clip->count < 0 || (clip->count > 0 && !clip->sums) || !(clip->max_norm >= 0.0)))
-        return fail(CFH_EINVAL, "adamw: clip: max_norm = %g must not be negative, sums and out not NULL", clip->max_norm);
+    if (clip && (!clip->norm || clip->count < 0 || (clip->count > 0 && !clip->sums) || !(clip->max_norm >= 0.0)))
+        return fail(CFH_EINVAL, "adamw: clip: max_norm = %g must not be negative, sums and norm not NULL", clip->max_norm);
     hipStream_t st = (hipStream_t)stream;
     const cfh::Moments W{state->exp_avg, state->exp_avg_sq, state->exp_avg_scale, state->exp_avg_sq_scale};
     cfh::AdamWStep* const S = reinterpret_cast<cfh::AdamWStep*>(scratch);
     const cfh::AdamWRates R{beta1, beta2, (float)eps};
     const bool past = 2 * tensor_bytes(jobs, njobs) + state->size * (state->bits / 4) >= 2 * cfh::CACHED_BYTES;
     cfh::GradClip C{};
-    if (clip) C = {clip->sums, clip->count, clip->max_norm, clip->out};
+    if (clip) C = {clip->sums, clip->count, clip->max_norm, clip->norm};
     hipLaunchKernelGGL(cfh::adamw_begin_kernel, dim3(1), dim3(256), 0, st, S, reinterpret_cast<unsigned long long*>(step_dev), lr, beta1, beta2,
                        weight_decay, C);
     const bool few = elements(jobs, njobs) < 512LL * cfh::ADAMW_CHUNK;

@@ -19,11 +19,20 @@ runs give equal bits).  ``max_grad_norm``: the gradients of all groups are clipp
 inside the step: the gradients are read once more and not written.  A group of float32 parameters with moments in 32 bits and
 no clipping takes ``cfh_adamw_step_batch``, anything else ``cfh_adamw_step_moments``.
 """
+import contextlib
 import ctypes
 
 import torch
 
 from . import _lib
+
+
+_here = contextlib.nullcontext()
+
+
+def _on(dev):
+    """A guard for ``dev``, or nothing where it is the current device already."""
+    return _here if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
 class AdamW(torch.optim.Optimizer):
@@ -138,7 +147,7 @@ class AdamW(torch.optim.Optimizer):
             if st["bits"] == 8:
                 dev, state = m.device, self._moments_struct(st)
                 m, v = (torch.empty(m.numel(), dtype=torch.float32, device=dev) for _ in range(2))
-                with torch.cuda.device(dev):
+                with _on(dev):
                     rc = lib.cfh_adamw_moments(ctypes.byref(state), m.data_ptr(), v.data_ptr(), _lib.raw_stream(dev))
                 _lib.check(rc, "cfh_adamw_moments")
             out.append((m, v))
@@ -199,15 +208,15 @@ class AdamW(torch.optim.Optimizer):
                 n, keep = self._fill_moments(plan, jobs)      # a gradient that has to be looked at
             if n:
                 filled.append((group, st, plan, jobs, n, keep))
-        clip = None
+        clip = sums = None
         if self.max_grad_norm is not None and filled:
-            clip = self._clip(lib, filled)
+            clip, sums = self._clip(lib, filled)      # (the sums live until the steps are on their way)
         elif self.max_grad_norm is not None:
             self.grad_norm = None
         for group, st, plan, jobs, n, keep in filled:
             dev, (b1, b2) = plan["device"], group["betas"]
             state = self._moments_struct(st)
-            with torch.cuda.device(dev):
+            with _on(dev):
                 rc = lib.cfh_adamw_step_moments(
                     jobs, n, ctypes.byref(state), float(group["lr"]), float(b1), float(b2), float(group["eps"]),
                     float(group["weight_decay"]), None if clip is None else ctypes.byref(clip), st["step"].data_ptr(),
@@ -230,15 +239,15 @@ class AdamW(torch.optim.Optimizer):
         clip.count = lib.cfh_grad_square_sums_count(jobs, total)
         if clip.count < 0:
             _lib.check(clip.count, "cfh_grad_square_sums_count")
-        # the norm (a double's place: the factor comes behind it), then the sums; memory of its own for every step, so that two captured
-        # steps never share it
-        memory = torch.empty(clip.count + 1, dtype=torch.float64, device=dev)
-        clip.out, clip.sums, clip.max_norm = memory.data_ptr(), memory.data_ptr() + 8, float(self.max_grad_norm)
-        with torch.cuda.device(dev):
+        # (memory of its own for every step: two captured steps never share it)
+        sums = torch.empty(clip.count, dtype=torch.float64, device=dev)
+        norm = torch.empty((), dtype=torch.float32, device=dev)
+        clip.sums, clip.norm, clip.max_norm = sums.data_ptr(), norm.data_ptr(), float(self.max_grad_norm)
+        with _on(dev):
             rc = lib.cfh_grad_square_sums(jobs, total, clip.sums, clip.count, _lib.raw_stream(dev))
         _lib.check(rc, "cfh_grad_square_sums")
-        self.grad_norm = memory.view(torch.float32)[0]
-        return clip
+        self.grad_norm = norm
+        return clip, sums
 
     @staticmethod
     def _fill_moments(plan, jobs):

@@ -558,7 +558,7 @@ typedef struct cfh_grad_clip {
     int32_t count;
     int32_t reserved0;
     double max_norm;
-    float* out;              /* device: |g| and c are written here                                */
+    float* norm;             /* device: |g| is written here                                       */
 } cfh_grad_clip;
 int cfh_adamw_step_moments(const cfh_param_job* jobs, int32_t njobs, const cfh_moments* state, double lr, double beta1,
                            double beta2, double eps, double weight_decay, const cfh_grad_clip* clip, uint64_t* step_dev,

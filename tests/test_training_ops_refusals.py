@@ -91,9 +91,9 @@ def test_sums_of_squares_clipping_and_values_of_moments():
     for args in ((None, 1, A, need), (jobs, -1, A, need), (jobs, 1, None, need), (jobs, 1, A, need - 1), (jobs, 1, A, need + 1), (jobs, 1, A + 4, need)):
         assert lib.cfh_grad_square_sums(*args, None) < 0
     assert lib.cfh_grad_square_sums_count(_job(dtype=7), 1) < 0
-    for change in (dict(out=None), dict(sums=None), dict(count=-1), dict(max_norm=-1.0), dict(max_norm=float("nan"))):
+    for change in (dict(norm=None), dict(sums=None), dict(count=-1), dict(max_norm=-1.0), dict(max_norm=float("nan"))):
         clip = _lib.CfhGradClip()
-        clip.sums, clip.count, clip.max_norm, clip.out = A, 1, 1.0, A
+        clip.sums, clip.count, clip.max_norm, clip.norm = A, 1, 1.0, A
         for k, v in change.items():
             setattr(clip, k, v)
         rc = lib.cfh_adamw_step_moments(jobs, 1, ctypes.byref(_state()), 1e-3, 0.9, 0.99, 1e-8, 0.0, ctypes.byref(clip), A, A, None)
