@@ -18,10 +18,9 @@
 
 namespace cfh {
 
-template <typename T>
+template <typename T, int E>
 struct Vec {
-    static constexpr int N = 16 / (int)sizeof(T);
-    T e[N];
+    T e[E];
 };
 
 // Sum over the lanes of a team; every lane gets it.  LANES 16, 32 or 64: a part of a wavefront, in DPP and lane swaps; 0: the whole
@@ -71,12 +70,12 @@ struct TeamSum {
     }
 };
 
-// A lane's part of a row: VPT pieces of 16 bytes, a team's width apart.  TAIL: the pieces of a team reach over
+// A lane's part of a row: VPT pieces of E elements (16 bytes; one element where a row is shorter than that), a team's width apart.  TAIL: the pieces of a team reach over
 // the row's end; else they are the row, and nothing has to be looked at.
-template <typename T, int LANES, int VPT, bool TAIL>
+template <typename T, int E_, int LANES, int VPT, bool TAIL>
 struct Share {
-    static constexpr int E = Vec<T>::N, N = VPT * E, CAP = LANES * N, TEAMS = LANES ? 256 / LANES : 1;
-    struct Raw { Vec<T> v[VPT]; };
+    static constexpr int E = E_, BYTES = E * (int)sizeof(T), N = VPT * E, CAP = LANES * N, TEAMS = LANES ? 256 / LANES : 1;
+    struct Raw { Vec<T, E> v[VPT]; };
     int lane, dim, width;
     __device__ __forceinline__ explicit Share(int dim_) : dim(dim_) {
         width = LANES ? LANES : (int)blockDim.x;
@@ -85,50 +84,40 @@ struct Share {
     __device__ __forceinline__ static int team() { return LANES ? (int)threadIdx.x / (LANES ? LANES : 1) : 0; }
     __device__ __forceinline__ int col(int k) const { return (k * width + lane) * E; }
     __device__ __forceinline__ bool live(int i) const { return !TAIL || col(i / E) + i % E < dim; }
-    // What lies behind the row's end is not read.  TAIL: a piece that reaches over it, or lies behind it, is read from the last 16 bytes of
-    // the row and moved into place by trim(), so that no load waits behind a branch.  (Rows shorter than a piece: element by element.)
+    // What lies behind the row's end is not read.  TAIL: a piece that reaches over it, or lies behind it, is read from the row's last E
+    // elements and moved into place by trim(), so that no load waits behind a branch.
     __device__ __forceinline__ void load(Raw& r, const T* row) const {
-        if (!TAIL) {
 #pragma unroll
-            for (int k = 0; k < VPT; k++) __builtin_memcpy(&r.v[k], row + col(k), 16);
-        } else if (dim >= E) {
-#pragma unroll
-            for (int k = 0; k < VPT; k++) __builtin_memcpy(&r.v[k], row + min(col(k), dim - E), 16);
-        } else {
-#pragma unroll
-            for (int k = 0; k < VPT; k++)
-#pragma unroll
-                for (int j = 0; j < E; j++) r.v[k].e[j] = col(k) + j < dim ? row[col(k) + j] : (T)0.0f;
-        }
+        for (int k = 0; k < VPT; k++) __builtin_memcpy(&r.v[k], row + (TAIL ? min(col(k), dim - E) : col(k)), BYTES);
     }
     __device__ __forceinline__ void trim(Raw& r) const {
-        if (!TAIL) return;
+        if constexpr (!TAIL) return;
 #pragma unroll
         for (int k = 0; k < VPT; k++) {
             const int over = col(k) + E - dim;
-            if (over > 0 && dim >= E) {
-                uint64_t w[2];
-                __builtin_memcpy(w, &r.v[k], 16);
-                const int bits = over * 8 * (int)sizeof(T);
-                if (bits >= 64) {
-                    w[0] = bits >= 128 ? 0 : w[1] >> (bits - 64);
-                    w[1] = 0;
-                } else {
-                    w[0] = w[0] >> bits | w[1] << (64 - bits);
-                    w[1] >>= bits;
+            if (over > 0) {
+                if constexpr (E == 1) r.v[k].e[0] = (T)0.0f;
+                else {
+                    uint64_t w[2];
+                    __builtin_memcpy(w, &r.v[k], 16);
+                    const int bits = over * 8 * (int)sizeof(T);
+                    if (bits >= 64) {
+                        w[0] = bits >= 128 ? 0 : w[1] >> (bits - 64);
+                        w[1] = 0;
+                    } else {
+                        w[0] = w[0] >> bits | w[1] << (64 - bits);
+                        w[1] >>= bits;
+                    }
+                    __builtin_memcpy(&r.v[k], w, 16);
                 }
-                __builtin_memcpy(&r.v[k], w, 16);
             }
         }
     }
     // weights: of the type of the rows or float32; `none` where there are none, 0 behind the last
     __device__ __forceinline__ void weights(float (&o)[N], const void* w, bool f32, float none) const {
-        if (!w || (TAIL && dim < E)) {
+        if (!w) {
 #pragma unroll
-            for (int i = 0; i < N; i++) {
-                const int c = col(i / E) + i % E;
-                o[i] = !live(i) ? 0.0f : !w ? none : f32 ? reinterpret_cast<const float*>(w)[c] : to_float(reinterpret_cast<const T*>(w)[c]);
-            }
+            for (int i = 0; i < N; i++) o[i] = live(i) ? none : 0.0f;
             return;
         }
         if (sizeof(T) < 4 && !f32) {
@@ -166,10 +155,10 @@ struct Share {
 #pragma unroll
         for (int k = 0; k < VPT; k++) {
             const int c = col(k);
-            Vec<T> v;
+            Vec<T, E> v;
 #pragma unroll
             for (int j = 0; j < E; j++) v.e[j] = from_float<T>(o[k * E + j]);
-            if (!TAIL || c + E <= dim) __builtin_memcpy(row + c, &v, 16);
+            if (!TAIL || c + E <= dim) __builtin_memcpy(row + c, &v, BYTES);
             else if (TAIL) {
 #pragma unroll
                 for (int j = 0; j < E; j++)
@@ -206,10 +195,10 @@ __device__ __forceinline__ void row_stats(const S& sh, const float (&v)[S::N], i
 }
 
 // GENERAL: some norm is a layer norm or has a bias; else root-mean-square norms with weights alone.
-template <typename T, int LANES, int VPT, bool TAIL, bool BN, bool GENERAL>
+template <typename T, int E, int LANES, int VPT, bool TAIL, bool BN, bool GENERAL>
 __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_forward_kernel(const ResidualNorm A, T* h_out, T* y_out,
                                                                                           float* stats) {
-    using S = Share<T, LANES, VPT, TAIL>;
+    using S = Share<T, E, LANES, VPT, TAIL>;
     constexpr int N = S::N, TEAMS = S::TEAMS;
     __shared__ float part[TeamSum<LANES>::WORDS];
     TeamSum<LANES> sum(part);
@@ -265,9 +254,9 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_forward_kern
 // written down per workgroup (or strip, for the gate); a second launch adds these in a fixed order.
 // GATE: 0 none, 1 a row for several rows (its gradient is a column sum), 2 one for each row.
 // GENERAL as above, or the gradient of a bias is wanted.
-template <typename T, int LANES, int VPT, bool TAIL, bool BN, int GATE, bool GENERAL>
+template <typename T, int E, int LANES, int VPT, bool TAIL, bool BN, int GATE, bool GENERAL>
 __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_backward_kernel(const ResidualNorm A, const NormGrads G) {
-    using S = Share<T, LANES, VPT, TAIL>;
+    using S = Share<T, E, LANES, VPT, TAIL>;
     constexpr int N = S::N, TEAMS = S::TEAMS;
     __shared__ float part[TeamSum<LANES>::WORDS];
     __shared__ float cols[TEAMS > 1 ? TEAMS * S::CAP : 1];
@@ -284,6 +273,33 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_backward_ker
         if constexpr (GENERAL) db[i] = 0.0f;
         if constexpr (BN) dwf[i] = 0.0f;
         if constexpr (BN && GENERAL) dbf[i] = 0.0f;
+    }
+
+    // The weights (w, wf, bf) of rows with a piece per lane are kept in LDS, in quads of a piece a team's width apart, so that lanes that
+    // read together read what lies together.  (Longer rows have no room there and read them from the caches.)
+    constexpr bool HELD = VPT == 1;
+    constexpr int QUAD = E < 4 ? E : 4;
+    extern __shared__ float held[];
+    auto place = [&](int k, int i) { return (k * N + i / QUAD * QUAD) * sh.width + sh.lane * QUAD + i % QUAD; };
+    auto weights = [&](int k, float (&o)[N], const void* from, float none) {
+        if constexpr (HELD) {
+#pragma unroll
+            for (int i = 0; i < N; i++) o[i] = held[place(k, i)];
+        } else sh.weights(o, from, A.w_float, none);
+    };
+    if constexpr (HELD) {
+        if (team == 0) {
+            float o[N];
+            auto hold = [&](int k, const void* from, float none) {
+                sh.weights(o, from, A.w_float, none);
+#pragma unroll
+                for (int i = 0; i < N; i++) held[place(k, i)] = o[i];
+            };
+            hold(0, A.w, 1.0f);
+            if constexpr (BN) hold(1, A.wf, 1.0f);
+            if constexpr (BN && GENERAL) hold(2, A.bf, 0.0f);
+        }
+        __syncthreads();
     }
 
     // the workgroup's sum of a column each: to float32 `sums`, or (NULL) rounded to `out`
@@ -315,31 +331,37 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_backward_ker
     for (int64_t strip = blockIdx.x; strip < G.strips; strip += gridDim.x) {
         const int64_t segment = strip / G.parts, sub = strip - segment * G.parts;
         const int64_t row0 = segment * span + span * sub / G.parts, row1 = segment * span + span * (sub + 1) / G.parts;
-        typename S::Raw rg;
+        typename S::Raw rg, rx, rf, rgh, rgy;
         if constexpr (GATE == 1) {
             sh.load(rg, reinterpret_cast<const T*>(A.gate) + segment * A.dim);
             sh.trim(rg);
 #pragma unroll
             for (int i = 0; i < N; i++) dg[i] = 0.0f;
         }
-        for (int64_t row = row0 + team; row < row1; row += TEAMS) {
-            typename S::Raw rx, rf, rgh, rgy;
-            sh.load(rx, reinterpret_cast<const T*>(A.x) + row * A.xs);
-            if (A.f) sh.load(rf, reinterpret_cast<const T*>(A.f) + row * A.fs);
-            if constexpr (GATE == 2) sh.load(rg, reinterpret_cast<const T*>(A.gate) + row * A.dim);
+        // The next row's pieces are asked for as soon as this row's are done with, so that they are on their way through its sums.
+        auto fetch_x = [&](int64_t r) { sh.load(rx, reinterpret_cast<const T*>(A.x) + r * A.xs); };
+        auto fetch_f = [&](int64_t r) { sh.load(rf, reinterpret_cast<const T*>(A.f) + r * A.fs); };
+        auto fetch_gate = [&](int64_t r) { sh.load(rg, reinterpret_cast<const T*>(A.gate) + r * A.dim); };
+        if (row0 + team < row1) {
+            const int64_t row = row0 + team;
+            if (gy) { fetch_x(row); sh.load(rgy, gy + row * A.dim); }
+            if (A.f) fetch_f(row);
+            if constexpr (GATE == 2) fetch_gate(row);
             if (gh) sh.load(rgh, gh + row * A.dim);
-            if (gy) sh.load(rgy, gy + row * A.dim);
+        }
+        for (int64_t row = row0 + team; row < row1; row += TEAMS) {
+            const int64_t next = row + TEAMS;
+            const bool more = next < row1;
             const float4 st = *reinterpret_cast<const float4*>(G.stats + 4 * row);
-            sh.trim(rx);
+            if (gy) { sh.trim(rx); sh.trim(rgy); }
             if (A.f) sh.trim(rf);
             if constexpr (GATE == 2) sh.trim(rg);
             if (gh) sh.trim(rgh);
-            if (gy) sh.trim(rgy);
             // What the rows' own values give is computed again where it is needed a second time, and the weights are read again for every
-            // row, from the caches: kept in registers, they would halve the wavefronts.
+            // row: kept in registers, they would halve the wavefronts.
             float wf[BN ? N : 1], bf[BN && GENERAL ? N : 1];
-            if constexpr (BN) sh.weights(wf, A.wf, A.w_float, 1.0f);
-            if constexpr (BN && GENERAL) sh.weights(bf, A.bf, A.w_float, 0.0f);
+            if constexpr (BN) weights(1, wf, A.wf, 1.0f);
+            if constexpr (BN && GENERAL) weights(2, bf, A.bf, 0.0f);
             auto gate = [&](int i) { return GATE ? S::at(rg, i) : 1.0f; };
             const float off_a = -st.x * st.y, off_h = -st.z * st.w;
             auto ahat = [&](int i) { return GENERAL ? fmaf(S::at(rf, i), st.y, off_a) : S::at(rf, i) * st.y; };
@@ -351,7 +373,7 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_backward_ker
             float dh[N];
             if (gy) {
                 float w[N], xhat[N], s = 0.0f, t = 0.0f;
-                sh.weights(w, A.w, A.w_float, 1.0f);
+                weights(0, w, A.w, 1.0f);
 #pragma unroll
                 for (int i = 0; i < N; i++) {
                     float v = A.in_scale * S::at(rx, i);
@@ -363,6 +385,10 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_backward_ker
                     dh[i] = e * w[i];
                     if constexpr (GENERAL) s += dh[i];
                     t = fmaf(dh[i], xhat[i], t);
+                }
+                if (more) {
+                    fetch_x(next);
+                    sh.load(rgy, gy + next * A.dim);
                 }
                 if constexpr (GENERAL) {
                     sum(s, t);
@@ -378,6 +404,7 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_backward_ker
 #pragma unroll
                 for (int i = 0; i < N; i++) dh[i] = gh ? S::at(rgh, i) : 0.0f;
             }
+            if (gh && more) sh.load(rgh, gh + next * A.dim);
             if (G.dx) {
                 float o[N];
 #pragma unroll
@@ -398,6 +425,9 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_backward_ker
             }
 #pragma unroll
             for (int i = 0; i < N; i++) dh[i] *= GATE ? A.sf * gate(i) : A.sf;
+            if constexpr (GATE == 2) {
+                if (more) fetch_gate(next);
+            }
             if constexpr (BN) {
                 float s = 0.0f, t = 0.0f;
 #pragma unroll
@@ -416,6 +446,7 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_backward_ker
 #pragma unroll
                 for (int i = 0; i < N; i++) dh[i] = st.y * fmaf(dh[i], wf[i], fmaf(-ahat(i), t, -s));
             }
+            if (A.f && more) fetch_f(next);
             if (G.df) sh.store(reinterpret_cast<T*>(G.df) + row * A.dim, dh);
         }
         if constexpr (GATE == 1)
@@ -469,18 +500,20 @@ __global__ __launch_bounds__(256) void residual_norm_columns_kernel(const NormGr
 }
 
 // ------------------------------------------------------------------------------------------------- launches
-// f(lanes of a team, pieces of 16 bytes per lane, whether they reach over a row's end, threads of a workgroup): see norm_threads.
+// f(elements of a piece, lanes of a team, pieces per lane, whether they reach over a row's end, threads of a workgroup): see norm_threads.
 template <typename T, typename F>
 void with_share(int64_t dim, F f) {
-    constexpr int E = Vec<T>::N;
+    constexpr int E = 16 / (int)sizeof(T);
     const int threads = norm_threads(dim, E);
     using std::integral_constant;
     auto share = [&](auto lanes, auto vpt) {
+        const integral_constant<int, E> e;
         const int64_t whole = (int64_t)(decltype(lanes)::value ? decltype(lanes)::value : threads) * decltype(vpt)::value * E;
-        if (dim == whole) f(lanes, vpt, std::false_type(), threads);
-        else f(lanes, vpt, std::true_type(), threads);
+        if (dim == whole) f(e, lanes, vpt, std::false_type(), threads);
+        else f(e, lanes, vpt, std::true_type(), threads);
     };
-    if (dim <= 16 * E) share(integral_constant<int, 16>(), integral_constant<int, 1>());
+    if (dim < E) f(integral_constant<int, 1>(), integral_constant<int, 16>(), integral_constant<int, 1>(), std::true_type(), threads);
+    else if (dim <= 16 * E) share(integral_constant<int, 16>(), integral_constant<int, 1>());
     else if (dim <= 32 * E) share(integral_constant<int, 32>(), integral_constant<int, 1>());
     else if (dim <= 64 * E) share(integral_constant<int, 64>(), integral_constant<int, 1>());
     else if (dim <= 1024 * E) share(integral_constant<int, 0>(), integral_constant<int, 1>());
@@ -490,13 +523,13 @@ void with_share(int64_t dim, F f) {
 
 template <typename T>
 void residual_norm_forward(const ResidualNorm& A, T* h, T* y, float* stats, hipStream_t st) {
-    with_share<T>(A.dim, [&](auto lanes, auto vpt, auto tail, int threads) {
-        constexpr int L = decltype(lanes)::value, V = decltype(vpt)::value, TEAMS = L ? 256 / L : 1;
+    with_share<T>(A.dim, [&](auto e, auto lanes, auto vpt, auto tail, int threads) {
+        constexpr int E = decltype(e)::value, L = decltype(lanes)::value, V = decltype(vpt)::value, TEAMS = L ? 256 / L : 1;
         constexpr bool TAIL = decltype(tail)::value;
         const int64_t blocks = (A.rows + TEAMS - 1) / TEAMS, most = (int64_t)NORM_CUS * (2048 / threads);
         const dim3 grid((unsigned)(blocks < most ? blocks : most));
         auto launch = [&](auto bn, auto general) {
-            hipLaunchKernelGGL((residual_norm_forward_kernel<T, L, V, TAIL, decltype(bn)::value, decltype(general)::value>), grid, dim3(threads), 0, st, A,
+            hipLaunchKernelGGL((residual_norm_forward_kernel<T, E, L, V, TAIL, decltype(bn)::value, decltype(general)::value>), grid, dim3(threads), 0, st, A,
                                h, y, stats);
         };
         auto kind_of = [&](auto bn) {
@@ -510,19 +543,23 @@ void residual_norm_forward(const ResidualNorm& A, T* h, T* y, float* stats, hipS
 
 template <typename T>
 void residual_norm_backward(const ResidualNorm& A, NormGrads G, int64_t gate_rows, float* scratch, hipStream_t st) {
-    const NormPlan P = norm_plan(A.rows, A.dim, Vec<T>::N, gate_rows);
+    const NormPlan P = norm_plan(A.rows, A.dim, 16 / (int)sizeof(T), gate_rows);
     G.column = P.column_floats ? scratch : nullptr;
     G.gate_column = P.gate_floats ? scratch + P.column_floats : nullptr;
     G.strips = P.strips;
     G.parts = P.parts;
     int blocks = P.blocks;
     if (A.rows > 0) {
-        with_share<T>(A.dim, [&](auto lanes, auto vpt, auto tail, int threads) {
-            constexpr int L = decltype(lanes)::value, V = decltype(vpt)::value;
+        with_share<T>(A.dim, [&](auto e, auto lanes, auto vpt, auto tail, int threads) {
+            constexpr int E = decltype(e)::value, L = decltype(lanes)::value, V = decltype(vpt)::value;
             constexpr bool TAIL = decltype(tail)::value;
-            auto launch = [&](auto bn, auto gate, auto bias) {
-                hipLaunchKernelGGL((residual_norm_backward_kernel<T, L, V, TAIL, decltype(bn)::value, decltype(gate)::value, decltype(bias)::value>),
-                                   dim3((unsigned)blocks), dim3(threads), 0, st, A, G);
+            auto launch = [&](auto bn, auto gate, auto kind) {
+                const auto kernel = residual_norm_backward_kernel<T, E, L, V, TAIL, decltype(bn)::value, decltype(gate)::value, decltype(kind)::value>;
+                constexpr int ARRAYS = V > 1 ? 0 : 1 + decltype(bn)::value + (decltype(bn)::value && decltype(kind)::value);
+                const size_t lds = sizeof(float) * ARRAYS * (L ? L : threads) * E;
+                // (beside up to 17 KB of the kernel's own; more than 64 KB has to be asked for)
+                if (lds > 40 * 1024) (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+                hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), lds, st, A, G);
             };
             const bool general = A.norm == 1 || A.block_norm == 1 || A.bf || G.db || G.dbf;
             auto kind_of = [&](auto bn, auto gate) {
