@@ -287,21 +287,6 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_backward_ker
             for (int i = 0; i < N; i++) o[i] = held[place(k, i)];
         } else sh.weights(o, from, A.w_float, none);
     };
-    if constexpr (HELD) {
-        if (team == 0) {
-            float o[N];
-            auto hold = [&](int k, const void* from, float none) {
-                sh.weights(o, from, A.w_float, none);
-#pragma unroll
-                for (int i = 0; i < N; i++) held[place(k, i)] = o[i];
-            };
-            hold(0, A.w, 1.0f);
-            if constexpr (BN) hold(1, A.wf, 1.0f);
-            if constexpr (BN && GENERAL) hold(2, A.bf, 0.0f);
-        }
-        __syncthreads();
-    }
-
     // the workgroup's sum of a column each: to float32 `sums`, or (NULL) rounded to `out`
     auto flush = [&](const float (&acc)[N], float* sums, void* out, bool f32) {
         auto put = [&](int c, float v) {
@@ -312,8 +297,16 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_backward_ker
         if (!sums && !out) return;
         if constexpr (TEAMS == 1) {
 #pragma unroll
-            for (int i = 0; i < N; i++)
-                if (sh.live(i)) put(sh.col(i / S::E) + i % S::E, acc[i]);
+            for (int k = 0; k < VPT; k++) {
+                const int c = sh.col(k);
+                if (sums && (!TAIL || c + E <= A.dim)) {
+                    __builtin_memcpy(sums + c, acc + k * E, E * sizeof(float));
+                    continue;
+                }
+#pragma unroll
+                for (int j = 0; j < E; j++)
+                    if (sh.live(k * E + j)) put(c + j, acc[k * E + j]);
+            }
         } else {
             __syncthreads();
 #pragma unroll
@@ -348,6 +341,23 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_backward_ker
             if (A.f) fetch_f(row);
             if constexpr (GATE == 2) fetch_gate(row);
             if (gh) sh.load(rgh, gh + row * A.dim);
+        }
+        // (behind the first row's fetch: the two wait together)
+        if constexpr (HELD) {
+            if (strip == blockIdx.x) {
+                if (team == 0) {
+                    float o[N];
+                    auto hold = [&](int k, const void* from, float none) {
+                        sh.weights(o, from, A.w_float, none);
+#pragma unroll
+                        for (int i = 0; i < N; i++) held[place(k, i)] = o[i];
+                    };
+                    hold(0, A.w, 1.0f);
+                    if constexpr (BN) hold(1, A.wf, 1.0f);
+                    if constexpr (BN && GENERAL) hold(2, A.bf, 0.0f);
+                }
+                __syncthreads();
+            }
         }
         for (int64_t row = row0 + team; row < row1; row += TEAMS) {
             const int64_t next = row + TEAMS;
@@ -467,32 +477,32 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_backward_ker
 }
 
 // Adds the `count` rows of a column sum: blockIdx.y 0 to 3 dw, db, dwf, dbf (count: the workgroups of the launch before), 4 on: rows of
-// the gate (count: parts).  16 columns per workgroup, 16 lanes for each.
+// the gate (count: parts).  16 columns per workgroup, eight loads under way per lane; 64 lanes for a column where the
+// launch has few workgroups (1021 x 1001: 16 lanes 6.6 us, 64 lanes 4.9), 16 where it has many (16384 x 4096: 10.6, 16.8).
 template <typename T>
-__global__ __launch_bounds__(256) void residual_norm_columns_kernel(const NormGrads G, int dim, int blocks, int w_float) {
+__global__ __launch_bounds__(1024) void residual_norm_columns_kernel(const NormGrads G, int dim, int blocks, int w_float) {
     __shared__ float part[16][16];
     const int k = (int)blockIdx.y, c = (int)blockIdx.x * 16 + (threadIdx.x & 15), lane = threadIdx.x >> 4;
     void* const out = k == 0 ? G.dw : k == 1 ? G.db : k == 2 ? G.dwf : k == 3 ? G.dbf : G.dgate;
     if (!out) return;
     const int64_t count = k < 4 ? blocks : G.parts;
     const float* const src = k < 4 ? G.column + (int64_t)k * blocks * dim : G.gate_column + (int64_t)(k - 4) * G.parts * dim;
+    const int lanes = (int)blockDim.x / 16;
     float s = 0.0f;
-    if (c < dim) {
-        int64_t r = lane;
-        for (; r + 7 * 16 < count; r += 8 * 16) {          // eight loads under way
+    if (c < dim)
+        for (int64_t r0 = lane; r0 < count; r0 += 8 * lanes) {
             float v[8];
 #pragma unroll
-            for (int k = 0; k < 8; k++) v[k] = src[(r + 16 * k) * dim + c];
+            for (int j = 0; j < 8; j++) v[j] = r0 + lanes * j < count ? src[(r0 + lanes * j) * dim + c] : 0.0f;
 #pragma unroll
-            for (int k = 0; k < 8; k++) s += v[k];
+            for (int j = 0; j < 8; j++) s += v[j];
         }
-        for (; r < count; r += 16) s += src[r * dim + c];
-    }
-    part[lane][threadIdx.x & 15] = s;
+    s = rows_sum(s);
+    if ((threadIdx.x & 48) == 0) part[threadIdx.x >> 6][threadIdx.x & 15] = s;
     __syncthreads();
     if (lane == 0 && c < dim) {
         s = 0.0f;
-        for (int t = 0; t < 16; t++) s += part[t][threadIdx.x];
+        for (int t = 0; t < lanes / 4; t++) s += part[t][threadIdx.x];
         const int64_t o = k < 4 ? c : (int64_t)(k - 4) * dim + c;
         if (k < 4 && w_float) reinterpret_cast<float*>(out)[o] = s;
         else reinterpret_cast<T*>(out)[o] = from_float<T>(s);
@@ -583,8 +593,9 @@ void residual_norm_backward(const ResidualNorm& A, NormGrads G, int64_t gate_row
     if (columns || gates) {
         if (!columns) G.dw = G.db = G.dwf = G.dbf = nullptr;
         const int64_t y = 4 + (gates ? (A.rows == 0 ? gate_rows : P.segments) : 0);
-        hipLaunchKernelGGL(residual_norm_columns_kernel<T>, dim3((unsigned)((A.dim + 15) / 16), (unsigned)y), dim3(256), 0, st, G, A.dim, blocks,
-                           A.w_float);
+        const dim3 grid((unsigned)((A.dim + 15) / 16), (unsigned)y);
+        const unsigned columns_threads = (int64_t)grid.x * grid.y >= 2 * NORM_CUS ? 256 : 1024;
+        hipLaunchKernelGGL(residual_norm_columns_kernel<T>, grid, dim3(columns_threads), 0, st, G, A.dim, blocks, A.w_float);
     }
 }
 
