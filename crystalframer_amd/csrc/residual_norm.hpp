@@ -253,8 +253,8 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_forward_kern
 // Sums over rows are kept per lane, for its columns, while a workgroup goes through its strips, then added over its teams and
 // written down per workgroup (or strip, for the gate); a second launch adds these in a fixed order.
 // GATE: 0 none, 1 a row for several rows (its gradient is a column sum), 2 one for each row.
-// GENERAL as above, or the gradient of a bias is wanted.
-template <typename T, int E, int LANES, int VPT, bool TAIL, bool BN, int GATE, bool GENERAL>
+// GENERAL as above, or the gradient of a bias is wanted.  SUMS: else the column sums are the column kernel's, and the rows' means are left to it.
+template <typename T, int E, int LANES, int VPT, bool TAIL, bool BN, int GATE, bool GENERAL, bool SUMS>
 __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_backward_kernel(const ResidualNorm A, const NormGrads G) {
     using S = Share<T, E, LANES, VPT, TAIL>;
     constexpr int N = S::N, TEAMS = S::TEAMS;
@@ -266,13 +266,14 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_backward_ker
     const T* const gh = reinterpret_cast<const T*>(G.gh);
     const T* const gy = reinterpret_cast<const T*>(G.gy);
     const float inv = 1.0f / (float)A.dim;
-    float dw[N], db[GENERAL ? N : 1], dwf[BN ? N : 1], dbf[BN && GENERAL ? N : 1], dg[GATE == 1 ? N : 1];
+    constexpr bool SUM_B = SUMS && GENERAL, SUM_WF = SUMS && BN, SUM_BF = SUMS && BN && GENERAL, SUM_G = SUMS && GATE == 1;
+    float dw[SUMS ? N : 1], db[SUM_B ? N : 1], dwf[SUM_WF ? N : 1], dbf[SUM_BF ? N : 1], dg[SUM_G ? N : 1];
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        dw[i] = 0.0f;
-        if constexpr (GENERAL) db[i] = 0.0f;
-        if constexpr (BN) dwf[i] = 0.0f;
-        if constexpr (BN && GENERAL) dbf[i] = 0.0f;
+        if constexpr (SUMS) dw[i] = 0.0f;
+        if constexpr (SUM_B) db[i] = 0.0f;
+        if constexpr (SUM_WF) dwf[i] = 0.0f;
+        if constexpr (SUM_BF) dbf[i] = 0.0f;
     }
 
     // The weights (w, wf, bf) of rows with a piece per lane are kept in LDS, in quads of a piece a team's width apart, so that lanes that
@@ -294,7 +295,6 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_backward_ker
             else if (f32) reinterpret_cast<float*>(out)[c] = v;
             else reinterpret_cast<T*>(out)[c] = from_float<T>(v);
         };
-        if (!sums && !out) return;
         if constexpr (TEAMS == 1) {
 #pragma unroll
             for (int k = 0; k < VPT; k++) {
@@ -328,6 +328,8 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_backward_ker
         if constexpr (GATE == 1) {
             sh.load(rg, reinterpret_cast<const T*>(A.gate) + segment * A.dim);
             sh.trim(rg);
+        }
+        if constexpr (SUM_G) {
 #pragma unroll
             for (int i = 0; i < N; i++) dg[i] = 0.0f;
         }
@@ -381,6 +383,7 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_backward_ker
                 else return S::at(rf, i);
             };
             float dh[N];
+            float4 mid = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (gy) {
                 float w[N], xhat[N], s = 0.0f, t = 0.0f;
                 weights(0, w, A.w, 1.0f);
@@ -390,8 +393,8 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_backward_ker
                     if (BN || GATE || A.f) v = fmaf(A.sf, GATE ? gate(i) * block_out(i) : block_out(i), v);
                     xhat[i] = GENERAL ? fmaf(v, st.w, off_h) : v * st.w;
                     const float e = S::at(rgy, i);
-                    dw[i] = fmaf(e, xhat[i], dw[i]);
-                    if constexpr (GENERAL) db[i] += e;
+                    if constexpr (SUMS) dw[i] = fmaf(e, xhat[i], dw[i]);
+                    if constexpr (SUM_B) db[i] += e;
                     dh[i] = e * w[i];
                     if constexpr (GENERAL) s += dh[i];
                     t = fmaf(dh[i], xhat[i], t);
@@ -405,6 +408,8 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_backward_ker
                     s = A.norm == 1 ? s * inv : 0.0f;
                 } else t = sum(t);
                 t *= inv;
+                mid.x = s;
+                mid.y = t;
 #pragma unroll
                 for (int i = 0; i < N; i++) {
                     const float v = fmaf(-xhat[i], t, GENERAL ? dh[i] - s : dh[i]);
@@ -421,7 +426,7 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_backward_ker
                 for (int i = 0; i < N; i++) o[i] = A.sx * dh[i];
                 sh.store(reinterpret_cast<T*>(G.dx) + row * A.dim, o);
             }
-            if constexpr (GATE == 1) {
+            if constexpr (SUM_G) {
 #pragma unroll
                 for (int i = 0; i < N; i++) dg[i] = fmaf(A.sf * block_out(i), dh[i], dg[i]);
             }
@@ -445,25 +450,136 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_backward_ker
                     const float u = dh[i] * wf[i], v = ahat(i);
                     if constexpr (GENERAL) s += u;
                     t = fmaf(u, v, t);
-                    dwf[i] = fmaf(dh[i], v, dwf[i]);
-                    if constexpr (GENERAL) dbf[i] += dh[i];
+                    if constexpr (SUM_WF) dwf[i] = fmaf(dh[i], v, dwf[i]);
+                    if constexpr (SUM_BF) dbf[i] += dh[i];
                 }
                 if constexpr (GENERAL) {
                     sum(s, t);
                     s = A.block_norm == 1 ? s * inv : 0.0f;
                 } else t = sum(t);
                 t *= inv;
+                mid.z = s;
+                mid.w = t;
 #pragma unroll
                 for (int i = 0; i < N; i++) dh[i] = st.y * fmaf(dh[i], wf[i], fmaf(-ahat(i), t, -s));
+            }
+            if constexpr (!SUMS) {
+                if (sh.lane == 0) *reinterpret_cast<float4*>(G.mid + 4 * row) = mid;
             }
             if (A.f && more) fetch_f(next);
             if (G.df) sh.store(reinterpret_cast<T*>(G.df) + row * A.dim, dh);
         }
-        if constexpr (GATE == 1)
-            flush(dg, G.gate_column ? G.gate_column + strip * A.dim : nullptr,
-                  G.dgate ? reinterpret_cast<T*>(G.dgate) + segment * A.dim : nullptr, false);
+        if constexpr (SUM_G) {
+            if (G.dgate) flush(dg, G.gate_column ? G.gate_column + strip * A.dim : nullptr, reinterpret_cast<T*>(G.dgate) + segment * A.dim, false);
+        }
     }
     auto column = [&](int k) { return G.column ? G.column + ((int64_t)k * gridDim.x + blockIdx.x) * A.dim : nullptr; };
+    if constexpr (SUMS) {
+        if (G.dw) flush(dw, column(0), G.dw, A.w_float);
+    }
+    if constexpr (SUM_B) {
+        if (G.db) flush(db, column(1), G.db, A.w_float);
+    }
+    if constexpr (SUM_WF) {
+        if (G.dwf) flush(dwf, column(2), G.dwf, A.w_float);
+    }
+    if constexpr (SUM_BF) {
+        if (G.dbf) flush(dbf, column(3), G.dbf, A.w_float);
+    }
+}
+
+// The column sums alone, with the rows' means known: a lane goes down the rows of its strip with a piece of 16 bytes of each array, four
+// wavefronts of a workgroup over the same columns.  Nothing is exchanged before the end.
+template <typename T, bool TAIL, bool BN, int GATE, bool GENERAL>
+__global__ __launch_bounds__(256) void residual_norm_column_kernel(const ResidualNorm A, const NormGrads G) {
+    constexpr int E = 16 / (int)sizeof(T), N = E, WIDE = 64 * E;
+    using S = Share<T, E, 64, 1, TAIL>;
+    __shared__ float cols[4][WIDE];
+    S sh(A.dim);
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), c0 = (int)blockIdx.x * WIDE;
+    sh.lane += (int)blockIdx.x * 64;
+    const T* const gh = reinterpret_cast<const T*>(G.gh);
+    const T* const gy = reinterpret_cast<const T*>(G.gy);
+    float w[N], wf[BN ? N : 1], bf[BN && GENERAL ? N : 1];
+    sh.weights(w, A.w, A.w_float, 1.0f);
+    if constexpr (BN) sh.weights(wf, A.wf, A.w_float, 1.0f);
+    if constexpr (BN && GENERAL) sh.weights(bf, A.bf, A.w_float, 0.0f);
+    float dw[N], db[GENERAL ? N : 1], dwf[BN ? N : 1], dbf[BN && GENERAL ? N : 1], dg[GATE == 1 ? N : 1];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        dw[i] = 0.0f;
+        if constexpr (GENERAL) db[i] = 0.0f;
+        if constexpr (BN) dwf[i] = 0.0f;
+        if constexpr (BN && GENERAL) dbf[i] = 0.0f;
+    }
+    auto flush = [&](const float (&acc)[N], float* sums, void* out, bool f32) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; i++) cols[wave][sh.col(0) - c0 + i] = acc[i];
+        __syncthreads();
+        for (int c = threadIdx.x; c < min(WIDE, A.dim - c0); c += 256) {
+            const float s = cols[0][c] + cols[1][c] + cols[2][c] + cols[3][c];
+            if (sums) sums[c0 + c] = s;
+            else if (f32) reinterpret_cast<float*>(out)[c0 + c] = s;
+            else reinterpret_cast<T*>(out)[c0 + c] = from_float<T>(s);
+        }
+    };
+    const int64_t span = GATE == 1 ? A.gate_span : A.rows;
+    for (int64_t strip = blockIdx.y; strip < G.strips; strip += gridDim.y) {
+        const int64_t segment = strip / G.parts, sub = strip - segment * G.parts;
+        const int64_t row0 = segment * span + span * sub / G.parts, row1 = segment * span + span * (sub + 1) / G.parts;
+        typename S::Raw rx, rf, rg, rgh, rgy;
+        if constexpr (GATE == 1) {
+            sh.load(rg, reinterpret_cast<const T*>(A.gate) + segment * A.dim);
+            sh.trim(rg);
+#pragma unroll
+            for (int i = 0; i < N; i++) dg[i] = 0.0f;
+        }
+        for (int64_t row = row0 + wave; row < row1; row += 4) {
+            if (gy) {
+                sh.load(rx, reinterpret_cast<const T*>(A.x) + row * A.xs);
+                sh.load(rgy, gy + row * A.dim);
+            }
+            if (A.f) sh.load(rf, reinterpret_cast<const T*>(A.f) + row * A.fs);
+            if constexpr (GATE == 2) sh.load(rg, reinterpret_cast<const T*>(A.gate) + row * A.dim);
+            if (gh) sh.load(rgh, gh + row * A.dim);
+            const float4 st = *reinterpret_cast<const float4*>(G.stats + 4 * row);
+            const float4 mid = *reinterpret_cast<const float4*>(G.mid + 4 * row);
+            if (gy) { sh.trim(rx); sh.trim(rgy); }
+            if (A.f) sh.trim(rf);
+            if constexpr (GATE == 2) sh.trim(rg);
+            if (gh) sh.trim(rgh);
+            const float off_a = -st.x * st.y, off_h = -st.z * st.w;
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const float g = GATE ? S::at(rg, i) : 1.0f;
+                float ahat = 0.0f, a = 0.0f;
+                if (BN || GATE || A.f) {
+                    ahat = !BN ? S::at(rf, i) : GENERAL ? fmaf(S::at(rf, i), st.y, off_a) : S::at(rf, i) * st.y;
+                    a = !BN ? ahat : GENERAL ? fmaf(ahat, wf[i], bf[i]) : ahat * wf[i];
+                }
+                float dh = gh ? S::at(rgh, i) : 0.0f;
+                if (gy) {
+                    const float v = fmaf(A.sf, GATE ? g * a : a, A.in_scale * S::at(rx, i)), xhat = GENERAL ? fmaf(v, st.w, off_h) : v * st.w;
+                    const float e = S::at(rgy, i);
+                    dw[i] = fmaf(e, xhat, dw[i]);
+                    if constexpr (GENERAL) db[i] += e;
+                    const float u = fmaf(-xhat, mid.y, GENERAL ? e * w[i] - mid.x : e * w[i]);
+                    dh = fmaf(st.w, u, dh);
+                }
+                if constexpr (GATE == 1) dg[i] = fmaf(A.sf * a, dh, dg[i]);
+                if constexpr (BN) {
+                    const float da = dh * (GATE ? A.sf * g : A.sf);
+                    dwf[i] = fmaf(da, ahat, dwf[i]);
+                    if constexpr (GENERAL) dbf[i] += da;
+                }
+            }
+        }
+        if constexpr (GATE == 1) {
+            if (G.dgate) flush(dg, G.gate_column ? G.gate_column + strip * A.dim : nullptr, reinterpret_cast<T*>(G.dgate) + segment * A.dim, false);
+        }
+    }
+    auto column = [&](int k) { return G.column ? G.column + ((int64_t)k * gridDim.y + blockIdx.y) * A.dim : nullptr; };
     if (G.dw) flush(dw, column(0), G.dw, A.w_float);
     if constexpr (GENERAL) {
         if (G.db) flush(db, column(1), G.db, A.w_float);
@@ -476,36 +592,39 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_backward_ker
     }
 }
 
-// Adds the `count` rows of a column sum: blockIdx.y 0 to 3 dw, db, dwf, dbf (count: the workgroups of the launch before), 4 on: rows of
-// the gate (count: parts).  16 columns per workgroup, eight loads under way per lane; 64 lanes for a column where the
+// Adds the `count` rows of a column sum: blockIdx.y 0 to 3 dw, db, dwf, dbf (count: the workgroups of the launch before), 4: the `gates`
+// rows of the gate, a gridDim.z'th of them (count: parts).  16 columns per workgroup, eight loads under way per lane; 64 lanes for a column where the
 // launch has few workgroups (1021 x 1001: 16 lanes 6.6 us, 64 lanes 4.9), 16 where it has many (16384 x 4096: 10.6, 16.8).
 template <typename T>
-__global__ __launch_bounds__(1024) void residual_norm_columns_kernel(const NormGrads G, int dim, int blocks, int w_float) {
+__global__ __launch_bounds__(1024) void residual_norm_columns_kernel(const NormGrads G, int dim, int64_t blocks, int64_t gates, int w_float) {
     __shared__ float part[16][16];
     const int k = (int)blockIdx.y, c = (int)blockIdx.x * 16 + (threadIdx.x & 15), lane = threadIdx.x >> 4;
     void* const out = k == 0 ? G.dw : k == 1 ? G.db : k == 2 ? G.dwf : k == 3 ? G.dbf : G.dgate;
     if (!out) return;
     const int64_t count = k < 4 ? blocks : G.parts;
-    const float* const src = k < 4 ? G.column + (int64_t)k * blocks * dim : G.gate_column + (int64_t)(k - 4) * G.parts * dim;
     const int lanes = (int)blockDim.x / 16;
-    float s = 0.0f;
-    if (c < dim)
-        for (int64_t r0 = lane; r0 < count; r0 += 8 * lanes) {
-            float v[8];
+    for (int64_t segment = blockIdx.z; segment < (k < 4 ? 1 : gates); segment += gridDim.z) {
+        const float* const src = k < 4 ? G.column + (int64_t)k * blocks * dim : G.gate_column + segment * G.parts * dim;
+        float s = 0.0f;
+        if (c < dim)
+            for (int64_t r0 = lane; r0 < count; r0 += 8 * lanes) {
+                float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = r0 + lanes * j < count ? src[(r0 + lanes * j) * dim + c] : 0.0f;
+                for (int j = 0; j < 8; j++) v[j] = r0 + lanes * j < count ? src[(r0 + lanes * j) * dim + c] : 0.0f;
 #pragma unroll
-            for (int j = 0; j < 8; j++) s += v[j];
+                for (int j = 0; j < 8; j++) s += v[j];
+            }
+        s = rows_sum(s);
+        if ((threadIdx.x & 48) == 0) part[threadIdx.x >> 6][threadIdx.x & 15] = s;
+        __syncthreads();
+        if (lane == 0 && c < dim) {
+            s = 0.0f;
+            for (int t = 0; t < lanes / 4; t++) s += part[t][threadIdx.x];
+            const int64_t o = k < 4 ? c : segment * dim + c;
+            if (k < 4 && w_float) reinterpret_cast<float*>(out)[o] = s;
+            else reinterpret_cast<T*>(out)[o] = from_float<T>(s);
         }
-    s = rows_sum(s);
-    if ((threadIdx.x & 48) == 0) part[threadIdx.x >> 6][threadIdx.x & 15] = s;
-    __syncthreads();
-    if (lane == 0 && c < dim) {
-        s = 0.0f;
-        for (int t = 0; t < lanes / 4; t++) s += part[t][threadIdx.x];
-        const int64_t o = k < 4 ? c : (int64_t)(k - 4) * dim + c;
-        if (k < 4 && w_float) reinterpret_cast<float*>(out)[o] = s;
-        else reinterpret_cast<T*>(out)[o] = from_float<T>(s);
+        __syncthreads();
     }
 }
 
@@ -551,39 +670,70 @@ void residual_norm_forward(const ResidualNorm& A, T* h, T* y, float* stats, hipS
     });
 }
 
+// f(whether the block is normed, the kind of gate, general), as the kernels' parameters.
+template <typename F>
+void with_form(const ResidualNorm& A, const NormGrads& G, int64_t gate_rows, bool shared, F f) {
+    using std::integral_constant;
+    auto kind_of = [&](auto bn, auto gate) {
+        if (A.norm == 1 || A.block_norm == 1 || A.b || A.bf || G.db || G.dbf) f(bn, gate, std::true_type());
+        else f(bn, gate, std::false_type());
+    };
+    auto gated = [&](auto bn) {
+        if (gate_rows == 0) kind_of(bn, integral_constant<int, 0>());
+        else if (shared) kind_of(bn, integral_constant<int, 1>());
+        else kind_of(bn, integral_constant<int, 2>());
+    };
+    if (A.block_norm) gated(std::true_type());
+    else gated(std::false_type());
+}
+
 template <typename T>
 void residual_norm_backward(const ResidualNorm& A, NormGrads G, int64_t gate_rows, float* scratch, hipStream_t st) {
-    const NormPlan P = norm_plan(A.rows, A.dim, 16 / (int)sizeof(T), gate_rows);
+    const NormPlan P = norm_plan(A.rows, A.dim, 16 / (int)sizeof(T), gate_rows, A.block_norm != 0,
+                                 A.norm == 1 || A.block_norm == 1 || A.b || A.bf);
+    const bool wanted = G.dw || G.db || G.dwf || G.dbf || (G.dgate && P.gate_rows_shared);
     G.column = P.column_floats ? scratch : nullptr;
     G.gate_column = P.gate_floats ? scratch + P.column_floats : nullptr;
-    G.strips = P.strips;
-    G.parts = P.parts;
-    int blocks = P.blocks;
+    G.mid = P.mid_floats ? scratch + (P.column_floats + P.gate_floats + 3) / 4 * 4 : nullptr;
+    int64_t blocks = P.column_blocks;
     if (A.rows > 0) {
         with_share<T>(A.dim, [&](auto e, auto lanes, auto vpt, auto tail, int threads) {
             constexpr int E = decltype(e)::value, L = decltype(lanes)::value, V = decltype(vpt)::value;
             constexpr bool TAIL = decltype(tail)::value;
-            auto launch = [&](auto bn, auto gate, auto kind) {
-                const auto kernel = residual_norm_backward_kernel<T, E, L, V, TAIL, decltype(bn)::value, decltype(gate)::value, decltype(kind)::value>;
-                constexpr int ARRAYS = V > 1 ? 0 : 1 + decltype(bn)::value + (decltype(bn)::value && decltype(kind)::value);
-                const size_t lds = sizeof(float) * ARRAYS * (L ? L : threads) * E;
-                // (beside up to 17 KB of the kernel's own; more than 64 KB has to be asked for)
-                if (lds > 40 * 1024) (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-                hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), lds, st, A, G);
-            };
-            const bool general = A.norm == 1 || A.block_norm == 1 || A.bf || G.db || G.dbf;
-            auto kind_of = [&](auto bn, auto gate) {
-                if (general) launch(bn, gate, std::true_type());
-                else launch(bn, gate, std::false_type());
-            };
-            auto gated = [&](auto bn) {
-                if (gate_rows == 0) kind_of(bn, std::integral_constant<int, 0>());
-                else if (P.gate_rows_shared) kind_of(bn, std::integral_constant<int, 1>());
-                else kind_of(bn, std::integral_constant<int, 2>());
-            };
-            if (A.block_norm) gated(std::true_type());
-            else gated(std::false_type());
+            with_form(A, G, gate_rows, P.gate_rows_shared, [&](auto bn, auto gate, auto general) {
+                constexpr bool BN = decltype(bn)::value, GENERAL = decltype(general)::value;
+                constexpr int GATE = decltype(gate)::value;
+                auto launch = [&](auto sums) {
+                    const auto kernel = residual_norm_backward_kernel<T, E, L, V, TAIL, BN, GATE, GENERAL, decltype(sums)::value>;
+                    constexpr int ARRAYS = V > 1 ? 0 : 1 + BN + (BN && GENERAL);
+                    const size_t lds = sizeof(float) * ARRAYS * (L ? L : threads) * E;
+                    // (beside up to 17 KB of the kernel's own; more than 64 KB has to be asked for)
+                    if (lds > 40 * 1024) (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+                    NormGrads R = G;
+                    R.strips = P.strips;
+                    R.parts = P.parts;
+                    hipLaunchKernelGGL(kernel, dim3((unsigned)P.blocks), dim3(threads), lds, st, A, R);
+                };
+                // (what norm_split can say for these parameters; GENERAL without a norm or bias that is: a bias' gradient alone is wanted)
+                constexpr bool ALWAYS = V > 1, SOMETIMES = L == 0 && sizeof(T) == 2 && BN && GENERAL && GATE != 0;
+                if constexpr (!ALWAYS) {
+                    if (!P.split) launch(std::true_type());
+                }
+                if constexpr (ALWAYS || SOMETIMES) {
+                    if (P.split) launch(std::false_type());
+                    if (P.split && wanted) {
+                        constexpr int WIDE = 64 * E;
+                        const dim3 grid((unsigned)((A.dim + WIDE - 1) / WIDE), (unsigned)P.column_blocks);
+                        NormGrads C = G;
+                        C.strips = P.column_strips;
+                        C.parts = P.column_parts;
+                        if (A.dim % WIDE) hipLaunchKernelGGL((residual_norm_column_kernel<T, true, BN, GATE, GENERAL>), grid, dim3(256), 0, st, A, C);
+                        else hipLaunchKernelGGL((residual_norm_column_kernel<T, false, BN, GATE, GENERAL>), grid, dim3(256), 0, st, A, C);
+                    }
+                }
+            });
         });
+        G.parts = P.split ? P.column_parts : P.parts;
     } else {
         blocks = 0;         // sums over no rows
         G.parts = 0;
@@ -592,10 +742,11 @@ void residual_norm_backward(const ResidualNorm& A, NormGrads G, int64_t gate_row
     const bool gates = G.dgate && (G.gate_column || A.rows == 0);
     if (columns || gates) {
         if (!columns) G.dw = G.db = G.dwf = G.dbf = nullptr;
-        const int64_t y = 4 + (gates ? (A.rows == 0 ? gate_rows : P.segments) : 0);
-        const dim3 grid((unsigned)((A.dim + 15) / 16), (unsigned)y);
-        const unsigned columns_threads = (int64_t)grid.x * grid.y >= 2 * NORM_CUS ? 256 : 1024;
-        hipLaunchKernelGGL(residual_norm_columns_kernel<T>, grid, dim3(columns_threads), 0, st, G, A.dim, blocks, A.w_float);
+        if (!gates) G.dgate = nullptr;
+        const int64_t segments = !gates ? 1 : A.rows == 0 ? gate_rows : P.segments;
+        const dim3 grid((unsigned)((A.dim + 15) / 16), 5, (unsigned)(segments < 64 ? segments : 64));
+        const unsigned columns_threads = (int64_t)grid.x * (4 + grid.z) >= 2 * NORM_CUS ? 256 : 1024;
+        hipLaunchKernelGGL(residual_norm_columns_kernel<T>, grid, dim3(columns_threads), 0, st, G, A.dim, blocks, segments, A.w_float);
     }
 }
 

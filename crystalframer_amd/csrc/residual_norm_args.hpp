@@ -21,6 +21,7 @@ struct NormGrads {
     void *dx, *df, *dgate, *dw, *db, *dwf, *dbf;
     float* column;           // (4, gridDim.x, dim): sums of the workgroups, in the order dw, db, dwf, dbf; NULL: one workgroup, final
     float* gate_column;      // (strips, dim): sums of the strips; NULL: a strip is all that shares its row of the gate, final
+    float* mid;              // (rows, 4): mean u and mean u xhat of N and of N_b, for the column kernel; NULL: column sums with the rows
     int64_t strips;
     int32_t parts;           // strips of the rows that share a row of the gate
 };
@@ -28,10 +29,10 @@ struct NormGrads {
 constexpr int NORM_CUS = 256;
 
 struct NormPlan {
-    int teams, blocks, parts;
-    int64_t segments, strips;
-    bool gate_rows_shared;
-    size_t column_floats, gate_floats;
+    int teams, blocks, parts, column_blocks, column_parts;
+    int64_t segments, strips, column_strips;
+    bool gate_rows_shared, split;       // split: column sums in a kernel of their own: column_blocks workgroups to a group of columns
+    size_t column_floats, gate_floats, mid_floats;
 };
 
 // Threads of a workgroup: for rows of up to 64 pieces of 16 bytes 256, in teams of 16, 32 or 64 lanes with a piece each; else one team of as
@@ -47,24 +48,48 @@ inline int norm_teams(int64_t dim, int elements) {
     return pieces <= 16 ? 16 : pieces <= 32 ? 8 : pieces <= 64 ? 4 : 1;
 }
 
+// Whether the backward pass makes its column sums in a kernel of its own, which reads the rows' arrays again but keeps no lane waiting for
+// another: where one kernel has no registers for both.  These are rows of more than 1024 pieces (4096 x 16384 bfloat16, layer norms on
+// both sides and a gate: 1365 us in one kernel, 424 in two; 4096 x 12288, one norm: 451, 194; 4096 x 8192 float32, gated: 371, 273), and
+// rows in 16 bits, where a lane has eight columns, with both norms, biases and a gate (32768 x 1024: 221, 168; 8192 x 4096: 215, 176;
+// without the gate 114, 129, and root-mean-square norms alone 104, 135: one kernel).
+inline bool norm_split(int64_t dim, int elements, int64_t gate_rows, bool block_norm, bool general) {
+    return dim > 1024 * elements || (elements == 8 && dim > 64 * elements && block_norm && general && gate_rows > 0);
+}
+
 // Strips of rows: as many as there are workgroups at once, but with two rows for each team of a workgroup where there are fewer, and
 // none across two rows of the gate.
-inline NormPlan norm_plan(int64_t rows, int64_t dim, int elements, int64_t gate_rows) {
+inline NormPlan norm_plan(int64_t rows, int64_t dim, int elements, int64_t gate_rows, bool block_norm, bool general) {
     NormPlan P{};
     P.teams = norm_teams(dim, elements);
     P.gate_rows_shared = gate_rows > 0 && gate_rows < rows;
     P.segments = P.gate_rows_shared ? gate_rows : 1;
-    const int64_t resident = 1024 / norm_threads(dim, elements), target = NORM_CUS * (resident < 1 ? 1 : resident), span = rows / P.segments;
-    int64_t strips = rows / (2 * P.teams);
-    strips = strips < 1 ? 1 : strips > target ? target : strips;
-    int64_t parts = strips / P.segments;
-    if (parts < 1) parts = 1;
-    if (parts > span) parts = span > 0 ? span : 1;
-    P.parts = (int)parts;
-    P.strips = P.segments * parts;
+    const int threads = norm_threads(dim, elements);
+    const int64_t resident = 1024 / threads, target = NORM_CUS * (resident < 1 ? 1 : resident), span = rows / P.segments;
+    auto in_parts = [&](int64_t strips, int64_t most) {
+        strips = strips < 1 ? 1 : strips > most ? most : strips;
+        int64_t parts = strips / P.segments;
+        if (parts < 1) parts = 1;
+        if (parts > span) parts = span > 0 ? span : 1;
+        return (int)parts;
+    };
+    P.parts = in_parts(rows / (2 * P.teams), target);
+    P.strips = P.segments * P.parts;
     P.blocks = (int)(P.strips < target ? P.strips : target);
-    P.column_floats = P.blocks > 1 ? (size_t)4 * P.blocks * dim : 0;
-    P.gate_floats = P.gate_rows_shared && P.parts > 1 ? (size_t)P.strips * dim : 0;
+    P.split = norm_split(dim, elements, gate_rows, block_norm, general);
+    P.column_strips = P.strips;
+    P.column_parts = P.parts;
+    P.column_blocks = P.blocks;
+    if (P.split) {
+        const int64_t groups = (dim + 64 * elements - 1) / (64 * elements);
+        const int64_t most = 4 * NORM_CUS / groups;      // (at least 16: there are up to 64 groups)
+        P.column_parts = in_parts(rows / 16, most);
+        P.column_strips = P.segments * P.column_parts;
+        P.column_blocks = (int)(P.column_strips < most ? P.column_strips : most);
+        P.mid_floats = (size_t)rows * 4;
+    }
+    P.column_floats = P.column_blocks > 1 ? (size_t)4 * P.column_blocks * dim : 0;
+    P.gate_floats = P.gate_rows_shared && P.column_parts > 1 ? (size_t)P.column_strips * dim : 0;
     return P;
 }
 

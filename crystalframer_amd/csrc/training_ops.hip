@@ -221,8 +221,9 @@ int cfh_residual_norm_forward(const cfh_residual_norm* a, void* h, void* y, floa
 
 size_t cfh_residual_norm_backward_workspace_bytes(const cfh_residual_norm* a) {
     if (check_norm(a, true)) return 0;
-    const cfh::NormPlan P = cfh::norm_plan(a->rows, a->dim, a->dtype == CFH_FLOAT32 ? 4 : 8, a->gate_rows);
-    return (P.column_floats + P.gate_floats + 4) * sizeof(float);
+    const cfh::NormPlan P = cfh::norm_plan(a->rows, a->dim, a->dtype == CFH_FLOAT32 ? 4 : 8, a->gate_rows, a->block_norm != 0,
+                                           a->norm == CFH_NORM_LAYER || a->block_norm == CFH_NORM_LAYER || a->bias || a->block_bias);
+    return (P.column_floats + P.gate_floats + P.mid_floats + 8) * sizeof(float);
 }
 
 int cfh_residual_norm_backward(const cfh_residual_norm* a, const float* stats, const void* gh, const void* gy, void* dx, void* dblock,

@@ -13,7 +13,7 @@ pytestmark = pytest.mark.gpu
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 
 
-def _make(shape, dtype, wtype, norm, block_norm, gate, block=True, seed=0, offset=0.3):
+def _make(shape, dtype, wtype, norm, block_norm, gate, block=True, seed=0, offset=0.3, biases=False):
     gen = torch.Generator().manual_seed(seed)
     D = shape[-1]
     rnd = lambda s, at, by, t: (at + by * torch.randn(s, generator=gen)).to(t)  # noqa: E731
@@ -24,11 +24,11 @@ def _make(shape, dtype, wtype, norm, block_norm, gate, block=True, seed=0, offse
         k["gate"] = rnd(gate, 0.6, 0.5, dtype)
     if norm:
         k["weight"] = rnd((D,), 1.0, 0.2, wtype)
-        if norm == "layer":
+        if norm == "layer" or biases:
             k["bias"] = rnd((D,), 0.0, 0.2, wtype)
     if block_norm:
         k["block_weight"] = rnd((D,), 1.0, 0.2, wtype)
-        if block_norm == "layer":
+        if block_norm == "layer" or biases:
             k["block_bias"] = rnd((D,), 0.0, 0.2, wtype)
     return k, gen
 
@@ -41,10 +41,10 @@ def _check(got, ref, size, what):
 
 
 def _compare(shape, dtype, wtype=None, norm="layer", block_norm=None, gate=None, keep=True, block=True, scales=(1.0, 1.0), eps=1e-5,
-             seed=0, place=lambda name, t: t.cuda(), train=True):
+             seed=0, place=lambda name, t: t.cuda(), train=True, biases=False):
     from crystalframer_amd import cuda_funcs
     wtype = wtype or dtype
-    tensors, gen = _make(shape, dtype, wtype, norm, block_norm, gate, block, seed)
+    tensors, gen = _make(shape, dtype, wtype, norm, block_norm, gate, block, seed, biases=biases)
     opts = dict(norm=norm, eps=eps, residual_scale=scales[0], block_scale=scales[1], block_norm=block_norm, block_eps=eps)
     dev = {k: place(k, t).requires_grad_(train) for k, t in tensors.items()}
     ref = {k: t.double().requires_grad_(train) for k, t in tensors.items()}
@@ -158,6 +158,54 @@ def test_many_short_sequences():
     _compare((700, 2, 72), F32, norm="layer", gate=(700, 1, 72))
     _compare((350, 3, 2, 72), F32, norm="layer", gate=(350, 3, 1, 72))
     _compare((350, 3, 2, 72), F32, norm="layer", gate=(350, 1, 1, 72))
+
+
+@pytest.mark.parametrize("dim", [1032, 2048])
+def test_short_sequences_of_long_rows(dim):
+    """More rows of a gate than workgroups that add them, in rows whose column sums have a kernel of their own."""
+    _compare((700, 2, dim), BF16, norm="layer", block_norm="layer", gate=(700, 1, dim))
+    _compare((90, 3, dim), F16, F32, norm="layer", block_norm="layer", gate=(90, 1, dim))
+    _compare((130, 3, 16384), BF16, norm="rms", gate=(130, 1, 16384))
+
+
+def test_more_sequences_than_a_grid_is_high():
+    from crystalframer_amd import cuda_funcs
+    B, S, D = 66000, 2, 1032
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    rnd = lambda s, at, by: (at + by * torch.randn(s, generator=gen, device="cuda", dtype=BF16))  # noqa: E731
+    t = dict(x=rnd((B, S, D), 0.3, 1.5), block=rnd((B, S, D), 0.1, 0.8), gate=rnd((B, 1, D), 0.6, 0.5), weight=rnd((D,), 1.0, 0.2), bias=rnd((D,), 0.0, 0.2),
+             block_weight=rnd((D,), 1.0, 0.2), block_bias=rnd((D,), 0.0, 0.2))
+    t = {k: v.requires_grad_() for k, v in t.items()}
+    gy = rnd((B, S, D), 0.1, 1.0)
+    y = cuda_funcs.residual_norm(**t, block_norm="layer", keep_residual=False)
+    dg, dx, db = torch.autograd.grad(y, (t["gate"], t["x"], t["bias"]), gy)
+    _check(db, gy.cpu().double().sum((0, 1)), gy.abs().sum((0, 1), dtype=torch.float32).cpu().double(), ("gradient of bias", BF16))
+    for part in (slice(0, 5), slice(65530, 65540), slice(B - 5, B)):
+        ref = {k: (v.detach()[part] if v.dim() == 3 else v.detach()).cpu().double().requires_grad_() for k, v in t.items()}
+        h, ry = TR.residual_norm(**ref, block_norm="layer")
+        wg, wx = torch.autograd.grad(ry, (ref["gate"], ref["x"]), gy[part].cpu().double())
+        # normed values to 5 deviations, weights to 2, deviations of h from a half on: terms of dh below 2 * 2 * 5 * (1 + 5), of the gate's 10 such
+        _check(dx[part], wx, 120.0, ("gradient of x", BF16))
+        _check(dg[part], wg, 2 * 10 * 120.0, ("gradient of gate", BF16))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("dim", [96, 1032, 16384])
+def test_biases_beside_root_mean_squares(dim, dtype):
+    """Also where their gradients are not wanted: the others' are the same, bit for bit."""
+    from crystalframer_amd import cuda_funcs
+    shape, opts = (9, 4, dim), dict(norm="rms", block_norm="rms")
+    _compare(shape, dtype, gate=(9, 1, dim), biases=True, **opts)
+    for given in (("bias",), ("block_bias",), ("bias", "block_bias")):
+        t, gen = _make(shape, dtype, dtype, "rms", "rms", (9, 1, dim), biases=True)
+        t = {k: v.cuda() for k, v in t.items() if k not in ("bias", "block_bias") or k in given}
+        g = torch.randn(shape, generator=gen).to(dtype).cuda()
+        grads = []
+        for frozen in ((), given):
+            dev = {k: v.detach().clone().requires_grad_(k not in frozen) for k, v in t.items()}
+            wanted = [k for k in t if k not in given]
+            grads.append(torch.autograd.grad(cuda_funcs.residual_norm(**dev, **opts, keep_residual=False), [dev[k] for k in wanted], g))
+        assert all(torch.equal(a, b) for a, b in zip(*grads)), given
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
