@@ -11,6 +11,7 @@
 // The entry points are called through addresses that the Python side hands over: the module does not link the library.
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -411,16 +412,16 @@ cfh_residual_norm norm_args(NormTensors& t, const NormSpec& s) {
 void* raw_stream(const at::Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
 // A gradient of a leaf that an eager graph still holds is accumulated on that graph's stream, which a backward pass under capture must
-// not wait for: that ends the process, so it is refused here, before anything is recorded.
-void check_capture(const NormTensors& t) {
+// not wait for: that ends the process, so it is refused here, before this pass records anything.
+void check_capture(const torch::autograd::Node& node, const c10::Device& device) {
     if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
-    const c10::Stream now = c10::hip::getCurrentHIPStream(t[X].device().index()).unwrap();
-    for (const auto& u : t) {
-        if (!u.defined() || !u.requires_grad() || !u.is_leaf()) continue;
-        const auto node = torch::autograd::impl::try_get_grad_accumulator(u);
-        const auto stream = node ? node->stream() : c10::nullopt;
-        TORCH_CHECK(!stream || *stream == now, "a residual norm is captured while a graph that was made on another stream still holds one of "
-                    "its parameters or inputs: let go of that graph's outputs (a loss, a prediction) first");
+    const c10::StreamId now = c10::hip::getCurrentHIPStream(device.index()).unwrap().id();
+    for (const auto& edge : node.next_edges()) {
+        const auto* const leaf = dynamic_cast<const torch::autograd::AccumulateGrad*>(edge.function.get());
+        if (!leaf) continue;
+        const auto stream = edge.function->stream();
+        TORCH_CHECK(!stream || stream->device_index() != device.index() || stream->id() == now, "the backward pass of a residual norm is captured while a graph that was made on another stream "
+                    "still holds one of its parameters or inputs: let go of that graph's outputs (a loss, a prediction) first");
     }
 }
 
@@ -449,6 +450,7 @@ struct ResidualNormBackward : public torch::autograd::Node {
             if (t[k].defined()) t[k] = t[k].detach();
         }
         c10::DeviceGuard guard(t[X].device());
+        check_capture(*this, t[X].device());
         const bool differentiable = at::GradMode::is_enabled();
         {
             at::AutoDispatchBelowADInplaceOrView below;
@@ -501,7 +503,6 @@ py::object residual_norm(const at::Tensor& x, const c10::optional<at::Tensor>& b
     if (at::GradMode::is_enabled())
         for (const auto& t : inputs) train = train || (t.defined() && t.requires_grad());
     c10::DeviceGuard guard(x.device());
-    if (train) check_capture(inputs);
     NormTensors t = inputs;
     at::Tensor h, y, stats;
     {

@@ -294,6 +294,22 @@ def test_one_output_alone_has_a_gradient():
     assert torch.equal(a, c) and torch.equal(b, d)
 
 
+def test_the_same_tensor_as_stream_and_block():
+    from crystalframer_amd import cuda_funcs
+    x = torch.randn(11, 72, device="cuda", requires_grad=True)
+    g = torch.randn(11, 72, device="cuda")
+    for scales in ((1.0, 1.0), (0.5, 1.25)):
+        opts = dict(residual_scale=scales[0], block_scale=scales[1])
+        both, = torch.autograd.grad(cuda_funcs.residual_norm(x, x, **opts), x, (g, g))
+        a, b = x.detach().clone().requires_grad_(), x.detach().clone().requires_grad_()
+        cuda_funcs.residual_norm(a, b, **opts)[1].backward(g, retain_graph=True)
+        one = a.grad.clone()
+        b.grad.add_(1.0)                         # (the gradients are two tensors, also where they are equal)
+        assert torch.equal(a.grad, one)
+        ga, gb = torch.autograd.grad(cuda_funcs.residual_norm(a, b, **opts), (a, b), (g, g))
+        assert (both - (ga + gb)).abs().max() <= 2.0 ** -23 * (ga.abs() + gb.abs()).max()
+
+
 def test_no_rows():
     from crystalframer_amd import cuda_funcs
     x = torch.zeros(0, 64, device="cuda", requires_grad=True)
@@ -345,7 +361,13 @@ def test_capture_beside_an_eager_graph_of_the_same_leaves_is_refused():
     graph = torch.cuda.CUDAGraph()
     with pytest.raises(RuntimeError, match="let go"):
         with torch.cuda.graph(graph):
-            cuda_funcs.residual_norm(x, None, w, keep_residual=False)
+            cuda_funcs.residual_norm(x, None, w, keep_residual=False).sum().backward()
+    y = []
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):               # (the forward pass alone is nothing to refuse)
+        y.append(cuda_funcs.residual_norm(x, None, w, keep_residual=False).detach())
+    graph.replay()
+    assert torch.equal(y[0], cuda_funcs.residual_norm(x, None, w, keep_residual=False).detach())
     del loss
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
