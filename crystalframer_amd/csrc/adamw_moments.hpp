@@ -16,6 +16,7 @@ namespace cfh {
 constexpr int MOMENT_BLOCK = 64;          // elements that share a scale
 constexpr int PARAM_MAX_JOBS = 88;        // tensors per launch (kernel arguments: 4 KB)
 constexpr int ADAMW_CHUNK = 2048;         // elements per workgroup of 256 threads
+constexpr uint32_t MAX_CHUNKS = 0xffffff;     // workgroups of a launch: a grid counts its threads in 32 bits
 constexpr int ADAMW_FEW = 1024;           // the same where there are not enough of those to go round
 constexpr int64_t CACHED_BYTES = 256LL << 20;      // that the last cache holds
 constexpr int GRAD_NORM_CHUNK = 8192;     // elements per turn of a workgroup of 256 threads: eight (four) loads under way per lane
@@ -110,10 +111,28 @@ __device__ __forceinline__ uint32_t moment_hash(uint32_t x) {
     return x ^ (x >> 15);
 }
 
-// (The hardware's root and reciprocal: each within one unit of the last place of what is a thousandth of the parameter.)
-__device__ __forceinline__ float adamw_update(float p, float m, float v, const AdamWStep& S, float eps) {
-    const float root = __builtin_amdgcn_sqrtf(v) * S.inv_sqrt_bc2 + eps;
-    return p * S.decay - S.step_size * (m * __builtin_amdgcn_rcpf(root));
+// How a chunk is gone through.  WHOLE: all its elements are there; else a lane may find fewer, or none.  STREAM: past the caches.
+// EXACT: see adamw_update.
+template <bool WHOLE_, bool STREAM_, bool EXACT_ = false>
+struct Way {
+    static constexpr bool WHOLE = WHOLE_, STREAM = STREAM_, EXACT = EXACT_;
+};
+// The hardware's root and reciprocal: each within one unit of the last place of what is a thousandth of the parameter.  The root takes
+// what is below 2^-126 for zero: beside an eps of 2^-38 that is no difference (2^-63), beside a smaller one whole functions
+// are called (WAY::EXACT).
+template <typename WAY, typename T, typename M, int E>
+__device__ __forceinline__ void adamw_update(T (&p)[E], const M (&m)[E], const M (&v)[E], const AdamWStep& S, float eps) {
+    if constexpr (WAY::EXACT) {
+#pragma unroll
+        for (int j = 0; j < E; j++)
+            p[j] = from_float<T>(to_float(p[j]) * S.decay - S.step_size * ((float)m[j] / (sqrtf((float)v[j]) * S.inv_sqrt_bc2 + eps)));
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < E; j++) {
+        const float root = __builtin_amdgcn_sqrtf((float)v[j]) * S.inv_sqrt_bc2 + eps;
+        p[j] = from_float<T>(to_float(p[j]) * S.decay - S.step_size * ((float)m[j] * __builtin_amdgcn_rcpf(root)));
+    }
 }
 
 // An 8-bit code without its sign is a double's exponent and mantissa cut to three bits: its bits, moved under the high word's
@@ -174,11 +193,6 @@ CFH_WORDS(8, 2)
 #undef CFH_WORDS
 template <> struct Words<4, 1> { typedef uint32_t type __attribute__((aligned(1))); };
 
-// How a chunk is gone through.  WHOLE: all its elements are there; else a lane may find fewer, or none.  STREAM: past the caches.
-template <bool WHOLE_, bool STREAM_>
-struct Way {
-    static constexpr bool WHOLE = WHOLE_, STREAM = STREAM_;
-};
 // `E` elements of a tensor from `i` on, of which a lane takes care: a block of 64 lies in 64 / E lanes.
 template <typename WAY, typename T, int E>
 __device__ __forceinline__ void load_elements(T (&o)[E], const T* from, uint32_t i, uint32_t n) {
@@ -236,8 +250,8 @@ __device__ __forceinline__ void moments32(const ParamJob& J, uint32_t i, const T
         const float c = to_float(g[j]) * S.clip;
         m[j] = b1 * m[j] + a1 * c;
         v[j] = b2 * v[j] + a2 * c * c;
-        p[j] = from_float<T>(adamw_update(to_float(p[j]), m[j], v[j], S, R.eps));
     }
+    adamw_update<WAY>(p, m, v, S, R.eps);
     store_elements<WAY>(pm, m, i, J.n);
     store_elements<WAY>(pv, v, i, J.n);
 }
@@ -308,8 +322,8 @@ __device__ __forceinline__ void moments8(const ParamJob& J, uint32_t i, const T 
         }
         cm[j / 4] |= ((high_word(m[j]) >> 24 & 128u) | a) << 8 * (j % 4);
         cv[j / 4] |= b << 8 * (j % 4);
-        p[j] = from_float<T>(adamw_update(to_float(p[j]), (float)m[j], (float)v[j], S, R.eps));
     }
+    adamw_update<WAY>(p, m, v, S, R.eps);
     store_codes<WAY, E>(pm, cm, i, J.n);
     store_codes<WAY, E>(pv, cv, i, J.n);
     if (some && i % MOMENT_BLOCK == 0) {
@@ -336,28 +350,28 @@ __device__ __forceinline__ void adamw_chunk(const ParamJob& J, uint32_t base, co
 
 // STREAM: tensors and moments that the last cache does not hold from one step to the next go past it (151 M float32 parameters, 8 bits
 // 430 -> 420 us, 32 bits 764 -> 746); smaller ones stay for who reads them next (25 M bfloat16: the values of the moments 48 -> 36).
-template <int BITS, int CHUNK, bool STREAM>
+template <int BITS, int CHUNK, bool STREAM, bool EXACT>
 __global__ __launch_bounds__(256) void adamw_moments_kernel(const ParamJobs T, const Moments W, const AdamWStep* step,
                                                             const AdamWRates R) {
     const ParamJob& J = job_of(T, blockIdx.x);
     const uint32_t base = (blockIdx.x - J.chunk0) * CHUNK;
     auto run = [&](auto t) {
         using E = decltype(t);
-        if (base + CHUNK <= J.n) adamw_chunk<E, BITS, CHUNK, Way<true, STREAM>>(J, base, W, step, R);
-        else adamw_chunk<E, BITS, CHUNK, Way<false, STREAM>>(J, base, W, step, R);
+        if (base + CHUNK <= J.n) adamw_chunk<E, BITS, CHUNK, Way<true, STREAM, EXACT>>(J, base, W, step, R);
+        else adamw_chunk<E, BITS, CHUNK, Way<false, STREAM, EXACT>>(J, base, W, step, R);
     };
     if (J.dtype == TYPE_F32) run(float());
     else if (J.dtype == TYPE_BF16) run(bf16());
     else run(f16());
 }
 
-// Four elements of one of the moments (blockIdx.y) per lane, nothing of it left in the caches: bound by HBM's writes.  In 32 bits the
+// Four elements from `at` on of one of the moments (blockIdx.y) per lane, nothing of it left in the caches: bound by HBM's writes.  In 32 bits the
 // codes' bits, moved under a float's exponent field, are the values times 2^-120 and 2^-97.
 constexpr int VALUES_CHUNK = 256 * 4;
-__global__ __launch_bounds__(256) void moment_values_kernel(const Moments W, uint64_t size, float* m, float* v) {
+__global__ __launch_bounds__(256) void moment_values_kernel(const Moments W, uint64_t at, uint64_t size, float* m, float* v) {
     typedef float f4 __attribute__((ext_vector_type(4)));
     const bool first = blockIdx.y == 0;
-    const uint64_t e = (uint64_t)blockIdx.x * VALUES_CHUNK + threadIdx.x * 4;
+    const uint64_t e = at + (uint64_t)blockIdx.x * VALUES_CHUNK + threadIdx.x * 4;
     if (e >= size) return;
     const uint8_t* const codes = reinterpret_cast<const uint8_t*>(first ? W.m : W.v) + e;
     float* const out = (first ? m : v) + e;

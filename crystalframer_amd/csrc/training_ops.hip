@@ -41,7 +41,7 @@ void in_tables(const cfh_param_job* jobs, int32_t njobs, int64_t chunk, F launch
         for (int64_t at = 0; at < jobs[j].n; at += JOB_ELEMENTS) {
             const int64_t n = jobs[j].n - at < JOB_ELEMENTS ? jobs[j].n - at : JOB_ELEMENTS, size = jobs[j].dtype == CFH_FLOAT32 ? 4 : 2;
             const int64_t chunks = (n + chunk - 1) / chunk;
-            if (T.njobs == cfh::PARAM_MAX_JOBS || (int64_t)T.chunks + chunks > 0x3fffffff) {
+            if (T.njobs == cfh::PARAM_MAX_JOBS || (int64_t)T.chunks + chunks > cfh::MAX_CHUNKS) {
                 launch(T);
                 T.njobs = 0;
                 T.chunks = 0;
@@ -153,13 +153,17 @@ int cfh_adamw_step_moments(const cfh_param_job* jobs, int32_t njobs, const cfh_m
     if (clip) C = {clip->sums, clip->count, clip->max_norm, clip->norm};
     hipLaunchKernelGGL(cfh::adamw_begin_kernel, dim3(1), dim3(256), 0, st, S, reinterpret_cast<unsigned long long*>(step_dev), lr, beta1, beta2,
                        weight_decay, C);
-    const bool few = elements(jobs, njobs) < 512LL * cfh::ADAMW_CHUNK;
+    const bool exact = R.eps < 0x1p-38f, few = !exact && elements(jobs, njobs) < 512LL * cfh::ADAMW_CHUNK;
     in_tables(jobs, njobs, few ? cfh::ADAMW_FEW : cfh::ADAMW_CHUNK, [&](const cfh::ParamJobs& T) {
         using cfh::adamw_moments_kernel;
-        const auto kernel = state->bits == 8 ? (few ? adamw_moments_kernel<8, cfh::ADAMW_FEW, false>
-                                                : past ? adamw_moments_kernel<8, cfh::ADAMW_CHUNK, true> : adamw_moments_kernel<8, cfh::ADAMW_CHUNK, false>)
-                                             : (few ? adamw_moments_kernel<32, cfh::ADAMW_FEW, false>
-                                                : past ? adamw_moments_kernel<32, cfh::ADAMW_CHUNK, true> : adamw_moments_kernel<32, cfh::ADAMW_CHUNK, false>);
+        auto form = [&](auto bits) {
+            constexpr int BITS = decltype(bits)::value;
+            return exact  ? adamw_moments_kernel<BITS, cfh::ADAMW_CHUNK, false, true>
+                   : few  ? adamw_moments_kernel<BITS, cfh::ADAMW_FEW, false, false>
+                   : past ? adamw_moments_kernel<BITS, cfh::ADAMW_CHUNK, true, false>
+                          : adamw_moments_kernel<BITS, cfh::ADAMW_CHUNK, false, false>;
+        };
+        const auto kernel = state->bits == 8 ? form(std::integral_constant<int, 8>()) : form(std::integral_constant<int, 32>());
         hipLaunchKernelGGL(kernel, dim3(T.chunks), dim3(256), 0, st, T, W, S, R);
     });
     return finish_launch("adamw_step_moments");
@@ -172,9 +176,11 @@ int cfh_adamw_moments(const cfh_moments* state, float* exp_avg, float* exp_avg_s
     if (state->size == 0) return CFH_OK;
     if (!exp_avg || !exp_avg_sq) return fail(CFH_EINVAL, "adamw_moments: exp_avg and exp_avg_sq must not be NULL");
     const cfh::Moments W{state->exp_avg, state->exp_avg_sq, state->exp_avg_scale, state->exp_avg_sq_scale};
-    hipLaunchKernelGGL(cfh::moment_values_kernel, dim3((unsigned)((state->size + cfh::VALUES_CHUNK - 1) / cfh::VALUES_CHUNK), 2), dim3(256), 0,
-                       (hipStream_t)stream, W,
-                       (uint64_t)state->size, exp_avg, exp_avg_sq);
+    for (int64_t at = 0, most = (int64_t)cfh::MAX_CHUNKS * cfh::VALUES_CHUNK; at < state->size; at += most) {
+        const int64_t n = state->size - at < most ? state->size - at : most;
+        hipLaunchKernelGGL(cfh::moment_values_kernel, dim3((unsigned)((n + cfh::VALUES_CHUNK - 1) / cfh::VALUES_CHUNK), 2), dim3(256), 0,
+                           (hipStream_t)stream, W, (uint64_t)at, (uint64_t)state->size, exp_avg, exp_avg_sq);
+    }
     return finish_launch("adamw_moments");
 }
 

@@ -16,7 +16,8 @@ memory and of the traffic (``cfh_adamw_step_moments`` in the C header defines bo
 parameter share a power of two, rounding is stochastic and a function of the step and of the element alone, so that equal
 runs give equal bits).  ``max_grad_norm``: the gradients of all groups are clipped by their common norm, as
 ``torch.nn.utils.clip_grad_norm_`` does before a step (models/regression.py:137-156 of the reference: backward, clip, step), but
-inside the step: the gradients are read once more and not written.  A group of float32 parameters with moments in 32 bits and
+inside the step: the gradients are read once more and not written (``grad_norm``; a captured step has one of its own, written
+by every replay).  The first step, which makes the moments, is taken before a capture.  A group of float32 parameters with moments in 32 bits and
 no clipping takes ``cfh_adamw_step_batch``, anything else ``cfh_adamw_step_moments``.
 """
 import contextlib
@@ -75,6 +76,10 @@ class AdamW(torch.optim.Optimizer):
             for p in ps:
                 if p.dtype not in _lib.ELEMENT_TYPES or not p.is_cuda or p.device != dev:
                     raise RuntimeError("AdamW of crystalframer_amd needs float32 (or bfloat16, float16) parameters on one HIP device")
+            plain = bits == 32 and all(p.dtype == torch.float32 for p in ps)
+            if not (plain and self.max_grad_norm is None) and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the first step of a group makes its moments (every replay would clear them): take it, or load a "
+                                   "state, before the capture")
             offs, total, align = [], 0, _lib.MOMENT_BLOCK
             for p in ps:
                 offs.append(total)
@@ -102,7 +107,7 @@ class AdamW(torch.optim.Optimizer):
                 self.state[p] = own
             st.update(flat, step=step, bits=bits, scratch=zeros(16, torch.float32), offset={id(p): o for p, o in zip(ps, offs)},
                       numel={id(p): p.numel() for p in ps},
-                      legacy=bits == 32 and all(p.dtype == torch.float32 for p in ps))
+                      legacy=plain)
         return st
 
     def _check_loaded(self, ps, bits):
@@ -174,10 +179,13 @@ class AdamW(torch.optim.Optimizer):
             st = self._group_state(group)
             if st is not None:
                 work.append((group, st, self._plan(group, st)))
-        if self.max_grad_norm is not None or not all(st["legacy"] for _, st, _ in work):
-            self._step_moments(lib, work)
-            return loss
+        clipped = self.max_grad_norm is not None
+        typed = [w for w in work if clipped or not w[1]["legacy"]]
+        if typed:
+            self._step_moments(lib, typed)
         for group, st, plan in work:
+            if clipped or not st["legacy"]:
+                continue
             jobs = plan["jobs"]
             m0, v0 = st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr()
             n, keep = plan["native"].fill(ctypes.addressof(jobs), m0, v0), None
@@ -202,6 +210,8 @@ class AdamW(torch.optim.Optimizer):
         for group, st, plan in work:
             jobs = plan.get("param_jobs")
             if jobs is None:
+                if len({id(p) for p in plan["params"]}) != len(plan["params"]):
+                    raise RuntimeError("a parameter is in its group twice")
                 jobs = plan["param_jobs"] = (_lib.CfhParamJob * max(len(plan["params"]), 1))()
             n, keep = plan["native"].fill_params(ctypes.addressof(jobs)), None
             if n < 0:

@@ -52,7 +52,7 @@ def _numbers(ts):
 def _check(opt, params, before, want, ref, bits):
     # The kernel of float32 parameters with 32-bit moments and no clipping takes 1 - beta2 from beta2 in float32, which is off by half
     # of its last place, 2^-25: 2^-25 / (1 - beta2) of what is added to exp_avg_sq, half of that in its root.
-    whole = opt._flat[id(opt.param_groups[0])]["legacy"] and opt.max_grad_norm is None and len(opt.param_groups) == 1
+    whole = opt._flat[id(opt.param_groups[0])]["legacy"] and opt.max_grad_norm is None
     slack = 2.0 ** -25 / (1.0 - HYPER["betas"][1]) if whole else 0.0
     for k, (p, b, w, s) in enumerate(zip(params, _numbers(before), want, ref.states)):
         got = p.detach().cpu().double().numpy().ravel()
@@ -295,6 +295,31 @@ def test_captured_steps_keep_counting(bits):
     assert all(torch.equal(x, y) for x, y in zip(one.moments()[0], two.moments()[0]))
 
 
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("eps", [0.0, 1e-30])
+def test_small_roots_beside_a_small_eps(bits, eps):
+    """exp_avg_sq around 2^-130, where float32 holds 19 bits of it: 2^-19 of the update, and what the other steps round."""
+    from crystalframer_amd import optim
+    p = torch.nn.Parameter(torch.linspace(0.5, 1.0, 200, device="cuda"))
+    g = 1e-18 * (1.0 + torch.arange(200, dtype=torch.float64) % 7 / 7) * (1 - 2 * (torch.arange(200) % 2))
+    p.grad = g.float().cuda()
+    q = p.detach().cpu().double()
+    opt = optim.AdamW([p], lr=3e-3, eps=eps, weight_decay=0.0, state_bits=bits, max_grad_norm=1.0)
+    opt.step()
+    want = q - 3e-3 * g / (g.abs() + eps)
+    assert ((p.detach().cpu().double() - want).abs() <= 8 * 2.0 ** -24 + 3e-3 * 2.0 ** -19).all()
+
+
+def test_a_group_in_float32_is_stepped_alike_beside_others():
+    from crystalframer_amd import optim
+    a, b, c = _params(F32), _params(F32), _params(BF16, seed=1)
+    one, two = optim.AdamW(a, **HYPER), optim.AdamW([dict(params=b), dict(params=c, state_bits=8)], **HYPER)
+    for step in range(3):
+        _grads(a, step), _grads(b, step), _grads(c, step)
+        one.step(), two.step()
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
 def test_elements_beyond_what_one_table_entry_counts():
     from crystalframer_amd import optim
     n = (1 << 30) + 200
@@ -336,6 +361,17 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="state_bits"):
         opt.step()
     opt.param_groups[0]["state_bits"] = 8
+    q = torch.nn.Parameter(torch.zeros(70, device="cuda"))
+    q.grad = torch.ones_like(q)
+    for form in (dict(state_bits=8), dict(max_grad_norm=1.0)):
+        new = optim.AdamW([q], **form)
+        with pytest.raises(RuntimeError, match="before the capture"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                new.step()
+    with pytest.warns(UserWarning):
+        new = optim.AdamW([q, q], state_bits=8)
+    with pytest.raises(RuntimeError, match="twice"):
+        new.step()
     old = p.data
     for other in (torch.zeros(71, device="cuda", dtype=BF16), old.float(), torch.zeros(140, device="cuda", dtype=BF16)[::2]):
         p.grad = None
