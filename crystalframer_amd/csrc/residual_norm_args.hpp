@@ -35,7 +35,7 @@ struct NormPlan {
     size_t column_floats, gate_floats, mid_floats;
 };
 
-// Threads of a workgroup: for rows of up to 64 pieces of 16 bytes 256, in teams of 16, 32 or 64 lanes with a piece each; else one team of as
+// Threads of a workgroup: for rows of up to 64 pieces of 16 bytes 256, in teams of 8, 16, 32 or 64 lanes with a piece each; else one team of as
 // many wavefronts as there are 64 pieces in a row, up to 16, where lanes take two or four.  A piece per lane is what leaves the backward
 // pass, with its column sums, registers for four wavefronts per SIMD.
 inline int norm_threads(int64_t dim, int elements) {
@@ -45,7 +45,7 @@ inline int norm_threads(int64_t dim, int elements) {
 }
 inline int norm_teams(int64_t dim, int elements) {
     const int64_t pieces = (dim + elements - 1) / elements;
-    return pieces <= 16 ? 16 : pieces <= 32 ? 8 : pieces <= 64 ? 4 : 1;
+    return pieces <= 8 ? 32 : pieces <= 16 ? 16 : pieces <= 32 ? 8 : pieces <= 64 ? 4 : 1;
 }
 
 // Whether the backward pass makes its column sums in a kernel of its own, which reads the rows' arrays again but keeps no lane waiting for

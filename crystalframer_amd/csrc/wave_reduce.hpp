@@ -18,10 +18,14 @@ __device__ __forceinline__ float row_min(float x) {
     x = fminf(x, dpp_move<0x140>(x));
     return x;
 }
-__device__ __forceinline__ float row_sum(float x) {
+__device__ __forceinline__ float half_row_sum(float x) {      // over 8 lanes
     x += dpp_move<0xB1>(x);
     x += dpp_move<0x4E>(x);
     x += dpp_move<0x141>(x);
+    return x;
+}
+__device__ __forceinline__ float row_sum(float x) {
+    x = half_row_sum(x);
     x += dpp_move<0x140>(x);
     return x;
 }
