@@ -63,7 +63,7 @@ class KernelManager:
     # much as they gain there (False: inside every backward call)
     DEFER_CORE_WEIGHT_GRADS: bool = True
     COLLECT_STATS: bool = False         # count translations (read with _lib.read_stats)
-    EVENT_LOG = None                    # a list: every library call appends (name, start, end) events
+    EVENT_LOG = None                    # a list: every library call of this module appends (name, start, end) events
     _compiled_for = None
 
 

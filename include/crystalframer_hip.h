@@ -7,7 +7,7 @@
  * it is given (NULL = the default stream) and returns without synchronising.  The return value is
  * 0 on success or a negative CFH_E* code; cfh_last_error() then describes the failure.  The library
  * allocates nothing: scratch memory comes in through the `workspace` argument, whose required
- * size cfh_workspace_bytes() reports.  All floating-point tensors are contiguous float32, all
+ * size cfh_workspace_bytes() reports.  All floating-point tensors are contiguous float32 (but where a dtype is given), all
  * index tensors contiguous int64, exactly as the reference passes them to its kernels.
  *
  * Tensor naming (N atoms, E ordered atom pairs, B crystals, H heads, Dh head dim, K distance bins,
@@ -589,7 +589,8 @@ int cfh_grad_square_sums(const cfh_param_job* jobs, int32_t njobs, double* sums,
  *   backward   gh, gy: gradients of h and y, either may be NULL (zero).  dx, dblock, dgate, dweight, dbias, dblock_weight,
  *              dblock_bias: NULL where they are not wanted; dblock may be dx where both are the same (equal scales, no gate, no
  *              block norm).  joined != 0: `x` holds h, as the forward pass wrote it in float32, and block is not read
- *              (no gate, no block norm).  Column sums are added in a fixed order.
+ *              (no gate, no block norm).  Column sums are added in a fixed order.  No output overlaps an input; workspace:
+ *              aligned to 16 bytes, the call's own until it has run.
  */
 enum { CFH_NORM_NONE = 0, CFH_NORM_LAYER = 1, CFH_NORM_RMS = 2 };
 typedef struct cfh_residual_norm {
