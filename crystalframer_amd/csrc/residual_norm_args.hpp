@@ -52,9 +52,10 @@ inline int norm_teams(int64_t dim, int elements) {
 // another: where one kernel has no registers for both.  These are rows of more than 1024 pieces (4096 x 16384 bfloat16, layer norms on
 // both sides and a gate: 1365 us in one kernel, 424 in two; 4096 x 12288, one norm: 451, 194; 4096 x 8192 float32, gated: 371, 273), and
 // rows in 16 bits, where a lane has eight columns, with both norms, biases and a gate (32768 x 1024: 221, 168; 8192 x 4096: 215, 176;
-// without the gate 114, 129, and root-mean-square norms alone 104, 135: one kernel).
-inline bool norm_split(int64_t dim, int elements, int64_t gate_rows, bool block_norm, bool general) {
-    return dim > 1024 * elements || (elements == 8 && dim > 64 * elements && block_norm && general && gate_rows > 0);
+// without the gate 114, 129, and root-mean-square norms alone 104, 135: one kernel), from 2^20 elements on (both passes in a graph, float16,
+// a gate per element: 4096 x 1001 77, 54; 1021 x 1001 38.6, 37.4; 256 x 4096 29.5, 29.7; 256 x 1001 24.5, 27.8; 64 x 4096 21.9, 25.9).
+inline bool norm_split(int64_t rows, int64_t dim, int elements, int64_t gate_rows, bool block_norm, bool general) {
+    return dim > 1024 * elements || (elements == 8 && dim > 64 * elements && rows * dim >= 1 << 20 && block_norm && general && gate_rows > 0);
 }
 
 // Strips of rows: as many as there are workgroups at once, but with two rows for each team of a workgroup where there are fewer, and
@@ -76,7 +77,7 @@ inline NormPlan norm_plan(int64_t rows, int64_t dim, int elements, int64_t gate_
     P.parts = in_parts(rows / (2 * P.teams), target);
     P.strips = P.segments * P.parts;
     P.blocks = (int)(P.strips < target ? P.strips : target);
-    P.split = norm_split(dim, elements, gate_rows, block_norm, general);
+    P.split = norm_split(rows, dim, elements, gate_rows, block_norm, general);
     P.column_strips = P.strips;
     P.column_parts = P.parts;
     P.column_blocks = P.blocks;

@@ -165,7 +165,19 @@ def test_short_sequences_of_long_rows(dim):
     """More rows of a gate than workgroups that add them, in rows whose column sums have a kernel of their own."""
     _compare((700, 2, dim), BF16, norm="layer", block_norm="layer", gate=(700, 1, dim))
     _compare((90, 3, dim), F16, F32, norm="layer", block_norm="layer", gate=(90, 1, dim))
+    _compare((350, 3, dim), F16, F32, norm="layer", block_norm="layer", gate=(350, 1, dim))
     _compare((130, 3, 16384), BF16, norm="rms", gate=(130, 1, 16384))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dim", [1000, 1001, 1024, 5000])
+def test_gates_over_many_rows_of_16_bits(dim, dtype):
+    """Column sums in a kernel of their own (from 2^20 elements on), for each kind of gate and mixture of norms."""
+    rows = (1 << 20) // dim // 2 + 1
+    for gate in ((dim,), (2, rows, dim), (2, 1, dim)):
+        _compare((2, rows, dim), dtype, norm="layer", block_norm="layer", gate=gate, keep=dim % 2 == 0)
+        _compare((2, rows, dim), dtype, F32, norm="rms", block_norm="layer", gate=gate)
+        _compare((2, rows, dim), dtype, norm=None, block_norm="layer", gate=gate)
 
 
 def test_more_sequences_than_a_grid_is_high():
