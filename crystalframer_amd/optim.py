@@ -126,14 +126,29 @@ class AdamW(torch.optim.Optimizer):
                     raise RuntimeError(f"{name} of a loaded state does not fit a parameter of {p.numel()} elements with moments in {bits} bits")
 
     def load_state_dict(self, state_dict):
-        """Loads like torch.optim.AdamW, then moves the loaded moments into the flat buffers.  A checkpoint brings the options of
-        its groups with it, ``state_bits`` among them."""
-        super().load_state_dict(state_dict)
-        # (the base class gives floating-point states the type of their parameter: the moments keep theirs)
-        saved = [i for group in state_dict["param_groups"] for i in group["params"]]
-        for i, p in zip(saved, (p for group in self.param_groups for p in group["params"])):
-            if i in state_dict["state"]:
-                self.state[p] = dict(state_dict["state"][i])
+        """Loads like torch.optim.AdamW, hooks included, then moves the loaded moments into the flat buffers.  A checkpoint brings the
+        options of its groups with it, ``state_bits`` among them."""
+        given = {}
+
+        def keep(_, state):
+            given.update(state)
+
+        def types_as_given(_):
+            # (the base class gives floating-point parameters' states the type of their parameter: the moments keep theirs)
+            saved = [i for group in given["param_groups"] for i in group["params"]]
+            for i, p in zip(saved, (p for group in self.param_groups for p in group["params"])):
+                own = self.state.get(p) or {}
+                for name, t in (given["state"].get(i) or {}).items():
+                    now = own.get(name)
+                    if torch.is_tensor(t) and torch.is_tensor(now) and now.dtype != t.dtype:
+                        own[name] = t.to(now.device)
+        # between the hooks before the load, whose dict it is, and those after it, which may change the state
+        handles = [self.register_load_state_dict_pre_hook(keep), self.register_load_state_dict_post_hook(types_as_given, prepend=True)]
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for handle in handles:
+                handle.remove()
         self._flat = {}
         for group in self.param_groups:
             self._group_state(group)
