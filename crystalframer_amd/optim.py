@@ -51,10 +51,14 @@ class AdamW(torch.optim.Optimizer):
         self.max_grad_norm = max_grad_norm
         self.grad_norm = None      # of the last step with max_grad_norm: the norm before clipping, a float32 scalar on the device
 
+    def __getstate__(self):
+        # (the flat buffers are made anew from the moments in ``state``, as after a load)
+        return dict(super().__getstate__(), max_grad_norm=self.max_grad_norm, grad_norm=self.grad_norm)
+
     def __setstate__(self, state):
         super().__setstate__(state)
         self.__dict__.setdefault("_flat", {})
-        self.__dict__.setdefault("max_grad_norm", None)
+        self.__dict__.setdefault("max_grad_norm", None)          # (of a copy written without it)
         self.__dict__.setdefault("grad_norm", None)
         for group in self.param_groups:          # (of a checkpoint written without it)
             group.setdefault("state_bits", 32)

@@ -1,4 +1,8 @@
 """Checkpoints and copies of ``optim.AdamW`` on the device: what hooks make of a load reaches the moments that the kernels use."""
+import copy
+import io
+import pickle
+
 import pytest
 import torch
 
@@ -46,3 +50,20 @@ def test_hooks_of_a_load_reach_the_moments(dtype, bits):
     (m, v), = three.moments()
     (m2, v2), = two.moments()
     assert torch.equal(v, v2) and not m[64:64 + 70].any() and torch.equal(m[64 + 128:], m2[64 + 128:])
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_copies_go_on_clipping(bits):
+    a, one = _optimizer(torch.float32, bits, max_grad_norm=0.1)
+    _steps(a, one, (1, 2))
+    file = io.BytesIO()
+    torch.save(one, file)
+    file.seek(0)
+    copies = [copy.deepcopy(one), torch.load(file, weights_only=False)] + ([pickle.loads(pickle.dumps(one))] if bits == 32 else [])
+    for two in copies:
+        assert torch.equal(two.grad_norm, one.grad_norm)
+    _steps(a, one, (3, 4))
+    for two in copies:
+        b = two.param_groups[0]["params"]
+        _steps(b, two, (3, 4))
+        assert all(torch.equal(p, q) for p, q in zip(a, b)) and torch.equal(two.grad_norm, one.grad_norm)

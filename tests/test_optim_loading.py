@@ -1,6 +1,7 @@
 """What ``optim.AdamW`` takes from a checkpoint, and what a copy of the optimizer keeps: looked at on the CPU, where the moments are
 left as the load put them into ``state`` (the flat buffers of the kernels are on a device)."""
 import copy
+import pickle
 
 import pytest
 import torch
@@ -107,3 +108,32 @@ def test_the_hooks_of_a_load_are_the_callers_alone():
     opt = copy.deepcopy(opt)
     opt.load_state_dict(_checkpoint(opt))
     assert calls == ["before", "after"] * 2 + ["before"]
+
+
+def _pickled(opt):
+    return pickle.loads(pickle.dumps(opt))
+
+
+@pytest.mark.parametrize("copied", [copy.deepcopy, _pickled])
+def test_a_copy_clips_as_its_original(copied):
+    _, opt = _optimizer(max_grad_norm=0.5)
+    opt.grad_norm = torch.tensor(3.0)
+    opt.load_state_dict(_checkpoint(opt))
+    other = copied(opt)
+    assert other.max_grad_norm == 0.5 and float(other.grad_norm) == 3.0
+    assert other.param_groups[0]["state_bits"] == 32 and other._flat == {}
+    for p, q in zip(opt.param_groups[0]["params"][:2], other.param_groups[0]["params"]):
+        assert all(_same(opt.state[p][name], other.state[q][name]) for name in TYPES)
+    assert copied(_optimizer()[1]).max_grad_norm is None
+
+
+def test_a_copy_written_without_the_options():
+    _, opt = _optimizer()
+    old = opt.__getstate__()
+    for name in ("max_grad_norm", "grad_norm"):
+        del old[name]
+    for group in old["param_groups"]:
+        del group["state_bits"]
+    new = OnTheHost.__new__(OnTheHost)
+    new.__setstate__(old)
+    assert new.max_grad_norm is None and new.grad_norm is None and new.param_groups[0]["state_bits"] == 32
