@@ -20,6 +20,7 @@ inside the step: the gradients are read once more and not written (``grad_norm``
 by every replay).  The first step, which makes the moments, is taken before a capture.  A group of float32 parameters with moments in 32 bits and
 no clipping takes ``cfh_adamw_step_batch``, anything else ``cfh_adamw_step_moments``.
 """
+import collections
 import contextlib
 import ctypes
 
@@ -52,8 +53,13 @@ class AdamW(torch.optim.Optimizer):
         self.grad_norm = None      # of the last step with max_grad_norm: the norm before clipping, a float32 scalar on the device
 
     def __getstate__(self):
-        # (the flat buffers are made anew from the moments in ``state``, as after a load)
-        return dict(super().__getstate__(), max_grad_norm=self.max_grad_norm, grad_norm=self.grad_norm)
+        # (the flat buffers are made anew from the moments in ``state``, as after a load; 8-bit floats go as bytes: the framework writes
+        # them into a pickle, but does not read them from it)
+        whole = super().__getstate__()
+        state = collections.defaultdict(dict)
+        for p, own in whole["state"].items():
+            state[p] = {name: t.view(torch.uint8) if torch.is_tensor(t) and t.dtype == torch.float8_e4m3fn else t for name, t in own.items()}
+        return dict(whole, state=state, max_grad_norm=self.max_grad_norm, grad_norm=self.grad_norm)
 
     def __setstate__(self, state):
         super().__setstate__(state)
@@ -62,6 +68,10 @@ class AdamW(torch.optim.Optimizer):
         self.__dict__.setdefault("grad_norm", None)
         for group in self.param_groups:          # (of a checkpoint written without it)
             group.setdefault("state_bits", 32)
+        for own in self.state.values():
+            codes = own.get("exp_avg")
+            if "exp_avg_scale" in own and torch.is_tensor(codes) and codes.dtype == torch.uint8:
+                own["exp_avg"] = codes.view(torch.float8_e4m3fn)
 
     def _group_state(self, group):
         """Moments of all parameters of a group in flat buffers and the step word; ``self.state[p]`` holds the

@@ -137,3 +137,16 @@ def test_a_copy_written_without_the_options():
     new = OnTheHost.__new__(OnTheHost)
     new.__setstate__(old)
     assert new.max_grad_norm is None and new.grad_norm is None and new.param_groups[0]["state_bits"] == 32
+
+
+@pytest.mark.parametrize("copied", [copy.deepcopy, _pickled])
+def test_a_copy_has_its_originals_8_bit_moments(copied):
+    _, opt = _optimizer(state_bits=8)
+    opt.load_state_dict(_checkpoint(opt, TYPES_8))
+    other = copied(opt)
+    assert other.param_groups[0]["state_bits"] == 8
+    for p, q in zip(opt.param_groups[0]["params"][:2], other.param_groups[0]["params"]):
+        assert opt.state[p]["exp_avg"].dtype == torch.float8_e4m3fn
+        assert all(_same(opt.state[p][name], other.state[q][name]) for name in TYPES_8)
+    whole = opt.state_dict()
+    assert whole["state"][1]["exp_avg"].dtype == torch.float8_e4m3fn
