@@ -325,7 +325,7 @@ using NormTensors = std::array<at::Tensor, NORM_TENSORS>;
 struct NormSpec {
     int norm, block_norm;
     float eps, block_eps, residual_scale, block_scale;
-    bool keep;
+    bool keep, twice;
 };
 
 int element_type(at::ScalarType t) {
@@ -373,6 +373,8 @@ void check_norm(const NormTensors& t, const NormSpec& s) {
     }
     for (const auto& u : t) TORCH_CHECK(!u.defined() || u.device() == x.device(), "the tensors are on different devices");
     if (t[GATE].defined()) gate_rows(t[GATE], x);
+    TORCH_CHECK_VALUE(!s.twice || (s.norm == CFH_NORM_LAYER && !s.block_norm && !t[GATE].defined() && s.residual_scale == 1.0f && s.block_scale == 1.0f),
+                      "second derivatives are those of a layer norm of x or of x + block");
 }
 
 // t as rows of its last dimension, `stride` elements apart: in place if they lie evenly and their elements next to each other.
@@ -429,6 +431,7 @@ struct ResidualNormBackward : public torch::autograd::Node {
     NormSpec spec;
     bool joined = false;                       // `saved[X]` is h (the last of the outputs that are kept for this)
     std::vector<int64_t> shape;
+    at::ScalarType weight_type = at::kFloat;   // of weight and bias
     std::array<torch::autograd::SavedVariable, NORM_TENSORS> saved;
     at::Tensor stats;
     bool released = false;
@@ -438,6 +441,32 @@ struct ResidualNormBackward : public torch::autograd::Node {
         released = true;
         for (auto& s : saved) s.reset_data();
         stats.reset();
+    }
+    // The same gradients by the framework's operations, which have derivatives of their own: for a backward pass that is recorded
+    // (create_graph) through a layer norm with at most an addition before it.
+    torch::autograd::variable_list differentiable_gradients(const at::Tensor& gh, const at::Tensor& gy) {
+        torch::autograd::variable_list out(NORM_TENSORS);
+        at::Tensor dh = gh;
+        if (gy.defined()) {
+            auto wide = [&](int k) {
+                const at::Tensor t = saved[k].unpack(shared_from_this());
+                return t.defined() ? c10::optional<at::Tensor>(t.to(at::kFloat)) : c10::nullopt;
+            };
+            at::Tensor h = *wide(X);
+            if (const auto block = wide(BLOCK)) h = h + *block;
+            const auto weight = wide(WEIGHT), bias = wide(BIAS);
+            at::Tensor mean, inverse, dweight, dbias, dx;
+            std::tie(std::ignore, mean, inverse) = at::native_layer_norm(h.detach(), {shape.back()}, c10::nullopt, c10::nullopt, spec.eps);
+            std::tie(dx, dweight, dbias) = at::native_layer_norm_backward(
+                gy.to(at::kFloat), h, {shape.back()}, mean, inverse, weight, bias,
+                {task_should_compute_output(X) || task_should_compute_output(BLOCK), task_should_compute_output(WEIGHT), task_should_compute_output(BIAS)});
+            if (dx.defined()) dh = (gh.defined() ? gh.to(at::kFloat) + dx : dx).to(gy.scalar_type());
+            if (dweight.defined()) out[WEIGHT] = dweight.to(weight_type);
+            if (dbias.defined()) out[BIAS] = dbias.to(weight_type);
+        }
+        for (int k : {X, BLOCK})
+            if (task_should_compute_output(k)) out[k] = dh;
+        return out;
     }
     torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
         TORCH_CHECK(!released, "Trying to backward through a residual norm a second time: make the first pass with retain_graph=True");
@@ -452,6 +481,7 @@ struct ResidualNormBackward : public torch::autograd::Node {
         c10::DeviceGuard guard(t[X].device());
         check_capture(*this, t[X].device());
         const bool differentiable = at::GradMode::is_enabled();
+        if (differentiable && spec.twice) return differentiable_gradients(gh, gy);
         {
             at::AutoDispatchBelowADInplaceOrView below;
             const auto options = t[X].options();
@@ -493,10 +523,10 @@ struct ResidualNormBackward : public torch::autograd::Node {
 py::object residual_norm(const at::Tensor& x, const c10::optional<at::Tensor>& block, const c10::optional<at::Tensor>& gate,
                          const c10::optional<at::Tensor>& weight, const c10::optional<at::Tensor>& bias,
                          const c10::optional<at::Tensor>& block_weight, const c10::optional<at::Tensor>& block_bias, int norm, double eps,
-                         int block_norm, double block_eps, double residual_scale, double block_scale, bool keep) {
+                         int block_norm, double block_eps, double residual_scale, double block_scale, bool keep, bool twice) {
     auto given = [](const c10::optional<at::Tensor>& t) { return t ? *t : at::Tensor(); };
     const NormTensors inputs = {x, given(block), given(gate), given(weight), given(bias), given(block_weight), given(block_bias)};
-    const NormSpec s{norm, block_norm, (float)eps, (float)block_eps, (float)residual_scale, (float)block_scale, keep};
+    const NormSpec s{norm, block_norm, (float)eps, (float)block_eps, (float)residual_scale, (float)block_scale, keep, twice};
     check_norm(inputs, s);
     TORCH_CHECK(!(watchers() & WATCHED), "a residual norm is one call of the library: it cannot be traced or transformed");
     bool train = false;
@@ -518,6 +548,8 @@ py::object residual_norm(const at::Tensor& x, const c10::optional<at::Tensor>& b
         auto node = std::shared_ptr<ResidualNormBackward>(new ResidualNormBackward(), torch::autograd::deleteNode);
         node->spec = s;
         node->shape = x.sizes().vec();
+        for (int k : {WEIGHT, BIAS})
+            if (inputs[k].defined()) node->weight_type = inputs[k].scalar_type();
         node->stats = std::move(stats);
         torch::autograd::edge_list edges;
         for (const auto& u : inputs)

@@ -24,7 +24,8 @@ from .params import LatticeformerParams
 # (cuda_funcs.LayerBridgeHIP) when the layers have no layer norm, no active dropout and the ReLU activation.
 FUSED_LAYER_BRIDGE = True
 # Layers with layer norms: the residual addition and the norm behind it in one launch each way (cuda_funcs.residual_norm), to the
-# same values as the modules up to the rounding of float32 sums.  False: torch.nn.LayerNorm and the addition by themselves.
+# same values as the modules up to the rounding of float32 sums, second derivatives included.  False: torch.nn.LayerNorm and the addition by
+# themselves.
 FUSED_RESIDUAL_NORM = True
 
 
@@ -48,14 +49,14 @@ def _norm_is_plain(norm: nn.Module, x: Tensor) -> bool:
 def _normed(norm: nn.Module, x: Tensor) -> Tensor:
     """``norm(x)``."""
     if _norm_is_plain(norm, x):
-        return norms.residual_norm(x, None, norm.weight, norm.bias, eps=norm.eps, keep_residual=False)
+        return norms.residual_norm(x, None, norm.weight, norm.bias, eps=norm.eps, keep_residual=False, twice_differentiable=True)
     return norm(x)
 
 
 def _normed_sum(norm: nn.Module, x: Tensor, block: Tensor, keep_sum: bool = False):
     """``norm(x + block)``; with ``keep_sum`` (x + block, norm(x + block))."""
     if block.dtype == x.dtype and block.shape == x.shape and block.is_cuda and _norm_is_plain(norm, x):
-        return norms.residual_norm(x, block, norm.weight, norm.bias, eps=norm.eps, keep_residual=keep_sum)
+        return norms.residual_norm(x, block, norm.weight, norm.bias, eps=norm.eps, keep_residual=keep_sum, twice_differentiable=True)
     x = x + block
     return (x, norm(x)) if keep_sum else norm(x)
 

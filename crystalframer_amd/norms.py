@@ -22,7 +22,8 @@ def residual_norm(x: torch.Tensor, block: Optional[torch.Tensor] = None, weight:
                   bias: Optional[torch.Tensor] = None, *, norm: Optional[str] = "layer", eps: float = 1e-5,
                   gate: Optional[torch.Tensor] = None, residual_scale: float = 1.0, block_scale: float = 1.0,
                   block_norm: Optional[str] = None, block_weight: Optional[torch.Tensor] = None,
-                  block_bias: Optional[torch.Tensor] = None, block_eps: float = 1e-5, keep_residual: bool = True):
+                  block_bias: Optional[torch.Tensor] = None, block_eps: float = 1e-5, keep_residual: bool = True,
+                  twice_differentiable: bool = False):
     """h = residual_scale x + block_scale gate N_b(block),  y = N(h): the residual stream after a block and its norm for the next.
 
     ``norm``, ``block_norm``: "layer" ((h - mean) / sqrt(var + eps) weight + bias), "rms" (h / sqrt(mean h^2 + eps) weight + bias)
@@ -31,8 +32,9 @@ def residual_norm(x: torch.Tensor, block: Optional[torch.Tensor] = None, weight:
     (B, T, D)).  Returns (h, y); y alone with ``keep_residual`` False; h alone with ``norm`` None.
 
     x, block and gate have one type, float32, bfloat16 or float16, which is that of the results; weights and biases have it too,
-    or float32.  Everything between is in float32, and rounded once.  Up to 16384 channels.  All gradients are there (once: a
-    gradient of a gradient raises), with sums over rows in a fixed order."""
+    or float32.  Everything between is in float32, and rounded once.  Up to 16384 channels.  All gradients are there, with
+    sums over rows in a fixed order; a gradient of a gradient raises, but with ``twice_differentiable`` (a layer norm of x or of x + block):
+    a backward pass that is itself recorded then goes through the framework's operations."""
     global _native
     if _native is None:
         _native = _lib.load_host().residual_norm
@@ -42,4 +44,4 @@ def residual_norm(x: torch.Tensor, block: Optional[torch.Tensor] = None, weight:
     if norm not in kinds or block_norm not in kinds:
         raise ValueError(f"norm {norm!r}, block_norm {block_norm!r}: \"layer\", \"rms\" or None")
     return _native(x, block, gate, weight, bias, block_weight, block_bias, kinds[norm], eps, kinds[block_norm], block_eps, residual_scale,
-                   block_scale, keep_residual)
+                   block_scale, keep_residual, twice_differentiable)
