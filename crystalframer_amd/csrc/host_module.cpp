@@ -346,8 +346,13 @@ int64_t gate_rows(const at::Tensor& gate, const at::Tensor& x) {
                       "leading dimensions none, or those of x up to some dimension and 1 from there on");
 }
 
+// A tensor whose class makes the framework's operations itself: it has no memory of its own (its address is NULL, which the library
+// takes for an argument left out).
+bool wrapped(const at::Tensor& t) { return t.defined() && t.unsafeGetTensorImpl()->is_python_dispatch(); }
+
 void check_norm(const NormTensors& t, const NormSpec& s) {
     const at::Tensor& x = t[X];
+    for (int k = 0; k < NORM_TENSORS; k++) TORCH_CHECK_TYPE(!wrapped(t[k]), NORM_NAMES[k], " is a tensor of a class with operations of its own: one in memory is needed");
     for (const auto& u : t)
         TORCH_CHECK(!u.defined() || u.is_cuda(), "crystalframer_amd operators run on a HIP device only (tensor on ", u.device(),
                     "); there is no CPU path");
@@ -657,6 +662,7 @@ PYBIND11_MODULE(_host, mod) {
     });
     mod.def("residual_norm", &residual_norm);
     mod.def("gate_rows", &gate_rows);
+    mod.def("wrapped", &wrapped);
     mod.attr("abi") = CFH_ABI_VERSION;
     mod.attr("WATCHED") = (int)WATCHED;
     mod.attr("FUNCTION_MODE") = (int)FUNCTION_MODE;

@@ -31,7 +31,7 @@ FUSED_RESIDUAL_NORM = True
 
 def _norm_is_plain(norm: nn.Module, x: Tensor) -> bool:
     """Nobody but the library has to see this norm: a layer norm over the channels of ``x`` as torch makes it, without hooks, a
-    forward of its own, autocast, tracing or modes."""
+    forward of its own, autocast, tracing or modes, of tensors whose class leaves the operations to torch."""
     if not (FUSED_RESIDUAL_NORM and type(norm) is nn.LayerNorm and x.is_cuda and x.dtype in _lib.ELEMENT_TYPES
             and norm.normalized_shape == (x.shape[-1],) and x.shape[-1] <= norms.MAX_DIM):
         return False
@@ -42,8 +42,15 @@ def _norm_is_plain(norm: nn.Module, x: Tensor) -> bool:
     if any(t is not None and (t.dtype not in (x.dtype, torch.float32) or t.device != x.device) for t in (norm.weight, norm.bias)):
         return False
     host = _lib.load_host()
-    return not (host.watchers() & (host.WATCHED | host.FUNCTION_MODE) or torch.is_autocast_enabled("cuda")
-                or torch.autograd.forward_ad._current_level >= 0)
+    if host.watchers() & (host.WATCHED | host.FUNCTION_MODE) or torch.is_autocast_enabled("cuda") or torch.autograd.forward_ad._current_level >= 0:
+        return False
+    return _leave_it_to_torch(x, norm.weight, norm.bias)
+
+
+def _leave_it_to_torch(*tensors) -> bool:
+    """None of the tensors is of a class with operations of its own."""
+    host = _lib.load_host()
+    return not (torch.overrides.has_torch_function(tensors) or any(t is not None and host.wrapped(t) for t in tensors))
 
 
 def _normed(norm: nn.Module, x: Tensor) -> Tensor:
@@ -55,7 +62,7 @@ def _normed(norm: nn.Module, x: Tensor) -> Tensor:
 
 def _normed_sum(norm: nn.Module, x: Tensor, block: Tensor, keep_sum: bool = False):
     """``norm(x + block)``; with ``keep_sum`` (x + block, norm(x + block))."""
-    if block.dtype == x.dtype and block.shape == x.shape and block.is_cuda and _norm_is_plain(norm, x):
+    if block.dtype == x.dtype and block.shape == x.shape and block.is_cuda and _norm_is_plain(norm, x) and _leave_it_to_torch(block):
         return norms.residual_norm(x, block, norm.weight, norm.bias, eps=norm.eps, keep_residual=keep_sum, twice_differentiable=True)
     x = x + block
     return (x, norm(x)) if keep_sum else norm(x)
