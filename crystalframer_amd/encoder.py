@@ -31,7 +31,9 @@ FUSED_RESIDUAL_NORM = True
 
 def _norm_is_plain(norm: nn.Module, x: Tensor) -> bool:
     """Nobody but the library has to see this norm: a layer norm over the channels of ``x`` as torch makes it, without hooks, a
-    forward of its own, autocast, tracing or modes, of tensors whose class leaves the operations to torch."""
+    forward of its own, autocast, tracing, compilation or modes, of tensors whose class leaves the operations to torch."""
+    if torch.compiler.is_compiling():
+        return False
     if not (FUSED_RESIDUAL_NORM and type(norm) is nn.LayerNorm and x.is_cuda and x.dtype in _lib.ELEMENT_TYPES
             and norm.normalized_shape == (x.shape[-1],) and x.shape[-1] <= norms.MAX_DIM):
         return False

@@ -18,3 +18,18 @@ def test_a_class_that_overrides_torchs_functions_sees_the_norm():
         assert torch.allclose(y.as_subclass(torch.Tensor), norm(x + block))
     del Overriding.calls[:]
     assert type(encoder._normed(norm, x.as_subclass(Overriding))) is Overriding and torch.nn.functional.layer_norm in Overriding.calls
+
+
+def test_a_compiled_function_has_the_module_in_its_graph():
+    from crystalframer_amd import encoder
+    norm = torch.nn.LayerNorm(32).cuda()
+    x, block = torch.randn(5, 32, device="cuda", requires_grad=True), torch.randn(5, 32, device="cuda")
+    graphs = []
+
+    def backend(graph, example):
+        graphs.append(str(graph.code))
+        return graph.forward
+    whole = torch.compile(lambda a, b: encoder._normed_sum(norm, encoder._normed(norm, a), b), backend=backend, fullgraph=True)
+    y = whole(x, block)
+    assert len(graphs) == 1 and graphs[0].count("layer_norm(") == 2
+    assert torch.allclose(y, norm(norm(x) + block))
