@@ -7,7 +7,7 @@
 // 952 000 float32 in 65 tensors: 7 us, and 2 to 3 for the launch before.
 //
 // The tensors' addresses travel in the kernel arguments.  What all elements share (the step's bias corrections, its hash
-// key, the clipping factor) is made by a launch of one wavefront before, which also advances the step.
+// key, the clipping factor) is made by a launch of one workgroup before, which also advances the step.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>

@@ -520,8 +520,8 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void residual_norm_backward_ker
     }
 }
 
-// The column sums alone, with the rows' means known (4096 x 16384 bfloat16, layer norms and gate: both kernels 418 us for 0.8 GB once and
-// 0.5 GB a second time): a lane goes down the rows of its strip with a piece of 16 bytes of each array, four
+// The column sums alone, with the rows' means known (4096 x 16384 bfloat16, layer norms on both sides, gate per element: the rows 336 us,
+// the columns 132 for 0.7 GB, 5.1 TB/s): a lane goes down the rows of its strip with a piece of 16 bytes of each array, four
 // wavefronts of a workgroup over the same columns.  Nothing is exchanged before the end.
 template <typename T, bool TAIL, bool BN, int GATE, bool GENERAL>
 __global__ __launch_bounds__(256) void residual_norm_column_kernel(const ResidualNorm A, const NormGrads G) {

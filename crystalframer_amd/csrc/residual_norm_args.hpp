@@ -37,7 +37,9 @@ struct NormPlan {
 
 // Threads of a workgroup: for rows of up to 64 pieces of 16 bytes 256, in teams of 8, 16, 32 or 64 lanes with a piece each; else one team of as
 // many wavefronts as there are 64 pieces in a row, up to 16, where lanes take two or four.  A piece per lane is what leaves the backward
-// pass, with its column sums, registers for four wavefronts per SIMD.
+// pass, with its column sums, registers for four wavefronts per SIMD (128) in float32 and, in 16 bits, for one norm of whole rows;
+// 16-bit rows with both norms spill there: 20 bytes a lane for whole rows and root-mean-square norms with a shared gate, up to 276 for layer norms
+// with a tail and a gate.  Several pieces per lane spill in most forms (up to 476 bytes in 16 bits, 676 in float32).
 inline int norm_threads(int64_t dim, int elements) {
     const int64_t pieces = (dim + elements - 1) / elements;
     if (pieces <= 64) return 256;

@@ -24,8 +24,8 @@ from .params import LatticeformerParams
 # (cuda_funcs.LayerBridgeHIP) when the layers have no layer norm, no active dropout and the ReLU activation.
 FUSED_LAYER_BRIDGE = True
 # Layers with layer norms: the residual addition and the norm behind it in one launch each way (cuda_funcs.residual_norm), to the
-# same values as the modules up to the rounding of float32 sums, second derivatives included.  False: torch.nn.LayerNorm and the addition by
-# themselves.
+# same values as the modules up to the rounding of float32 sums (the sum of 16-bit tensors is not rounded before its norm), second
+# derivatives included.  False: torch.nn.LayerNorm and the addition by themselves.
 FUSED_RESIDUAL_NORM = True
 
 

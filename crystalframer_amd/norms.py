@@ -1,6 +1,6 @@
 """Norms before and after the blocks of a transformer, joined with the residual stream around them.
 
-One launch forward (and two backward) for what the encoder layers with layer norms do between two blocks
+One launch forward and two backward (three where the column sums have a kernel of their own) for what the encoder layers with layer norms do between two blocks
 (reference: models/indexed_latticeformer_encoder.py:848-877, ``torch.nn.LayerNorm`` and additions): the block's output is
 normed itself if asked for, gated, scaled and added to the scaled residual stream, and the sum is normed for what follows.
 Also reachable as ``cuda_funcs.residual_norm``.  The checks, the library's calls and the autograd function are native
