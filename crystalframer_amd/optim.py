@@ -58,7 +58,8 @@ class AdamW(torch.optim.Optimizer):
         whole = super().__getstate__()
         state = collections.defaultdict(dict)
         for p, own in whole["state"].items():
-            state[p] = {name: t.view(torch.uint8) if torch.is_tensor(t) and t.dtype == torch.float8_e4m3fn else t for name, t in own.items()}
+            state[p] = own if not isinstance(own, dict) else {
+                name: t.view(torch.uint8) if torch.is_tensor(t) and t.dtype == torch.float8_e4m3fn else t for name, t in own.items()}
         return dict(whole, state=state, max_grad_norm=self.max_grad_norm, grad_norm=self.grad_norm)
 
     def __setstate__(self, state):
@@ -69,8 +70,8 @@ class AdamW(torch.optim.Optimizer):
         for group in self.param_groups:          # (of a checkpoint written without it)
             group.setdefault("state_bits", 32)
         for own in self.state.values():
-            codes = own.get("exp_avg")
-            if "exp_avg_scale" in own and torch.is_tensor(codes) and codes.dtype == torch.uint8:
+            codes = own.get("exp_avg") if isinstance(own, dict) and "exp_avg_scale" in own else None
+            if torch.is_tensor(codes) and codes.dtype == torch.uint8:
                 own["exp_avg"] = codes.view(torch.float8_e4m3fn)
 
     def _group_state(self, group):

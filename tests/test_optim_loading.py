@@ -150,3 +150,13 @@ def test_a_copy_has_its_originals_8_bit_moments(copied):
         assert all(_same(opt.state[p][name], other.state[q][name]) for name in TYPES_8)
     whole = opt.state_dict()
     assert whole["state"][1]["exp_avg"].dtype == torch.float8_e4m3fn
+
+
+def test_entries_that_belong_to_no_parameter():
+    """The base class hands them through as they are."""
+    ps, opt = _optimizer()
+    whole = _checkpoint(opt)
+    whole["state"]["note"] = 3
+    opt.load_state_dict(whole)
+    assert opt.state["note"] == 3 and _same(opt.state[ps[1]]["exp_avg"], whole["state"][1]["exp_avg"])
+    assert copy.deepcopy(opt).state["note"] == 3
