@@ -662,7 +662,6 @@ PYBIND11_MODULE(_host, mod) {
     });
     mod.def("residual_norm", &residual_norm);
     mod.def("gate_rows", &gate_rows);
-    mod.def("wrapped", &wrapped);
     mod.attr("abi") = CFH_ABI_VERSION;
     mod.attr("WATCHED") = (int)WATCHED;
     mod.attr("FUNCTION_MODE") = (int)FUNCTION_MODE;

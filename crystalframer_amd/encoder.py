@@ -50,9 +50,11 @@ def _norm_is_plain(norm: nn.Module, x: Tensor) -> bool:
 
 
 def _leave_it_to_torch(*tensors) -> bool:
-    """None of the tensors is of a class with operations of its own."""
-    host = _lib.load_host()
-    return not (torch.overrides.has_torch_function(tensors) or any(t is not None and host.wrapped(t) for t in tensors))
+    """None of the tensors is of a class of its own, which may have operations of its own."""
+    for t in tensors:
+        if t is not None and type(t) is not nn.Parameter and type(t) is not Tensor:
+            return False
+    return True
 
 
 def _normed(norm: nn.Module, x: Tensor) -> Tensor:
