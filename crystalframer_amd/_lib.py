@@ -14,7 +14,7 @@ import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libcrystalframer_hip.so")
-ABI_VERSION = 15
+ABI_VERSION = 16
 
 CFH_WINDOW_REFERENCE = 0
 CFH_WINDOW_WIDE = 1
@@ -121,6 +121,20 @@ class CfhResidualNorm(ctypes.Structure):
                 + [(n, ctypes.c_void_p) for n in ("x", "block", "gate", "weight", "bias", "block_weight", "block_bias")])
 
 
+ATTENTION_MAX_REACH = 1024       # CFH_ATTENTION_MAX_REACH
+
+
+class CfhAttention(ctypes.Structure):
+    """Mirror of ``cfh_attention`` in include/crystalframer_hip.h."""
+    _fields_ = ([(n, ctypes.c_int32) for n in ("struct_size", "dtype", "table_dtype", "packed", "causal", "queries_last", "batch", "heads",
+                                               "kv_heads", "dim", "buckets", "reach")]
+                + [("scale", ctypes.c_float), ("reserved0", ctypes.c_int32)]
+                + [(n, ctypes.c_int64) for n in ("query_rows", "key_rows")]
+                + [(n, ctypes.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride")]
+                + [(n, ctypes.c_void_p) for n in ("q", "k", "v", "key_mask", "query_starts", "key_starts", "query_sizes", "key_sizes",
+                                                  "table", "bucket_of")])
+
+
 class CfhModelLayer(ctypes.Structure):
     """Mirror of ``cfh_model_layer`` in include/crystalframer_hip.h."""
     _fields_ = ([("core", CfhParams)]
@@ -170,7 +184,9 @@ EXPORTS = ("cfh_abi_version", "cfh_last_error", "cfh_workspace_bytes", "cfh_fram
            "cfh_fused_core_weight_gradients_workspace_bytes", "cfh_fused_core_weight_gradients",
            "cfh_model_sizes", "cfh_model_forward", "cfh_model_backward",
            "cfh_adamw_step_moments", "cfh_adamw_moments", "cfh_grad_square_sums_count", "cfh_grad_square_sums",
-           "cfh_residual_norm_forward", "cfh_residual_norm_backward_workspace_bytes", "cfh_residual_norm_backward")
+           "cfh_residual_norm_forward", "cfh_residual_norm_backward_workspace_bytes", "cfh_residual_norm_backward",
+           "cfh_attention_forward_workspace_bytes", "cfh_attention_forward", "cfh_attention_backward_workspace_bytes",
+           "cfh_attention_backward")
 
 _lib = None
 _lock = threading.Lock()
@@ -303,6 +319,13 @@ def load():
         lib.cfh_residual_norm_backward_workspace_bytes.argtypes = [_P]
         lib.cfh_residual_norm_backward.restype = ctypes.c_int
         lib.cfh_residual_norm_backward.argtypes = [_P] * 12 + [ctypes.c_size_t, _P]
+        for name in ("cfh_attention_forward_workspace_bytes", "cfh_attention_backward_workspace_bytes"):
+            getattr(lib, name).restype = ctypes.c_size_t
+            getattr(lib, name).argtypes = [_P]
+        lib.cfh_attention_forward.restype = ctypes.c_int
+        lib.cfh_attention_forward.argtypes = [_P] * 4 + [ctypes.c_size_t, _P]
+        lib.cfh_attention_backward.restype = ctypes.c_int
+        lib.cfh_attention_backward.argtypes = [_P] * 10 + [ctypes.c_size_t, _P]
         if lib.cfh_abi_version() != ABI_VERSION:
             raise RuntimeError(f"ABI version {lib.cfh_abi_version()} of {LIB_PATH} != {ABI_VERSION}")
         _lib = lib
@@ -351,6 +374,8 @@ def load_host():
         mod.bind(addr(lib.cfh_model_sizes), addr(lib.cfh_model_forward), addr(lib.cfh_model_backward), addr(lib.cfh_last_error))
         mod.bind_norm(addr(lib.cfh_residual_norm_forward), addr(lib.cfh_residual_norm_backward_workspace_bytes),
                       addr(lib.cfh_residual_norm_backward))
+        mod.bind_attention(addr(lib.cfh_attention_forward_workspace_bytes), addr(lib.cfh_attention_forward),
+                           addr(lib.cfh_attention_backward_workspace_bytes), addr(lib.cfh_attention_backward))
         _host = mod
     return _host
 

@@ -19,7 +19,8 @@ LIB_NAME = "libcrystalframer_hip.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 HOST_PATH = os.path.join(HERE, "_host.so")
 
-LIB_SOURCES = ("crystalframer_hip", "training_ops", "residual_norm_f32", "residual_norm_bf16", "residual_norm_f16")
+LIB_SOURCES = ("crystalframer_hip", "training_ops", "residual_norm_f32", "residual_norm_bf16", "residual_norm_f16",
+               "sequence_attention_ops", "sequence_attention_f32", "sequence_attention_bf16", "sequence_attention_f16")
 
 HIPCC_FLAGS = [
     "-O3", "--offload-arch=gfx950", "-std=c++17", "-fPIC",

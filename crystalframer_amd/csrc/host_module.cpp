@@ -420,14 +420,14 @@ void* raw_stream(const at::Tensor& t) { return (void*)c10::hip::getCurrentHIPStr
 
 // A gradient of a leaf that an eager graph still holds is accumulated on that graph's stream, which a backward pass under capture must
 // not wait for: that ends the process, so it is refused here, before this pass records anything.
-void check_capture(const torch::autograd::Node& node, const c10::Device& device) {
+void check_capture(const torch::autograd::Node& node, const c10::Device& device, const char* what) {
     if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
     const c10::StreamId now = c10::hip::getCurrentHIPStream(device.index()).unwrap().id();
     for (const auto& edge : node.next_edges()) {
         const auto* const leaf = dynamic_cast<const torch::autograd::AccumulateGrad*>(edge.function.get());
         if (!leaf) continue;
         const auto stream = edge.function->stream();
-        TORCH_CHECK(!stream || stream->device_index() != device.index() || stream->id() == now, "the backward pass of a residual norm is captured while a graph that was made on another stream "
+        TORCH_CHECK(!stream || stream->device_index() != device.index() || stream->id() == now, "the backward pass of ", what, " is captured while a graph that was made on another stream "
                     "still holds one of its parameters or inputs: let go of that graph's outputs (a loss, a prediction) first");
     }
 }
@@ -484,7 +484,7 @@ struct ResidualNormBackward : public torch::autograd::Node {
             if (t[k].defined()) t[k] = t[k].detach();
         }
         c10::DeviceGuard guard(t[X].device());
-        check_capture(*this, t[X].device());
+        check_capture(*this, t[X].device(), "a residual norm");
         const bool differentiable = at::GradMode::is_enabled();
         if (differentiable && spec.twice) return differentiable_gradients(gh, gy);
         {
@@ -576,6 +576,229 @@ py::object residual_norm(const at::Tensor& x, const c10::optional<at::Tensor>& b
     return py::make_tuple(py::cast(h), py::cast(y));
 }
 
+// ---- attention between sequences ---------------------------------------------------------------------------------------------------
+struct AttentionLibrary {
+    size_t (*forward_bytes)(const cfh_attention*) = nullptr;
+    int (*forward)(const cfh_attention*, void*, float*, void*, size_t, void*) = nullptr;
+    size_t (*backward_bytes)(const cfh_attention*) = nullptr;
+    int (*backward)(const cfh_attention*, const void*, const float*, const void*, const int64_t*, void*, void*, void*, void*, void*, size_t, void*) = nullptr;
+} g_attention;
+
+enum { QUERY, KEY, VALUE, TABLE, ATTENTION_LEAVES, BUCKETS = ATTENTION_LEAVES, QUERY_STARTS, KEY_STARTS, QUERY_SIZES, KEY_SIZES, KEY_MASK, ATTENTION_TENSORS };
+const char* const ATTENTION_NAMES[ATTENTION_TENSORS] = {"query", "key", "value", "table", "buckets", "query_starts", "key_starts", "query_sizes",
+                                                       "key_sizes", "key_mask"};
+using AttentionTensors = std::array<at::Tensor, ATTENTION_TENSORS>;
+
+struct AttentionSpec {
+    double scale;                              // 0: one over the root of the channels
+    bool causal, last;
+};
+
+void check_attention(const AttentionTensors& t, const AttentionSpec& s) {
+    const at::Tensor &q = t[QUERY], &k = t[KEY], &v = t[VALUE];
+    for (int n = 0; n < ATTENTION_TENSORS; n++)
+        TORCH_CHECK_TYPE(!wrapped(t[n]), ATTENTION_NAMES[n], " is a tensor of a class with operations of its own: one in memory is needed");
+    for (const auto& u : t) {
+        TORCH_CHECK(!u.defined() || u.is_cuda(), "crystalframer_amd operators run on a HIP device only (tensor on ", u.device(),
+                    "); there is no CPU path");
+        TORCH_CHECK(!u.defined() || u.layout() == at::kStrided, "a tensor of layout ", u.layout(), ": strided ones are needed");
+    }
+    TORCH_CHECK_TYPE(element_type(q.scalar_type()) >= 0, "query of ", q.scalar_type(), ": float32, bfloat16 or float16");
+    TORCH_CHECK_TYPE(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), "query of ", q.scalar_type(), ", key of ",
+                     k.scalar_type(), ", value of ", v.scalar_type(), ": they must have one type");
+    TORCH_CHECK_VALUE(q.dim() == 3 || q.dim() == 4, "query of shape ", q.sizes(), ": (rows, heads, channels) of packed sequences, or (batch, positions, heads, channels)");
+    const bool packed = q.dim() == 3;
+    TORCH_CHECK_VALUE(k.dim() == q.dim() && k.sizes() == v.sizes(), "query of shape ", q.sizes(), ", key of shape ", k.sizes(), ", value of shape ", v.sizes());
+    const int64_t H = q.size(-2), G = k.size(-2), D = q.size(-1);
+    TORCH_CHECK_VALUE(k.size(-1) == D && D >= 1 && D <= CFH_ATTENTION_MAX_DIM, "heads of ", D, " and ", k.size(-1), " channels: as many, from 1 to ", CFH_ATTENTION_MAX_DIM);
+    TORCH_CHECK_VALUE(H >= 1 && G >= 1 && H % G == 0, H, " heads of the query, ", G, " of key and value: each of these has to serve as many of those");
+    for (const auto& u : t) TORCH_CHECK(!u.defined() || u.device() == q.device(), "the tensors are on different devices");
+    int64_t batch = 0;
+    if (packed) {
+        TORCH_CHECK_VALUE(t[QUERY_STARTS].defined() && t[KEY_STARTS].defined(), "packed sequences need query_starts and key_starts");
+        TORCH_CHECK_VALUE(!t[QUERY_SIZES].defined() && !t[KEY_SIZES].defined(), "query_sizes and key_sizes are of sequences that are not packed");
+        for (int n : {QUERY_STARTS, KEY_STARTS})
+            TORCH_CHECK_VALUE(t[n].dim() == 1 && t[n].size(0) >= 1 && t[n].size(0) == t[QUERY_STARTS].size(0), ATTENTION_NAMES[n], " of shape ", t[n].sizes(),
+                              ": where each sequence begins and, behind them, where the last ends, for queries and keys alike");
+        batch = t[QUERY_STARTS].size(0) - 1;
+    } else {
+        batch = q.size(0);
+        TORCH_CHECK_VALUE(k.size(0) == batch, "batches of ", batch, " and ", k.size(0), " sequences");
+        TORCH_CHECK_VALUE(!t[QUERY_STARTS].defined() && !t[KEY_STARTS].defined(), "query_starts and key_starts are of packed sequences");
+        for (int n : {QUERY_SIZES, KEY_SIZES})
+            TORCH_CHECK_VALUE(!t[n].defined() || (t[n].dim() == 1 && t[n].size(0) == batch), ATTENTION_NAMES[n], " of shape ", t[n].sizes(), " for ", batch, " sequences");
+    }
+    TORCH_CHECK_VALUE(batch <= 0x7fffffffLL, batch, " sequences");
+    for (int n : {QUERY_STARTS, KEY_STARTS, QUERY_SIZES, KEY_SIZES})
+        TORCH_CHECK_TYPE(!t[n].defined() || t[n].scalar_type() == at::kLong, ATTENTION_NAMES[n], " of ", t[n].scalar_type(), ": int64");
+    if (t[KEY_MASK].defined()) {
+        TORCH_CHECK_TYPE(t[KEY_MASK].scalar_type() == at::kBool, "key_mask of ", t[KEY_MASK].scalar_type(), ": bool, true for keys that are there");
+        TORCH_CHECK_VALUE(t[KEY_MASK].sizes() == k.sizes().slice(0, k.dim() - 2), "key_mask of shape ", t[KEY_MASK].sizes(), " for keys of shape ", k.sizes());
+    }
+    if (t[TABLE].defined()) {
+        const at::Tensor& of = t[BUCKETS];
+        TORCH_CHECK_TYPE(t[TABLE].scalar_type() == q.scalar_type() || t[TABLE].scalar_type() == at::kFloat, "table of ", t[TABLE].scalar_type(),
+                         ": the type of the query, or float32");
+        TORCH_CHECK_VALUE(t[TABLE].dim() == 2 && t[TABLE].size(0) >= 1 && t[TABLE].size(0) <= 65535 && t[TABLE].size(1) == H, "table of shape ",
+                          t[TABLE].sizes(), ": (buckets, ", H, " heads)");
+        TORCH_CHECK_TYPE(of.scalar_type() == at::kInt, "buckets of ", of.scalar_type(), ": int32");
+        TORCH_CHECK_VALUE(of.dim() == 1 && of.size(0) % 2 == 1 && of.size(0) <= 2 * CFH_ATTENTION_MAX_REACH + 1, "buckets of shape ", of.sizes(),
+                          ": one for each relative position from -reach to reach, up to ", CFH_ATTENTION_MAX_REACH);
+    }
+    TORCH_CHECK_VALUE(s.scale == 0.0 || (s.scale > 0.0 && std::isfinite((float)s.scale) && (float)s.scale > 0.0f), "scale ", s.scale, " must be positive and finite");
+}
+
+// t with its channels next to one another.
+at::Tensor with_channels(const at::Tensor& t) { return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+// Strides of (batch, row, head); of a dimension that has one entry, 0.
+void strides_of(const at::Tensor& t, int64_t* out) {
+    const int64_t n = t.dim();
+    for (int64_t d = 0; d < 3; d++) {
+        const int64_t at = n - 4 + d;
+        out[d] = at < 0 || t.size(at) <= 1 ? 0 : t.stride(at);
+    }
+}
+// The library's arguments; `t` becomes the tensors that they point to.
+cfh_attention attention_args(AttentionTensors& t, const AttentionSpec& s) {
+    cfh_attention a;
+    std::memset(&a, 0, sizeof(a));
+    for (int n : {QUERY, KEY, VALUE}) t[n] = with_channels(t[n]);
+    for (int n = TABLE; n < ATTENTION_TENSORS; n++)
+        if (t[n].defined()) t[n] = t[n].contiguous();
+    const at::Tensor &q = t[QUERY], &k = t[KEY];
+    a.struct_size = (int32_t)sizeof(a);
+    a.dtype = a.table_dtype = element_type(q.scalar_type());
+    a.packed = q.dim() == 3;
+    a.causal = s.causal; a.queries_last = s.last;
+    a.batch = (int32_t)(a.packed ? t[QUERY_STARTS].size(0) - 1 : q.size(0));
+    a.heads = (int32_t)q.size(-2); a.kv_heads = (int32_t)k.size(-2); a.dim = (int32_t)q.size(-1);
+    a.scale = s.scale == 0.0 ? (float)(1.0 / std::sqrt((double)a.dim)) : (float)s.scale;
+    a.query_rows = q.size(-3); a.key_rows = k.size(-3);
+    strides_of(q, a.q_stride);
+    strides_of(k, a.k_stride);
+    strides_of(t[VALUE], a.v_stride);
+    auto p = [&](int n) { return t[n].defined() ? t[n].data_ptr() : nullptr; };
+    a.q = p(QUERY); a.k = p(KEY); a.v = p(VALUE);
+    a.key_mask = static_cast<const uint8_t*>(p(KEY_MASK));
+    a.query_starts = static_cast<const int64_t*>(p(QUERY_STARTS)); a.key_starts = static_cast<const int64_t*>(p(KEY_STARTS));
+    a.query_sizes = static_cast<const int64_t*>(p(QUERY_SIZES)); a.key_sizes = static_cast<const int64_t*>(p(KEY_SIZES));
+    if (t[TABLE].defined()) {
+        a.table = p(TABLE);
+        a.table_dtype = element_type(t[TABLE].scalar_type());
+        a.buckets = (int32_t)t[TABLE].size(0);
+        a.reach = (int32_t)(t[BUCKETS].size(0) / 2);
+        a.bucket_of = static_cast<const int32_t*>(p(BUCKETS));
+    }
+    return a;
+}
+
+struct SequenceAttentionBackward : public torch::autograd::Node {
+    AttentionSpec spec;
+    std::array<torch::autograd::SavedVariable, ATTENTION_TENSORS> saved;
+    torch::autograd::SavedVariable out;
+    at::Tensor stats;
+    bool released = false;
+
+    std::string name() const override { return "SequenceAttentionHIPBackward"; }
+    void release_variables() override {
+        released = true;
+        for (auto& s : saved) s.reset_data();
+        out.reset_data();
+        stats.reset();
+    }
+    torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+        TORCH_CHECK(!released, "Trying to backward through an attention a second time: make the first pass with retain_graph=True");
+        torch::autograd::variable_list result(ATTENTION_LEAVES);
+        if (!grads[0].defined()) return result;
+        AttentionTensors t;
+        for (int n = 0; n < ATTENTION_TENSORS; n++) {
+            t[n] = saved[n].unpack();
+            if (t[n].defined()) t[n] = t[n].detach();
+        }
+        const at::Tensor o = out.unpack(shared_from_this()).detach();
+        c10::DeviceGuard guard(o.device());
+        check_capture(*this, o.device(), "an attention");
+        {
+            at::AutoDispatchBelowADInplaceOrView below;
+            const std::array<bool, ATTENTION_LEAVES> wanted = {task_should_compute_output(QUERY), task_should_compute_output(KEY),
+                                                               task_should_compute_output(VALUE), task_should_compute_output(TABLE)};
+            const at::Tensor dq = at::empty(t[QUERY].sizes(), o.options());
+            at::Tensor dk, dv, dtable;
+            if (wanted[KEY] || wanted[VALUE]) {
+                dk = at::empty(t[KEY].sizes(), o.options());
+                dv = at::empty(t[KEY].sizes(), o.options());
+            }
+            if (wanted[TABLE]) dtable = at::empty(t[TABLE].sizes(), t[TABLE].options());
+            const at::Tensor go = with_channels(grads[0].detach());
+            const cfh_attention a = attention_args(t, spec);
+            int64_t go_stride[3];
+            strides_of(go, go_stride);
+            // (scratch of its own for every call: two captured passes never share it)
+            const at::Tensor scratch = bytes(g_attention.backward_bytes(&a), o.device());
+            auto p = [](const at::Tensor& u) { return u.defined() ? u.data_ptr() : nullptr; };
+            check(g_attention.backward(&a, p(o), stats.data_ptr<float>(), p(go), go_stride, p(dq), p(dk), p(dv), p(dtable), scratch.data_ptr(),
+                                       (size_t)scratch.numel(), raw_stream(o)),
+                  "cfh_attention_backward");
+            if (wanted[QUERY]) result[QUERY] = dq;
+            if (wanted[KEY]) result[KEY] = dk;
+            if (wanted[VALUE]) result[VALUE] = dv;
+            if (wanted[TABLE]) result[TABLE] = dtable;
+        }
+        if (at::GradMode::is_enabled()) {      // a gradient of this gradient would be wrong without a word
+            auto error = std::make_shared<torch::autograd::DelayedError>("the gradients of an attention are not differentiable", (int64_t)result.size());
+            torch::autograd::variable_list given = result;
+            for (auto& g : given)
+                if (g.defined()) g = g.detach().requires_grad_(true);
+            given = (*error)(std::move(given));
+            for (size_t n = 0; n < result.size(); n++)
+                if (result[n].defined()) result[n] = given[n];
+        }
+        return result;
+    }
+};
+
+at::Tensor sequence_attention(const at::Tensor& query, const at::Tensor& key, const at::Tensor& value, const c10::optional<at::Tensor>& table,
+                              const c10::optional<at::Tensor>& buckets, const c10::optional<at::Tensor>& query_starts,
+                              const c10::optional<at::Tensor>& key_starts, const c10::optional<at::Tensor>& query_sizes,
+                              const c10::optional<at::Tensor>& key_sizes, const c10::optional<at::Tensor>& key_mask, double scale, bool causal, bool last) {
+    auto given = [](const c10::optional<at::Tensor>& t) { return t ? *t : at::Tensor(); };
+    const AttentionTensors inputs = {query, key, value, given(table), given(buckets), given(query_starts), given(key_starts), given(query_sizes),
+                                     given(key_sizes), given(key_mask)};
+    const AttentionSpec s{scale, causal, last};
+    check_attention(inputs, s);
+    TORCH_CHECK(!(watchers() & WATCHED), "an attention is one call of the library: it cannot be traced or transformed");
+    bool train = false;
+    if (at::GradMode::is_enabled())
+        for (int n = 0; n < ATTENTION_LEAVES; n++) train = train || (inputs[n].defined() && inputs[n].requires_grad());
+    c10::DeviceGuard guard(query.device());
+    AttentionTensors t = inputs;
+    at::Tensor out, stats;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const cfh_attention a = attention_args(t, s);
+        out = at::empty(query.sizes(), query.options().memory_format(at::MemoryFormat::Contiguous));
+        if (train) stats = at::empty({query.numel() / query.size(-1), 2}, query.options().dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous));
+        const size_t need = g_attention.forward_bytes(&a);
+        const at::Tensor scratch = need ? bytes(need, query.device()) : at::Tensor();
+        check(g_attention.forward(&a, out.data_ptr(), train ? stats.data_ptr<float>() : nullptr, need ? scratch.data_ptr() : nullptr, need, raw_stream(query)),
+              "cfh_attention_forward");
+    }
+    if (train) {
+        auto node = std::shared_ptr<SequenceAttentionBackward>(new SequenceAttentionBackward(), torch::autograd::deleteNode);
+        node->spec = s;
+        node->stats = std::move(stats);
+        torch::autograd::edge_list edges;
+        for (int n = 0; n < ATTENTION_LEAVES; n++)
+            edges.push_back(inputs[n].defined() && inputs[n].requires_grad() ? torch::autograd::impl::gradient_edge(inputs[n]) : torch::autograd::Edge());
+        node->set_next_edges(std::move(edges));
+        torch::autograd::set_history(out, node);
+        for (int n = 0; n < ATTENTION_TENSORS; n++)
+            if (inputs[n].defined()) node->saved[n] = torch::autograd::SavedVariable(inputs[n], false);
+        node->out = torch::autograd::SavedVariable(out, true);
+    }
+    return out;
+}
+
 // Addresses of an optimizer's launch: fills the jobs of the parameters that have a gradient.  Returns how many, or -1 when a
 // gradient is one that the Python side has to look at (not contiguous, sparse, another type) or does not fit the moments:
 // the kernel goes over as many words of parameter, gradient and moments as the parameter had when these were made.
@@ -661,6 +884,13 @@ PYBIND11_MODULE(_host, mod) {
         g_norm.backward = reinterpret_cast<decltype(g_norm.backward)>(backward);
     });
     mod.def("residual_norm", &residual_norm);
+    mod.def("bind_attention", [](uintptr_t forward_bytes, uintptr_t forward, uintptr_t backward_bytes, uintptr_t backward) {
+        g_attention.forward_bytes = reinterpret_cast<decltype(g_attention.forward_bytes)>(forward_bytes);
+        g_attention.forward = reinterpret_cast<decltype(g_attention.forward)>(forward);
+        g_attention.backward_bytes = reinterpret_cast<decltype(g_attention.backward_bytes)>(backward_bytes);
+        g_attention.backward = reinterpret_cast<decltype(g_attention.backward)>(backward);
+    });
+    mod.def("sequence_attention", &sequence_attention);
     mod.def("gate_rows", &gate_rows);
     mod.attr("abi") = CFH_ABI_VERSION;
     mod.attr("WATCHED") = (int)WATCHED;

@@ -1,0 +1,1169 @@
+// Attention between the sequences of a batch and those of another, or the same, batch (cross_attention, relative_attention):
+//
+//   t_ij = scale q_i . k_j + table[bucket_of[j - i - shift]],   P_ij = exp(t_ij - m_i) / l_i,   o_i = sum_j P_ij v_j
+//   D_i = do_i . o_i,   ds_ij = P_ij (do_i . v_j - D_i)
+//   dv_j = sum_i P_ij do_i,   dq_i = scale sum_j ds_ij k_j,   dk_j = scale sum_i ds_ij q_i,   dtable[b] = sum over bucket b of ds_ij
+//
+// All products are matrix instructions of 32 x 32 results, 16 (16-bit types) or 2 (float32) terms deep.  A result has its column in
+// the lane (l % 32) and 16 of its rows in the lane's registers: rows 8 (r / 4) + 4 (l / 32) + r % 4.  The scores are made transposed
+// where sums over keys follow (rows: keys, columns: queries), and upright where sums over queries follow: either way the probabilities
+// are, register by register, the right operand of the product that follows, whose terms may come in any order as long as the left
+// operand has them in the same one.  That operand is the transpose of a tile in LDS (16 bits: ds_read_b64_tr_b16; float32: words).
+// Statistics of a row, its largest score and its sum, then live in one lane (two: the halves of the wavefront share a column).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "element_types.hpp"
+#include "sequence_attention_args.hpp"
+#include "wave_reduce.hpp"
+
+namespace cfh {
+namespace attention {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float NONE = -__builtin_inff();
+
+// ---- operands: 8 terms per lane, 16 per step -------------------------------------------------------------------------------------
+template <typename T> struct Operand;
+template <> struct Operand<bf16> {
+    typedef bf16 Eight __attribute__((ext_vector_type(8)));
+    static __device__ __forceinline__ f32x16 product(Eight a, Eight b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Operand<f16> {
+    typedef f16 Eight __attribute__((ext_vector_type(8)));
+    static __device__ __forceinline__ f32x16 product(Eight a, Eight b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Operand<float> {
+    typedef f32x8 Eight;
+    static __device__ __forceinline__ f32x16 product(Eight a, Eight b, f32x16 c) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+        return c;
+    }
+};
+template <typename T> using Eight = typename Operand<T>::Eight;
+
+// Registers 8 s ... 8 s + 7 of a result, rounded to T (half a unit each: 2^-9, 2^-12; float32 stays), as an operand of step s.
+template <typename T>
+__device__ __forceinline__ Eight<T> rounded(const f32x16& x, int s) {
+    Eight<T> y;
+#pragma unroll
+    for (int e = 0; e < 8; e++) y[e] = from_float<T>(x[8 * s + e]);
+    return y;
+}
+// Row of register r of a result, without the lane's 4 (l / 32).
+__device__ __forceinline__ constexpr int result_row(int r) { return 8 * (r / 4) + r % 4; }
+
+// What float16's range takes: powers of a running row, which reach 2^8 (see Running), are lifted by 2^6 and probabilities by 2^15 before
+// they are rounded, so that a term is lost only below 2^-31 of the row's largest, or 2^-40.  A gradient of scores has no bound: it is
+// multiplied by a power of two for each column, which brings the column's largest so far to 2^14 (Scaled).
+template <typename T> constexpr bool NARROW = std::is_same<T, f16>::value;
+template <typename T> constexpr float POWER_LIFT = NARROW<T> ? 6.0f : 0.0f;
+template <typename T> constexpr float P_LIFT = NARROW<T> ? 15.0f : 0.0f;
+
+// ---- tiles in LDS: rows of DP channels in pieces of 16 bytes, whose places are exchanged by the row so that 16 rows of one piece, and
+// the pieces of one transposed read, lie in different banks -------------------------------------------------------------------------
+template <typename T, int DP>
+struct Tile {
+    static constexpr int E = 16 / sizeof(T), PIECES = DP / E, ROW = DP * sizeof(T);
+    static __device__ __forceinline__ int mixed(int row) {
+        if (sizeof(T) == 4) return PIECES >= 16 ? ((row >> 2 & 1) << 3 | (row & 3) << 1 | (row >> 3 & 1)) : (row >> 1 & 7);
+        if (PIECES == 16) return (row & 3) << 2 | (row >> 2 & 3);
+        if (PIECES == 8) return (row >> 1 & 1) << 2 | (row >> 2 & 3);
+        return row >> 2 & 3;
+    }
+    // (base: a multiple of 16)
+    static __device__ __forceinline__ int place(int base, int row, int piece) { return base * ROW + row * ROW + ((piece ^ mixed(row)) << 4); }
+    // Channels 16 step + 8 (l / 32) ... of row base + l % 32.
+    static __device__ __forceinline__ Eight<T> rows(const char* tile, int base, int step, int lane) {
+        const int row = lane & 31, half = lane >> 5;
+        if constexpr (sizeof(T) == 2) {
+            return *reinterpret_cast<const Eight<T>*>(tile + place(base, row, 2 * step + half));
+        } else {
+            const f32x4 a = *reinterpret_cast<const f32x4*>(tile + place(base, row, 4 * step + 2 * half));
+            const f32x4 b = *reinterpret_cast<const f32x4*>(tile + place(base, row, 4 * step + 2 * half + 1));
+            return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+        }
+    }
+    // Channel 32 d + l % 32 of rows base + 8 (e / 4) + 4 (l / 32) + e % 4.
+    static __device__ __forceinline__ Eight<T> columns(const char* tile, int base, int d, int lane) {
+        const int half = lane >> 5;
+        if constexpr (sizeof(T) == 2) {
+            const int row = 4 * half + (lane & 15) / 4, piece = 4 * d + 2 * (lane >> 4 & 1) + (lane & 3) / 2, in = (lane & 1) * 8;
+            auto* a = (__attribute__((address_space(3))) char*)(tile);
+            const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a + place(base, row, piece) + in));
+            const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a + place(base, row + 8, piece) + in));
+            typedef short s16x8 __attribute__((ext_vector_type(8)));
+            return __builtin_bit_cast(Eight<T>, s16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]});
+        } else {
+            f32x8 x;
+            const int c = 32 * d + (lane & 31);
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                x[e] = *reinterpret_cast<const float*>(tile + place(base, 8 * (e / 4) + 4 * half + e % 4, c / 4) + (c % 4) * 4);
+            return x;
+        }
+    }
+};
+
+// ---- rows in memory ------------------------------------------------------------------------------------------------------------------
+// 16 bytes of a row from channel `from` on; channels that the row does not have are 0.
+template <typename T>
+__device__ __forceinline__ uint4 piece_of(const T* row, int from, int dim, int wide) {
+    uint4 x{0, 0, 0, 0};
+    constexpr int E = 16 / sizeof(T);
+    if (wide) {
+        if (from < dim) x = *reinterpret_cast<const uint4*>(row + from);
+    } else {
+        T e[E];
+#pragma unroll
+        for (int n = 0; n < E; n++) e[n] = from + n < dim ? row[from + n] : T(0);
+        __builtin_memcpy(&x, e, 16);
+    }
+    return x;
+}
+// Operand of step `step` straight from memory: channels 16 step + 8 (l / 32) ... of the lane's row.
+template <typename T>
+__device__ __forceinline__ Eight<T> row_operand(const T* row, bool there, int step, int dim, int wide, int lane) {
+    uint4 x[sizeof(T) / 2];
+    constexpr int E = 16 / sizeof(T);
+#pragma unroll
+    for (int n = 0; n < (int)sizeof(T) / 2; n++) {
+        x[n] = uint4{0, 0, 0, 0};
+        if (there) x[n] = piece_of<T>(row, 16 * step + 8 * (lane >> 5) + n * E, dim, wide);
+    }
+    Eight<T> y;
+    __builtin_memcpy(&y, x, sizeof(y));
+    return y;
+}
+
+// ROWS rows on their way into a tile through the registers of THREADS lanes.  A row that is not there is 0 in LDS: what memory holds
+// in its place, infinities and NaN among it, meets no product.
+template <typename T, int DP, int ROWS, int THREADS>
+struct Staged {
+    using L = Tile<T, DP>;
+    static constexpr int ALL = ROWS * L::PIECES, EACH = (ALL + THREADS - 1) / THREADS;
+    uint4 x[EACH];
+    __device__ __forceinline__ void load(const T* first, int64_t stride, int there, const uint8_t* mask, int dim, int wide, int thread) {
+#pragma unroll
+        for (int n = 0; n < EACH; n++) {
+            const int at = thread + n * THREADS, row = at / L::PIECES, piece = at % L::PIECES;
+            x[n] = uint4{0, 0, 0, 0};
+            if (at < ALL && row < there && (!mask || mask[row])) x[n] = piece_of<T>(first + row * stride, piece * L::E, dim, wide);
+        }
+    }
+    __device__ __forceinline__ void store(char* tile, int thread) const {
+#pragma unroll
+        for (int n = 0; n < EACH; n++) {
+            const int at = thread + n * THREADS, row = at / L::PIECES, piece = at % L::PIECES;
+            if (at < ALL) *reinterpret_cast<uint4*>(tile + L::place(row & ~15, row & 15, piece)) = x[n];
+        }
+    }
+};
+
+// Four neighbouring channels of a row (from: a multiple of 4).
+template <typename T>
+__device__ __forceinline__ void put_four(T* row, int from, int dim, f32x4 x) {
+    if ((dim & 3) == 0) {
+        if (from >= dim) return;
+        typedef T Four __attribute__((ext_vector_type(4)));
+        Four y;
+#pragma unroll
+        for (int n = 0; n < 4; n++) y[n] = from_float<T>(x[n]);
+        *reinterpret_cast<Four*>(row + from) = y;
+    } else {
+#pragma unroll
+        for (int n = 0; n < 4; n++)
+            if (from + n < dim) row[from + n] = from_float<T>(x[n]);
+    }
+}
+
+// ---- which rows a workgroup has --------------------------------------------------------------------------------------------------------
+struct Span {
+    int64_t first;      // row of the sequence's first position among all rows
+    int64_t batch;      // index of the sequence in tensors with a batch dimension
+    int there, rows;    // positions; rows to write (those that are no position get 0)
+};
+__device__ __forceinline__ int64_t between(int64_t x, int64_t lo, int64_t hi) { return x < lo ? lo : x > hi ? hi : x; }
+
+// Sequence b of a batch; packed sequence number `batch` is what lies behind the last one.
+__device__ __forceinline__ Span span_of(const int64_t* starts, const int64_t* sizes, int64_t rows, int packed, int batch, int b) {
+    Span s;
+    if (packed) {
+        const int64_t lo = b == 0 ? 0 : between(starts[b], 0, rows), hi = b == batch ? rows : between(starts[b + 1], lo, rows);
+        s.first = lo;
+        s.batch = 0;
+        s.rows = (int)(hi - lo);
+        s.there = b == batch ? 0 : s.rows;
+    } else {
+        s.first = (int64_t)b * rows;
+        s.batch = b;
+        s.rows = (int)rows;
+        s.there = sizes ? (int)between(sizes[b], 0, rows) : (int)rows;
+    }
+    return s;
+}
+// Sequence and first row in it of slot w; false: none.
+__device__ __forceinline__ bool find_slot(const int64_t* starts, int64_t rows, int packed, int batch, int tile, int w, int lane, int& b, int& from) {
+    if (!packed) {
+        const int per = (int)((rows + tile - 1) / tile);
+        b = w / per;
+        from = (w - b * per) * tile;
+        return b < batch;
+    }
+    auto base = [&](int n) { return (n == 0 ? 0 : between(starts[n], 0, rows) / tile) + n; };
+    int lo = 0, n = batch + 1;      // the last of n from lo on whose first slot is not behind w
+    while (n > 1) {
+        const int step = (n + 63) / 64, probe = lane * step;
+        const bool before = probe < n && base(lo + probe) <= w;
+        const int count = __popcll(__ballot(before));
+        const int skip = (count > 0 ? count - 1 : 0) * step;
+        lo += skip;
+        n = n - skip < step ? n - skip : step;
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    b = lo;
+    const int64_t at = (w - base(lo)) * (int64_t)tile;
+    if (at < 0 || at > rows) return false;
+    from = (int)at;
+    return true;
+}
+// Workgroups that follow one another on one of the 8 dies: they share what its cache holds.
+__device__ __forceinline__ int64_t die_order(int64_t id, int64_t count) {
+    const int64_t per = (count + 7) / 8;
+    return (id & 7) * per + (id >> 3);
+}
+
+template <typename T>
+__device__ __forceinline__ const T* row_start(const AttentionRows& r, const Span& s, int packed, int head) {
+    return static_cast<const T*>(r.at) + (packed ? s.first * r.row : s.batch * r.batch) + head * r.head;
+}
+__device__ __forceinline__ int shift_of(const SequenceAttention& A, const Span& q, const Span& k) { return A.last ? k.there - q.there : 0; }
+
+// ---- scores ----------------------------------------------------------------------------------------------------------------------------
+// t is what the maximum is taken of and exp2((t - m) rate) the probability: in 16 bits with a bias t has log2 as its unit (rate 1),
+// in float32 t is the score itself, so that the difference to the maximum is taken before anything is rounded.
+template <typename T, bool BIAS>
+struct Score {
+    static constexpr bool WIDE = sizeof(T) == 4;
+    float in, rate;
+    __device__ __forceinline__ explicit Score(float scale) {
+        in = BIAS ? (WIDE ? scale : scale * LOG2E) : 1.0f;
+        rate = BIAS ? (WIDE ? LOG2E : 1.0f) : scale * LOG2E;
+    }
+    static __device__ __forceinline__ float bias(float x) { return WIDE ? x : x * LOG2E; }
+    __device__ __forceinline__ float t(float s, float b) const { return BIAS ? __builtin_fmaf(s, in, b) : s; }
+    // exp of (t - m) in the score's own unit; `shift` = -m rate
+    __device__ __forceinline__ float power(float t, float m, float shift) const {
+        if (WIDE) return __builtin_amdgcn_exp2f((t - m) * rate);
+        return __builtin_amdgcn_exp2f(BIAS ? t + shift : __builtin_fmaf(t, rate, shift));
+    }
+};
+
+// Biases of one head by relative position in LDS, from -reach - MARGIN to reach + MARGIN: a tile that is not beyond the reach as a whole
+// needs no bounds.
+constexpr int MARGIN = 96;
+template <typename T>
+__device__ __forceinline__ float table_entry(const SequenceAttention& A, int at, int head) {
+    const int b = A.bucket_of[at];
+    if ((unsigned)b >= (unsigned)A.buckets) return 0.0f;
+    const int64_t n = (int64_t)b * A.heads + head;
+    return A.table_float ? static_cast<const float*>(A.table)[n] : to_float(static_cast<const T*>(A.table)[n]);
+}
+__device__ __forceinline__ int clamped(int r, int reach) { return (r < -reach ? -reach : r > reach ? reach : r) + reach; }
+template <typename T, bool BIAS>
+__device__ __forceinline__ void fill_line(const SequenceAttention& A, int head, float* line, int thread, int threads) {
+    for (int n = thread; n <= 2 * (A.reach + MARGIN); n += threads)
+        line[n] = Score<T, BIAS>::bias(table_entry<T>(A, clamped(n - A.reach - MARGIN, A.reach), head));
+}
+
+__device__ __forceinline__ float other_half_max(float x) { float a, b; swap32(x, a, b); return fmaxf(a, b); }
+__device__ __forceinline__ float other_half_sum(float x) { float a, b; swap32(x, a, b); return a + b; }
+
+// Which of the 32 keys of a tile are there, as the bits of a word.
+__device__ __forceinline__ uint32_t keys_there(int left, const uint8_t* mask, int lane) {
+    const int j = lane & 31;
+    return (uint32_t)__ballot(lane < 32 && j < left && (!mask || mask[j]));
+}
+
+// Running maximum, sum and weighted sum of one column.  The maximum that the powers are relative to follows the true one when that is
+// more than 2^8 ahead: the sums are scaled anew in few tiles only, and no power is above 2^8.
+template <int DP>
+struct Running {
+    float m = NONE, l = 0.0f;
+    f32x16 o[DP / 32];
+    __device__ __forceinline__ Running() {
+#pragma unroll
+        for (int d = 0; d < DP / 32; d++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
+    }
+    __device__ __forceinline__ void meet(float top, float rate) {
+        const bool ahead = (top - m) * rate > 8.0f;      // (no for -inf against -inf)
+        if (!__any(ahead)) return;
+        const float by = ahead ? __builtin_amdgcn_exp2f((m - top) * rate) : 1.0f;
+        m = ahead ? top : m;
+        l *= by;
+#pragma unroll
+        for (int d = 0; d < DP / 32; d++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) o[d][r] *= by;
+    }
+    __device__ __forceinline__ float base() const { return m == NONE ? 0.0f : m; }
+};
+
+// Gradients of scores on their way into a product whose sums `sum` are per column (see NARROW).
+template <typename T, int DP>
+struct Scaled {
+    float by = 1.0f;
+    bool met = false;
+    __device__ __forceinline__ void meet(f32x16& ds, f32x16* sum) {
+        if (!NARROW<T>) return;
+        float top = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; r++) top = fmaxf(top, fabsf(ds[r]));
+        top = other_half_max(top);
+        const bool ahead = top < __builtin_inff() && (met ? top * by >= 32768.0f : top > 0.0f);
+        if (__any(ahead)) {
+            const int e = (int)(__float_as_uint(top) >> 23);                                  // 2^(e - 127) <= top
+            const int to = 2 * 127 + 14 - e;
+            const float next = ahead ? __uint_as_float((uint32_t)(to > 253 ? 253 : to < 1 ? 1 : to) << 23) : by;
+            const float change = met ? next / by : 1.0f;                                      // (nothing but 0 is there before)
+#pragma unroll
+            for (int d = 0; d < DP / 32; d++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) sum[d][r] *= change;
+            by = next;
+            met = met || ahead;
+        }
+#pragma unroll
+        for (int r = 0; r < 16; r++) ds[r] *= by;
+    }
+    __device__ __forceinline__ float back() const { return NARROW<T> ? 1.0f / by : 1.0f; }
+};
+
+// Scores of 32 keys (rows) and 32 queries (columns) as t, without those that are masked.  bias(r): of register r.
+template <typename T, bool BIAS, typename F>
+__device__ __forceinline__ void scores(f32x16& s, const Score<T, BIAS>& score, uint32_t there, bool causal, int last, int lane, F bias) {
+    const int half4 = (lane >> 5) * 4;
+    if (BIAS)
+#pragma unroll
+        for (int r = 0; r < 16; r++) s[r] = score.t(s[r], bias(r));
+    if (there != 0xffffffffu) {
+        const uint32_t mine = there >> half4;
+#pragma unroll
+        for (int r = 0; r < 16; r++) s[r] = mine >> result_row(r) & 1 ? s[r] : NONE;
+    }
+    if (causal) {       // keys up to number `last` of the tile
+        const int mine = last - half4;
+#pragma unroll
+        for (int r = 0; r < 16; r++) s[r] = result_row(r) <= mine ? s[r] : NONE;
+    }
+}
+
+// ---- few queries: the keys in parts -----------------------------------------------------------------------------------------------------
+// 32 columns are (query, head of one key head): single tokens of shared heads fill them together.  Every wavefront goes through keys of
+// its own, in tiles of 32 that it alone puts into LDS and reads (no barrier in the loop), and the wavefronts' sums are joined at the end;
+// so are, by combine_parts, those of `splits` workgroups.  Bound by the bytes of keys and values for single tokens.
+template <typename T>
+__device__ __forceinline__ int heads_at_once(int share) { return share < 32 ? share : 32; }
+
+template <typename T, int DP, int NW>
+struct FewLds {
+    static constexpr int TILE = 32 * Tile<T, DP>::ROW, SUM = 32 * (DP + 4) * 4;
+    static constexpr int EACH = 2 * TILE > SUM ? 2 * TILE : SUM;
+    char wave[NW][EACH];
+    float m[NW][32], l[NW][32];
+};
+
+template <typename T, int DP, int NW, bool BIAS>
+__global__ __launch_bounds__(NW * 64) void few_kernel(SequenceAttention A, T* out, float* stats, float* part_o, float* part_ml, int splits) {
+    using L = Tile<T, DP>;
+    __shared__ __attribute__((aligned(16))) FewLds<T, DP, NW> S;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const int at_once = heads_at_once<T>(A.share), groups = (A.share + at_once - 1) / at_once, tile = 32 / at_once;
+    int b, i0;
+    if (!find_slot(A.q_starts, A.q_rows, A.packed, A.batch, tile, blockIdx.x, lane, b, i0)) return;
+    const Span q = span_of(A.q_starts, A.q_sizes, A.q_rows, A.packed, A.batch, b);
+    if (i0 >= q.rows) return;
+    Span k{0, 0, 0, 0};
+    if (!A.packed || b < A.batch) k = span_of(A.k_starts, A.k_sizes, A.k_rows, A.packed, A.batch, b);
+    const int kh = blockIdx.y / groups, h0 = kh * A.share + (blockIdx.y % groups) * at_once;
+    const int column = lane & 31, i = i0 + column / at_once, h = h0 + column % at_once;
+    const bool mine = column / at_once < tile && i < q.there && h < (kh + 1) * A.share;
+    const int shift = shift_of(A, q, k);
+    const Score<T, BIAS> score(A.scale);
+
+    // the tiles of this split that any of the queries sees
+    const int i_last = min(i0 + tile, q.there) - 1;
+    int seen = i0 < q.there ? k.there : 0;
+    if (A.causal) seen = min(seen, i_last + shift + 1);
+    const int tiles = seen > 0 ? (seen + 31) / 32 : 0;
+    const int first = (int)((int64_t)tiles * blockIdx.z / splits), end = (int)((int64_t)tiles * (blockIdx.z + 1) / splits);
+
+    Eight<T> qf[DP / 16];
+    const T* const q_row = row_start<T>(A.q, q, A.packed, mine ? h : 0) + (mine ? i : 0) * A.q.row;
+#pragma unroll
+    for (int s = 0; s < DP / 16; s++) qf[s] = row_operand<T>(q_row, mine, s, A.dim, A.q.wide, lane);
+    const T* const k_at = row_start<T>(A.k, k, A.packed, kh);
+    const T* const v_at = row_start<T>(A.v, k, A.packed, kh);
+    const uint8_t* const mask = A.mask ? A.mask + k.first : nullptr;
+    float far[2] = {0.0f, 0.0f};
+    if (BIAS && mine) {
+        far[0] = Score<T, BIAS>::bias(table_entry<T>(A, 0, h));
+        far[1] = Score<T, BIAS>::bias(table_entry<T>(A, 2 * A.reach, h));
+    }
+    char* const kt = S.wave[wave];
+    char* const vt = kt + FewLds<T, DP, NW>::TILE;
+    Running<DP> sum;
+    Staged<T, DP, 32, 64> kx, vx;
+    auto fetch = [&](int n) {
+        const int j0 = n * 32;
+        const uint8_t* const m = mask ? mask + j0 : nullptr;
+        kx.load(k_at + j0 * A.k.row, A.k.row, k.there - j0, m, A.dim, A.k.wide, lane);
+        vx.load(v_at + j0 * A.v.row, A.v.row, k.there - j0, m, A.dim, A.v.wide, lane);
+    };
+    if (first + wave < end) fetch(first + wave);
+    for (int n = first + wave; n < end; n += NW) {
+        const int j0 = n * 32;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        kx.store(kt, lane);
+        vx.store(vt, lane);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const uint32_t there = keys_there(k.there - j0, mask ? mask + j0 : nullptr, lane);
+        if (n + NW < end) fetch(n + NW);
+        f32x16 s;
+#pragma unroll
+        for (int r = 0; r < 16; r++) s[r] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < DP / 16; c++) s = Operand<T>::product(L::rows(kt, 0, c, lane), qf[c], s);
+        const int low = j0 - i_last - shift, high = j0 + 31 - i0 - shift;      // relative positions of the tile
+        const int r0 = j0 + 4 * half - i - shift;
+        const bool causal = A.causal && high > 0;
+        if (!BIAS || low >= A.reach || high <= -A.reach) {
+            const float flat = low >= A.reach ? far[1] : far[0];
+            scores<T, BIAS>(s, score, there, causal, i + shift - j0, lane, [&](int) { return flat; });
+        } else {
+            scores<T, BIAS>(s, score, there, causal, i + shift - j0, lane, [&](int r) {
+                return mine ? Score<T, BIAS>::bias(table_entry<T>(A, clamped(r0 + result_row(r), A.reach), h)) : 0.0f;
+            });
+        }
+        float top = s[0];
+#pragma unroll
+        for (int r = 1; r < 16; r++) top = fmaxf(top, s[r]);
+        sum.meet(other_half_max(top), score.rate);
+        const float m = sum.base(), off = POWER_LIFT<T> - m * score.rate;
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            s[r] = score.power(s[r], m, off);
+            sum.l += s[r];
+        }
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            const Eight<T> p = rounded<T>(s, c);
+#pragma unroll
+            for (int d = 0; d < DP / 32; d++) sum.o[d] = Operand<T>::product(L::columns(vt, 16 * c, d, lane), p, sum.o[d]);
+        }
+    }
+    // the wavefronts' sums, side by side in LDS
+    __syncthreads();
+    sum.l = other_half_sum(sum.l);
+    float* const mine_o = reinterpret_cast<float*>(S.wave[wave]);
+#pragma unroll
+    for (int d = 0; d < DP / 32; d++)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4)
+            *reinterpret_cast<f32x4*>(mine_o + column * (DP + 4) + 32 * d + result_row(r) + 4 * half) =
+                f32x4{sum.o[d][r], sum.o[d][r + 1], sum.o[d][r + 2], sum.o[d][r + 3]};
+    if (half == 0) {
+        S.m[wave][column] = sum.m;
+        S.l[wave][column] = sum.l;
+    }
+    __syncthreads();
+    const int fours = (A.dim + 3) / 4;
+    for (int n = threadIdx.x; n < 32 * fours; n += NW * 64) {
+        const int c = n / fours, from = (n - c * fours) * 4, ci = i0 + c / at_once, ch = h0 + c % at_once;
+        if (c / at_once >= tile || ci >= q.rows || ch >= (kh + 1) * A.share) continue;
+        float m = NONE, l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; w++) m = fmaxf(m, S.m[w][c]);
+        f32x4 o{0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            const float by = S.m[w][c] == NONE ? 0.0f : __builtin_amdgcn_exp2f((S.m[w][c] - m) * score.rate);
+            l += by * S.l[w][c];
+            o += by * *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(S.wave[w]) + c * (DP + 4) + from);
+        }
+        if (ci >= q.there) {
+            m = NONE;
+            l = 0.0f;
+            o = f32x4{0, 0, 0, 0};
+        }
+        const int64_t row = (q.first + ci) * A.heads + ch;
+        if (splits > 1) {
+            const int64_t rows = (A.packed ? A.q_rows : A.q_rows * A.batch) * A.heads, at = blockIdx.z * rows + row;
+            *reinterpret_cast<f32x4*>(part_o + at * DP + from) = o;
+            if (from == 0) {
+                part_ml[2 * at] = m;
+                part_ml[2 * at + 1] = l;
+            }
+            continue;
+        }
+        const float inverse = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+        put_four<T>(out + row * A.dim, from, A.dim, o * inverse);
+        if (stats && from == 0) {
+            stats[2 * row] = m == NONE ? -NONE : m;
+            stats[2 * row + 1] = inverse * (NARROW<T> ? 0x1p6f : 1.0f);
+        }
+    }
+}
+
+// Joins the splits: 8 rows to a workgroup, 32 lanes to a row.
+template <typename T, int DP, bool BIAS>
+__global__ __launch_bounds__(256) void combine_parts(SequenceAttention A, const float* part_o, const float* part_ml, int splits, int64_t rows, T* out,
+                                                     float* stats) {
+    const int64_t row = blockIdx.x * 8LL + threadIdx.x / 32;
+    const int from = (threadIdx.x & 31) * 4;
+    if (row >= rows || from >= DP) return;
+    const Score<T, BIAS> score(A.scale);
+    float m = NONE, l = 0.0f;
+    for (int z = 0; z < splits; z++) m = fmaxf(m, part_ml[2 * (z * rows + row)]);
+    f32x4 o{0, 0, 0, 0};
+    for (int z = 0; z < splits; z++) {
+        const float mz = part_ml[2 * (z * rows + row)];
+        const float by = mz == NONE ? 0.0f : __builtin_amdgcn_exp2f((mz - m) * score.rate);
+        l += by * part_ml[2 * (z * rows + row) + 1];
+        if (from < A.dim) o += by * *reinterpret_cast<const f32x4*>(part_o + (z * rows + row) * DP + from);
+    }
+    const float inverse = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+    if (from < A.dim) put_four<T>(out + row * A.dim, from, A.dim, o * inverse);
+    if (stats && from == 0) {
+        stats[2 * row] = m == NONE ? -NONE : m;
+        stats[2 * row + 1] = inverse * (NARROW<T> ? 0x1p6f : 1.0f);
+    }
+}
+
+// ---- many queries: tiles of keys shared by the wavefronts of a workgroup ------------------------------------------------------------------
+template <typename T, int NW>
+constexpr int keys_at_once() { return sizeof(T) == 2 && NW >= 4 ? 64 : 32; }
+
+template <typename T, int DP, int NW, bool BIAS>
+__global__ __launch_bounds__(NW * 64) void tiles_kernel(SequenceAttention A, T* out, float* stats, int64_t slots) {
+    using L = Tile<T, DP>;
+    constexpr int KEYS = keys_at_once<T, NW>(), TILE = KEYS * L::ROW;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    char* const tiles = lds;                    // two pairs of a tile of keys and one of values
+    float* const line = reinterpret_cast<float*>(lds + 4 * TILE);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, column = lane & 31;
+    const int64_t id = die_order(blockIdx.x, slots * A.heads);
+    if (id >= slots * A.heads) return;
+    const int h = (int)(id / slots), slot = (int)(id - h * slots), kh = h / A.share;
+    int b, from;
+    if (!find_slot(A.q_starts, A.q_rows, A.packed, A.batch, NW * 32, slot, lane, b, from)) return;
+    const Span q = span_of(A.q_starts, A.q_sizes, A.q_rows, A.packed, A.batch, b);
+    if (from >= q.rows) return;
+    Span k{0, 0, 0, 0};
+    if (!A.packed || b < A.batch) k = span_of(A.k_starts, A.k_sizes, A.k_rows, A.packed, A.batch, b);
+    const int i0 = from + wave * 32, i = i0 + column;
+    const bool mine = i < q.there;
+    const int shift = shift_of(A, q, k);
+    const Score<T, BIAS> score(A.scale);
+    int seen = from < q.there ? k.there : 0;
+    if (A.causal) seen = min(seen, min(from + NW * 32, q.there) + shift);
+    const int count = seen > 0 ? (seen + KEYS - 1) / KEYS : 0;
+
+    Eight<T> qf[DP / 16];
+    const T* const q_row = row_start<T>(A.q, q, A.packed, h) + (mine ? i : 0) * A.q.row;
+#pragma unroll
+    for (int s = 0; s < DP / 16; s++) qf[s] = row_operand<T>(q_row, mine, s, A.dim, A.q.wide, lane);
+    const T* const k_at = row_start<T>(A.k, k, A.packed, kh);
+    const T* const v_at = row_start<T>(A.v, k, A.packed, kh);
+    const uint8_t* const mask = A.mask ? A.mask + k.first : nullptr;
+    if (BIAS) fill_line<T, BIAS>(A, h, line, threadIdx.x, NW * 64);
+    Running<DP> sum;
+    Staged<T, DP, KEYS, NW * 64> kx, vx;
+    auto fetch = [&](int n) {
+        const int j0 = n * KEYS;
+        const uint8_t* const m = mask ? mask + j0 : nullptr;
+        kx.load(k_at + j0 * A.k.row, A.k.row, k.there - j0, m, A.dim, A.k.wide, threadIdx.x);
+        vx.load(v_at + j0 * A.v.row, A.v.row, k.there - j0, m, A.dim, A.v.wide, threadIdx.x);
+    };
+    auto put = [&](int n) {
+        kx.store(tiles + (n & 1) * 2 * TILE, threadIdx.x);
+        vx.store(tiles + (n & 1) * 2 * TILE + TILE, threadIdx.x);
+    };
+    if (count > 0) {
+        fetch(0);
+        put(0);
+    }
+    __syncthreads();
+    for (int n = 0; n < count; n++) {
+        const char* const kt = tiles + (n & 1) * 2 * TILE;
+        const char* const vt = kt + TILE;
+        if (n + 1 < count) fetch(n + 1);
+        f32x16 s[KEYS / 32];
+        float top = NONE;
+#pragma unroll
+        for (int u = 0; u < KEYS / 32; u++) {
+            const int j0 = n * KEYS + 32 * u;
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[u][r] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < DP / 16; c++) s[u] = Operand<T>::product(L::rows(kt, 32 * u, c, lane), qf[c], s[u]);
+            const uint32_t there = keys_there(k.there - j0, mask ? mask + j0 : nullptr, lane);
+            const int low = j0 - (i0 + 31) - shift, high = j0 + 31 - i0 - shift;
+            const bool causal = A.causal && high > 0;
+            if (!BIAS || low >= A.reach || high <= -A.reach) {
+                const float flat = BIAS ? line[low >= A.reach ? 2 * (A.reach + MARGIN) : 0] : 0.0f;
+                scores<T, BIAS>(s[u], score, there, causal, i + shift - j0, lane, [&](int) { return flat; });
+            } else {
+                const float* const at = line + (j0 + 4 * half - i - shift + A.reach + MARGIN);
+                scores<T, BIAS>(s[u], score, there, causal, i + shift - j0, lane, [&](int r) { return at[result_row(r)]; });
+            }
+#pragma unroll
+            for (int r = 0; r < 16; r++) top = fmaxf(top, s[u][r]);
+        }
+        sum.meet(other_half_max(top), score.rate);
+        const float m = sum.base(), off = POWER_LIFT<T> - m * score.rate;
+#pragma unroll
+        for (int u = 0; u < KEYS / 32; u++) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                s[u][r] = score.power(s[u][r], m, off);
+                sum.l += s[u][r];
+            }
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                const Eight<T> p = rounded<T>(s[u], c);
+#pragma unroll
+                for (int d = 0; d < DP / 32; d++) sum.o[d] = Operand<T>::product(L::columns(vt, 32 * u + 16 * c, d, lane), p, sum.o[d]);
+            }
+        }
+        if (n + 1 < count) put(n + 1);
+        __syncthreads();
+    }
+    if (i >= q.rows) return;
+    const float l = other_half_sum(sum.l);
+    const float inverse = mine && (l > 0.0f || l != l) ? 1.0f / l : 0.0f;
+    const int64_t row = (q.first + i) * A.heads + h;
+#pragma unroll
+    for (int d = 0; d < DP / 32; d++)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            f32x4 x{sum.o[d][r], sum.o[d][r + 1], sum.o[d][r + 2], sum.o[d][r + 3]};
+            x *= inverse;
+            put_four<T>(out + row * A.dim, 32 * d + result_row(r) + 4 * half, A.dim, mine ? x : f32x4{0, 0, 0, 0});
+        }
+    if (stats && half == 0) {
+        stats[2 * row] = mine && sum.m != NONE ? sum.m : -NONE;
+        stats[2 * row + 1] = inverse * (NARROW<T> ? 0x1p6f : 1.0f);
+    }
+}
+
+// ---- backward: queries' side ---------------------------------------------------------------------------------------------------------------
+// Probability of a stored row: exp2((t - m) rate) / l; 16 bits: with 1 / l in the exponent (0 for a row without keys).
+template <typename T, bool BIAS>
+__device__ __forceinline__ float row_shift(const Score<T, BIAS>& score, float m, float inverse) {
+    return sizeof(T) == 4 ? 0.0f : __builtin_amdgcn_logf(inverse) - m * score.rate;
+}
+template <typename T, bool BIAS>
+__device__ __forceinline__ float probability(const Score<T, BIAS>& score, float t, float m, float inverse, float shift) {
+    const float p = score.power(t, m, shift);
+    return sizeof(T) == 4 ? p * inverse : p;
+}
+
+// dq, D, and the table's gradient: scores transposed as in the forward pass.  The gradients of the biases are summed in float32 by
+// relative position (a column of sums for each half wavefront, so that no two lanes meet in one), those beyond the reach in the lane.
+// D comes from a rounded output, so that the ds of a row add up to a small e instead of 0; what lies beyond the reach, where most of
+// a long row's probability is, gets its share of -e back.
+template <typename T, int DP, int NW, bool BIAS>
+__global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, AttentionGrads G, int64_t slots, int splits) {
+    using L = Tile<T, DP>;
+    constexpr int KEYS = 32, TILE = KEYS * L::ROW;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    char* const tiles = lds;
+    float* const line = reinterpret_cast<float*>(lds + 4 * TILE);
+    const int entries = 2 * A.reach + 1;
+    float* const sums = line + 2 * (A.reach + MARGIN) + 1;      // (2 NW, entries), then two for each wavefront
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, column = lane & 31;
+    const int64_t total = slots * A.heads, id = die_order(blockIdx.x, total);
+    if (id >= total) return;
+    const int h = (int)(id / slots), slot = (int)(id - h * slots), kh = h / A.share, z = blockIdx.y;
+    float* const dtable = BIAS && G.dtable ? G.dtable + (((int64_t)h * splits + z) * slots + slot) * A.buckets : nullptr;
+    int b, from;
+    bool any = find_slot(A.q_starts, A.q_rows, A.packed, A.batch, NW * 32, slot, lane, b, from);
+    Span q{0, 0, 0, 0}, k{0, 0, 0, 0};
+    if (any) q = span_of(A.q_starts, A.q_sizes, A.q_rows, A.packed, A.batch, b);
+    if (!any || from >= q.rows) {
+        if (dtable)
+            for (int n = threadIdx.x; n < A.buckets; n += NW * 64) dtable[n] = 0.0f;
+        return;
+    }
+    if (!A.packed || b < A.batch) k = span_of(A.k_starts, A.k_sizes, A.k_rows, A.packed, A.batch, b);
+    const int i0 = from + wave * 32, i = i0 + column;
+    const bool mine = i < q.there;
+    const int shift = shift_of(A, q, k);
+    const Score<T, BIAS> score(A.scale);
+    int seen = from < q.there ? k.there : 0;
+    if (A.causal) seen = min(seen, min(from + NW * 32, q.there) + shift);
+    const int whole = seen > 0 ? (seen + KEYS - 1) / KEYS : 0;
+    const int first = (int)((int64_t)whole * z / splits), end = (int)((int64_t)whole * (z + 1) / splits);
+
+    const int64_t row = (q.first + i) * A.heads + h;
+    Eight<T> qf[DP / 16], gf[DP / 16];
+    float D = 0.0f;
+    {
+        const T* const q_row = row_start<T>(A.q, q, A.packed, h) + (mine ? i : 0) * A.q.row;
+        const T* const g_row = row_start<T>(G.go, q, A.packed, h) + (mine ? i : 0) * G.go.row;
+        const T* const o_row = static_cast<const T*>(G.out) + (mine ? row : 0) * A.dim;
+        const int o_wide = A.dim % L::E == 0;
+#pragma unroll
+        for (int s = 0; s < DP / 16; s++) {
+            qf[s] = row_operand<T>(q_row, mine, s, A.dim, A.q.wide, lane);
+            gf[s] = row_operand<T>(g_row, mine, s, A.dim, G.go.wide, lane);
+            const Eight<T> of = row_operand<T>(o_row, mine, s, A.dim, o_wide, lane);
+#pragma unroll
+            for (int e = 0; e < 8; e++) D = __builtin_fmaf(to_float(gf[s][e]), to_float(of[e]), D);
+        }
+        D = other_half_sum(D);
+    }
+    float m = -NONE, inverse = 0.0f;
+    if (mine) {
+        m = G.stats[2 * row];
+        inverse = G.stats[2 * row + 1];
+    }
+    if (z == 0 && half == 0 && i < q.rows) G.rows[row] = D;
+    const float off = row_shift(score, m, inverse);
+    const T* const k_at = row_start<T>(A.k, k, A.packed, kh);
+    const T* const v_at = row_start<T>(A.v, k, A.packed, kh);
+    const uint8_t* const mask = A.mask ? A.mask + k.first : nullptr;
+    if (BIAS) {
+        fill_line<T, BIAS>(A, h, line, threadIdx.x, NW * 64);
+        for (int n = threadIdx.x; n < 2 * NW * entries; n += NW * 64) sums[n] = 0.0f;
+    }
+    float* const own_sums = sums + (2 * wave + half) * entries;
+    float far_ds[2] = {0.0f, 0.0f}, far_p[2] = {0.0f, 0.0f}, all_ds = 0.0f;
+    f32x16 dq[DP / 32];
+    Scaled<T, DP> scaled;
+#pragma unroll
+    for (int d = 0; d < DP / 32; d++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) dq[d][r] = 0.0f;
+    Staged<T, DP, KEYS, NW * 64> kx, vx;
+    auto fetch = [&](int n) {
+        const int j0 = n * KEYS;
+        const uint8_t* const mk = mask ? mask + j0 : nullptr;
+        kx.load(k_at + j0 * A.k.row, A.k.row, k.there - j0, mk, A.dim, A.k.wide, threadIdx.x);
+        vx.load(v_at + j0 * A.v.row, A.v.row, k.there - j0, mk, A.dim, A.v.wide, threadIdx.x);
+    };
+    auto put = [&](int n) {
+        kx.store(tiles + (n & 1) * 2 * TILE, threadIdx.x);
+        vx.store(tiles + (n & 1) * 2 * TILE + TILE, threadIdx.x);
+    };
+    if (first < end) {
+        fetch(first);
+        put(first);
+    }
+    __syncthreads();
+    for (int n = first; n < end; n++) {
+        const char* const kt = tiles + (n & 1) * 2 * TILE;
+        const char* const vt = kt + TILE;
+        if (n + 1 < end) fetch(n + 1);
+        const int j0 = n * KEYS;
+        f32x16 s, dp;
+#pragma unroll
+        for (int r = 0; r < 16; r++) s[r] = dp[r] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < DP / 16; c++) s = Operand<T>::product(L::rows(kt, 0, c, lane), qf[c], s);
+#pragma unroll
+        for (int c = 0; c < DP / 16; c++) dp = Operand<T>::product(L::rows(vt, 0, c, lane), gf[c], dp);
+        const uint32_t there = keys_there(k.there - j0, mask ? mask + j0 : nullptr, lane);
+        const int low = j0 - (i0 + 31) - shift, high = j0 + 31 - i0 - shift, r0 = j0 + 4 * half - i - shift;
+        const bool causal = A.causal && high > 0, beyond = low >= A.reach || high <= -A.reach;
+        if (!BIAS || beyond) {
+            const float flat = BIAS ? line[low >= A.reach ? 2 * (A.reach + MARGIN) : 0] : 0.0f;
+            scores<T, BIAS>(s, score, there, causal, i + shift - j0, lane, [&](int) { return flat; });
+        } else {
+            const float* const at = line + (r0 + A.reach + MARGIN);
+            scores<T, BIAS>(s, score, there, causal, i + shift - j0, lane, [&](int r) { return at[result_row(r)]; });
+        }
+        if (!BIAS) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[r] = probability(score, s[r], m, inverse, off) * (dp[r] - D);
+        } else if (beyond) {
+            float ds = 0.0f, ps = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const float p = probability(score, s[r], m, inverse, off);
+                s[r] = p * (dp[r] - D);
+                ds += s[r];
+                ps += p;
+            }
+            const int side = low >= A.reach;
+            far_ds[0] += side ? 0.0f : ds; far_p[0] += side ? 0.0f : ps;
+            far_ds[1] += side ? ds : 0.0f; far_p[1] += side ? ps : 0.0f;
+            all_ds += ds;
+        } else {
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const float p = probability(score, s[r], m, inverse, off);
+                s[r] = p * (dp[r] - D);
+                all_ds += s[r];
+                const int rel = r0 + result_row(r);
+                if (rel > -A.reach && rel < A.reach) {
+                    if (mine) atomicAdd(own_sums + rel + A.reach, s[r]);
+                } else {
+                    const bool up = rel > 0;
+                    far_ds[0] += up ? 0.0f : s[r]; far_p[0] += up ? 0.0f : p;
+                    far_ds[1] += up ? s[r] : 0.0f; far_p[1] += up ? p : 0.0f;
+                }
+            }
+        }
+        scaled.meet(s, dq);
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            const Eight<T> ds = rounded<T>(s, c);
+#pragma unroll
+            for (int d = 0; d < DP / 32; d++) dq[d] = Operand<T>::product(L::columns(kt, 16 * c, d, lane), ds, dq[d]);
+        }
+        if (n + 1 < end) put(n + 1);
+        __syncthreads();
+    }
+    if (i < q.rows) {
+        const float factor = A.scale * scaled.back();
+        const int64_t rows = (A.packed ? A.q_rows : A.q_rows * A.batch) * A.heads;
+#pragma unroll
+        for (int d = 0; d < DP / 32; d++)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                f32x4 x{dq[d][r], dq[d][r + 1], dq[d][r + 2], dq[d][r + 3]};
+                x *= factor;
+                if (!mine) x = f32x4{0, 0, 0, 0};
+                const int c = 32 * d + result_row(r) + 4 * half;
+                if (G.dq_parts) put_four<float>(G.dq_parts + (z * rows + row) * A.dim, c, A.dim, x);
+                else put_four<T>(static_cast<T*>(G.dq) + row * A.dim, c, A.dim, x);
+            }
+    }
+    if (!BIAS || !dtable) return;
+    all_ds = other_half_sum(all_ds);
+    float* const far_sums = sums + 2 * NW * entries;
+#pragma unroll
+    for (int side = 0; side < 2; side++) {
+        const float ds = other_half_sum(far_ds[side]), p = other_half_sum(far_p[side]);
+        const float x = wave_sum(mine && half == 0 ? (splits > 1 ? ds : ds - all_ds * p) : 0.0f);
+        if (lane == 0) far_sums[2 * wave + side] = x;
+    }
+    __syncthreads();
+    for (int n = threadIdx.x; n < entries; n += NW * 64) {
+        float x = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 2 * NW; w++) x += sums[w * entries + n];
+#pragma unroll
+        for (int side = 0; side < 2; side++)      // (one entry is both)
+            if (n == side * (entries - 1))
+#pragma unroll
+                for (int w = 0; w < NW; w++) x += far_sums[2 * w + side];
+        line[n] = x;
+    }
+    __syncthreads();
+    for (int n = threadIdx.x; n < A.buckets; n += NW * 64) {
+        float x = 0.0f;
+        for (int e = 0; e < entries; e++) x += A.bucket_of[e] == n ? line[e] : 0.0f;
+        dtable[n] = x;
+    }
+}
+
+// Table's gradient: the workgroups' sums in a fixed order, in 64 bits.  A wavefront to a (head, bucket).
+template <typename T>
+__global__ __launch_bounds__(64) void table_gradient(const float* parts, int64_t count, int buckets, int heads, int table_float, void* dtable) {
+    const int n = blockIdx.x, h = blockIdx.y;
+    double x = 0.0;
+    for (int64_t w = threadIdx.x; w < count; w += 64) x += parts[((int64_t)h * count + w) * buckets + n];
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d);
+    if (threadIdx.x) return;
+    if (table_float) static_cast<float*>(dtable)[(int64_t)n * heads + h] = (float)x;
+    else static_cast<T*>(dtable)[(int64_t)n * heads + h] = from_float<T>((float)x);
+}
+
+// ---- backward: keys' side --------------------------------------------------------------------------------------------------------------------
+// A wavefront has 32 keys (columns), whose gradients stay in its registers; the workgroup goes through the queries of the heads that
+// share the key head, in tiles of 32.
+template <typename T, int DP, int NW, bool BIAS>
+__global__ __launch_bounds__(NW * 64) void keys_kernel(SequenceAttention A, AttentionGrads G, int64_t slots, int splits) {
+    using L = Tile<T, DP>;
+    constexpr int ROWS = 32, TILE = ROWS * L::ROW;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    char* const tiles = lds;                                            // two pairs: q, do
+    float* const row_stats = reinterpret_cast<float*>(lds + 4 * TILE);  // two times (3, ROWS): m or shift, 1 / l, D
+    float* const line = row_stats + 2 * 3 * ROWS;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, column = lane & 31;
+    const int64_t total = slots * A.kv_heads, id = die_order(blockIdx.x, total);
+    if (id >= total) return;
+    const int kh = (int)(id / slots), slot = (int)(id - kh * slots), z = blockIdx.y;
+    int b, from;
+    if (!find_slot(A.k_starts, A.k_rows, A.packed, A.batch, NW * 32, slot, lane, b, from)) return;
+    const Span k = span_of(A.k_starts, A.k_sizes, A.k_rows, A.packed, A.batch, b);
+    if (from >= k.rows) return;
+    Span q{0, 0, 0, 0};
+    if (!A.packed || b < A.batch) q = span_of(A.q_starts, A.q_sizes, A.q_rows, A.packed, A.batch, b);
+    const int j0 = from + wave * 32, j = j0 + column;
+    const bool mine = j < k.there && (!A.mask || A.mask[k.first + j]);
+    const int shift = shift_of(A, q, k);
+    const Score<T, BIAS> score(A.scale);
+    // the first tile of queries that sees a key of this workgroup
+    int skip = 0;
+    if (A.causal) skip = max(0, from - shift) / ROWS;
+    const int each = from < k.there ? max(0, (q.there + ROWS - 1) / ROWS - skip) : 0, whole = each * A.share;
+    const int first = (int)((int64_t)whole * z / splits), end = (int)((int64_t)whole * (z + 1) / splits);
+
+    Eight<T> kf[DP / 16], vf[DP / 16];
+    {
+        const T* const k_row = row_start<T>(A.k, k, A.packed, kh) + (mine ? j : 0) * A.k.row;
+        const T* const v_row = row_start<T>(A.v, k, A.packed, kh) + (mine ? j : 0) * A.v.row;
+#pragma unroll
+        for (int s = 0; s < DP / 16; s++) {
+            kf[s] = row_operand<T>(k_row, mine, s, A.dim, A.k.wide, lane);
+            vf[s] = row_operand<T>(v_row, mine, s, A.dim, A.v.wide, lane);
+        }
+    }
+    f32x16 dk[DP / 32], dv[DP / 32];
+    Scaled<T, DP> scaled;
+#pragma unroll
+    for (int d = 0; d < DP / 32; d++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) dk[d][r] = dv[d][r] = 0.0f;
+    Staged<T, DP, ROWS, NW * 64> qx, gx;
+    float sx[3];
+    auto fetch = [&](int n) {
+        const int h = kh * A.share + n / each, i0 = (skip + n % each) * ROWS;
+        qx.load(row_start<T>(A.q, q, A.packed, h) + i0 * A.q.row, A.q.row, q.there - i0, nullptr, A.dim, A.q.wide, threadIdx.x);
+        gx.load(row_start<T>(G.go, q, A.packed, h) + i0 * G.go.row, G.go.row, q.there - i0, nullptr, A.dim, G.go.wide, threadIdx.x);
+        if (threadIdx.x < ROWS) {
+            float m = -NONE, inverse = 0.0f, D = 0.0f;
+            if (i0 + (int)threadIdx.x < q.there) {
+                const int64_t row = (q.first + i0 + threadIdx.x) * A.heads + h;
+                m = G.stats[2 * row];
+                inverse = G.stats[2 * row + 1];
+                D = G.rows[row];
+            }
+            sx[0] = sizeof(T) == 4 ? m : P_LIFT<T> + row_shift(score, m, inverse);
+            sx[1] = inverse;
+            sx[2] = D;
+        }
+    };
+    auto put = [&](int n) {
+        qx.store(tiles + (n & 1) * 2 * TILE, threadIdx.x);
+        gx.store(tiles + (n & 1) * 2 * TILE + TILE, threadIdx.x);
+        if (threadIdx.x < ROWS)
+#pragma unroll
+            for (int c = 0; c < 3; c++) row_stats[((n & 1) * 3 + c) * ROWS + threadIdx.x] = sx[c];
+    };
+    if (first < end) {
+        fetch(first);
+        put(first);
+    }
+    int line_of = -1;
+    for (int n = first; n < end; n++) {
+        const int h = kh * A.share + n / each, i0 = (skip + n % each) * ROWS;
+        if (BIAS && h != line_of) {
+            __syncthreads();
+            fill_line<T, BIAS>(A, h, line, threadIdx.x, NW * 64);
+            line_of = h;
+        }
+        __syncthreads();
+        const char* const qt = tiles + (n & 1) * 2 * TILE;
+        const char* const gt = qt + TILE;
+        const float* const st = row_stats + (n & 1) * 3 * ROWS + 4 * half;
+        if (n + 1 < end) fetch(n + 1);
+        f32x16 s, dp;
+#pragma unroll
+        for (int r = 0; r < 16; r++) s[r] = dp[r] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < DP / 16; c++) s = Operand<T>::product(L::rows(qt, 0, c, lane), kf[c], s);
+#pragma unroll
+        for (int c = 0; c < DP / 16; c++) dp = Operand<T>::product(L::rows(gt, 0, c, lane), vf[c], dp);
+        if (BIAS) {
+            const int low = j0 - (i0 + 31) - shift, high = j0 + 31 - i0 - shift;
+            if (low >= A.reach || high <= -A.reach) {
+                const float flat = line[low >= A.reach ? 2 * (A.reach + MARGIN) : 0];
+#pragma unroll
+                for (int r = 0; r < 16; r++) s[r] = score.t(s[r], flat);
+            } else {
+                const float* const at = line + (j - i0 - 4 * half - shift + A.reach + MARGIN);
+#pragma unroll
+                for (int r = 0; r < 16; r++) s[r] = score.t(s[r], at[-result_row(r)]);
+            }
+        }
+        if (A.causal && j0 + 31 > i0 + shift) {
+            const int least = j - shift - i0 - 4 * half;      // first row that sees the column's key
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[r] = result_row(r) >= least ? s[r] : NONE;
+        }
+        f32x16 p;
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const f32x4 m4 = *reinterpret_cast<const f32x4*>(st + result_row(r)), D4 = *reinterpret_cast<const f32x4*>(st + 2 * ROWS + result_row(r));
+            f32x4 l4{1, 1, 1, 1};
+            if (sizeof(T) == 4) l4 = *reinterpret_cast<const f32x4*>(st + ROWS + result_row(r));
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                p[r + e] = probability(score, s[r + e], m4[e], l4[e], m4[e]);
+                s[r + e] = p[r + e] * (dp[r + e] - D4[e]);
+            }
+        }
+        scaled.meet(s, dk);
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            const Eight<T> pf = rounded<T>(p, c), ds = rounded<T>(s, c);
+#pragma unroll
+            for (int d = 0; d < DP / 32; d++) {
+                dv[d] = Operand<T>::product(L::columns(gt, 16 * c, d, lane), pf, dv[d]);
+                dk[d] = Operand<T>::product(L::columns(qt, 16 * c, d, lane), ds, dk[d]);
+            }
+        }
+        if (n + 1 < end) put(n + 1);
+    }
+    if (j >= k.rows) return;
+    const float lift = NARROW<T> ? 0x1p-15f : 1.0f, factor = A.scale * scaled.back() * lift;
+    const int64_t row = (k.first + j) * A.kv_heads + kh, rows = (A.packed ? A.k_rows : A.k_rows * A.batch) * A.kv_heads;
+#pragma unroll
+    for (int d = 0; d < DP / 32; d++)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            f32x4 x{dk[d][r], dk[d][r + 1], dk[d][r + 2], dk[d][r + 3]}, y{dv[d][r], dv[d][r + 1], dv[d][r + 2], dv[d][r + 3]};
+            x *= factor;
+            y *= lift;
+            if (!mine) x = y = f32x4{0, 0, 0, 0};
+            const int c = 32 * d + result_row(r) + 4 * half;
+            if (G.dk_parts) {
+                put_four<float>(G.dk_parts + (z * rows + row) * A.dim, c, A.dim, x);
+                put_four<float>(G.dv_parts + (z * rows + row) * A.dim, c, A.dim, y);
+            } else {
+                put_four<T>(static_cast<T*>(G.dk) + row * A.dim, c, A.dim, x);
+                put_four<T>(static_cast<T*>(G.dv) + row * A.dim, c, A.dim, y);
+            }
+        }
+}
+
+// out = the sum of the splits, in their order.
+template <typename T>
+__global__ __launch_bounds__(256) void add_parts(const float* parts, int splits, int64_t count, T* out) {
+    const int64_t n = (blockIdx.x * 256LL + threadIdx.x) * 4;
+    if (n >= count) return;
+    if (n + 4 <= count && (count & 3) == 0) {
+        f32x4 x{0, 0, 0, 0};
+        for (int z = 0; z < splits; z++) x += *reinterpret_cast<const f32x4*>(parts + z * count + n);
+        put_four<T>(out + n, 0, 4, x);
+        return;
+    }
+    for (int64_t e = n; e < n + 4 && e < count; e++) {
+        float x = 0.0f;
+        for (int z = 0; z < splits; z++) x += parts[z * count + e];
+        out[e] = from_float<T>(x);
+    }
+}
+}  // namespace attention
+
+// ---- launches ----------------------------------------------------------------------------------------------------------------------------------
+template <typename K, typename... P>
+void launch_attention(K kernel, dim3 grid, int threads, size_t lds, hipStream_t st, P... p) {
+    if (lds > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    hipLaunchKernelGGL(kernel, grid, dim3(threads), lds, st, p...);
+}
+template <typename F>
+void with_padded_dim(int dim, F f) {
+    if (dim <= 32) f(std::integral_constant<int, 32>());
+    else if (dim <= 64) f(std::integral_constant<int, 64>());
+    else f(std::integral_constant<int, 128>());
+}
+template <typename F>
+void with_choice(bool yes, F f) {
+    if (yes) f(std::true_type());
+    else f(std::false_type());
+}
+inline unsigned die_grid(int64_t count) { return (unsigned)((count + 7) / 8 * 8); }
+
+template <typename T>
+void sequence_attention_forward(const SequenceAttention& A, const AttentionPlan& P, T* out, float* stats, float* scratch, hipStream_t st) {
+    using namespace attention;
+    with_padded_dim(A.dim, [&](auto dp) {
+        with_choice(A.table != nullptr, [&](auto bias) {
+            constexpr int DP = decltype(dp)::value;
+            constexpr bool BIAS = decltype(bias)::value;
+            const int64_t rows = (A.packed ? A.q_rows : A.q_rows * A.batch) * A.heads;
+            if (!P.few) {
+                const size_t lds = 4 * keys_at_once<T, 4>() * Tile<T, DP>::ROW + (BIAS ? (2 * (A.reach + MARGIN) + 1) * sizeof(float) : 0);
+                launch_attention(tiles_kernel<T, DP, 4, BIAS>, dim3(die_grid((int64_t)P.slots * A.heads)), 256, lds, st, A, out, stats, P.slots);
+                return;
+            }
+            float* const part_o = scratch;
+            float* const part_ml = scratch + P.splits * rows * DP;
+            const dim3 grid(P.slots, A.kv_heads * ((A.share + 31) / 32), P.splits);
+            if (P.waves == 1) launch_attention(few_kernel<T, DP, 1, BIAS>, grid, 64, 0, st, A, out, stats, part_o, part_ml, P.splits);
+            else launch_attention(few_kernel<T, DP, 4, BIAS>, grid, 256, 0, st, A, out, stats, part_o, part_ml, P.splits);
+            if (P.splits > 1)
+                launch_attention(combine_parts<T, DP, BIAS>, dim3((unsigned)((rows + 7) / 8)), 256, 0, st, A, part_o, part_ml, P.splits, rows, out, stats);
+        });
+    });
+}
+
+template <typename T>
+void sequence_attention_backward(const SequenceAttention& A, const AttentionGradPlan& P, AttentionGrads G, void* dtable, float* scratch, hipStream_t st) {
+    using namespace attention;
+    const int64_t q_all = (A.packed ? A.q_rows : A.q_rows * A.batch) * A.heads, k_all = (A.packed ? A.k_rows : A.k_rows * A.batch) * A.kv_heads;
+    float* next = scratch;
+    auto take = [&](int64_t floats) {      // aligned to 16 bytes
+        float* const at = next;
+        next += (floats + 3) / 4 * 4;
+        return at;
+    };
+    G.rows = take(q_all);
+    if (P.q_splits > 1) G.dq_parts = take(P.q_splits * q_all * A.dim);
+    if (P.k_splits > 1) {
+        G.dk_parts = take(P.k_splits * k_all * A.dim);
+        G.dv_parts = take(P.k_splits * k_all * A.dim);
+    }
+    G.dtable = dtable ? next : nullptr;
+    with_padded_dim(A.dim, [&](auto dp) {
+        with_choice(A.table != nullptr, [&](auto bias) {
+            constexpr int DP = decltype(dp)::value;
+            constexpr bool BIAS = decltype(bias)::value;
+            const size_t line = BIAS ? (2 * (A.reach + MARGIN) + 1) * sizeof(float) : 0, tiles = 4 * 32 * Tile<T, DP>::ROW;
+            const size_t sums = BIAS ? (2 * P.q_waves * (2 * A.reach + 1) + 2 * P.q_waves) * sizeof(float) : 0;
+            if (q_all > 0) {
+                const dim3 grid(die_grid((int64_t)P.q_slots * A.heads), P.q_splits);
+                if (P.q_waves == 1) launch_attention(queries_kernel<T, DP, 1, BIAS>, grid, 64, tiles + line + sums, st, A, G, P.q_slots, P.q_splits);
+                else launch_attention(queries_kernel<T, DP, 4, BIAS>, grid, 256, tiles + line + sums, st, A, G, P.q_slots, P.q_splits);
+            }
+            if (k_all > 0 && G.dk) {
+                const dim3 grid(die_grid((int64_t)P.k_slots * A.kv_heads), P.k_splits);
+                const size_t lds = tiles + 6 * 32 * sizeof(float) + line;
+                if (P.k_waves == 1) launch_attention(keys_kernel<T, DP, 1, BIAS>, grid, 64, lds, st, A, G, P.k_slots, P.k_splits);
+                else launch_attention(keys_kernel<T, DP, 4, BIAS>, grid, 256, lds, st, A, G, P.k_slots, P.k_splits);
+            }
+        });
+    });
+    auto add = [&](const float* parts, int splits, int64_t count, void* to) {
+        if (count > 0) launch_attention(add_parts<T>, dim3((unsigned)((count + 1023) / 1024)), 256, 0, st, parts, splits, count, static_cast<T*>(to));
+    };
+    if (P.q_splits > 1) add(G.dq_parts, P.q_splits, q_all * A.dim, G.dq);
+    if (P.k_splits > 1 && G.dk) {
+        add(G.dk_parts, P.k_splits, k_all * A.dim, G.dk);
+        add(G.dv_parts, P.k_splits, k_all * A.dim, G.dv);
+    }
+    if (dtable) {
+        const int64_t count = q_all > 0 ? (int64_t)P.q_slots * P.q_splits : 0;
+        launch_attention(table_gradient<T>, dim3(A.buckets, A.heads), 64, 0, st, G.dtable, count, A.buckets, A.heads, A.table_float, dtable);
+    }
+}
+}  // namespace cfh

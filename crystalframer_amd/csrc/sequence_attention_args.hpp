@@ -1,0 +1,91 @@
+// What the kernels of attention between sequences are told, and which of them a call takes.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace cfh {
+
+constexpr int ATTENTION_MAX_DIM = 128;
+constexpr int ATTENTION_MAX_REACH = 1024;      // relative positions beyond this (either way) share a bucket
+constexpr int ATTENTION_CUS = 256;
+
+// Element strides of (batch, position, head); channels lie next to one another.  16-byte loads where `wide`.
+struct AttentionRows {
+    const void* at;
+    int64_t batch, row, head;
+    int32_t wide;
+};
+
+struct SequenceAttention {
+    AttentionRows q, k, v;
+    const uint8_t* mask;               // per key: 0 = not there; packed (k_rows) or (batch, k_rows); NULL: all are
+    const int64_t *q_starts, *k_starts, *q_sizes, *k_sizes;
+    const void* table;                 // (buckets, heads)
+    const int32_t* bucket_of;          // (2 reach + 1): of the relative positions -reach ... reach
+    int64_t q_rows, k_rows;            // packed: of all sequences; else of one
+    int32_t packed, batch, heads, kv_heads, share, dim, buckets, reach, causal, last, table_float;
+    float scale;
+};
+
+struct AttentionGrads {
+    AttentionRows go;
+    const void* out;                   // (rows, heads, dim), as all that follows
+    const float* stats;                // (rows, heads, 2): largest score, one over the sum
+    float* rows;                       // (rows, heads): D, from the queries' kernel for the keys'
+    void *dq, *dk, *dv;                // (dk, dv over kv_heads)
+    float *dq_parts, *dk_parts, *dv_parts;      // of the splits, or NULL
+    float* dtable;                     // (workgroups, buckets), or NULL
+};
+
+// Tiles of the grid for rows of `tile`: packed sequence b begins at tile starts[b] / tile + b, which leaves every sequence as many as it
+// needs without anyone adding up lengths.
+inline int64_t tile_slots(int packed, int64_t rows, int batch, int tile) {
+    return packed ? rows / tile + batch + 1 : (int64_t)batch * ((rows + tile - 1) / tile);
+}
+inline int64_t split_count(int64_t workgroups, int64_t wanted, int64_t most) {
+    const int64_t n = workgroups > 0 ? wanted / workgroups : 1;
+    return n < 1 || most < 1 ? 1 : n > most ? most : n;
+}
+
+struct AttentionPlan {
+    bool few;              // few_kernel
+    int waves, splits;
+    int64_t slots;
+};
+inline AttentionPlan attention_plan(const SequenceAttention& A) {
+    AttentionPlan P{};
+    const int64_t q_each = A.packed && A.batch > 0 ? A.q_rows / A.batch : A.q_rows, k_each = A.packed && A.batch > 0 ? A.k_rows / A.batch : A.k_rows;
+    const int64_t whole = tile_slots(A.packed, A.q_rows, A.batch, 128);
+    P.few = q_each * (A.share < 32 ? A.share : 32) <= 32 || whole * A.heads < 192;
+    P.splits = 1;
+    P.slots = whole;
+    P.waves = 4;
+    if (!P.few) return P;
+    const int at_once = A.share < 32 ? A.share : 32, groups = (A.share + at_once - 1) / at_once;
+    P.slots = tile_slots(A.packed, A.q_rows, A.batch, 32 / at_once);
+    P.waves = k_each > 64 ? 4 : 1;
+    P.splits = (int)split_count(P.slots * A.kv_heads * groups, 4 * ATTENTION_CUS, k_each / (64 * P.waves));
+    return P;
+}
+
+struct AttentionGradPlan {
+    int q_waves, q_splits, k_waves, k_splits;
+    int64_t q_slots, k_slots;
+};
+inline AttentionGradPlan attention_grad_plan(const SequenceAttention& A) {
+    AttentionGradPlan P{};
+    const int64_t q_each = A.packed && A.batch > 0 ? A.q_rows / A.batch : A.q_rows, k_each = A.packed && A.batch > 0 ? A.k_rows / A.batch : A.k_rows;
+    P.q_waves = q_each > 64 ? 4 : 1;
+    P.k_waves = k_each > 64 ? 4 : 1;
+    P.q_slots = tile_slots(A.packed, A.q_rows, A.batch, 32 * P.q_waves);
+    P.k_slots = tile_slots(A.packed, A.k_rows, A.batch, 32 * P.k_waves);
+    P.q_splits = (int)split_count(P.q_slots * A.heads, 2 * ATTENTION_CUS, k_each / 256);
+    P.k_splits = (int)split_count(P.k_slots * A.kv_heads, 2 * ATTENTION_CUS, q_each * A.share / 256);
+    return P;
+}
+
+template <typename T>
+void sequence_attention_forward(const SequenceAttention& A, const AttentionPlan& P, T* out, float* stats, float* scratch, hipStream_t st);
+template <typename T>
+void sequence_attention_backward(const SequenceAttention& A, const AttentionGradPlan& P, AttentionGrads G, void* dtable, float* scratch, hipStream_t st);
+}  // namespace cfh

@@ -1,0 +1,155 @@
+// C ABI of attention between sequences (see include/crystalframer_hip.h): argument checks and launches.  Nothing here allocates or
+// synchronises.
+#include "../../include/crystalframer_hip.h"
+
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+
+#include "element_types.hpp"
+#include "host_error.hpp"
+#include "sequence_attention_args.hpp"
+
+namespace {
+
+using cfh::fail;
+using cfh::finish_launch;
+
+constexpr int64_t MAX_ROWS = 0x7fffff00LL;      // of a sequence, and of all packed ones
+constexpr int64_t MAX_GRID = 0x7fffff00LL;
+
+int check_attention(const cfh_attention* a) {
+    if (!a || a->struct_size != (int32_t)sizeof(cfh_attention)) return fail(CFH_EINVAL, "attention: struct_size does not match");
+    if (a->dtype < CFH_FLOAT32 || a->dtype > CFH_FLOAT16) return fail(CFH_EINVAL, "attention: dtype %d", (int)a->dtype);
+    if (a->dim < 1 || a->dim > CFH_ATTENTION_MAX_DIM)
+        return fail(CFH_EINVAL, "attention: dim = %d: 1 to %d channels of a head", (int)a->dim, CFH_ATTENTION_MAX_DIM);
+    if (a->heads < 1 || a->heads > 65535 || a->kv_heads < 1 || a->heads % a->kv_heads)
+        return fail(CFH_EINVAL, "attention: heads = %d, kv_heads = %d: every key head serves as many of up to 65535 heads", (int)a->heads, (int)a->kv_heads);
+    if (a->batch < 0 || a->query_rows < 0 || a->query_rows > MAX_ROWS || a->key_rows < 0 || a->key_rows > MAX_ROWS)
+        return fail(CFH_EINVAL, "attention: batch = %d, query_rows = %lld, key_rows = %lld out of range", (int)a->batch, (long long)a->query_rows,
+                    (long long)a->key_rows);
+    if (!(a->scale > 0.0f) || std::isinf(a->scale)) return fail(CFH_EINVAL, "attention: scale = %g must be positive and finite", a->scale);
+    for (int n = 0; n < 3; n++)
+        if (a->q_stride[n] < 0 || a->k_stride[n] < 0 || a->v_stride[n] < 0) return fail(CFH_EINVAL, "attention: strides must not be negative");
+    if (a->packed && (!a->query_starts || !a->key_starts)) return fail(CFH_EINVAL, "attention: packed sequences need query_starts and key_starts");
+    if (a->packed && (a->query_sizes || a->key_sizes)) return fail(CFH_EINVAL, "attention: query_sizes and key_sizes are of sequences that are not packed");
+    if (!a->packed && (a->query_starts || a->key_starts)) return fail(CFH_EINVAL, "attention: query_starts and key_starts are of packed sequences");
+    const int64_t q_all = a->packed ? a->query_rows : a->query_rows * a->batch, k_all = a->packed ? a->key_rows : a->key_rows * a->batch;
+    if ((q_all > 0 && !a->q) || (k_all > 0 && (!a->k || !a->v))) return fail(CFH_EINVAL, "attention: q, k and v must not be NULL");
+    const uintptr_t element = a->dtype == CFH_FLOAT32 ? 3 : 1;
+    if (((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v) & element) return fail(CFH_EINVAL, "attention: an address is not one of an element");
+    if (a->table) {
+        if (a->table_dtype != a->dtype && a->table_dtype != CFH_FLOAT32)
+            return fail(CFH_EINVAL, "attention: table_dtype %d is neither dtype nor float32", (int)a->table_dtype);
+        if (a->reach < 0 || a->reach > CFH_ATTENTION_MAX_REACH)
+            return fail(CFH_EINVAL, "attention: reach = %d: 0 to %d", (int)a->reach, CFH_ATTENTION_MAX_REACH);
+        if (a->buckets < 1 || a->buckets > 65535) return fail(CFH_EINVAL, "attention: buckets = %d: 1 to 65535", (int)a->buckets);
+        if (!a->bucket_of) return fail(CFH_EINVAL, "attention: a table needs bucket_of");
+    } else if (a->buckets || a->reach || a->bucket_of) {
+        return fail(CFH_EINVAL, "attention: buckets, reach and bucket_of belong to a table");
+    }
+    // (the smallest tile of either side is one row)
+    const int64_t slots = cfh::tile_slots(a->packed, a->query_rows > a->key_rows ? a->query_rows : a->key_rows, a->batch, 1);
+    if (slots > MAX_GRID / a->heads) return fail(CFH_EINVAL, "attention: %lld rows of %d heads are more than a grid holds", (long long)slots, (int)a->heads);
+    return CFH_OK;
+}
+
+// 16 bytes at a time: where they begin at multiples of 16 and hold whole rows of channels.
+cfh::AttentionRows rows_of(const void* at, const int64_t* stride, int dtype, int dim) {
+    const int64_t bytes = dtype == CFH_FLOAT32 ? 4 : 2;
+    uint64_t all = (uint64_t)(uintptr_t)at | (uint64_t)(dim * bytes);
+    for (int n = 0; n < 3; n++) all |= (uint64_t)(stride[n] * bytes);
+    return {at, stride[0], stride[1], stride[2], (all & 15) == 0};
+}
+
+cfh::SequenceAttention device_args(const cfh_attention* a) {
+    cfh::SequenceAttention A{};
+    A.q = rows_of(a->q, a->q_stride, a->dtype, a->dim);
+    A.k = rows_of(a->k, a->k_stride, a->dtype, a->dim);
+    A.v = rows_of(a->v, a->v_stride, a->dtype, a->dim);
+    A.mask = a->key_mask;
+    A.q_starts = a->query_starts; A.k_starts = a->key_starts; A.q_sizes = a->query_sizes; A.k_sizes = a->key_sizes;
+    A.table = a->table; A.bucket_of = a->bucket_of;
+    A.q_rows = a->query_rows; A.k_rows = a->key_rows;
+    A.packed = a->packed; A.batch = a->batch; A.heads = a->heads; A.kv_heads = a->kv_heads; A.share = a->heads / a->kv_heads;
+    A.dim = a->dim; A.buckets = a->buckets; A.reach = a->reach; A.causal = a->causal; A.last = a->queries_last;
+    A.table_float = a->table_dtype == CFH_FLOAT32;
+    A.scale = a->scale;
+    return A;
+}
+int padded_dim(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : 128; }
+int64_t q_all(const cfh::SequenceAttention& A) { return (A.packed ? A.q_rows : A.q_rows * A.batch) * A.heads; }
+int64_t k_all(const cfh::SequenceAttention& A) { return (A.packed ? A.k_rows : A.k_rows * A.batch) * A.kv_heads; }
+
+int check_workspace(const void* workspace, size_t have, size_t need) {
+    if (need > 0 && (!workspace || ((uintptr_t)workspace & 15) || have < need))
+        return fail(CFH_EWORKSPACE, "attention: workspace of %zu bytes, aligned to 16, is missing", need);
+    return CFH_OK;
+}
+template <typename F>
+void with_type(int dtype, F f) {
+    if (dtype == CFH_FLOAT32) f(float());
+    else if (dtype == CFH_BFLOAT16) f(cfh::bf16());
+    else f(cfh::f16());
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t cfh_attention_forward_workspace_bytes(const cfh_attention* a) {
+    if (check_attention(a)) return 0;
+    const cfh::SequenceAttention A = device_args(a);
+    const cfh::AttentionPlan P = cfh::attention_plan(A);
+    return P.splits > 1 ? (size_t)P.splits * q_all(A) * (padded_dim(A.dim) + 2) * sizeof(float) : 0;
+}
+
+int cfh_attention_forward(const cfh_attention* a, void* out, float* stats, void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = check_attention(a);
+    if (rc) return rc;
+    const cfh::SequenceAttention A = device_args(a);
+    if (q_all(A) == 0) return CFH_OK;
+    if (!out || ((uintptr_t)out & 15)) return fail(CFH_EINVAL, "attention: out must not be NULL, and aligned to 16 bytes");
+    if ((rc = check_workspace(workspace, workspace_bytes, cfh_attention_forward_workspace_bytes(a)))) return rc;
+    with_type(a->dtype, [&](auto t) {
+        using T = decltype(t);
+        cfh::sequence_attention_forward<T>(A, cfh::attention_plan(A), (T*)out, stats, (float*)workspace, (hipStream_t)stream);
+    });
+    return finish_launch("attention_forward");
+}
+
+size_t cfh_attention_backward_workspace_bytes(const cfh_attention* a) {
+    if (check_attention(a)) return 0;
+    const cfh::SequenceAttention A = device_args(a);
+    const cfh::AttentionGradPlan P = cfh::attention_grad_plan(A);
+    size_t floats = (size_t)q_all(A) + 32;
+    if (P.q_splits > 1) floats += (size_t)P.q_splits * q_all(A) * A.dim;
+    if (P.k_splits > 1) floats += 2 * (size_t)P.k_splits * k_all(A) * A.dim;
+    if (A.table) floats += (size_t)P.q_slots * P.q_splits * A.heads * A.buckets;
+    return floats * sizeof(float);
+}
+
+int cfh_attention_backward(const cfh_attention* a, const void* out, const float* stats, const void* gout, const int64_t gout_stride[3],
+                           void* dq, void* dk, void* dv, void* dtable, void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = check_attention(a);
+    if (rc) return rc;
+    const cfh::SequenceAttention A = device_args(a);
+    if (dtable && !a->table) return fail(CFH_EINVAL, "attention: a gradient of a table that is not there");
+    if (q_all(A) > 0 && (!out || !stats || !gout || !gout_stride || !dq)) return fail(CFH_EINVAL, "attention: out, stats, gout, its strides and dq must not be NULL");
+    if (k_all(A) > 0 && !dk != !dv) return fail(CFH_EINVAL, "attention: dk and dv go together");
+    if (((uintptr_t)out | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15) return fail(CFH_EINVAL, "attention: out, dq, dk and dv must be aligned to 16 bytes");
+    const int64_t none[3] = {0, 0, 0};
+    const int64_t* const gs = gout_stride ? gout_stride : none;
+    if (gs[0] < 0 || gs[1] < 0 || gs[2] < 0 || ((uintptr_t)gout & (a->dtype == CFH_FLOAT32 ? 3 : 1)))
+        return fail(CFH_EINVAL, "attention: strides must not be negative, addresses those of elements");
+    if ((rc = check_workspace(workspace, workspace_bytes, cfh_attention_backward_workspace_bytes(a)))) return rc;
+    cfh::AttentionGrads G{};
+    G.go = rows_of(gout, gs, a->dtype, a->dim);
+    G.out = out; G.stats = stats; G.dq = dq; G.dk = dk; G.dv = dv;
+    with_type(a->dtype, [&](auto t) {
+        cfh::sequence_attention_backward<decltype(t)>(A, cfh::attention_grad_plan(A), G, dtable, (float*)workspace, (hipStream_t)stream);
+    });
+    return finish_launch("attention_backward");
+}
+
+}  // extern "C"

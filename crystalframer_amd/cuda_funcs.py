@@ -17,6 +17,7 @@ import torch
 
 from . import _lib
 from .norms import residual_norm  # noqa: F401
+from .sequence_attention import cross_attention, position_buckets, relative_attention  # noqa: F401
 
 CUPY_AVAILABLE = True   # name kept from the reference: "the native path is usable"
 

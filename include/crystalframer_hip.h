@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define CFH_ABI_VERSION 15
+#define CFH_ABI_VERSION 16
 
 enum {
     CFH_OK = 0,
@@ -771,6 +771,50 @@ int cfh_model_forward(const cfh_model* m, const cfh_model_batch* b, float* out);
  * head W, b.  `b` is the forward's (same arena, untouched since). */
 int cfh_model_backward(const cfh_model* m, const cfh_model_batch* b, const float* gout, void* scratch,
                        size_t scratch_bytes, float* grads);
+
+/*
+ * Attention between the sequences of a batch and those of another (cross attention), or of the same with a learned bias by relative
+ * position.  No counterpart in the reference, whose attention is over the atoms of one crystal.
+ *
+ *   t_ij = scale q_i . k_j + table[bucket_of[reach + j - i - shift], head],  o_i = sum_j softmax_j(t_ij) v_j
+ *
+ * over the keys j of the query's own sequence which key_mask keeps and, with causal, j <= i + shift; shift = keys - queries of the
+ * sequence with queries_last, else 0; relative positions beyond +-reach count as +-reach.  Head h has key head h / (heads / kv_heads).
+ * A row without keys is 0.  In place of a key that is not there, anything may be in memory, NaN included.
+ *
+ * packed = 1: the sequences lie behind one another, query_starts and key_starts (batch + 1, int64, beginning with 0) say where, rows
+ *   behind the last are 0 in every result; query_rows, key_rows are those of all sequences.
+ * packed = 0: (batch, query_rows) and (batch, key_rows); query_sizes, key_sizes (batch, int64, or NULL: whole rows).
+ * Values of these arrays are cut to what is there; an entry of bucket_of outside 0 ... buckets - 1 means no bias.
+ * Strides are in elements; channels lie next to one another.  out and gradients are contiguous: (rows, heads or kv_heads, dim).
+ */
+#define CFH_ATTENTION_MAX_DIM 128
+#define CFH_ATTENTION_MAX_REACH 1024
+typedef struct cfh_attention {
+    int32_t struct_size;                  /* = sizeof(cfh_attention)                                     */
+    int32_t dtype, table_dtype;           /* table_dtype: dtype or CFH_FLOAT32                           */
+    int32_t packed, causal, queries_last;
+    int32_t batch, heads, kv_heads, dim;
+    int32_t buckets, reach;               /* 0 without a table                                           */
+    float scale;                          /* positive                                                    */
+    int32_t reserved0;
+    int64_t query_rows, key_rows;
+    int64_t q_stride[3], k_stride[3], v_stride[3];      /* of batch (packed: unused), row, head          */
+    const void* q; const void* k; const void* v;
+    const uint8_t* key_mask;              /* (key_rows) or (batch, key_rows), 0: not there; NULL: all are */
+    const int64_t* query_starts; const int64_t* key_starts;
+    const int64_t* query_sizes; const int64_t* key_sizes;
+    const void* table;                    /* (buckets, heads) or NULL                                    */
+    const int32_t* bucket_of;             /* (2 reach + 1)                                               */
+} cfh_attention;
+/* stats (rows, heads, 2): for the backward pass, or NULL.  workspace aligned to 16 bytes; 0 bytes may be needed. */
+size_t cfh_attention_forward_workspace_bytes(const cfh_attention* a);
+int cfh_attention_forward(const cfh_attention* a, void* out, float* stats, void* workspace, size_t workspace_bytes, void* stream);
+/* gout with strides as q_stride; dk and dv may both be NULL (states that are not trained); dtable (buckets, heads) in table_dtype, or
+ * NULL.  Every sum in a fixed order. */
+size_t cfh_attention_backward_workspace_bytes(const cfh_attention* a);
+int cfh_attention_backward(const cfh_attention* a, const void* out, const float* stats, const void* gout, const int64_t gout_stride[3],
+                           void* dq, void* dk, void* dv, void* dtable, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
