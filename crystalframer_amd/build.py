@@ -28,6 +28,9 @@ HIPCC_FLAGS = [
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]
 
+# results of matrix instructions stay in the registers that all others use: sums that are scaled between products are not moved
+SOURCE_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for name in LIB_SOURCES if name.startswith("sequence_attention_")}
+
 
 def hipcc_path() -> str:
     for cand in (shutil.which("hipcc"), "/opt/rocm/bin/hipcc"):
@@ -48,7 +51,7 @@ def build_library(verbose: bool = True) -> str:
     extra = os.environ.get("CFH_EXTRA_HIPCC_FLAGS", "").split()
     tmp = LIB_PATH + ".tmp"
     objects = [os.path.join(HERE, name + ".o") for name in LIB_SOURCES]
-    cmds = [[hipcc_path(), *HIPCC_FLAGS, *extra, "-c", "-o", obj, os.path.join(CSRC, name + ".hip")]
+    cmds = [[hipcc_path(), *HIPCC_FLAGS, *SOURCE_FLAGS.get(name, []), *extra, "-c", "-o", obj, os.path.join(CSRC, name + ".hip")]
             for name, obj in zip(LIB_SOURCES, objects)]
     try:
         with concurrent.futures.ThreadPoolExecutor(len(cmds)) as pool:

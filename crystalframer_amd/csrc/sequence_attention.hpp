@@ -116,56 +116,95 @@ struct Tile {
 };
 
 // ---- rows in memory ------------------------------------------------------------------------------------------------------------------
+// Where rows lie at multiples of 16 bytes they are read as pieces of a buffer that ends behind the last row that is there: what is
+// beyond comes back as 0, without a branch.  Others are read element by element.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+constexpr int BEYOND = 0x40000000;      // behind any buffer here
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* at, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(at), 0, bytes, 0x00027000);
+}
 // 16 bytes of a row from channel `from` on; channels that the row does not have are 0.
 template <typename T>
-__device__ __forceinline__ uint4 piece_of(const T* row, int from, int dim, int wide) {
-    uint4 x{0, 0, 0, 0};
+__device__ __forceinline__ u32x4 elements_of(const T* row, int from, int dim) {
     constexpr int E = 16 / sizeof(T);
-    if (wide) {
-        if (from < dim) x = *reinterpret_cast<const uint4*>(row + from);
-    } else {
-        T e[E];
+    T e[E];
 #pragma unroll
-        for (int n = 0; n < E; n++) e[n] = from + n < dim ? row[from + n] : T(0);
-        __builtin_memcpy(&x, e, 16);
-    }
+    for (int n = 0; n < E; n++) e[n] = from + n < dim ? row[from + n] : T(0);
+    u32x4 x;
+    __builtin_memcpy(&x, e, 16);
     return x;
 }
-// Operand of step `step` straight from memory: channels 16 step + 8 (l / 32) ... of the lane's row.
-template <typename T>
-__device__ __forceinline__ Eight<T> row_operand(const T* row, bool there, int step, int dim, int wide, int lane) {
-    uint4 x[sizeof(T) / 2];
-    constexpr int E = 16 / sizeof(T);
+// Operands of all steps straight from memory: channels 16 step + 8 (l / 32) ... of the lane's row.
+template <typename T, int DP>
+__device__ __forceinline__ void row_operands(Eight<T> (&y)[DP / 16], const T* row, bool there, int dim, int wide, int lane) {
+    constexpr int E = 16 / sizeof(T), EACH = sizeof(T) / 2;
+    u32x4 x[DP / 16 * EACH];
 #pragma unroll
-    for (int n = 0; n < (int)sizeof(T) / 2; n++) {
-        x[n] = uint4{0, 0, 0, 0};
-        if (there) x[n] = piece_of<T>(row, 16 * step + 8 * (lane >> 5) + n * E, dim, wide);
+    for (int n = 0; n < DP / 16 * EACH; n++) x[n] = u32x4{0, 0, 0, 0};
+    if (there) {
+        const int first = 8 * (lane >> 5);
+        if (wide) {
+#pragma unroll
+            for (int n = 0; n < DP / 16 * EACH; n++) {
+                const int from = 16 * (n / EACH) + first + n % EACH * E;
+                if (from < dim) x[n] = *reinterpret_cast<const u32x4*>(row + from);
+            }
+        } else {
+#pragma unroll
+            for (int n = 0; n < DP / 16 * EACH; n++) x[n] = elements_of<T>(row, 16 * (n / EACH) + first + n % EACH * E, dim);
+        }
     }
-    Eight<T> y;
-    __builtin_memcpy(&y, x, sizeof(y));
-    return y;
+    __builtin_memcpy(y, x, sizeof(x));
 }
+
+// Which of the next keys are there: a bit for each, of the mask's bytes on their way (lane l: key l), or of their number.
+struct KeyBits {
+    uint32_t byte = 0;
+    int left = 0;
+    __device__ __forceinline__ void load(const uint8_t* mask, int left_, int lane) {
+        left = left_;
+        if (mask) byte = __builtin_amdgcn_raw_buffer_load_b8(buffer(mask, left < 0 ? 0 : left), lane, 0, 0);
+    }
+    __device__ __forceinline__ uint64_t get(const uint8_t* mask) const {
+        if (mask) return __ballot((byte & 255) != 0);
+        return left >= 64 ? ~0ull : left <= 0 ? 0ull : (1ull << left) - 1;
+    }
+};
 
 // ROWS rows on their way into a tile through the registers of THREADS lanes.  A row that is not there is 0 in LDS: what memory holds
 // in its place, infinities and NaN among it, meets no product.
 template <typename T, int DP, int ROWS, int THREADS>
 struct Staged {
     using L = Tile<T, DP>;
-    static constexpr int ALL = ROWS * L::PIECES, EACH = (ALL + THREADS - 1) / THREADS;
-    uint4 x[EACH];
-    __device__ __forceinline__ void load(const T* first, int64_t stride, int there, const uint8_t* mask, int dim, int wide, int thread) {
+    static constexpr int ALL = ROWS * L::PIECES, EACH = (ALL + THREADS - 1) / THREADS, EVERY = THREADS / L::PIECES;
+    static_assert(THREADS % L::PIECES == 0, "a lane has one piece of several rows");
+    u32x4 x[EACH];
+    __device__ __forceinline__ void load(const T* first, int64_t stride, int there, int dim, int wide, int thread) {
+        const int row = thread / L::PIECES, piece = thread % L::PIECES;
+        if (wide) {
+            const int rows = there < ROWS ? there : ROWS, step = (int)stride * (int)sizeof(T);
+            const auto from = buffer(first, rows <= 0 ? 0 : (rows - 1) * step + dim * (int)sizeof(T));
+            const int at = piece * L::E < dim && row < ROWS ? row * step + piece * 16 : BEYOND;
 #pragma unroll
-        for (int n = 0; n < EACH; n++) {
-            const int at = thread + n * THREADS, row = at / L::PIECES, piece = at % L::PIECES;
-            x[n] = uint4{0, 0, 0, 0};
-            if (at < ALL && row < there && (!mask || mask[row])) x[n] = piece_of<T>(first + row * stride, piece * L::E, dim, wide);
+            for (int n = 0; n < EACH; n++) x[n] = __builtin_amdgcn_raw_buffer_load_b128(from, at + n * EVERY * step, 0, 0);
+        } else {
+#pragma unroll
+            for (int n = 0; n < EACH; n++) {
+                x[n] = u32x4{0, 0, 0, 0};
+                if (row + n * EVERY < ROWS && row + n * EVERY < there) x[n] = elements_of<T>(first + (row + n * EVERY) * stride, piece * L::E, dim);
+            }
         }
     }
-    __device__ __forceinline__ void store(char* tile, int thread) const {
+    // rows whose bit is 0 are not there
+    __device__ __forceinline__ void store(char* tile, int thread, uint64_t bits = ~0ull) const {
+        const int row = thread / L::PIECES, piece = thread % L::PIECES;
+        const bool whole = bits == ~0ull;
 #pragma unroll
         for (int n = 0; n < EACH; n++) {
-            const int at = thread + n * THREADS, row = at / L::PIECES, piece = at % L::PIECES;
-            if (at < ALL) *reinterpret_cast<uint4*>(tile + L::place(row & ~15, row & 15, piece)) = x[n];
+            const int r = row + n * EVERY;
+            if (ALL % THREADS != 0 && r >= ROWS) continue;
+            const bool keep = whole || (bits >> (r & 63) & 1);
+            *reinterpret_cast<u32x4*>(tile + L::place(r & ~15, r & 15, piece)) = keep ? x[n] : u32x4{0, 0, 0, 0};
         }
     }
 };
@@ -289,12 +328,6 @@ __device__ __forceinline__ void fill_line(const SequenceAttention& A, int head, 
 __device__ __forceinline__ float other_half_max(float x) { float a, b; swap32(x, a, b); return fmaxf(a, b); }
 __device__ __forceinline__ float other_half_sum(float x) { float a, b; swap32(x, a, b); return a + b; }
 
-// Which of the 32 keys of a tile are there, as the bits of a word.
-__device__ __forceinline__ uint32_t keys_there(int left, const uint8_t* mask, int lane) {
-    const int j = lane & 31;
-    return (uint32_t)__ballot(lane < 32 && j < left && (!mask || mask[j]));
-}
-
 // Running maximum, sum and weighted sum of one column.  The maximum that the powers are relative to follows the true one when that is
 // more than 2^8 ahead: the sums are scaled anew in few tiles only, and no power is above 2^8.
 template <int DP>
@@ -412,8 +445,7 @@ __global__ __launch_bounds__(NW * 64) void few_kernel(SequenceAttention A, T* ou
 
     Eight<T> qf[DP / 16];
     const T* const q_row = row_start<T>(A.q, q, A.packed, mine ? h : 0) + (mine ? i : 0) * A.q.row;
-#pragma unroll
-    for (int s = 0; s < DP / 16; s++) qf[s] = row_operand<T>(q_row, mine, s, A.dim, A.q.wide, lane);
+    row_operands<T, DP>(qf, q_row, mine, A.dim, A.q.wide, lane);
     const T* const k_at = row_start<T>(A.k, k, A.packed, kh);
     const T* const v_at = row_start<T>(A.v, k, A.packed, kh);
     const uint8_t* const mask = A.mask ? A.mask + k.first : nullptr;
@@ -426,20 +458,22 @@ __global__ __launch_bounds__(NW * 64) void few_kernel(SequenceAttention A, T* ou
     char* const vt = kt + FewLds<T, DP, NW>::TILE;
     Running<DP> sum;
     Staged<T, DP, 32, 64> kx, vx;
+    KeyBits bits;
     auto fetch = [&](int n) {
         const int j0 = n * 32;
-        const uint8_t* const m = mask ? mask + j0 : nullptr;
-        kx.load(k_at + j0 * A.k.row, A.k.row, k.there - j0, m, A.dim, A.k.wide, lane);
-        vx.load(v_at + j0 * A.v.row, A.v.row, k.there - j0, m, A.dim, A.v.wide, lane);
+        bits.load(mask ? mask + j0 : nullptr, min(k.there - j0, 32), lane);
+        kx.load(k_at + j0 * A.k.row, A.k.row, k.there - j0, A.dim, A.k.wide, lane);
+        vx.load(v_at + j0 * A.v.row, A.v.row, k.there - j0, A.dim, A.v.wide, lane);
     };
     if (first + wave < end) fetch(first + wave);
     for (int n = first + wave; n < end; n += NW) {
         const int j0 = n * 32;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        kx.store(kt, lane);
-        vx.store(vt, lane);
+        const uint32_t there = (uint32_t)bits.get(mask);
+        const uint64_t rows = mask ? there | ~0xffffffffull : ~0ull;      // (rows behind the last are 0 already)
+        kx.store(kt, lane, rows);
+        vx.store(vt, lane, rows);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        const uint32_t there = keys_there(k.there - j0, mask ? mask + j0 : nullptr, lane);
         if (n + NW < end) fetch(n + NW);
         f32x16 s;
 #pragma unroll
@@ -583,23 +617,26 @@ __global__ __launch_bounds__(NW * 64) void tiles_kernel(SequenceAttention A, T* 
 
     Eight<T> qf[DP / 16];
     const T* const q_row = row_start<T>(A.q, q, A.packed, h) + (mine ? i : 0) * A.q.row;
-#pragma unroll
-    for (int s = 0; s < DP / 16; s++) qf[s] = row_operand<T>(q_row, mine, s, A.dim, A.q.wide, lane);
+    row_operands<T, DP>(qf, q_row, mine, A.dim, A.q.wide, lane);
     const T* const k_at = row_start<T>(A.k, k, A.packed, kh);
     const T* const v_at = row_start<T>(A.v, k, A.packed, kh);
     const uint8_t* const mask = A.mask ? A.mask + k.first : nullptr;
     if (BIAS) fill_line<T, BIAS>(A, h, line, threadIdx.x, NW * 64);
     Running<DP> sum;
     Staged<T, DP, KEYS, NW * 64> kx, vx;
+    KeyBits bits;
+    uint64_t there = 0;                         // keys of the tile in LDS
     auto fetch = [&](int n) {
         const int j0 = n * KEYS;
-        const uint8_t* const m = mask ? mask + j0 : nullptr;
-        kx.load(k_at + j0 * A.k.row, A.k.row, k.there - j0, m, A.dim, A.k.wide, threadIdx.x);
-        vx.load(v_at + j0 * A.v.row, A.v.row, k.there - j0, m, A.dim, A.v.wide, threadIdx.x);
+        bits.load(mask ? mask + j0 : nullptr, min(k.there - j0, KEYS), lane);
+        kx.load(k_at + j0 * A.k.row, A.k.row, k.there - j0, A.dim, A.k.wide, threadIdx.x);
+        vx.load(v_at + j0 * A.v.row, A.v.row, k.there - j0, A.dim, A.v.wide, threadIdx.x);
     };
     auto put = [&](int n) {
-        kx.store(tiles + (n & 1) * 2 * TILE, threadIdx.x);
-        vx.store(tiles + (n & 1) * 2 * TILE + TILE, threadIdx.x);
+        there = bits.get(mask);
+        const uint64_t rows = mask ? there | (KEYS < 64 ? ~0ull << (KEYS & 63) : 0ull) : ~0ull;      // (rows behind the last are 0 already)
+        kx.store(tiles + (n & 1) * 2 * TILE, threadIdx.x, rows);
+        vx.store(tiles + (n & 1) * 2 * TILE + TILE, threadIdx.x, rows);
     };
     if (count > 0) {
         fetch(0);
@@ -613,21 +650,24 @@ __global__ __launch_bounds__(NW * 64) void tiles_kernel(SequenceAttention A, T* 
         f32x16 s[KEYS / 32];
         float top = NONE;
 #pragma unroll
-        for (int u = 0; u < KEYS / 32; u++) {
-            const int j0 = n * KEYS + 32 * u;
+        for (int u = 0; u < KEYS / 32; u++)
 #pragma unroll
             for (int r = 0; r < 16; r++) s[u][r] = 0.0f;
 #pragma unroll
-            for (int c = 0; c < DP / 16; c++) s[u] = Operand<T>::product(L::rows(kt, 32 * u, c, lane), qf[c], s[u]);
-            const uint32_t there = keys_there(k.there - j0, mask ? mask + j0 : nullptr, lane);
+        for (int c = 0; c < DP / 16; c++)
+#pragma unroll
+            for (int u = 0; u < KEYS / 32; u++) s[u] = Operand<T>::product(L::rows(kt, 32 * u, c, lane), qf[c], s[u]);
+#pragma unroll
+        for (int u = 0; u < KEYS / 32; u++) {
+            const int j0 = n * KEYS + 32 * u;
             const int low = j0 - (i0 + 31) - shift, high = j0 + 31 - i0 - shift;
             const bool causal = A.causal && high > 0;
             if (!BIAS || low >= A.reach || high <= -A.reach) {
                 const float flat = BIAS ? line[low >= A.reach ? 2 * (A.reach + MARGIN) : 0] : 0.0f;
-                scores<T, BIAS>(s[u], score, there, causal, i + shift - j0, lane, [&](int) { return flat; });
+                scores<T, BIAS>(s[u], score, (uint32_t)(there >> 32 * u), causal, i + shift - j0, lane, [&](int) { return flat; });
             } else {
                 const float* const at = line + (j0 + 4 * half - i - shift + A.reach + MARGIN);
-                scores<T, BIAS>(s[u], score, there, causal, i + shift - j0, lane, [&](int r) { return at[result_row(r)]; });
+                scores<T, BIAS>(s[u], score, (uint32_t)(there >> 32 * u), causal, i + shift - j0, lane, [&](int r) { return at[result_row(r)]; });
             }
 #pragma unroll
             for (int r = 0; r < 16; r++) top = fmaxf(top, s[u][r]);
@@ -726,14 +766,14 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
         const T* const g_row = row_start<T>(G.go, q, A.packed, h) + (mine ? i : 0) * G.go.row;
         const T* const o_row = static_cast<const T*>(G.out) + (mine ? row : 0) * A.dim;
         const int o_wide = A.dim % L::E == 0;
+        Eight<T> of[DP / 16];
+        row_operands<T, DP>(qf, q_row, mine, A.dim, A.q.wide, lane);
+        row_operands<T, DP>(gf, g_row, mine, A.dim, G.go.wide, lane);
+        row_operands<T, DP>(of, o_row, mine, A.dim, o_wide, lane);
 #pragma unroll
-        for (int s = 0; s < DP / 16; s++) {
-            qf[s] = row_operand<T>(q_row, mine, s, A.dim, A.q.wide, lane);
-            gf[s] = row_operand<T>(g_row, mine, s, A.dim, G.go.wide, lane);
-            const Eight<T> of = row_operand<T>(o_row, mine, s, A.dim, o_wide, lane);
+        for (int s = 0; s < DP / 16; s++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) D = __builtin_fmaf(to_float(gf[s][e]), to_float(of[e]), D);
-        }
+            for (int e = 0; e < 8; e++) D = __builtin_fmaf(to_float(gf[s][e]), to_float(of[s][e]), D);
         D = other_half_sum(D);
     }
     float m = -NONE, inverse = 0.0f;
@@ -759,15 +799,19 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
 #pragma unroll
         for (int r = 0; r < 16; r++) dq[d][r] = 0.0f;
     Staged<T, DP, KEYS, NW * 64> kx, vx;
+    KeyBits bits;
+    uint64_t there = 0;                         // keys of the tile in LDS
     auto fetch = [&](int n) {
         const int j0 = n * KEYS;
-        const uint8_t* const mk = mask ? mask + j0 : nullptr;
-        kx.load(k_at + j0 * A.k.row, A.k.row, k.there - j0, mk, A.dim, A.k.wide, threadIdx.x);
-        vx.load(v_at + j0 * A.v.row, A.v.row, k.there - j0, mk, A.dim, A.v.wide, threadIdx.x);
+        bits.load(mask ? mask + j0 : nullptr, min(k.there - j0, KEYS), lane);
+        kx.load(k_at + j0 * A.k.row, A.k.row, k.there - j0, A.dim, A.k.wide, threadIdx.x);
+        vx.load(v_at + j0 * A.v.row, A.v.row, k.there - j0, A.dim, A.v.wide, threadIdx.x);
     };
     auto put = [&](int n) {
-        kx.store(tiles + (n & 1) * 2 * TILE, threadIdx.x);
-        vx.store(tiles + (n & 1) * 2 * TILE + TILE, threadIdx.x);
+        there = bits.get(mask);
+        const uint64_t rows = mask ? there | (KEYS < 64 ? ~0ull << (KEYS & 63) : 0ull) : ~0ull;      // (rows behind the last are 0 already)
+        kx.store(tiles + (n & 1) * 2 * TILE, threadIdx.x, rows);
+        vx.store(tiles + (n & 1) * 2 * TILE + TILE, threadIdx.x, rows);
     };
     if (first < end) {
         fetch(first);
@@ -786,15 +830,14 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
         for (int c = 0; c < DP / 16; c++) s = Operand<T>::product(L::rows(kt, 0, c, lane), qf[c], s);
 #pragma unroll
         for (int c = 0; c < DP / 16; c++) dp = Operand<T>::product(L::rows(vt, 0, c, lane), gf[c], dp);
-        const uint32_t there = keys_there(k.there - j0, mask ? mask + j0 : nullptr, lane);
         const int low = j0 - (i0 + 31) - shift, high = j0 + 31 - i0 - shift, r0 = j0 + 4 * half - i - shift;
         const bool causal = A.causal && high > 0, beyond = low >= A.reach || high <= -A.reach;
         if (!BIAS || beyond) {
             const float flat = BIAS ? line[low >= A.reach ? 2 * (A.reach + MARGIN) : 0] : 0.0f;
-            scores<T, BIAS>(s, score, there, causal, i + shift - j0, lane, [&](int) { return flat; });
+            scores<T, BIAS>(s, score, (uint32_t)there, causal, i + shift - j0, lane, [&](int) { return flat; });
         } else {
             const float* const at = line + (r0 + A.reach + MARGIN);
-            scores<T, BIAS>(s, score, there, causal, i + shift - j0, lane, [&](int r) { return at[result_row(r)]; });
+            scores<T, BIAS>(s, score, (uint32_t)there, causal, i + shift - j0, lane, [&](int r) { return at[result_row(r)]; });
         }
         if (!BIAS) {
 #pragma unroll
@@ -930,11 +973,8 @@ __global__ __launch_bounds__(NW * 64) void keys_kernel(SequenceAttention A, Atte
     {
         const T* const k_row = row_start<T>(A.k, k, A.packed, kh) + (mine ? j : 0) * A.k.row;
         const T* const v_row = row_start<T>(A.v, k, A.packed, kh) + (mine ? j : 0) * A.v.row;
-#pragma unroll
-        for (int s = 0; s < DP / 16; s++) {
-            kf[s] = row_operand<T>(k_row, mine, s, A.dim, A.k.wide, lane);
-            vf[s] = row_operand<T>(v_row, mine, s, A.dim, A.v.wide, lane);
-        }
+        row_operands<T, DP>(kf, k_row, mine, A.dim, A.k.wide, lane);
+        row_operands<T, DP>(vf, v_row, mine, A.dim, A.v.wide, lane);
     }
     f32x16 dk[DP / 32], dv[DP / 32];
     Scaled<T, DP> scaled;
@@ -946,8 +986,8 @@ __global__ __launch_bounds__(NW * 64) void keys_kernel(SequenceAttention A, Atte
     float sx[3];
     auto fetch = [&](int n) {
         const int h = kh * A.share + n / each, i0 = (skip + n % each) * ROWS;
-        qx.load(row_start<T>(A.q, q, A.packed, h) + i0 * A.q.row, A.q.row, q.there - i0, nullptr, A.dim, A.q.wide, threadIdx.x);
-        gx.load(row_start<T>(G.go, q, A.packed, h) + i0 * G.go.row, G.go.row, q.there - i0, nullptr, A.dim, G.go.wide, threadIdx.x);
+        qx.load(row_start<T>(A.q, q, A.packed, h) + i0 * A.q.row, A.q.row, q.there - i0, A.dim, A.q.wide, threadIdx.x);
+        gx.load(row_start<T>(G.go, q, A.packed, h) + i0 * G.go.row, G.go.row, q.there - i0, A.dim, G.go.wide, threadIdx.x);
         if (threadIdx.x < ROWS) {
             float m = -NONE, inverse = 0.0f, D = 0.0f;
             if (i0 + (int)threadIdx.x < q.there) {

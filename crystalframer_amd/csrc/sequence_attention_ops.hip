@@ -54,12 +54,12 @@ int check_attention(const cfh_attention* a) {
     return CFH_OK;
 }
 
-// 16 bytes at a time: where they begin at multiples of 16 and hold whole rows of channels.
+// 16 bytes at a time: where they begin at multiples of 16 and hold whole rows of channels, and 64 rows are less than 2^30 bytes.
 cfh::AttentionRows rows_of(const void* at, const int64_t* stride, int dtype, int dim) {
     const int64_t bytes = dtype == CFH_FLOAT32 ? 4 : 2;
     uint64_t all = (uint64_t)(uintptr_t)at | (uint64_t)(dim * bytes);
     for (int n = 0; n < 3; n++) all |= (uint64_t)(stride[n] * bytes);
-    return {at, stride[0], stride[1], stride[2], (all & 15) == 0};
+    return {at, stride[0], stride[1], stride[2], (all & 15) == 0 && stride[1] * bytes < (1 << 24)};
 }
 
 cfh::SequenceAttention device_args(const cfh_attention* a) {
