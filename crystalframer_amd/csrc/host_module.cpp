@@ -648,8 +648,16 @@ void check_attention(const AttentionTensors& t, const AttentionSpec& s) {
     TORCH_CHECK_VALUE(s.scale == 0.0 || (s.scale > 0.0 && std::isfinite((float)s.scale) && (float)s.scale > 0.0f), "scale ", s.scale, " must be positive and finite");
 }
 
-// t with its channels next to one another.
-at::Tensor with_channels(const at::Tensor& t) { return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+// t as the library reads it: rows of neighbouring channels that begin at multiples of 16 bytes and fill them; others are laid out again.
+at::Tensor aligned_rows(const at::Tensor& t) {
+    const int64_t size = (int64_t)t.element_size(), D = t.size(-1), n = t.dim();
+    uint64_t all = (uint64_t)reinterpret_cast<uintptr_t>(t.data_ptr());
+    for (int64_t d = 0; d + 1 < n; d++)
+        if (t.size(d) > 1) all |= (uint64_t)(t.stride(d) * size);
+    const bool near = t.size(n - 3) <= 1 || t.stride(n - 3) * size < 1 << 24;
+    if (D * size % 16) return at::constant_pad_nd(t, {0, (16 - D * size % 16) / size});
+    return (D == 1 || t.stride(-1) == 1) && !(all & 15) && near ? t : t.clone(at::MemoryFormat::Contiguous);
+}
 // Strides of (batch, row, head); of a dimension that has one entry, 0.
 void strides_of(const at::Tensor& t, int64_t* out) {
     const int64_t n = t.dim();
@@ -662,7 +670,8 @@ void strides_of(const at::Tensor& t, int64_t* out) {
 cfh_attention attention_args(AttentionTensors& t, const AttentionSpec& s) {
     cfh_attention a;
     std::memset(&a, 0, sizeof(a));
-    for (int n : {QUERY, KEY, VALUE}) t[n] = with_channels(t[n]);
+    const int64_t channels = t[QUERY].size(-1);
+    for (int n : {QUERY, KEY, VALUE}) t[n] = aligned_rows(t[n]);
     for (int n = TABLE; n < ATTENTION_TENSORS; n++)
         if (t[n].defined()) t[n] = t[n].contiguous();
     const at::Tensor &q = t[QUERY], &k = t[KEY];
@@ -671,7 +680,7 @@ cfh_attention attention_args(AttentionTensors& t, const AttentionSpec& s) {
     a.packed = q.dim() == 3;
     a.causal = s.causal; a.queries_last = s.last;
     a.batch = (int32_t)(a.packed ? t[QUERY_STARTS].size(0) - 1 : q.size(0));
-    a.heads = (int32_t)q.size(-2); a.kv_heads = (int32_t)k.size(-2); a.dim = (int32_t)q.size(-1);
+    a.heads = (int32_t)q.size(-2); a.kv_heads = (int32_t)k.size(-2); a.dim = (int32_t)channels;
     a.scale = s.scale == 0.0 ? (float)(1.0 / std::sqrt((double)a.dim)) : (float)s.scale;
     a.query_rows = q.size(-3); a.key_rows = k.size(-3);
     strides_of(q, a.q_stride);
@@ -729,7 +738,7 @@ struct SequenceAttentionBackward : public torch::autograd::Node {
                 dv = at::empty(t[KEY].sizes(), o.options());
             }
             if (wanted[TABLE]) dtable = at::empty(t[TABLE].sizes(), t[TABLE].options());
-            const at::Tensor go = with_channels(grads[0].detach());
+            const at::Tensor go = aligned_rows(grads[0].detach());
             const cfh_attention a = attention_args(t, spec);
             int64_t go_stride[3];
             strides_of(go, go_stride);

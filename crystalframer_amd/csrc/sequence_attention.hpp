@@ -71,53 +71,62 @@ template <typename T> constexpr float POWER_LIFT = NARROW<T> ? 6.0f : 0.0f;
 template <typename T> constexpr float P_LIFT = NARROW<T> ? 15.0f : 0.0f;
 
 // ---- tiles in LDS: rows of DP channels in pieces of 16 bytes, whose places are exchanged by the row so that 16 rows of one piece, and
-// the pieces of one transposed read, lie in different banks -------------------------------------------------------------------------
+// the pieces of one transposed read, lie in different banks (no conflict counted in any kernel) ----------------------------------------
+// A lane's address is made once per tile; what changes inside a tile is exclusive-ored into it or lies in the instruction's offset, which
+// leaves registers to the sums.  Tiles begin at multiples of their rows' length.
+typedef __attribute__((address_space(3))) char lds_char;
+__device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_t)(uintptr_t)(lds_char*)p; }
+template <typename V>
+__device__ __forceinline__ V lds_read(uint32_t at) { return *reinterpret_cast<__attribute__((address_space(3))) const V*>(at); }
+
 template <typename T, int DP>
 struct Tile {
     static constexpr int E = 16 / sizeof(T), PIECES = DP / E, ROW = DP * sizeof(T);
-    static __device__ __forceinline__ int mixed(int row) {
+    static __device__ __forceinline__ constexpr int mixed(int row) {
         if (sizeof(T) == 4) return PIECES >= 16 ? ((row >> 2 & 1) << 3 | (row & 3) << 1 | (row >> 3 & 1)) : (row >> 1 & 7);
         if (PIECES == 16) return (row & 3) << 2 | (row >> 2 & 3);
         if (PIECES == 8) return (row >> 1 & 1) << 2 | (row >> 2 & 3);
         return row >> 2 & 3;
     }
-    // (base: a multiple of 16)
-    static __device__ __forceinline__ int place(int base, int row, int piece) { return base * ROW + row * ROW + ((piece ^ mixed(row)) << 4); }
+    static __device__ __forceinline__ int place(int row, int piece) { return row * ROW + ((piece ^ mixed(row)) << 4); }
+    // The lane's part of an address for rows() and columns().
+    static __device__ __forceinline__ uint32_t rows_at(int lane) { return place(lane & 31, (lane >> 5) * (sizeof(T) / 2)); }
+    static __device__ __forceinline__ uint32_t columns_at(int lane) {
+        const int half = lane >> 5;
+        if (sizeof(T) == 2) return place(4 * half + (lane & 15) / 4, 2 * (lane >> 4 & 1) + (lane & 3) / 2) + (lane & 1) * 8;
+        return place(4 * half, (lane & 31) / 4) + (lane & 3) * 4;
+    }
     // Channels 16 step + 8 (l / 32) ... of row base + l % 32.
-    static __device__ __forceinline__ Eight<T> rows(const char* tile, int base, int step, int lane) {
-        const int row = lane & 31, half = lane >> 5;
+    static __device__ __forceinline__ Eight<T> rows(uint32_t at, int base, int step) {
         if constexpr (sizeof(T) == 2) {
-            return *reinterpret_cast<const Eight<T>*>(tile + place(base, row, 2 * step + half));
+            return lds_read<Eight<T>>((at ^ step << 5) + base * ROW);
         } else {
-            const f32x4 a = *reinterpret_cast<const f32x4*>(tile + place(base, row, 4 * step + 2 * half));
-            const f32x4 b = *reinterpret_cast<const f32x4*>(tile + place(base, row, 4 * step + 2 * half + 1));
+            const f32x4 a = lds_read<f32x4>((at ^ step << 6) + base * ROW), b = lds_read<f32x4>((at ^ (step << 6 | 16)) + base * ROW);
             return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
         }
     }
     // Channel 32 d + l % 32 of rows base + 8 (e / 4) + 4 (l / 32) + e % 4.
-    static __device__ __forceinline__ Eight<T> columns(const char* tile, int base, int d, int lane) {
-        const int half = lane >> 5;
+    static __device__ __forceinline__ Eight<T> columns(uint32_t at, int base, int d) {
         if constexpr (sizeof(T) == 2) {
-            const int row = 4 * half + (lane & 15) / 4, piece = 4 * d + 2 * (lane >> 4 & 1) + (lane & 3) / 2, in = (lane & 1) * 8;
-            auto* a = (__attribute__((address_space(3))) char*)(tile);
-            const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a + place(base, row, piece) + in));
-            const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a + place(base, row + 8, piece) + in));
+            const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4*>((at ^ d << 6) + base * ROW));
+            const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4*>((at ^ (d << 6 | 32)) + (base + 8) * ROW));
             typedef short s16x8 __attribute__((ext_vector_type(8)));
             return __builtin_bit_cast(Eight<T>, s16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]});
         } else {
             f32x8 x;
-            const int c = 32 * d + (lane & 31);
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-                x[e] = *reinterpret_cast<const float*>(tile + place(base, 8 * (e / 4) + 4 * half + e % 4, c / 4) + (c % 4) * 4);
+            for (int e = 0; e < 8; e++) {      // (the row's part in the exchange: 4 (l / 32) is in the lane's, 8 (e / 4) + e % 4 here)
+                const int row = 8 * (e / 4) + e % 4;
+                x[e] = lds_read<float>((at ^ (d << 7 | mixed(row) << 4)) + (base + row) * ROW);
+            }
             return x;
         }
     }
 };
 
 // ---- rows in memory ------------------------------------------------------------------------------------------------------------------
-// Where rows lie at multiples of 16 bytes they are read as pieces of a buffer that ends behind the last row that is there: what is
-// beyond comes back as 0, without a branch.  Others are read element by element.
+// Rows lie at multiples of 16 bytes and are read as pieces of a buffer that ends behind the last row that is there: what is beyond
+// comes back as 0, without a branch.  (A last piece that the row's channels do not fill is filled with zeros in memory.)
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr int BEYOND = 0x40000000;      // behind any buffer here
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* at, int bytes) {
@@ -134,27 +143,33 @@ __device__ __forceinline__ u32x4 elements_of(const T* row, int from, int dim) {
     __builtin_memcpy(&x, e, 16);
     return x;
 }
-// Operands of all steps straight from memory: channels 16 step + 8 (l / 32) ... of the lane's row.
+// Operands of all steps straight from memory: channels 16 step + 8 (l / 32) ... of the lane's row.  `whole`: of rows as above.
 template <typename T, int DP>
-__device__ __forceinline__ void row_operands(Eight<T> (&y)[DP / 16], const T* row, bool there, int dim, int wide, int lane) {
+__device__ __forceinline__ void row_operands(Eight<T> (&y)[DP / 16], const T* row, bool there, int dim, bool whole, int lane) {
     constexpr int E = 16 / sizeof(T), EACH = sizeof(T) / 2;
     u32x4 x[DP / 16 * EACH];
 #pragma unroll
     for (int n = 0; n < DP / 16 * EACH; n++) x[n] = u32x4{0, 0, 0, 0};
     if (there) {
         const int first = 8 * (lane >> 5);
-        if (wide) {
 #pragma unroll
-            for (int n = 0; n < DP / 16 * EACH; n++) {
-                const int from = 16 * (n / EACH) + first + n % EACH * E;
+        for (int n = 0; n < DP / 16 * EACH; n++) {
+            const int from = 16 * (n / EACH) + first + n % EACH * E;
+            if (whole) {
                 if (from < dim) x[n] = *reinterpret_cast<const u32x4*>(row + from);
+            } else {
+                x[n] = elements_of<T>(row, from, dim);
             }
-        } else {
-#pragma unroll
-            for (int n = 0; n < DP / 16 * EACH; n++) x[n] = elements_of<T>(row, 16 * (n / EACH) + first + n % EACH * E, dim);
         }
     }
     __builtin_memcpy(y, x, sizeof(x));
+}
+
+// Waits for operands here.  (Left to their first use, in the loop, the wait would also be for the tile that was asked for last.)
+template <typename T, int N>
+__device__ __forceinline__ void settle(Eight<T> (&y)[N]) {
+#pragma unroll
+    for (int n = 0; n < N; n++) asm volatile("" : "+v"(y[n]));
 }
 
 // Which of the next keys are there: a bit for each, of the mask's bytes on their way (lane l: key l), or of their number.
@@ -179,21 +194,13 @@ struct Staged {
     static constexpr int ALL = ROWS * L::PIECES, EACH = (ALL + THREADS - 1) / THREADS, EVERY = THREADS / L::PIECES;
     static_assert(THREADS % L::PIECES == 0, "a lane has one piece of several rows");
     u32x4 x[EACH];
-    __device__ __forceinline__ void load(const T* first, int64_t stride, int there, int dim, int wide, int thread) {
+    __device__ __forceinline__ void load(const T* first, int64_t stride, int there, int dim, int thread) {
         const int row = thread / L::PIECES, piece = thread % L::PIECES;
-        if (wide) {
-            const int rows = there < ROWS ? there : ROWS, step = (int)stride * (int)sizeof(T);
-            const auto from = buffer(first, rows <= 0 ? 0 : (rows - 1) * step + dim * (int)sizeof(T));
-            const int at = piece * L::E < dim && row < ROWS ? row * step + piece * 16 : BEYOND;
+        const int rows = there < ROWS ? there : ROWS, step = (int)stride * (int)sizeof(T), last = (dim + L::E - 1) / L::E * 16;
+        const auto from = buffer(first, rows <= 0 ? 0 : (rows - 1) * step + last);
+        const int at = piece * 16 < last && row < ROWS ? row * step + piece * 16 : BEYOND;
 #pragma unroll
-            for (int n = 0; n < EACH; n++) x[n] = __builtin_amdgcn_raw_buffer_load_b128(from, at + n * EVERY * step, 0, 0);
-        } else {
-#pragma unroll
-            for (int n = 0; n < EACH; n++) {
-                x[n] = u32x4{0, 0, 0, 0};
-                if (row + n * EVERY < ROWS && row + n * EVERY < there) x[n] = elements_of<T>(first + (row + n * EVERY) * stride, piece * L::E, dim);
-            }
-        }
+        for (int n = 0; n < EACH; n++) x[n] = __builtin_amdgcn_raw_buffer_load_b128(from, at + n * EVERY * step, 0, 0);
     }
     // rows whose bit is 0 are not there
     __device__ __forceinline__ void store(char* tile, int thread, uint64_t bits = ~0ull) const {
@@ -204,7 +211,7 @@ struct Staged {
             const int r = row + n * EVERY;
             if (ALL % THREADS != 0 && r >= ROWS) continue;
             const bool keep = whole || (bits >> (r & 63) & 1);
-            *reinterpret_cast<u32x4*>(tile + L::place(r & ~15, r & 15, piece)) = keep ? x[n] : u32x4{0, 0, 0, 0};
+            *reinterpret_cast<u32x4*>(tile + L::place(r, piece)) = keep ? x[n] : u32x4{0, 0, 0, 0};
         }
     }
 };
@@ -252,11 +259,11 @@ __device__ __forceinline__ Span span_of(const int64_t* starts, const int64_t* si
     return s;
 }
 // Sequence and first row in it of slot w; false: none.
-__device__ __forceinline__ bool find_slot(const int64_t* starts, int64_t rows, int packed, int batch, int tile, int w, int lane, int& b, int& from) {
+__device__ __forceinline__ bool find_slot(const int64_t* starts, int64_t rows, int packed, int batch, int tile, int64_t w, int lane, int& b, int& from) {
     if (!packed) {
         const int per = (int)((rows + tile - 1) / tile);
-        b = w / per;
-        from = (w - b * per) * tile;
+        b = (int)(w / per);
+        from = (int)(w - (int64_t)b * per) * tile;
         return b < batch;
     }
     auto base = [&](int n) { return (n == 0 ? 0 : between(starts[n], 0, rows) / tile) + n; };
@@ -276,10 +283,24 @@ __device__ __forceinline__ bool find_slot(const int64_t* starts, int64_t rows, i
     from = (int)at;
     return true;
 }
-// Workgroups that follow one another on one of the 8 dies: they share what its cache holds.
-__device__ __forceinline__ int64_t die_order(int64_t id, int64_t count) {
-    const int64_t per = (count + 7) / 8;
-    return (id & 7) * per + (id >> 3);
+// Head and slot of a workgroup (false: none).  Workgroups that follow one another on one of the 8 dies share what its cache holds: the
+// tiles of a head.  Causal tiles differ in their work: a die takes its sequences' and heads' longest ones first.
+__device__ __forceinline__ bool workgroup_item(int64_t id, int64_t slots, int heads, const SequenceAttention& A, bool last_first, int& head, int64_t& slot) {
+    const int64_t count = slots * heads, pairs = (int64_t)A.batch * heads;
+    if (A.causal && !A.packed && (pairs & 7) == 0) {
+        const int64_t mine = pairs / 8, tiles = slots / A.batch, local = id >> 3, pair = (id & 7) * mine + local % mine;
+        int64_t tile = local / mine;
+        if (tile >= tiles) return false;
+        if (last_first) tile = tiles - 1 - tile;
+        head = (int)(pair / A.batch);
+        slot = (pair - (int64_t)head * A.batch) * tiles + tile;
+        return true;
+    }
+    const int64_t at = (id & 7) * ((count + 7) / 8) + (id >> 3);
+    if (at >= count) return false;
+    head = (int)(at / slots);
+    slot = at - head * slots;
+    return true;
 }
 
 template <typename T>
@@ -414,12 +435,12 @@ template <typename T, int DP, int NW>
 struct FewLds {
     static constexpr int TILE = 32 * Tile<T, DP>::ROW, SUM = 32 * (DP + 4) * 4;
     static constexpr int EACH = 2 * TILE > SUM ? 2 * TILE : SUM;
-    char wave[NW][EACH];
+    alignas(512) char wave[NW][(EACH + 511) / 512 * 512];
     float m[NW][32], l[NW][32];
 };
 
 template <typename T, int DP, int NW, bool BIAS>
-__global__ __launch_bounds__(NW * 64) void few_kernel(SequenceAttention A, T* out, float* stats, float* part_o, float* part_ml, int splits) {
+__global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && NW == 4 ? 2 : 1)) void few_kernel(SequenceAttention A, T* out, float* stats, float* part_o, float* part_ml, int splits) {
     using L = Tile<T, DP>;
     __shared__ __attribute__((aligned(16))) FewLds<T, DP, NW> S;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
@@ -445,7 +466,7 @@ __global__ __launch_bounds__(NW * 64) void few_kernel(SequenceAttention A, T* ou
 
     Eight<T> qf[DP / 16];
     const T* const q_row = row_start<T>(A.q, q, A.packed, mine ? h : 0) + (mine ? i : 0) * A.q.row;
-    row_operands<T, DP>(qf, q_row, mine, A.dim, A.q.wide, lane);
+    row_operands<T, DP>(qf, q_row, mine, A.dim, true, lane);
     const T* const k_at = row_start<T>(A.k, k, A.packed, kh);
     const T* const v_at = row_start<T>(A.v, k, A.packed, kh);
     const uint8_t* const mask = A.mask ? A.mask + k.first : nullptr;
@@ -456,15 +477,17 @@ __global__ __launch_bounds__(NW * 64) void few_kernel(SequenceAttention A, T* ou
     }
     char* const kt = S.wave[wave];
     char* const vt = kt + FewLds<T, DP, NW>::TILE;
+    const uint32_t kr = lds_address(kt) + L::rows_at(lane), vc = lds_address(vt) + L::columns_at(lane);
     Running<DP> sum;
     Staged<T, DP, 32, 64> kx, vx;
     KeyBits bits;
     auto fetch = [&](int n) {
         const int j0 = n * 32;
         bits.load(mask ? mask + j0 : nullptr, min(k.there - j0, 32), lane);
-        kx.load(k_at + j0 * A.k.row, A.k.row, k.there - j0, A.dim, A.k.wide, lane);
-        vx.load(v_at + j0 * A.v.row, A.v.row, k.there - j0, A.dim, A.v.wide, lane);
+        kx.load(k_at + j0 * A.k.row, A.k.row, k.there - j0, A.dim, lane);
+        vx.load(v_at + j0 * A.v.row, A.v.row, k.there - j0, A.dim, lane);
     };
+    settle<T>(qf);
     if (first + wave < end) fetch(first + wave);
     for (int n = first + wave; n < end; n += NW) {
         const int j0 = n * 32;
@@ -479,7 +502,7 @@ __global__ __launch_bounds__(NW * 64) void few_kernel(SequenceAttention A, T* ou
 #pragma unroll
         for (int r = 0; r < 16; r++) s[r] = 0.0f;
 #pragma unroll
-        for (int c = 0; c < DP / 16; c++) s = Operand<T>::product(L::rows(kt, 0, c, lane), qf[c], s);
+        for (int c = 0; c < DP / 16; c++) s = Operand<T>::product(L::rows(kr, 0, c), qf[c], s);
         const int low = j0 - i_last - shift, high = j0 + 31 - i0 - shift;      // relative positions of the tile
         const int r0 = j0 + 4 * half - i - shift;
         const bool causal = A.causal && high > 0;
@@ -505,7 +528,7 @@ __global__ __launch_bounds__(NW * 64) void few_kernel(SequenceAttention A, T* ou
         for (int c = 0; c < 2; c++) {
             const Eight<T> p = rounded<T>(s, c);
 #pragma unroll
-            for (int d = 0; d < DP / 32; d++) sum.o[d] = Operand<T>::product(L::columns(vt, 16 * c, d, lane), p, sum.o[d]);
+            for (int d = 0; d < DP / 32; d++) sum.o[d] = Operand<T>::product(L::columns(vc, 16 * c, d), p, sum.o[d]);
         }
     }
     // the wavefronts' sums, side by side in LDS
@@ -591,16 +614,17 @@ template <typename T, int NW>
 constexpr int keys_at_once() { return sizeof(T) == 2 && NW >= 4 ? 64 : 32; }
 
 template <typename T, int DP, int NW, bool BIAS>
-__global__ __launch_bounds__(NW * 64) void tiles_kernel(SequenceAttention A, T* out, float* stats, int64_t slots) {
+__global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 ? 2 : 1)) void tiles_kernel(SequenceAttention A, T* out, float* stats, int64_t slots) {
     using L = Tile<T, DP>;
     constexpr int KEYS = keys_at_once<T, NW>(), TILE = KEYS * L::ROW;
-    extern __shared__ __attribute__((aligned(16))) char lds[];
+    extern __shared__ __attribute__((aligned(512))) char lds[];
     char* const tiles = lds;                    // two pairs of a tile of keys and one of values
     float* const line = reinterpret_cast<float*>(lds + 4 * TILE);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, column = lane & 31;
-    const int64_t id = die_order(blockIdx.x, slots * A.heads);
-    if (id >= slots * A.heads) return;
-    const int h = (int)(id / slots), slot = (int)(id - h * slots), kh = h / A.share;
+    int h;
+    int64_t slot;
+    if (!workgroup_item(blockIdx.x, slots, A.heads, A, true, h, slot)) return;
+    const int kh = h / A.share;
     int b, from;
     if (!find_slot(A.q_starts, A.q_rows, A.packed, A.batch, NW * 32, slot, lane, b, from)) return;
     const Span q = span_of(A.q_starts, A.q_sizes, A.q_rows, A.packed, A.batch, b);
@@ -617,7 +641,7 @@ __global__ __launch_bounds__(NW * 64) void tiles_kernel(SequenceAttention A, T* 
 
     Eight<T> qf[DP / 16];
     const T* const q_row = row_start<T>(A.q, q, A.packed, h) + (mine ? i : 0) * A.q.row;
-    row_operands<T, DP>(qf, q_row, mine, A.dim, A.q.wide, lane);
+    row_operands<T, DP>(qf, q_row, mine, A.dim, true, lane);
     const T* const k_at = row_start<T>(A.k, k, A.packed, kh);
     const T* const v_at = row_start<T>(A.v, k, A.packed, kh);
     const uint8_t* const mask = A.mask ? A.mask + k.first : nullptr;
@@ -629,8 +653,8 @@ __global__ __launch_bounds__(NW * 64) void tiles_kernel(SequenceAttention A, T* 
     auto fetch = [&](int n) {
         const int j0 = n * KEYS;
         bits.load(mask ? mask + j0 : nullptr, min(k.there - j0, KEYS), lane);
-        kx.load(k_at + j0 * A.k.row, A.k.row, k.there - j0, A.dim, A.k.wide, threadIdx.x);
-        vx.load(v_at + j0 * A.v.row, A.v.row, k.there - j0, A.dim, A.v.wide, threadIdx.x);
+        kx.load(k_at + j0 * A.k.row, A.k.row, k.there - j0, A.dim, threadIdx.x);
+        vx.load(v_at + j0 * A.v.row, A.v.row, k.there - j0, A.dim, threadIdx.x);
     };
     auto put = [&](int n) {
         there = bits.get(mask);
@@ -638,14 +662,14 @@ __global__ __launch_bounds__(NW * 64) void tiles_kernel(SequenceAttention A, T* 
         kx.store(tiles + (n & 1) * 2 * TILE, threadIdx.x, rows);
         vx.store(tiles + (n & 1) * 2 * TILE + TILE, threadIdx.x, rows);
     };
+    settle<T>(qf);
     if (count > 0) {
         fetch(0);
         put(0);
     }
     __syncthreads();
     for (int n = 0; n < count; n++) {
-        const char* const kt = tiles + (n & 1) * 2 * TILE;
-        const char* const vt = kt + TILE;
+        const uint32_t tile = lds_address(tiles) + (n & 1) * 2 * TILE, kr = tile + L::rows_at(lane), vc = tile + TILE + L::columns_at(lane);
         if (n + 1 < count) fetch(n + 1);
         f32x16 s[KEYS / 32];
         float top = NONE;
@@ -656,7 +680,7 @@ __global__ __launch_bounds__(NW * 64) void tiles_kernel(SequenceAttention A, T* 
 #pragma unroll
         for (int c = 0; c < DP / 16; c++)
 #pragma unroll
-            for (int u = 0; u < KEYS / 32; u++) s[u] = Operand<T>::product(L::rows(kt, 32 * u, c, lane), qf[c], s[u]);
+            for (int u = 0; u < KEYS / 32; u++) s[u] = Operand<T>::product(L::rows(kr, 32 * u, c), qf[c], s[u]);
 #pragma unroll
         for (int u = 0; u < KEYS / 32; u++) {
             const int j0 = n * KEYS + 32 * u;
@@ -685,7 +709,7 @@ __global__ __launch_bounds__(NW * 64) void tiles_kernel(SequenceAttention A, T* 
             for (int c = 0; c < 2; c++) {
                 const Eight<T> p = rounded<T>(s[u], c);
 #pragma unroll
-                for (int d = 0; d < DP / 32; d++) sum.o[d] = Operand<T>::product(L::columns(vt, 32 * u + 16 * c, d, lane), p, sum.o[d]);
+                for (int d = 0; d < DP / 32; d++) sum.o[d] = Operand<T>::product(L::columns(vc, 32 * u + 16 * c, d), p, sum.o[d]);
             }
         }
         if (n + 1 < count) put(n + 1);
@@ -729,15 +753,16 @@ template <typename T, int DP, int NW, bool BIAS>
 __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, AttentionGrads G, int64_t slots, int splits) {
     using L = Tile<T, DP>;
     constexpr int KEYS = 32, TILE = KEYS * L::ROW;
-    extern __shared__ __attribute__((aligned(16))) char lds[];
+    extern __shared__ __attribute__((aligned(512))) char lds[];
     char* const tiles = lds;
     float* const line = reinterpret_cast<float*>(lds + 4 * TILE);
     const int entries = 2 * A.reach + 1;
     float* const sums = line + 2 * (A.reach + MARGIN) + 1;      // (2 NW, entries), then two for each wavefront
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, column = lane & 31;
-    const int64_t total = slots * A.heads, id = die_order(blockIdx.x, total);
-    if (id >= total) return;
-    const int h = (int)(id / slots), slot = (int)(id - h * slots), kh = h / A.share, z = blockIdx.y;
+    int h;
+    int64_t slot;
+    if (!workgroup_item(blockIdx.x, slots, A.heads, A, true, h, slot)) return;
+    const int kh = h / A.share, z = blockIdx.y;
     float* const dtable = BIAS && G.dtable ? G.dtable + (((int64_t)h * splits + z) * slots + slot) * A.buckets : nullptr;
     int b, from;
     bool any = find_slot(A.q_starts, A.q_rows, A.packed, A.batch, NW * 32, slot, lane, b, from);
@@ -765,11 +790,11 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
         const T* const q_row = row_start<T>(A.q, q, A.packed, h) + (mine ? i : 0) * A.q.row;
         const T* const g_row = row_start<T>(G.go, q, A.packed, h) + (mine ? i : 0) * G.go.row;
         const T* const o_row = static_cast<const T*>(G.out) + (mine ? row : 0) * A.dim;
-        const int o_wide = A.dim % L::E == 0;
+        const bool o_whole = A.dim % L::E == 0;
         Eight<T> of[DP / 16];
-        row_operands<T, DP>(qf, q_row, mine, A.dim, A.q.wide, lane);
-        row_operands<T, DP>(gf, g_row, mine, A.dim, G.go.wide, lane);
-        row_operands<T, DP>(of, o_row, mine, A.dim, o_wide, lane);
+        row_operands<T, DP>(qf, q_row, mine, A.dim, true, lane);
+        row_operands<T, DP>(gf, g_row, mine, A.dim, true, lane);
+        row_operands<T, DP>(of, o_row, mine, A.dim, o_whole, lane);
 #pragma unroll
         for (int s = 0; s < DP / 16; s++)
 #pragma unroll
@@ -804,8 +829,8 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
     auto fetch = [&](int n) {
         const int j0 = n * KEYS;
         bits.load(mask ? mask + j0 : nullptr, min(k.there - j0, KEYS), lane);
-        kx.load(k_at + j0 * A.k.row, A.k.row, k.there - j0, A.dim, A.k.wide, threadIdx.x);
-        vx.load(v_at + j0 * A.v.row, A.v.row, k.there - j0, A.dim, A.v.wide, threadIdx.x);
+        kx.load(k_at + j0 * A.k.row, A.k.row, k.there - j0, A.dim, threadIdx.x);
+        vx.load(v_at + j0 * A.v.row, A.v.row, k.there - j0, A.dim, threadIdx.x);
     };
     auto put = [&](int n) {
         there = bits.get(mask);
@@ -813,23 +838,25 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
         kx.store(tiles + (n & 1) * 2 * TILE, threadIdx.x, rows);
         vx.store(tiles + (n & 1) * 2 * TILE + TILE, threadIdx.x, rows);
     };
+    settle<T>(qf);
+    settle<T>(gf);
+    asm volatile("" : "+v"(m), "+v"(inverse));
     if (first < end) {
         fetch(first);
         put(first);
     }
     __syncthreads();
     for (int n = first; n < end; n++) {
-        const char* const kt = tiles + (n & 1) * 2 * TILE;
-        const char* const vt = kt + TILE;
+        const uint32_t tile = lds_address(tiles) + (n & 1) * 2 * TILE, kr = tile + L::rows_at(lane), vr = kr + TILE, kc = tile + L::columns_at(lane);
         if (n + 1 < end) fetch(n + 1);
         const int j0 = n * KEYS;
         f32x16 s, dp;
 #pragma unroll
         for (int r = 0; r < 16; r++) s[r] = dp[r] = 0.0f;
 #pragma unroll
-        for (int c = 0; c < DP / 16; c++) s = Operand<T>::product(L::rows(kt, 0, c, lane), qf[c], s);
+        for (int c = 0; c < DP / 16; c++) s = Operand<T>::product(L::rows(kr, 0, c), qf[c], s);
 #pragma unroll
-        for (int c = 0; c < DP / 16; c++) dp = Operand<T>::product(L::rows(vt, 0, c, lane), gf[c], dp);
+        for (int c = 0; c < DP / 16; c++) dp = Operand<T>::product(L::rows(vr, 0, c), gf[c], dp);
         const int low = j0 - (i0 + 31) - shift, high = j0 + 31 - i0 - shift, r0 = j0 + 4 * half - i - shift;
         const bool causal = A.causal && high > 0, beyond = low >= A.reach || high <= -A.reach;
         if (!BIAS || beyond) {
@@ -876,7 +903,7 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
         for (int c = 0; c < 2; c++) {
             const Eight<T> ds = rounded<T>(s, c);
 #pragma unroll
-            for (int d = 0; d < DP / 32; d++) dq[d] = Operand<T>::product(L::columns(kt, 16 * c, d, lane), ds, dq[d]);
+            for (int d = 0; d < DP / 32; d++) dq[d] = Operand<T>::product(L::columns(kc, 16 * c, d), ds, dq[d]);
         }
         if (n + 1 < end) put(n + 1);
         __syncthreads();
@@ -940,19 +967,24 @@ __global__ __launch_bounds__(64) void table_gradient(const float* parts, int64_t
 
 // ---- backward: keys' side --------------------------------------------------------------------------------------------------------------------
 // A wavefront has 32 keys (columns), whose gradients stay in its registers; the workgroup goes through the queries of the heads that
-// share the key head, in tiles of 32.
+// share the key head, in tiles of 32.  Heads of 128 channels in 16 bits: the wavefront's values stay in LDS, so that two wavefronts
+// have room on a SIMD.
+template <typename T, int DP>
+constexpr bool values_in_lds() { return sizeof(T) == 2 && DP == 128; }
 template <typename T, int DP, int NW, bool BIAS>
-__global__ __launch_bounds__(NW * 64) void keys_kernel(SequenceAttention A, AttentionGrads G, int64_t slots, int splits) {
+__global__ __launch_bounds__(NW * 64, (NW == 4 && values_in_lds<T, DP>() ? 2 : 1)) void keys_kernel(SequenceAttention A, AttentionGrads G, int64_t slots, int splits) {
     using L = Tile<T, DP>;
     constexpr int ROWS = 32, TILE = ROWS * L::ROW;
-    extern __shared__ __attribute__((aligned(16))) char lds[];
+    extern __shared__ __attribute__((aligned(512))) char lds[];
     char* const tiles = lds;                                            // two pairs: q, do
-    float* const row_stats = reinterpret_cast<float*>(lds + 4 * TILE);  // two times (3, ROWS): m or shift, 1 / l, D
-    float* const line = row_stats + 2 * 3 * ROWS;
+    float* const row_stats = reinterpret_cast<float*>(lds + 4 * TILE);  // two times (3, ROWS): m or shift, 1 / l, -D
+    char* const values = lds + 4 * TILE + 2 * 3 * ROWS * sizeof(float) + (values_in_lds<T, DP>() ? (threadIdx.x >> 6) * TILE : 0);
+    float* const line = row_stats + 2 * 3 * ROWS + (values_in_lds<T, DP>() ? NW * TILE / sizeof(float) : 0);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, column = lane & 31;
-    const int64_t total = slots * A.kv_heads, id = die_order(blockIdx.x, total);
-    if (id >= total) return;
-    const int kh = (int)(id / slots), slot = (int)(id - kh * slots), z = blockIdx.y;
+    int kh;
+    int64_t slot;
+    if (!workgroup_item(blockIdx.x, slots, A.kv_heads, A, false, kh, slot)) return;
+    const int z = blockIdx.y;
     int b, from;
     if (!find_slot(A.k_starts, A.k_rows, A.packed, A.batch, NW * 32, slot, lane, b, from)) return;
     const Span k = span_of(A.k_starts, A.k_sizes, A.k_rows, A.packed, A.batch, b);
@@ -969,12 +1001,20 @@ __global__ __launch_bounds__(NW * 64) void keys_kernel(SequenceAttention A, Atte
     const int each = from < k.there ? max(0, (q.there + ROWS - 1) / ROWS - skip) : 0, whole = each * A.share;
     const int first = (int)((int64_t)whole * z / splits), end = (int)((int64_t)whole * (z + 1) / splits);
 
-    Eight<T> kf[DP / 16], vf[DP / 16];
+    Eight<T> kf[DP / 16], vf[values_in_lds<T, DP>() ? 1 : DP / 16];
     {
         const T* const k_row = row_start<T>(A.k, k, A.packed, kh) + (mine ? j : 0) * A.k.row;
         const T* const v_row = row_start<T>(A.v, k, A.packed, kh) + (mine ? j : 0) * A.v.row;
-        row_operands<T, DP>(kf, k_row, mine, A.dim, A.k.wide, lane);
-        row_operands<T, DP>(vf, v_row, mine, A.dim, A.v.wide, lane);
+        row_operands<T, DP>(kf, k_row, mine, A.dim, true, lane);
+        if constexpr (values_in_lds<T, DP>()) {
+            Staged<T, DP, 32, 64> vx;
+            vx.load(row_start<T>(A.v, k, A.packed, kh) + j0 * A.v.row, A.v.row, k.there - j0, A.dim, lane);
+            vx.store(values, lane);      // (read by this wavefront alone)
+            (void)v_row;
+        } else {
+            row_operands<T, DP>(vf, v_row, mine, A.dim, true, lane);
+            settle<T>(vf);
+        }
     }
     f32x16 dk[DP / 32], dv[DP / 32];
     Scaled<T, DP> scaled;
@@ -986,8 +1026,8 @@ __global__ __launch_bounds__(NW * 64) void keys_kernel(SequenceAttention A, Atte
     float sx[3];
     auto fetch = [&](int n) {
         const int h = kh * A.share + n / each, i0 = (skip + n % each) * ROWS;
-        qx.load(row_start<T>(A.q, q, A.packed, h) + i0 * A.q.row, A.q.row, q.there - i0, A.dim, A.q.wide, threadIdx.x);
-        gx.load(row_start<T>(G.go, q, A.packed, h) + i0 * G.go.row, G.go.row, q.there - i0, A.dim, G.go.wide, threadIdx.x);
+        qx.load(row_start<T>(A.q, q, A.packed, h) + i0 * A.q.row, A.q.row, q.there - i0, A.dim, threadIdx.x);
+        gx.load(row_start<T>(G.go, q, A.packed, h) + i0 * G.go.row, G.go.row, q.there - i0, A.dim, threadIdx.x);
         if (threadIdx.x < ROWS) {
             float m = -NONE, inverse = 0.0f, D = 0.0f;
             if (i0 + (int)threadIdx.x < q.there) {
@@ -996,7 +1036,7 @@ __global__ __launch_bounds__(NW * 64) void keys_kernel(SequenceAttention A, Atte
                 inverse = G.stats[2 * row + 1];
                 D = G.rows[row];
             }
-            sx[0] = sizeof(T) == 4 ? m : P_LIFT<T> + row_shift(score, m, inverse);
+            sx[0] = m;
             sx[1] = inverse;
             sx[2] = D;
         }
@@ -1004,15 +1044,21 @@ __global__ __launch_bounds__(NW * 64) void keys_kernel(SequenceAttention A, Atte
     auto put = [&](int n) {
         qx.store(tiles + (n & 1) * 2 * TILE, threadIdx.x);
         gx.store(tiles + (n & 1) * 2 * TILE + TILE, threadIdx.x);
-        if (threadIdx.x < ROWS)
-#pragma unroll
-            for (int c = 0; c < 3; c++) row_stats[((n & 1) * 3 + c) * ROWS + threadIdx.x] = sx[c];
+        if (threadIdx.x < ROWS) {
+            float* const st = row_stats + (n & 1) * 3 * ROWS + threadIdx.x;
+            st[0] = sizeof(T) == 4 ? sx[0] : P_LIFT<T> + row_shift(score, sx[0], sx[1]);
+            st[ROWS] = sx[1];
+            st[2 * ROWS] = -sx[2];
+        }
     };
+    settle<T>(kf);
     if (first < end) {
         fetch(first);
         put(first);
     }
     int line_of = -1;
+    const uint32_t vr = lds_address(values) + L::rows_at(lane);
+    (void)vr;
     for (int n = first; n < end; n++) {
         const int h = kh * A.share + n / each, i0 = (skip + n % each) * ROWS;
         if (BIAS && h != line_of) {
@@ -1021,17 +1067,26 @@ __global__ __launch_bounds__(NW * 64) void keys_kernel(SequenceAttention A, Atte
             line_of = h;
         }
         __syncthreads();
-        const char* const qt = tiles + (n & 1) * 2 * TILE;
-        const char* const gt = qt + TILE;
+        const uint32_t tile = lds_address(tiles) + (n & 1) * 2 * TILE, qr = tile + L::rows_at(lane), gr = qr + TILE, qc = tile + L::columns_at(lane),
+                       gc = qc + TILE;
         const float* const st = row_stats + (n & 1) * 3 * ROWS + 4 * half;
-        if (n + 1 < end) fetch(n + 1);
         f32x16 s, dp;
 #pragma unroll
-        for (int r = 0; r < 16; r++) s[r] = dp[r] = 0.0f;
+        for (int r = 0; r < 16; r++) s[r] = 0.0f;
 #pragma unroll
-        for (int c = 0; c < DP / 16; c++) s = Operand<T>::product(L::rows(qt, 0, c, lane), kf[c], s);
+        for (int r = 0; r < 16; r += 4) {      // do . v - D
+            const f32x4 D4 = *reinterpret_cast<const f32x4*>(st + 2 * ROWS + result_row(r));
 #pragma unroll
-        for (int c = 0; c < DP / 16; c++) dp = Operand<T>::product(L::rows(gt, 0, c, lane), vf[c], dp);
+            for (int e = 0; e < 4; e++) dp[r + e] = D4[e];
+        }
+#pragma unroll
+        for (int c = 0; c < DP / 16; c++) s = Operand<T>::product(L::rows(qr, 0, c), kf[c], s);
+#pragma unroll
+        for (int c = 0; c < DP / 16; c++) {
+            const Eight<T> gx8 = L::rows(gr, 0, c);
+            if constexpr (values_in_lds<T, DP>()) dp = Operand<T>::product(gx8, L::rows(vr, 0, c), dp);
+            else dp = Operand<T>::product(gx8, vf[c], dp);
+        }
         if (BIAS) {
             const int low = j0 - (i0 + 31) - shift, high = j0 + 31 - i0 - shift;
             if (low >= A.reach || high <= -A.reach) {
@@ -1052,25 +1107,25 @@ __global__ __launch_bounds__(NW * 64) void keys_kernel(SequenceAttention A, Atte
         f32x16 p;
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {
-            const f32x4 m4 = *reinterpret_cast<const f32x4*>(st + result_row(r)), D4 = *reinterpret_cast<const f32x4*>(st + 2 * ROWS + result_row(r));
+            const f32x4 m4 = *reinterpret_cast<const f32x4*>(st + result_row(r));
             f32x4 l4{1, 1, 1, 1};
             if (sizeof(T) == 4) l4 = *reinterpret_cast<const f32x4*>(st + ROWS + result_row(r));
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 p[r + e] = probability(score, s[r + e], m4[e], l4[e], m4[e]);
-                s[r + e] = p[r + e] * (dp[r + e] - D4[e]);
+                s[r + e] = p[r + e] * dp[r + e];
             }
         }
         scaled.meet(s, dk);
+        const Eight<T> pf[2] = {rounded<T>(p, 0), rounded<T>(p, 1)}, ds[2] = {rounded<T>(s, 0), rounded<T>(s, 1)};
+        if (n + 1 < end) fetch(n + 1);      // (here: registers that the scores had)
 #pragma unroll
-        for (int c = 0; c < 2; c++) {
-            const Eight<T> pf = rounded<T>(p, c), ds = rounded<T>(s, c);
+        for (int c = 0; c < 2; c++)
 #pragma unroll
             for (int d = 0; d < DP / 32; d++) {
-                dv[d] = Operand<T>::product(L::columns(gt, 16 * c, d, lane), pf, dv[d]);
-                dk[d] = Operand<T>::product(L::columns(qt, 16 * c, d, lane), ds, dk[d]);
+                dv[d] = Operand<T>::product(L::columns(gc, 16 * c, d), pf[c], dv[d]);
+                dk[d] = Operand<T>::product(L::columns(qc, 16 * c, d), ds[c], dk[d]);
             }
-        }
         if (n + 1 < end) put(n + 1);
     }
     if (j >= k.rows) return;
@@ -1187,7 +1242,7 @@ void sequence_attention_backward(const SequenceAttention& A, const AttentionGrad
             }
             if (k_all > 0 && G.dk) {
                 const dim3 grid(die_grid((int64_t)P.k_slots * A.kv_heads), P.k_splits);
-                const size_t lds = tiles + 6 * 32 * sizeof(float) + line;
+                const size_t lds = tiles + 6 * 32 * sizeof(float) + line + (values_in_lds<T, DP>() ? P.k_waves * 32 * Tile<T, DP>::ROW : 0);
                 if (P.k_waves == 1) launch_attention(keys_kernel<T, DP, 1, BIAS>, grid, 64, lds, st, A, G, P.k_slots, P.k_splits);
                 else launch_attention(keys_kernel<T, DP, 4, BIAS>, grid, 256, lds, st, A, G, P.k_slots, P.k_splits);
             }

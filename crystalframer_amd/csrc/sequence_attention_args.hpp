@@ -9,11 +9,10 @@ constexpr int ATTENTION_MAX_DIM = 128;
 constexpr int ATTENTION_MAX_REACH = 1024;      // relative positions beyond this (either way) share a bucket
 constexpr int ATTENTION_CUS = 256;
 
-// Element strides of (batch, position, head); channels lie next to one another.  16-byte loads where `wide`.
+// Element strides of (batch, position, head); channels lie next to one another, rows at multiples of 16 bytes.
 struct AttentionRows {
     const void* at;
     int64_t batch, row, head;
-    int32_t wide;
 };
 
 struct SequenceAttention {

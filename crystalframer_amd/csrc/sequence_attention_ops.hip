@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cmath>
+#include <cstdint>
 
 #include "element_types.hpp"
 #include "host_error.hpp"
@@ -18,6 +19,19 @@ using cfh::finish_launch;
 constexpr int64_t MAX_ROWS = 0x7fffff00LL;      // of a sequence, and of all packed ones
 constexpr int64_t MAX_GRID = 0x7fffff00LL;
 
+// Rows begin at multiples of 16 bytes, and a tile of them is less than 2^30 bytes.
+int check_rows(const void* at, const int64_t* stride, int dtype) {
+    const int64_t bytes = dtype == CFH_FLOAT32 ? 4 : 2;
+    uint64_t all = (uint64_t)(uintptr_t)at;
+    for (int n = 0; n < 3; n++) {
+        if (stride[n] < 0 || stride[n] > INT64_MAX / 8) return fail(CFH_EINVAL, "attention: strides must not be negative");
+        all |= (uint64_t)(stride[n] * bytes);
+    }
+    if (all & 15) return fail(CFH_EINVAL, "attention: an address or a stride is no multiple of 16 bytes");
+    if (stride[1] * bytes >= 1 << 24) return fail(CFH_EINVAL, "attention: strides: rows %lld bytes apart: less than 2^24", (long long)(stride[1] * bytes));
+    return CFH_OK;
+}
+
 int check_attention(const cfh_attention* a) {
     if (!a || a->struct_size != (int32_t)sizeof(cfh_attention)) return fail(CFH_EINVAL, "attention: struct_size does not match");
     if (a->dtype < CFH_FLOAT32 || a->dtype > CFH_FLOAT16) return fail(CFH_EINVAL, "attention: dtype %d", (int)a->dtype);
@@ -29,15 +43,13 @@ int check_attention(const cfh_attention* a) {
         return fail(CFH_EINVAL, "attention: batch = %d, query_rows = %lld, key_rows = %lld out of range", (int)a->batch, (long long)a->query_rows,
                     (long long)a->key_rows);
     if (!(a->scale > 0.0f) || std::isinf(a->scale)) return fail(CFH_EINVAL, "attention: scale = %g must be positive and finite", a->scale);
-    for (int n = 0; n < 3; n++)
-        if (a->q_stride[n] < 0 || a->k_stride[n] < 0 || a->v_stride[n] < 0) return fail(CFH_EINVAL, "attention: strides must not be negative");
     if (a->packed && (!a->query_starts || !a->key_starts)) return fail(CFH_EINVAL, "attention: packed sequences need query_starts and key_starts");
     if (a->packed && (a->query_sizes || a->key_sizes)) return fail(CFH_EINVAL, "attention: query_sizes and key_sizes are of sequences that are not packed");
     if (!a->packed && (a->query_starts || a->key_starts)) return fail(CFH_EINVAL, "attention: query_starts and key_starts are of packed sequences");
     const int64_t q_all = a->packed ? a->query_rows : a->query_rows * a->batch, k_all = a->packed ? a->key_rows : a->key_rows * a->batch;
     if ((q_all > 0 && !a->q) || (k_all > 0 && (!a->k || !a->v))) return fail(CFH_EINVAL, "attention: q, k and v must not be NULL");
-    const uintptr_t element = a->dtype == CFH_FLOAT32 ? 3 : 1;
-    if (((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v) & element) return fail(CFH_EINVAL, "attention: an address is not one of an element");
+    for (int rc : {check_rows(a->q, a->q_stride, a->dtype), check_rows(a->k, a->k_stride, a->dtype), check_rows(a->v, a->v_stride, a->dtype)})
+        if (rc) return rc;
     if (a->table) {
         if (a->table_dtype != a->dtype && a->table_dtype != CFH_FLOAT32)
             return fail(CFH_EINVAL, "attention: table_dtype %d is neither dtype nor float32", (int)a->table_dtype);
@@ -54,19 +66,11 @@ int check_attention(const cfh_attention* a) {
     return CFH_OK;
 }
 
-// 16 bytes at a time: where they begin at multiples of 16 and hold whole rows of channels, and 64 rows are less than 2^30 bytes.
-cfh::AttentionRows rows_of(const void* at, const int64_t* stride, int dtype, int dim) {
-    const int64_t bytes = dtype == CFH_FLOAT32 ? 4 : 2;
-    uint64_t all = (uint64_t)(uintptr_t)at | (uint64_t)(dim * bytes);
-    for (int n = 0; n < 3; n++) all |= (uint64_t)(stride[n] * bytes);
-    return {at, stride[0], stride[1], stride[2], (all & 15) == 0 && stride[1] * bytes < (1 << 24)};
-}
-
 cfh::SequenceAttention device_args(const cfh_attention* a) {
     cfh::SequenceAttention A{};
-    A.q = rows_of(a->q, a->q_stride, a->dtype, a->dim);
-    A.k = rows_of(a->k, a->k_stride, a->dtype, a->dim);
-    A.v = rows_of(a->v, a->v_stride, a->dtype, a->dim);
+    A.q = {a->q, a->q_stride[0], a->q_stride[1], a->q_stride[2]};
+    A.k = {a->k, a->k_stride[0], a->k_stride[1], a->k_stride[2]};
+    A.v = {a->v, a->v_stride[0], a->v_stride[1], a->v_stride[2]};
     A.mask = a->key_mask;
     A.q_starts = a->query_starts; A.k_starts = a->key_starts; A.q_sizes = a->query_sizes; A.k_sizes = a->key_sizes;
     A.table = a->table; A.bucket_of = a->bucket_of;
@@ -140,11 +144,10 @@ int cfh_attention_backward(const cfh_attention* a, const void* out, const float*
     if (((uintptr_t)out | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15) return fail(CFH_EINVAL, "attention: out, dq, dk and dv must be aligned to 16 bytes");
     const int64_t none[3] = {0, 0, 0};
     const int64_t* const gs = gout_stride ? gout_stride : none;
-    if (gs[0] < 0 || gs[1] < 0 || gs[2] < 0 || ((uintptr_t)gout & (a->dtype == CFH_FLOAT32 ? 3 : 1)))
-        return fail(CFH_EINVAL, "attention: strides must not be negative, addresses those of elements");
+    if ((rc = check_rows(gout, gs, a->dtype))) return rc;
     if ((rc = check_workspace(workspace, workspace_bytes, cfh_attention_backward_workspace_bytes(a)))) return rc;
     cfh::AttentionGrads G{};
-    G.go = rows_of(gout, gs, a->dtype, a->dim);
+    G.go = {gout, gs[0], gs[1], gs[2]};
     G.out = out; G.stats = stats; G.dq = dq; G.dk = dk; G.dv = dv;
     with_type(a->dtype, [&](auto t) {
         cfh::sequence_attention_backward<decltype(t)>(A, cfh::attention_grad_plan(A), G, dtable, (float*)workspace, (hipStream_t)stream);

@@ -46,8 +46,8 @@ def cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
 
     The heads may be a multiple of the key heads: head h reads key head h // (heads // key heads).  1 to 128 channels of a head;
     ``scale``: one over their root.  One type, float32, bfloat16 or float16, for all and for the result; sums, maxima and the gradients'
-    sums are in float32, probabilities and the scores' gradients are rounded to the type before their products.  Any strides; channels
-    that do not lie next to one another are laid out again.  The values of starts and sizes are cut to the rows that are there.
+    sums are in float32, probabilities and the scores' gradients are rounded to the type before their products.  Any strides; rows
+    that do not begin at multiples of 16 bytes, or do not fill them, are laid out again first.  The values of starts and sizes are cut to the rows that are there.
 
     All gradients are there, with sums in a fixed order; a gradient of a gradient raises."""
     return _call(query, key, value, None, None, query_starts, key_starts, query_sizes, key_sizes, key_mask, scale, False, False)

@@ -31,7 +31,8 @@ TABLE = dict(table=A, buckets=4, reach=8, bucket_of=A)
     (dict(scale=-1.0), b"scale"), (dict(scale=math.nan), b"scale"), (dict(scale=math.inf), b"scale"), (dict(q_stride=(1, -1, 1)), b"strides"),
     (dict(packed=1), b"query_starts"), (dict(packed=1, query_starts=A), b"query_starts"), (dict(query_starts=A, key_starts=A), b"packed"),
     (dict(packed=1, query_starts=A, key_starts=A, key_sizes=A), b"sizes"), (dict(q=None), b"NULL"), (dict(v=None), b"NULL"),
-    (dict(k=A + 1), b"address"), (dict(dtype=1, q=A + 1), b"address"), (dict(TABLE, dtype=1, table_dtype=2), b"table_dtype"),
+    (dict(k=A + 4), b"address"), (dict(dtype=1, q=A + 2), b"address"), (dict(k_stride=(224, 30, 16)), b"16 bytes"),
+    (dict(v_stride=(0, 1 << 22, 16)), b"strides"), (dict(q_stride=(1 << 62, 64, 16)), b"strides"), (dict(TABLE, dtype=1, table_dtype=2), b"table_dtype"),
     (dict(TABLE, reach=1025), b"reach"), (dict(TABLE, reach=-1), b"reach"), (dict(TABLE, buckets=0), b"buckets"), (dict(TABLE, bucket_of=None), b"bucket_of"),
     (dict(buckets=3), b"table"), (dict(bucket_of=A), b"table"), (dict(batch=1 << 20, query_rows=1 << 20), b"grid"),
     (dict(batch=0x7fffffff, key_rows=0x7fffff00), b"grid")])
@@ -55,7 +56,7 @@ def test_results_and_workspaces():
     for change, word in ((dict(out=None), b"NULL"), (dict(stats=None), b"NULL"), (dict(go=None), b"NULL"), (dict(st=None), b"NULL"),
                          (dict(dq=None), b"NULL"), (dict(dk=None), b"together"), (dict(dv=None), b"together"), (dict(dq=A + 8), b"16"),
                          (dict(out=A + 4), b"16"), (dict(table=A), b"table"), (dict(ws=None), b"workspace"), (dict(n=need - 1), b"workspace"),
-                         (dict(ws=A + 4), b"workspace"), (dict(go=A + 2), b"address"), (dict(st=(ctypes.c_int64 * 3)(1, -1, 1)), b"strides")):
+                         (dict(ws=A + 4), b"workspace"), (dict(go=A + 4), b"address"), (dict(st=(ctypes.c_int64 * 3)(4, -4, 4)), b"strides")):
         assert backward(**change) < 0 and word in lib.cfh_last_error(), (change, lib.cfh_last_error())
     assert lib.cfh_attention_forward(ctypes.byref(a), None, None, None, 0, None) < 0 and b"out" in lib.cfh_last_error()
     assert lib.cfh_attention_forward(ctypes.byref(a), A + 8, None, None, 0, None) < 0 and b"out" in lib.cfh_last_error()
