@@ -15,6 +15,7 @@
 #include <stdint.h>
 
 #include <type_traits>
+#include <utility>
 
 #include "element_types.hpp"
 #include "sequence_attention_args.hpp"
@@ -745,8 +746,31 @@ __device__ __forceinline__ float probability(const Score<T, BIAS>& score, float 
     return sizeof(T) == 4 ? p * inverse : p;
 }
 
+// Sums of a 32 x 32 result over its diagonals: column l of 16 and row 16 a + b meet in place (l - b) of sum a, or of sum a + 1 where that
+// is negative.  A shift within 16 lanes that fills with zeros is part of the addition (DPP): two instructions for a register, none of
+// them an LDS atomic, of which one takes 94 cycles for a wavefront (16 of them per tile: 330 us where this takes NEARUS, 32 x 512 tokens, 12 heads
+// of 64).  Register r is row 8 (r / 4) + r % 4; the 4 of the upper half wavefront are in the place that the sums are added to.
+template <int CTRL>
+__device__ __forceinline__ float shifted(float x) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+template <int R>
+__device__ __forceinline__ void add_diagonal(float s, float (&x)[3]) {
+    constexpr int a = result_row(R) / 16, b = result_row(R) % 16;
+    if constexpr (b == 0) {
+        x[a] += s;
+    } else {
+        x[a] += shifted<0x100 + b>(s);              // from b lanes further
+        x[a + 1] += shifted<0x110 + 16 - b>(s);     // from 16 - b lanes before
+    }
+}
+template <int... R>
+__device__ __forceinline__ void add_diagonals(const f32x16& s, float (&x)[3], std::integer_sequence<int, R...>) {
+    (add_diagonal<R>(s[R], x), ...);
+}
+
 // dq, D, and the table's gradient: scores transposed as in the forward pass.  The gradients of the biases are summed in float32 by
-// relative position (a column of sums for each half wavefront, so that no two lanes meet in one), those beyond the reach in the lane.
+// relative position (for each half wavefront by itself), those of tiles beyond the reach in the lane.
 // D comes from a rounded output, so that the ds of a row add up to a small e instead of 0; what lies beyond the reach, where most of
 // a long row's probability is, gets its share of -e back.
 template <typename T, int DP, int NW, bool BIAS>
@@ -756,8 +780,8 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
     extern __shared__ __attribute__((aligned(512))) char lds[];
     char* const tiles = lds;
     float* const line = reinterpret_cast<float*>(lds + 4 * TILE);
-    const int entries = 2 * A.reach + 1;
-    float* const sums = line + 2 * (A.reach + MARGIN) + 1;      // (2 NW, entries), then two for each wavefront
+    const int entries = 2 * (A.reach + MARGIN) + 1;
+    float* const sums = line + entries;                         // (2 NW, entries), then two for each wavefront
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, column = lane & 31;
     int h;
     int64_t slot;
@@ -885,17 +909,16 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
         } else {
 #pragma unroll
             for (int r = 0; r < 16; r++) {
-                const float p = probability(score, s[r], m, inverse, off);
-                s[r] = p * (dp[r] - D);
+                s[r] = probability(score, s[r], m, inverse, off) * (dp[r] - D);
                 all_ds += s[r];
-                const int rel = r0 + result_row(r);
-                if (rel > -A.reach && rel < A.reach) {
-                    if (mine) atomicAdd(own_sums + rel + A.reach, s[r]);
-                } else {
-                    const bool up = rel > 0;
-                    far_ds[0] += up ? 0.0f : s[r]; far_p[0] += up ? 0.0f : p;
-                    far_ds[1] += up ? s[r] : 0.0f; far_p[1] += up ? p : 0.0f;
-                }
+            }
+            float x[3] = {0.0f, 0.0f, 0.0f};
+            add_diagonals(s, x, std::make_integer_sequence<int, 16>());
+            float* const at = own_sums + (j0 - i0 - shift + 4 * half - (lane & 31) + A.reach + MARGIN);
+#pragma unroll
+            for (int n16 = 0; n16 < 3; n16++) {      // (no two lanes of a half wavefront in one place, but in those of the next 16)
+                at[16 * n16] += x[n16];
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             }
         }
         scaled.meet(s, dq);
@@ -938,17 +961,19 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
 #pragma unroll
         for (int w = 0; w < 2 * NW; w++) x += sums[w * entries + n];
 #pragma unroll
-        for (int side = 0; side < 2; side++)      // (one entry is both)
+        for (int side = 0; side < 2; side++)
             if (n == side * (entries - 1))
 #pragma unroll
                 for (int w = 0; w < NW; w++) x += far_sums[2 * w + side];
         line[n] = x;
+        sums[n] = __int_as_float(A.bucket_of[clamped(n - A.reach - MARGIN, A.reach)]);      // (where the entry's first sum was)
     }
     __syncthreads();
-    for (int n = threadIdx.x; n < A.buckets; n += NW * 64) {
+    for (int n = wave; n < A.buckets; n += NW) {
         float x = 0.0f;
-        for (int e = 0; e < entries; e++) x += A.bucket_of[e] == n ? line[e] : 0.0f;
-        dtable[n] = x;
+        for (int e = lane; e < entries; e += 64) x += __float_as_int(sums[e]) == n ? line[e] : 0.0f;
+        x = wave_sum(x);
+        if (lane == 0) dtable[n] = x;
     }
 }
 
@@ -1234,7 +1259,7 @@ void sequence_attention_backward(const SequenceAttention& A, const AttentionGrad
             constexpr int DP = decltype(dp)::value;
             constexpr bool BIAS = decltype(bias)::value;
             const size_t line = BIAS ? (2 * (A.reach + MARGIN) + 1) * sizeof(float) : 0, tiles = 4 * 32 * Tile<T, DP>::ROW;
-            const size_t sums = BIAS ? (2 * P.q_waves * (2 * A.reach + 1) + 2 * P.q_waves) * sizeof(float) : 0;
+            const size_t sums = BIAS ? (2 * P.q_waves * (2 * (A.reach + MARGIN) + 1) + 2 * P.q_waves) * sizeof(float) : 0;
             if (q_all > 0) {
                 const dim3 grid(die_grid((int64_t)P.q_slots * A.heads), P.q_splits);
                 if (P.q_waves == 1) launch_attention(queries_kernel<T, DP, 1, BIAS>, grid, 64, tiles + line + sums, st, A, G, P.q_slots, P.q_splits);
