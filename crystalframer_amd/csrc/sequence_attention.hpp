@@ -80,6 +80,8 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_
 template <typename V>
 __device__ __forceinline__ V lds_read(uint32_t at) { return *reinterpret_cast<__attribute__((address_space(3))) const V*>(at); }
 
+// Channels of a row in LDS, for heads of up to DC (a multiple of 16).
+constexpr int pitch(int dc) { return dc <= 32 ? 32 : dc <= 64 ? 64 : 128; }
 template <typename T, int DP>
 struct Tile {
     static constexpr int E = 16 / sizeof(T), PIECES = DP / E, ROW = DP * sizeof(T);
@@ -145,16 +147,16 @@ __device__ __forceinline__ u32x4 elements_of(const T* row, int from, int dim) {
     return x;
 }
 // Operands of all steps straight from memory: channels 16 step + 8 (l / 32) ... of the lane's row.  `whole`: of rows as above.
-template <typename T, int DP>
-__device__ __forceinline__ void row_operands(Eight<T> (&y)[DP / 16], const T* row, bool there, int dim, bool whole, int lane) {
+template <typename T, int DC>
+__device__ __forceinline__ void row_operands(Eight<T> (&y)[DC / 16], const T* row, bool there, int dim, bool whole, int lane) {
     constexpr int E = 16 / sizeof(T), EACH = sizeof(T) / 2;
-    u32x4 x[DP / 16 * EACH];
+    u32x4 x[DC / 16 * EACH];
 #pragma unroll
-    for (int n = 0; n < DP / 16 * EACH; n++) x[n] = u32x4{0, 0, 0, 0};
+    for (int n = 0; n < DC / 16 * EACH; n++) x[n] = u32x4{0, 0, 0, 0};
     if (there) {
         const int first = 8 * (lane >> 5);
 #pragma unroll
-        for (int n = 0; n < DP / 16 * EACH; n++) {
+        for (int n = 0; n < DC / 16 * EACH; n++) {
             const int from = 16 * (n / EACH) + first + n % EACH * E;
             if (whole) {
                 if (from < dim) x[n] = *reinterpret_cast<const u32x4*>(row + from);
@@ -267,7 +269,7 @@ __device__ __forceinline__ bool find_slot(const int64_t* starts, int64_t rows, i
         from = (int)(w - (int64_t)b * per) * tile;
         return b < batch;
     }
-    auto base = [&](int n) { return (n == 0 ? 0 : between(starts[n], 0, rows) / tile) + n; };
+    auto base = [&](int n) { return (n == 0 ? 0 : (int64_t)((uint32_t)between(starts[n], 0, rows) / (uint32_t)tile)) + n; };
     int lo = 0, n = batch + 1;      // the last of n from lo on whose first slot is not behind w
     while (n > 1) {
         const int step = (n + 63) / 64, probe = lane * step;
@@ -352,13 +354,13 @@ __device__ __forceinline__ float other_half_sum(float x) { float a, b; swap32(x,
 
 // Running maximum, sum and weighted sum of one column.  The maximum that the powers are relative to follows the true one when that is
 // more than 2^8 ahead: the sums are scaled anew in few tiles only, and no power is above 2^8.
-template <int DP>
+template <int ND>
 struct Running {
     float m = NONE, l = 0.0f;
-    f32x16 o[DP / 32];
+    f32x16 o[ND];
     __device__ __forceinline__ Running() {
 #pragma unroll
-        for (int d = 0; d < DP / 32; d++)
+        for (int d = 0; d < ND; d++)
 #pragma unroll
             for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
     }
@@ -369,7 +371,7 @@ struct Running {
         m = ahead ? top : m;
         l *= by;
 #pragma unroll
-        for (int d = 0; d < DP / 32; d++)
+        for (int d = 0; d < ND; d++)
 #pragma unroll
             for (int r = 0; r < 16; r++) o[d][r] *= by;
     }
@@ -377,7 +379,7 @@ struct Running {
 };
 
 // Gradients of scores on their way into a product whose sums `sum` are per column (see NARROW).
-template <typename T, int DP>
+template <typename T, int ND>
 struct Scaled {
     float by = 1.0f;
     bool met = false;
@@ -394,7 +396,7 @@ struct Scaled {
             const float next = ahead ? __uint_as_float((uint32_t)(to > 253 ? 253 : to < 1 ? 1 : to) << 23) : by;
             const float change = met ? next / by : 1.0f;                                      // (nothing but 0 is there before)
 #pragma unroll
-            for (int d = 0; d < DP / 32; d++)
+            for (int d = 0; d < ND; d++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) sum[d][r] *= change;
             by = next;
@@ -440,8 +442,9 @@ struct FewLds {
     float m[NW][32], l[NW][32];
 };
 
-template <typename T, int DP, int NW, bool BIAS>
+template <typename T, int DC, int NW, bool BIAS>
 __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && NW == 4 ? 2 : 1)) void few_kernel(SequenceAttention A, T* out, float* stats, float* part_o, float* part_ml, int splits) {
+    constexpr int DP = pitch(DC), ND = (DC + 31) / 32;
     using L = Tile<T, DP>;
     __shared__ __attribute__((aligned(16))) FewLds<T, DP, NW> S;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
@@ -465,9 +468,9 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && NW == 4 ? 2 : 1)) void 
     const int tiles = seen > 0 ? (seen + 31) / 32 : 0;
     const int first = (int)((int64_t)tiles * blockIdx.z / splits), end = (int)((int64_t)tiles * (blockIdx.z + 1) / splits);
 
-    Eight<T> qf[DP / 16];
+    Eight<T> qf[DC / 16];
     const T* const q_row = row_start<T>(A.q, q, A.packed, mine ? h : 0) + (mine ? i : 0) * A.q.row;
-    row_operands<T, DP>(qf, q_row, mine, A.dim, true, lane);
+    row_operands<T, DC>(qf, q_row, mine, A.dim, true, lane);
     const T* const k_at = row_start<T>(A.k, k, A.packed, kh);
     const T* const v_at = row_start<T>(A.v, k, A.packed, kh);
     const uint8_t* const mask = A.mask ? A.mask + k.first : nullptr;
@@ -479,7 +482,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && NW == 4 ? 2 : 1)) void 
     char* const kt = S.wave[wave];
     char* const vt = kt + FewLds<T, DP, NW>::TILE;
     const uint32_t kr = lds_address(kt) + L::rows_at(lane), vc = lds_address(vt) + L::columns_at(lane);
-    Running<DP> sum;
+    Running<ND> sum;
     Staged<T, DP, 32, 64> kx, vx;
     KeyBits bits;
     auto fetch = [&](int n) {
@@ -503,7 +506,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && NW == 4 ? 2 : 1)) void 
 #pragma unroll
         for (int r = 0; r < 16; r++) s[r] = 0.0f;
 #pragma unroll
-        for (int c = 0; c < DP / 16; c++) s = Operand<T>::product(L::rows(kr, 0, c), qf[c], s);
+        for (int c = 0; c < DC / 16; c++) s = Operand<T>::product(L::rows(kr, 0, c), qf[c], s);
         const int low = j0 - i_last - shift, high = j0 + 31 - i0 - shift;      // relative positions of the tile
         const int r0 = j0 + 4 * half - i - shift;
         const bool causal = A.causal && high > 0;
@@ -529,7 +532,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && NW == 4 ? 2 : 1)) void 
         for (int c = 0; c < 2; c++) {
             const Eight<T> p = rounded<T>(s, c);
 #pragma unroll
-            for (int d = 0; d < DP / 32; d++) sum.o[d] = Operand<T>::product(L::columns(vc, 16 * c, d), p, sum.o[d]);
+            for (int d = 0; d < ND; d++) sum.o[d] = Operand<T>::product(L::columns(vc, 16 * c, d), p, sum.o[d]);
         }
     }
     // the wavefronts' sums, side by side in LDS
@@ -537,7 +540,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && NW == 4 ? 2 : 1)) void 
     sum.l = other_half_sum(sum.l);
     float* const mine_o = reinterpret_cast<float*>(S.wave[wave]);
 #pragma unroll
-    for (int d = 0; d < DP / 32; d++)
+    for (int d = 0; d < ND; d++)
 #pragma unroll
         for (int r = 0; r < 16; r += 4)
             *reinterpret_cast<f32x4*>(mine_o + column * (DP + 4) + 32 * d + result_row(r) + 4 * half) =
@@ -586,9 +589,10 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && NW == 4 ? 2 : 1)) void 
 }
 
 // Joins the splits: 8 rows to a workgroup, 32 lanes to a row.
-template <typename T, int DP, bool BIAS>
+template <typename T, int DC, bool BIAS>
 __global__ __launch_bounds__(256) void combine_parts(SequenceAttention A, const float* part_o, const float* part_ml, int splits, int64_t rows, T* out,
                                                      float* stats) {
+    constexpr int DP = pitch(DC);
     const int64_t row = blockIdx.x * 8LL + threadIdx.x / 32;
     const int from = (threadIdx.x & 31) * 4;
     if (row >= rows || from >= DP) return;
@@ -614,8 +618,9 @@ __global__ __launch_bounds__(256) void combine_parts(SequenceAttention A, const 
 template <typename T, int NW>
 constexpr int keys_at_once() { return sizeof(T) == 2 && NW >= 4 ? 64 : 32; }
 
-template <typename T, int DP, int NW, bool BIAS>
+template <typename T, int DC, int NW, bool BIAS>
 __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 ? 2 : 1)) void tiles_kernel(SequenceAttention A, T* out, float* stats, int64_t slots) {
+    constexpr int DP = pitch(DC), ND = (DC + 31) / 32;
     using L = Tile<T, DP>;
     constexpr int KEYS = keys_at_once<T, NW>(), TILE = KEYS * L::ROW;
     extern __shared__ __attribute__((aligned(512))) char lds[];
@@ -640,14 +645,14 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 ? 2 : 1)) void tiles_kerne
     if (A.causal) seen = min(seen, min(from + NW * 32, q.there) + shift);
     const int count = seen > 0 ? (seen + KEYS - 1) / KEYS : 0;
 
-    Eight<T> qf[DP / 16];
+    Eight<T> qf[DC / 16];
     const T* const q_row = row_start<T>(A.q, q, A.packed, h) + (mine ? i : 0) * A.q.row;
-    row_operands<T, DP>(qf, q_row, mine, A.dim, true, lane);
+    row_operands<T, DC>(qf, q_row, mine, A.dim, true, lane);
     const T* const k_at = row_start<T>(A.k, k, A.packed, kh);
     const T* const v_at = row_start<T>(A.v, k, A.packed, kh);
     const uint8_t* const mask = A.mask ? A.mask + k.first : nullptr;
     if (BIAS) fill_line<T, BIAS>(A, h, line, threadIdx.x, NW * 64);
-    Running<DP> sum;
+    Running<ND> sum;
     Staged<T, DP, KEYS, NW * 64> kx, vx;
     KeyBits bits;
     uint64_t there = 0;                         // keys of the tile in LDS
@@ -679,7 +684,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 ? 2 : 1)) void tiles_kerne
 #pragma unroll
             for (int r = 0; r < 16; r++) s[u][r] = 0.0f;
 #pragma unroll
-        for (int c = 0; c < DP / 16; c++)
+        for (int c = 0; c < DC / 16; c++)
 #pragma unroll
             for (int u = 0; u < KEYS / 32; u++) s[u] = Operand<T>::product(L::rows(kr, 32 * u, c), qf[c], s[u]);
 #pragma unroll
@@ -710,7 +715,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 ? 2 : 1)) void tiles_kerne
             for (int c = 0; c < 2; c++) {
                 const Eight<T> p = rounded<T>(s[u], c);
 #pragma unroll
-                for (int d = 0; d < DP / 32; d++) sum.o[d] = Operand<T>::product(L::columns(vc, 32 * u + 16 * c, d), p, sum.o[d]);
+                for (int d = 0; d < ND; d++) sum.o[d] = Operand<T>::product(L::columns(vc, 32 * u + 16 * c, d), p, sum.o[d]);
             }
         }
         if (n + 1 < count) put(n + 1);
@@ -721,7 +726,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 ? 2 : 1)) void tiles_kerne
     const float inverse = mine && (l > 0.0f || l != l) ? 1.0f / l : 0.0f;
     const int64_t row = (q.first + i) * A.heads + h;
 #pragma unroll
-    for (int d = 0; d < DP / 32; d++)
+    for (int d = 0; d < ND; d++)
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {
             f32x4 x{sum.o[d][r], sum.o[d][r + 1], sum.o[d][r + 2], sum.o[d][r + 3]};
@@ -773,8 +778,9 @@ __device__ __forceinline__ void add_diagonals(const f32x16& s, float (&x)[3], st
 // relative position (for each half wavefront by itself), those of tiles beyond the reach in the lane.
 // D comes from a rounded output, so that the ds of a row add up to a small e instead of 0; what lies beyond the reach, where most of
 // a long row's probability is, gets its share of -e back.
-template <typename T, int DP, int NW, bool BIAS>
+template <typename T, int DC, int NW, bool BIAS>
 __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, AttentionGrads G, int64_t slots, int splits) {
+    constexpr int DP = pitch(DC), ND = (DC + 31) / 32;
     using L = Tile<T, DP>;
     constexpr int KEYS = 32, TILE = KEYS * L::ROW;
     extern __shared__ __attribute__((aligned(512))) char lds[];
@@ -808,19 +814,19 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
     const int first = (int)((int64_t)whole * z / splits), end = (int)((int64_t)whole * (z + 1) / splits);
 
     const int64_t row = (q.first + i) * A.heads + h;
-    Eight<T> qf[DP / 16], gf[DP / 16];
+    Eight<T> qf[DC / 16], gf[DC / 16];
     float D = 0.0f;
     {
         const T* const q_row = row_start<T>(A.q, q, A.packed, h) + (mine ? i : 0) * A.q.row;
         const T* const g_row = row_start<T>(G.go, q, A.packed, h) + (mine ? i : 0) * G.go.row;
         const T* const o_row = static_cast<const T*>(G.out) + (mine ? row : 0) * A.dim;
         const bool o_whole = A.dim % L::E == 0;
-        Eight<T> of[DP / 16];
-        row_operands<T, DP>(qf, q_row, mine, A.dim, true, lane);
-        row_operands<T, DP>(gf, g_row, mine, A.dim, true, lane);
-        row_operands<T, DP>(of, o_row, mine, A.dim, o_whole, lane);
+        Eight<T> of[DC / 16];
+        row_operands<T, DC>(qf, q_row, mine, A.dim, true, lane);
+        row_operands<T, DC>(gf, g_row, mine, A.dim, true, lane);
+        row_operands<T, DC>(of, o_row, mine, A.dim, o_whole, lane);
 #pragma unroll
-        for (int s = 0; s < DP / 16; s++)
+        for (int s = 0; s < DC / 16; s++)
 #pragma unroll
             for (int e = 0; e < 8; e++) D = __builtin_fmaf(to_float(gf[s][e]), to_float(of[s][e]), D);
         D = other_half_sum(D);
@@ -841,10 +847,10 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
     }
     float* const own_sums = sums + (2 * wave + half) * entries;
     float far_ds[2] = {0.0f, 0.0f}, far_p[2] = {0.0f, 0.0f}, all_ds = 0.0f;
-    f32x16 dq[DP / 32];
-    Scaled<T, DP> scaled;
+    f32x16 dq[ND];
+    Scaled<T, ND> scaled;
 #pragma unroll
-    for (int d = 0; d < DP / 32; d++)
+    for (int d = 0; d < ND; d++)
 #pragma unroll
         for (int r = 0; r < 16; r++) dq[d][r] = 0.0f;
     Staged<T, DP, KEYS, NW * 64> kx, vx;
@@ -878,9 +884,9 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
 #pragma unroll
         for (int r = 0; r < 16; r++) s[r] = dp[r] = 0.0f;
 #pragma unroll
-        for (int c = 0; c < DP / 16; c++) s = Operand<T>::product(L::rows(kr, 0, c), qf[c], s);
+        for (int c = 0; c < DC / 16; c++) s = Operand<T>::product(L::rows(kr, 0, c), qf[c], s);
 #pragma unroll
-        for (int c = 0; c < DP / 16; c++) dp = Operand<T>::product(L::rows(vr, 0, c), gf[c], dp);
+        for (int c = 0; c < DC / 16; c++) dp = Operand<T>::product(L::rows(vr, 0, c), gf[c], dp);
         const int low = j0 - (i0 + 31) - shift, high = j0 + 31 - i0 - shift, r0 = j0 + 4 * half - i - shift;
         const bool causal = A.causal && high > 0, beyond = low >= A.reach || high <= -A.reach;
         if (!BIAS || beyond) {
@@ -926,7 +932,7 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
         for (int c = 0; c < 2; c++) {
             const Eight<T> ds = rounded<T>(s, c);
 #pragma unroll
-            for (int d = 0; d < DP / 32; d++) dq[d] = Operand<T>::product(L::columns(kc, 16 * c, d), ds, dq[d]);
+            for (int d = 0; d < ND; d++) dq[d] = Operand<T>::product(L::columns(kc, 16 * c, d), ds, dq[d]);
         }
         if (n + 1 < end) put(n + 1);
         __syncthreads();
@@ -935,7 +941,7 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
         const float factor = A.scale * scaled.back();
         const int64_t rows = (A.packed ? A.q_rows : A.q_rows * A.batch) * A.heads;
 #pragma unroll
-        for (int d = 0; d < DP / 32; d++)
+        for (int d = 0; d < ND; d++)
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
                 f32x4 x{dq[d][r], dq[d][r + 1], dq[d][r + 2], dq[d][r + 3]};
@@ -977,34 +983,22 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
     }
 }
 
-// Table's gradient: the workgroups' sums in a fixed order, in 64 bits.  A wavefront to a (head, bucket).
-template <typename T>
-__global__ __launch_bounds__(64) void table_gradient(const float* parts, int64_t count, int buckets, int heads, int table_float, void* dtable) {
-    const int n = blockIdx.x, h = blockIdx.y;
-    double x = 0.0;
-    for (int64_t w = threadIdx.x; w < count; w += 64) x += parts[((int64_t)h * count + w) * buckets + n];
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d);
-    if (threadIdx.x) return;
-    if (table_float) static_cast<float*>(dtable)[(int64_t)n * heads + h] = (float)x;
-    else static_cast<T*>(dtable)[(int64_t)n * heads + h] = from_float<T>((float)x);
-}
-
 // ---- backward: keys' side --------------------------------------------------------------------------------------------------------------------
 // A wavefront has 32 keys (columns), whose gradients stay in its registers; the workgroup goes through the queries of the heads that
 // share the key head, in tiles of 32.  Heads of 128 channels in 16 bits: the wavefront's values stay in LDS, so that two wavefronts
 // have room on a SIMD.
-template <typename T, int DP>
-constexpr bool values_in_lds() { return sizeof(T) == 2 && DP == 128; }
-template <typename T, int DP, int NW, bool BIAS>
-__global__ __launch_bounds__(NW * 64, (NW == 4 && values_in_lds<T, DP>() ? 2 : 1)) void keys_kernel(SequenceAttention A, AttentionGrads G, int64_t slots, int splits) {
+template <typename T, int DC>
+constexpr bool values_in_lds() { return sizeof(T) == 2 && DC == 128; }
+template <typename T, int DC, int NW, bool BIAS>
+__global__ __launch_bounds__(NW * 64, (NW == 4 && values_in_lds<T, DC>() ? 2 : 1)) void keys_kernel(SequenceAttention A, AttentionGrads G, int64_t slots, int splits) {
+    constexpr int DP = pitch(DC), ND = (DC + 31) / 32;
     using L = Tile<T, DP>;
     constexpr int ROWS = 32, TILE = ROWS * L::ROW;
     extern __shared__ __attribute__((aligned(512))) char lds[];
     char* const tiles = lds;                                            // two pairs: q, do
     float* const row_stats = reinterpret_cast<float*>(lds + 4 * TILE);  // two times (3, ROWS): m or shift, 1 / l, -D
-    char* const values = lds + 4 * TILE + 2 * 3 * ROWS * sizeof(float) + (values_in_lds<T, DP>() ? (threadIdx.x >> 6) * TILE : 0);
-    float* const line = row_stats + 2 * 3 * ROWS + (values_in_lds<T, DP>() ? NW * TILE / sizeof(float) : 0);
+    char* const values = lds + 4 * TILE + 2 * 3 * ROWS * sizeof(float) + (values_in_lds<T, DC>() ? (threadIdx.x >> 6) * TILE : 0);
+    float* const line = row_stats + 2 * 3 * ROWS + (values_in_lds<T, DC>() ? NW * TILE / sizeof(float) : 0);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, column = lane & 31;
     int kh;
     int64_t slot;
@@ -1026,25 +1020,25 @@ __global__ __launch_bounds__(NW * 64, (NW == 4 && values_in_lds<T, DP>() ? 2 : 1
     const int each = from < k.there ? max(0, (q.there + ROWS - 1) / ROWS - skip) : 0, whole = each * A.share;
     const int first = (int)((int64_t)whole * z / splits), end = (int)((int64_t)whole * (z + 1) / splits);
 
-    Eight<T> kf[DP / 16], vf[values_in_lds<T, DP>() ? 1 : DP / 16];
+    Eight<T> kf[DC / 16], vf[values_in_lds<T, DC>() ? 1 : DC / 16];
     {
         const T* const k_row = row_start<T>(A.k, k, A.packed, kh) + (mine ? j : 0) * A.k.row;
         const T* const v_row = row_start<T>(A.v, k, A.packed, kh) + (mine ? j : 0) * A.v.row;
-        row_operands<T, DP>(kf, k_row, mine, A.dim, true, lane);
-        if constexpr (values_in_lds<T, DP>()) {
+        row_operands<T, DC>(kf, k_row, mine, A.dim, true, lane);
+        if constexpr (values_in_lds<T, DC>()) {
             Staged<T, DP, 32, 64> vx;
             vx.load(row_start<T>(A.v, k, A.packed, kh) + j0 * A.v.row, A.v.row, k.there - j0, A.dim, lane);
             vx.store(values, lane);      // (read by this wavefront alone)
             (void)v_row;
         } else {
-            row_operands<T, DP>(vf, v_row, mine, A.dim, true, lane);
+            row_operands<T, DC>(vf, v_row, mine, A.dim, true, lane);
             settle<T>(vf);
         }
     }
-    f32x16 dk[DP / 32], dv[DP / 32];
-    Scaled<T, DP> scaled;
+    f32x16 dk[ND], dv[ND];
+    Scaled<T, ND> scaled;
 #pragma unroll
-    for (int d = 0; d < DP / 32; d++)
+    for (int d = 0; d < ND; d++)
 #pragma unroll
         for (int r = 0; r < 16; r++) dk[d][r] = dv[d][r] = 0.0f;
     Staged<T, DP, ROWS, NW * 64> qx, gx;
@@ -1105,11 +1099,11 @@ __global__ __launch_bounds__(NW * 64, (NW == 4 && values_in_lds<T, DP>() ? 2 : 1
             for (int e = 0; e < 4; e++) dp[r + e] = D4[e];
         }
 #pragma unroll
-        for (int c = 0; c < DP / 16; c++) s = Operand<T>::product(L::rows(qr, 0, c), kf[c], s);
+        for (int c = 0; c < DC / 16; c++) s = Operand<T>::product(L::rows(qr, 0, c), kf[c], s);
 #pragma unroll
-        for (int c = 0; c < DP / 16; c++) {
+        for (int c = 0; c < DC / 16; c++) {
             const Eight<T> gx8 = L::rows(gr, 0, c);
-            if constexpr (values_in_lds<T, DP>()) dp = Operand<T>::product(gx8, L::rows(vr, 0, c), dp);
+            if constexpr (values_in_lds<T, DC>()) dp = Operand<T>::product(gx8, L::rows(vr, 0, c), dp);
             else dp = Operand<T>::product(gx8, vf[c], dp);
         }
         if (BIAS) {
@@ -1147,7 +1141,7 @@ __global__ __launch_bounds__(NW * 64, (NW == 4 && values_in_lds<T, DP>() ? 2 : 1
 #pragma unroll
         for (int c = 0; c < 2; c++)
 #pragma unroll
-            for (int d = 0; d < DP / 32; d++) {
+            for (int d = 0; d < ND; d++) {
                 dv[d] = Operand<T>::product(L::columns(gc, 16 * c, d), pf[c], dv[d]);
                 dk[d] = Operand<T>::product(L::columns(qc, 16 * c, d), ds[c], dk[d]);
             }
@@ -1157,7 +1151,7 @@ __global__ __launch_bounds__(NW * 64, (NW == 4 && values_in_lds<T, DP>() ? 2 : 1
     const float lift = NARROW<T> ? 0x1p-15f : 1.0f, factor = A.scale * scaled.back() * lift;
     const int64_t row = (k.first + j) * A.kv_heads + kh, rows = (A.packed ? A.k_rows : A.k_rows * A.batch) * A.kv_heads;
 #pragma unroll
-    for (int d = 0; d < DP / 32; d++)
+    for (int d = 0; d < ND; d++)
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {
             f32x4 x{dk[d][r], dk[d][r + 1], dk[d][r + 2], dk[d][r + 3]}, y{dv[d][r], dv[d][r + 1], dv[d][r + 2], dv[d][r + 3]};
@@ -1175,22 +1169,53 @@ __global__ __launch_bounds__(NW * 64, (NW == 4 && values_in_lds<T, DP>() ? 2 : 1
         }
 }
 
-// out = the sum of the splits, in their order.
+// What the passes left in parts, in one launch: gradients as the sum of their splits, in their order, and the table's.
+struct Finish {
+    const float* parts[3];
+    void* to[3];
+    int64_t count[3], blocks[3];      // elements; workgroups (1024 elements each)
+    int splits[3];
+    const float* table_parts;
+    void* dtable;
+    int64_t table_count;              // workgroups' sums for a (head, bucket)
+    int buckets, heads, table_float;
+};
 template <typename T>
-__global__ __launch_bounds__(256) void add_parts(const float* parts, int splits, int64_t count, T* out) {
-    const int64_t n = (blockIdx.x * 256LL + threadIdx.x) * 4;
-    if (n >= count) return;
-    if (n + 4 <= count && (count & 3) == 0) {
-        f32x4 x{0, 0, 0, 0};
-        for (int z = 0; z < splits; z++) x += *reinterpret_cast<const f32x4*>(parts + z * count + n);
-        put_four<T>(out + n, 0, 4, x);
+__global__ __launch_bounds__(256) void finish_kernel(Finish F) {
+    int64_t block = blockIdx.x;
+#pragma unroll
+    for (int a = 0; a < 3; a++) {
+        if (block >= F.blocks[a]) {
+            block -= F.blocks[a];
+            continue;
+        }
+        const int64_t n = (block * 256 + threadIdx.x) * 4, count = F.count[a];
+        T* const out = static_cast<T*>(F.to[a]);
+        if ((count & 3) == 0) {
+            if (n >= count) return;
+            f32x4 x{0, 0, 0, 0};
+            for (int z = 0; z < F.splits[a]; z++) x += *reinterpret_cast<const f32x4*>(F.parts[a] + z * count + n);
+            put_four<T>(out + n, 0, 4, x);
+        } else {
+            for (int64_t e = n; e < n + 4 && e < count; e++) {
+                float x = 0.0f;
+                for (int z = 0; z < F.splits[a]; z++) x += F.parts[a][z * count + e];
+                out[e] = from_float<T>(x);
+            }
+        }
         return;
     }
-    for (int64_t e = n; e < n + 4 && e < count; e++) {
-        float x = 0.0f;
-        for (int z = 0; z < splits; z++) x += parts[z * count + e];
-        out[e] = from_float<T>(x);
-    }
+    // a wavefront to a (head, bucket): the workgroups' sums in a fixed order, in 64 bits
+    const int64_t at = block * 4 + (threadIdx.x >> 6);
+    if (at >= (int64_t)F.heads * F.buckets) return;
+    const int h = (int)(at / F.buckets), n = (int)(at - (int64_t)h * F.buckets), lane = threadIdx.x & 63;
+    double x = 0.0;
+    for (int64_t w = lane; w < F.table_count; w += 64) x += F.table_parts[(h * F.table_count + w) * F.buckets + n];
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d);
+    if (lane) return;
+    if (F.table_float) static_cast<float*>(F.dtable)[(int64_t)n * F.heads + h] = (float)x;
+    else static_cast<T*>(F.dtable)[(int64_t)n * F.heads + h] = from_float<T>((float)x);
 }
 }  // namespace attention
 
@@ -1202,8 +1227,10 @@ void launch_attention(K kernel, dim3 grid, int threads, size_t lds, hipStream_t 
 }
 template <typename F>
 void with_padded_dim(int dim, F f) {
-    if (dim <= 32) f(std::integral_constant<int, 32>());
+    if (dim <= 16) f(std::integral_constant<int, 16>());
+    else if (dim <= 32) f(std::integral_constant<int, 32>());
     else if (dim <= 64) f(std::integral_constant<int, 64>());
+    else if (dim <= 96) f(std::integral_constant<int, 96>());
     else f(std::integral_constant<int, 128>());
 }
 template <typename F>
@@ -1216,23 +1243,23 @@ inline unsigned die_grid(int64_t count) { return (unsigned)((count + 7) / 8 * 8)
 template <typename T>
 void sequence_attention_forward(const SequenceAttention& A, const AttentionPlan& P, T* out, float* stats, float* scratch, hipStream_t st) {
     using namespace attention;
-    with_padded_dim(A.dim, [&](auto dp) {
+    with_padded_dim(A.dim, [&](auto dc) {
         with_choice(A.table != nullptr, [&](auto bias) {
-            constexpr int DP = decltype(dp)::value;
+            constexpr int DC = decltype(dc)::value, DP = pitch(DC);
             constexpr bool BIAS = decltype(bias)::value;
             const int64_t rows = (A.packed ? A.q_rows : A.q_rows * A.batch) * A.heads;
             if (!P.few) {
                 const size_t lds = 4 * keys_at_once<T, 4>() * Tile<T, DP>::ROW + (BIAS ? (2 * (A.reach + MARGIN) + 1) * sizeof(float) : 0);
-                launch_attention(tiles_kernel<T, DP, 4, BIAS>, dim3(die_grid((int64_t)P.slots * A.heads)), 256, lds, st, A, out, stats, P.slots);
+                launch_attention(tiles_kernel<T, DC, 4, BIAS>, dim3(die_grid((int64_t)P.slots * A.heads)), 256, lds, st, A, out, stats, P.slots);
                 return;
             }
             float* const part_o = scratch;
             float* const part_ml = scratch + P.splits * rows * DP;
             const dim3 grid(P.slots, A.kv_heads * ((A.share + 31) / 32), P.splits);
-            if (P.waves == 1) launch_attention(few_kernel<T, DP, 1, BIAS>, grid, 64, 0, st, A, out, stats, part_o, part_ml, P.splits);
-            else launch_attention(few_kernel<T, DP, 4, BIAS>, grid, 256, 0, st, A, out, stats, part_o, part_ml, P.splits);
+            if (P.waves == 1) launch_attention(few_kernel<T, DC, 1, BIAS>, grid, 64, 0, st, A, out, stats, part_o, part_ml, P.splits);
+            else launch_attention(few_kernel<T, DC, 4, BIAS>, grid, 256, 0, st, A, out, stats, part_o, part_ml, P.splits);
             if (P.splits > 1)
-                launch_attention(combine_parts<T, DP, BIAS>, dim3((unsigned)((rows + 7) / 8)), 256, 0, st, A, part_o, part_ml, P.splits, rows, out, stats);
+                launch_attention(combine_parts<T, DC, BIAS>, dim3((unsigned)((rows + 7) / 8)), 256, 0, st, A, part_o, part_ml, P.splits, rows, out, stats);
         });
     });
 }
@@ -1254,36 +1281,41 @@ void sequence_attention_backward(const SequenceAttention& A, const AttentionGrad
         G.dv_parts = take(P.k_splits * k_all * A.dim);
     }
     G.dtable = dtable ? next : nullptr;
-    with_padded_dim(A.dim, [&](auto dp) {
+    with_padded_dim(A.dim, [&](auto dc) {
         with_choice(A.table != nullptr, [&](auto bias) {
-            constexpr int DP = decltype(dp)::value;
+            constexpr int DC = decltype(dc)::value, DP = pitch(DC);
             constexpr bool BIAS = decltype(bias)::value;
             const size_t line = BIAS ? (2 * (A.reach + MARGIN) + 1) * sizeof(float) : 0, tiles = 4 * 32 * Tile<T, DP>::ROW;
             const size_t sums = BIAS ? (2 * P.q_waves * (2 * (A.reach + MARGIN) + 1) + 2 * P.q_waves) * sizeof(float) : 0;
             if (q_all > 0) {
                 const dim3 grid(die_grid((int64_t)P.q_slots * A.heads), P.q_splits);
-                if (P.q_waves == 1) launch_attention(queries_kernel<T, DP, 1, BIAS>, grid, 64, tiles + line + sums, st, A, G, P.q_slots, P.q_splits);
-                else launch_attention(queries_kernel<T, DP, 4, BIAS>, grid, 256, tiles + line + sums, st, A, G, P.q_slots, P.q_splits);
+                if (P.q_waves == 1) launch_attention(queries_kernel<T, DC, 1, BIAS>, grid, 64, tiles + line + sums, st, A, G, P.q_slots, P.q_splits);
+                else launch_attention(queries_kernel<T, DC, 4, BIAS>, grid, 256, tiles + line + sums, st, A, G, P.q_slots, P.q_splits);
             }
             if (k_all > 0 && G.dk) {
                 const dim3 grid(die_grid((int64_t)P.k_slots * A.kv_heads), P.k_splits);
-                const size_t lds = tiles + 6 * 32 * sizeof(float) + line + (values_in_lds<T, DP>() ? P.k_waves * 32 * Tile<T, DP>::ROW : 0);
-                if (P.k_waves == 1) launch_attention(keys_kernel<T, DP, 1, BIAS>, grid, 64, lds, st, A, G, P.k_slots, P.k_splits);
-                else launch_attention(keys_kernel<T, DP, 4, BIAS>, grid, 256, lds, st, A, G, P.k_slots, P.k_splits);
+                const size_t lds = tiles + 6 * 32 * sizeof(float) + line + (values_in_lds<T, DC>() ? P.k_waves * 32 * Tile<T, DP>::ROW : 0);
+                if (P.k_waves == 1) launch_attention(keys_kernel<T, DC, 1, BIAS>, grid, 64, lds, st, A, G, P.k_slots, P.k_splits);
+                else launch_attention(keys_kernel<T, DC, 4, BIAS>, grid, 256, lds, st, A, G, P.k_slots, P.k_splits);
             }
         });
     });
-    auto add = [&](const float* parts, int splits, int64_t count, void* to) {
-        if (count > 0) launch_attention(add_parts<T>, dim3((unsigned)((count + 1023) / 1024)), 256, 0, st, parts, splits, count, static_cast<T*>(to));
+    Finish F{};
+    int64_t blocks = 0;
+    auto add = [&](int at, const float* parts, int splits, int64_t count, void* to) {
+        if (!parts || !to) return;
+        F.parts[at] = parts; F.to[at] = to; F.splits[at] = splits; F.count[at] = count;
+        blocks += F.blocks[at] = (count + 1023) / 1024;
     };
-    if (P.q_splits > 1) add(G.dq_parts, P.q_splits, q_all * A.dim, G.dq);
-    if (P.k_splits > 1 && G.dk) {
-        add(G.dk_parts, P.k_splits, k_all * A.dim, G.dk);
-        add(G.dv_parts, P.k_splits, k_all * A.dim, G.dv);
-    }
+    add(0, G.dq_parts, P.q_splits, q_all * A.dim, G.dq);
+    add(1, G.dk_parts, P.k_splits, k_all * A.dim, G.dk);
+    add(2, G.dv_parts, P.k_splits, k_all * A.dim, G.dv);
     if (dtable) {
-        const int64_t count = q_all > 0 ? (int64_t)P.q_slots * P.q_splits : 0;
-        launch_attention(table_gradient<T>, dim3(A.buckets, A.heads), 64, 0, st, G.dtable, count, A.buckets, A.heads, A.table_float, dtable);
+        F.table_parts = G.dtable; F.dtable = dtable;
+        F.table_count = q_all > 0 ? P.q_slots * P.q_splits : 0;
+        F.buckets = A.buckets; F.heads = A.heads; F.table_float = A.table_float;
+        blocks += ((int64_t)A.heads * A.buckets + 3) / 4;
     }
+    if (blocks > 0) launch_attention(finish_kernel<T>, dim3((unsigned)blocks), 256, 0, st, F);
 }
 }  // namespace cfh

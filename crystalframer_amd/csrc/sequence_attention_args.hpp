@@ -41,9 +41,10 @@ struct AttentionGrads {
 inline int64_t tile_slots(int packed, int64_t rows, int batch, int tile) {
     return packed ? rows / tile + batch + 1 : (int64_t)batch * ((rows + tile - 1) / tile);
 }
-inline int64_t split_count(int64_t workgroups, int64_t wanted, int64_t most) {
-    const int64_t n = workgroups > 0 ? wanted / workgroups : 1;
-    return n < 1 || most < 1 ? 1 : n > most ? most : n;
+// Into how many parts an axis goes so that there are about `wanted` wavefronts, with at least `least` rows of the axis to each.
+inline int split_count(int64_t wavefronts, int64_t wanted, int64_t rows, int64_t least) {
+    const int64_t n = wavefronts > 0 ? wanted / wavefronts : 1, most = rows / least;
+    return (int)(n < 1 || most < 1 ? 1 : n > most ? most : n);
 }
 
 struct AttentionPlan {
@@ -63,7 +64,7 @@ inline AttentionPlan attention_plan(const SequenceAttention& A) {
     const int at_once = A.share < 32 ? A.share : 32, groups = (A.share + at_once - 1) / at_once;
     P.slots = tile_slots(A.packed, A.q_rows, A.batch, 32 / at_once);
     P.waves = k_each > 64 ? 4 : 1;
-    P.splits = (int)split_count(P.slots * A.kv_heads * groups, 4 * ATTENTION_CUS, k_each / (64 * P.waves));
+    P.splits = split_count(P.slots * A.kv_heads * groups * P.waves, 16 * ATTENTION_CUS, k_each, 64 * P.waves);
     return P;
 }
 
@@ -78,8 +79,8 @@ inline AttentionGradPlan attention_grad_plan(const SequenceAttention& A) {
     P.k_waves = k_each > 64 ? 4 : 1;
     P.q_slots = tile_slots(A.packed, A.q_rows, A.batch, 32 * P.q_waves);
     P.k_slots = tile_slots(A.packed, A.k_rows, A.batch, 32 * P.k_waves);
-    P.q_splits = (int)split_count(P.q_slots * A.heads, 2 * ATTENTION_CUS, k_each / 256);
-    P.k_splits = (int)split_count(P.k_slots * A.kv_heads, 2 * ATTENTION_CUS, q_each * A.share / 256);
+    P.q_splits = split_count(P.q_slots * A.heads * P.q_waves, 8 * ATTENTION_CUS, k_each, 128);
+    P.k_splits = split_count(P.k_slots * A.kv_heads * P.k_waves, 8 * ATTENTION_CUS, q_each * A.share, 128);
     return P;
 }
 
