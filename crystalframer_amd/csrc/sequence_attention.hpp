@@ -213,8 +213,9 @@ struct Staged {
         for (int n = 0; n < EACH; n++) {
             const int r = row + n * EVERY;
             if (ALL % THREADS != 0 && r >= ROWS) continue;
-            const bool keep = whole || (bits >> (r & 63) & 1);
-            *reinterpret_cast<u32x4*>(tile + L::place(r, piece)) = keep ? x[n] : u32x4{0, 0, 0, 0};
+            u32x4 y = x[n];
+            if (!whole) y &= (uint32_t)((int64_t)(bits << (63 - (r & 63))) >> 63);      // all bits of the row's
+            *reinterpret_cast<u32x4*>(tile + L::place(r, piece)) = y;
         }
     }
 };
@@ -313,22 +314,17 @@ __device__ __forceinline__ const T* row_start(const AttentionRows& r, const Span
 __device__ __forceinline__ int shift_of(const SequenceAttention& A, const Span& q, const Span& k) { return A.last ? k.there - q.there : 0; }
 
 // ---- scores ----------------------------------------------------------------------------------------------------------------------------
-// t is what the maximum is taken of and exp2((t - m) rate) the probability: in 16 bits with a bias t has log2 as its unit (rate 1),
-// in float32 t is the score itself, so that the difference to the maximum is taken before anything is rounded.
-template <typename T, bool BIAS>
+// A score t is what the product sums up to, q . k + bias / scale, and exp2((t - m) rate) its power.  The bias costs no instruction of its
+// own that way: near ones are what the product's sum begins with, and one that is the same for a whole tile goes into m.  float32 takes
+// the difference to the maximum before anything is rounded, 16-bit types in one instruction with the factor.
+template <typename T>
 struct Score {
     static constexpr bool WIDE = sizeof(T) == 4;
-    float in, rate;
-    __device__ __forceinline__ explicit Score(float scale) {
-        in = BIAS ? (WIDE ? scale : scale * LOG2E) : 1.0f;
-        rate = BIAS ? (WIDE ? LOG2E : 1.0f) : scale * LOG2E;
-    }
-    static __device__ __forceinline__ float bias(float x) { return WIDE ? x : x * LOG2E; }
-    __device__ __forceinline__ float t(float s, float b) const { return BIAS ? __builtin_fmaf(s, in, b) : s; }
-    // exp of (t - m) in the score's own unit; `shift` = -m rate
+    float rate;
+    __device__ __forceinline__ explicit Score(float scale) : rate(scale * LOG2E) {}
+    // `shift` = -m rate
     __device__ __forceinline__ float power(float t, float m, float shift) const {
-        if (WIDE) return __builtin_amdgcn_exp2f((t - m) * rate);
-        return __builtin_amdgcn_exp2f(BIAS ? t + shift : __builtin_fmaf(t, rate, shift));
+        return __builtin_amdgcn_exp2f(WIDE ? (t - m) * rate : __builtin_fmaf(t, rate, shift));
     }
 };
 
@@ -343,10 +339,11 @@ __device__ __forceinline__ float table_entry(const SequenceAttention& A, int at,
     return A.table_float ? static_cast<const float*>(A.table)[n] : to_float(static_cast<const T*>(A.table)[n]);
 }
 __device__ __forceinline__ int clamped(int r, int reach) { return (r < -reach ? -reach : r > reach ? reach : r) + reach; }
-template <typename T, bool BIAS>
+template <typename T>
 __device__ __forceinline__ void fill_line(const SequenceAttention& A, int head, float* line, int thread, int threads) {
+    const float by = 1.0f / A.scale;
     for (int n = thread; n <= 2 * (A.reach + MARGIN); n += threads)
-        line[n] = Score<T, BIAS>::bias(table_entry<T>(A, clamped(n - A.reach - MARGIN, A.reach), head));
+        line[n] = table_entry<T>(A, clamped(n - A.reach - MARGIN, A.reach), head) * by;
 }
 
 __device__ __forceinline__ float other_half_max(float x) { float a, b; swap32(x, a, b); return fmaxf(a, b); }
@@ -408,24 +405,34 @@ struct Scaled {
     __device__ __forceinline__ float back() const { return NARROW<T> ? 1.0f / by : 1.0f; }
 };
 
-// Scores of 32 keys (rows) and 32 queries (columns) as t, without those that are masked.  bias(r): of register r.
-template <typename T, bool BIAS, typename F>
-__device__ __forceinline__ void scores(f32x16& s, const Score<T, BIAS>& score, uint32_t there, bool causal, int last, int lane, F bias) {
-    const int half4 = (lane >> 5) * 4;
-    if (BIAS)
+// Without the keys (rows) that are not there: `there` holds 0 for one that is and minus infinity for others, in LDS.
+__device__ __forceinline__ void drop_keys(f32x16& s, uint32_t there, int lane) {
 #pragma unroll
-        for (int r = 0; r < 16; r++) s[r] = score.t(s[r], bias(r));
-    if (there != 0xffffffffu) {
-        const uint32_t mine = there >> half4;
+    for (int r = 0; r < 16; r += 4) {
+        const f32x4 x = lds_read<f32x4>(there + (result_row(r) + 4 * (lane >> 5)) * 4);
 #pragma unroll
-        for (int r = 0; r < 16; r++) s[r] = mine >> result_row(r) & 1 ? s[r] : NONE;
-    }
-    if (causal) {       // keys up to number `last` of the tile
-        const int mine = last - half4;
-#pragma unroll
-        for (int r = 0; r < 16; r++) s[r] = result_row(r) <= mine ? s[r] : NONE;
+        for (int e = 0; e < 4; e++) s[r + e] += x[e];
     }
 }
+// Without the keys behind number `last` of the tile.
+__device__ __forceinline__ void drop_behind(f32x16& s, int last, int lane) {
+    const int mine = last - (lane >> 5) * 4;
+#pragma unroll
+    for (int r = 0; r < 16; r++) s[r] = result_row(r) <= mine ? s[r] : NONE;
+}
+// For keys in columns: without the queries (rows) before number `first`.
+__device__ __forceinline__ void drop_before(f32x16& s, int first, int lane) {
+    const int mine = first - (lane >> 5) * 4;
+#pragma unroll
+    for (int r = 0; r < 16; r++) s[r] = result_row(r) >= mine ? s[r] : NONE;
+}
+// Writes what drop_keys() reads, for COUNT keys.
+template <int COUNT>
+__device__ __forceinline__ void put_keys(float* at, uint64_t bits, int thread) {
+    if (thread < COUNT) at[thread] = bits >> thread & 1 ? 0.0f : NONE;
+}
+template <int COUNT>
+__device__ __forceinline__ bool all_there(uint64_t bits) { return COUNT == 64 ? bits == ~0ull : (uint32_t)bits == ~0u; }
 
 // ---- few queries: the keys in parts -----------------------------------------------------------------------------------------------------
 // 32 columns are (query, head of one key head): single tokens of shared heads fill them together.  Every wavefront goes through keys of
@@ -439,7 +446,7 @@ struct FewLds {
     static constexpr int TILE = 32 * Tile<T, DP>::ROW, SUM = 32 * (DP + 4) * 4;
     static constexpr int EACH = 2 * TILE > SUM ? 2 * TILE : SUM;
     alignas(512) char wave[NW][(EACH + 511) / 512 * 512];
-    float m[NW][32], l[NW][32];
+    float m[NW][32], l[NW][32], there[NW][32];
 };
 
 template <typename T, int DC, int NW, bool BIAS>
@@ -459,7 +466,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && NW == 4 ? 2 : 1)) void 
     const int column = lane & 31, i = i0 + column / at_once, h = h0 + column % at_once;
     const bool mine = column / at_once < tile && i < q.there && h < (kh + 1) * A.share;
     const int shift = shift_of(A, q, k);
-    const Score<T, BIAS> score(A.scale);
+    const Score<T> score(A.scale);
 
     // the tiles of this split that any of the queries sees
     const int i_last = min(i0 + tile, q.there) - 1;
@@ -474,10 +481,11 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && NW == 4 ? 2 : 1)) void 
     const T* const k_at = row_start<T>(A.k, k, A.packed, kh);
     const T* const v_at = row_start<T>(A.v, k, A.packed, kh);
     const uint8_t* const mask = A.mask ? A.mask + k.first : nullptr;
+    const float by = 1.0f / A.scale;
     float far[2] = {0.0f, 0.0f};
     if (BIAS && mine) {
-        far[0] = Score<T, BIAS>::bias(table_entry<T>(A, 0, h));
-        far[1] = Score<T, BIAS>::bias(table_entry<T>(A, 2 * A.reach, h));
+        far[0] = table_entry<T>(A, 0, h) * by;
+        far[1] = table_entry<T>(A, 2 * A.reach, h) * by;
     }
     char* const kt = S.wave[wave];
     char* const vt = kt + FewLds<T, DP, NW>::TILE;
@@ -498,31 +506,32 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && NW == 4 ? 2 : 1)) void 
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         const uint32_t there = (uint32_t)bits.get(mask);
         const uint64_t rows = mask ? there | ~0xffffffffull : ~0ull;      // (rows behind the last are 0 already)
+        if (!all_there<32>(there)) put_keys<32>(S.there[wave], there, lane);
         kx.store(kt, lane, rows);
         vx.store(vt, lane, rows);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         if (n + NW < end) fetch(n + NW);
         f32x16 s;
+        const int low = j0 - i_last - shift, high = j0 + 31 - i0 - shift;      // relative positions of the tile
+        const bool near = BIAS && low < A.reach && high > -A.reach;
+        if (near) {
+            const int r0 = j0 + 4 * half - i - shift;
 #pragma unroll
-        for (int r = 0; r < 16; r++) s[r] = 0.0f;
+            for (int r = 0; r < 16; r++) s[r] = mine ? table_entry<T>(A, clamped(r0 + result_row(r), A.reach), h) * by : 0.0f;
+        } else {
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[r] = 0.0f;
+        }
 #pragma unroll
         for (int c = 0; c < DC / 16; c++) s = Operand<T>::product(L::rows(kr, 0, c), qf[c], s);
-        const int low = j0 - i_last - shift, high = j0 + 31 - i0 - shift;      // relative positions of the tile
-        const int r0 = j0 + 4 * half - i - shift;
-        const bool causal = A.causal && high > 0;
-        if (!BIAS || low >= A.reach || high <= -A.reach) {
-            const float flat = low >= A.reach ? far[1] : far[0];
-            scores<T, BIAS>(s, score, there, causal, i + shift - j0, lane, [&](int) { return flat; });
-        } else {
-            scores<T, BIAS>(s, score, there, causal, i + shift - j0, lane, [&](int r) {
-                return mine ? Score<T, BIAS>::bias(table_entry<T>(A, clamped(r0 + result_row(r), A.reach), h)) : 0.0f;
-            });
-        }
+        if (!all_there<32>(there)) drop_keys(s, lds_address(S.there[wave]), lane);
+        if (A.causal && high > 0) drop_behind(s, i + shift - j0, lane);
+        const float flat = BIAS && !near ? low >= A.reach ? far[1] : far[0] : 0.0f;
         float top = s[0];
 #pragma unroll
         for (int r = 1; r < 16; r++) top = fmaxf(top, s[r]);
-        sum.meet(other_half_max(top), score.rate);
-        const float m = sum.base(), off = POWER_LIFT<T> - m * score.rate;
+        sum.meet(other_half_max(top) + flat, score.rate);
+        const float m = sum.base() - flat, off = POWER_LIFT<T> - m * score.rate;
 #pragma unroll
         for (int r = 0; r < 16; r++) {
             s[r] = score.power(s[r], m, off);
@@ -596,7 +605,7 @@ __global__ __launch_bounds__(256) void combine_parts(SequenceAttention A, const 
     const int64_t row = blockIdx.x * 8LL + threadIdx.x / 32;
     const int from = (threadIdx.x & 31) * 4;
     if (row >= rows || from >= DP) return;
-    const Score<T, BIAS> score(A.scale);
+    const Score<T> score(A.scale);
     float m = NONE, l = 0.0f;
     for (int z = 0; z < splits; z++) m = fmaxf(m, part_ml[2 * (z * rows + row)]);
     f32x4 o{0, 0, 0, 0};
@@ -625,7 +634,8 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 ? 2 : 1)) void tiles_kerne
     constexpr int KEYS = keys_at_once<T, NW>(), TILE = KEYS * L::ROW;
     extern __shared__ __attribute__((aligned(512))) char lds[];
     char* const tiles = lds;                    // two pairs of a tile of keys and one of values
-    float* const line = reinterpret_cast<float*>(lds + 4 * TILE);
+    float* const keys = reinterpret_cast<float*>(lds + 4 * TILE);       // which are there: two times KEYS
+    float* const line = keys + 2 * KEYS;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, column = lane & 31;
     int h;
     int64_t slot;
@@ -640,7 +650,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 ? 2 : 1)) void tiles_kerne
     const int i0 = from + wave * 32, i = i0 + column;
     const bool mine = i < q.there;
     const int shift = shift_of(A, q, k);
-    const Score<T, BIAS> score(A.scale);
+    const Score<T> score(A.scale);
     int seen = from < q.there ? k.there : 0;
     if (A.causal) seen = min(seen, min(from + NW * 32, q.there) + shift);
     const int count = seen > 0 ? (seen + KEYS - 1) / KEYS : 0;
@@ -651,7 +661,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 ? 2 : 1)) void tiles_kerne
     const T* const k_at = row_start<T>(A.k, k, A.packed, kh);
     const T* const v_at = row_start<T>(A.v, k, A.packed, kh);
     const uint8_t* const mask = A.mask ? A.mask + k.first : nullptr;
-    if (BIAS) fill_line<T, BIAS>(A, h, line, threadIdx.x, NW * 64);
+    if (BIAS) fill_line<T>(A, h, line, threadIdx.x, NW * 64);
     Running<ND> sum;
     Staged<T, DP, KEYS, NW * 64> kx, vx;
     KeyBits bits;
@@ -665,6 +675,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 ? 2 : 1)) void tiles_kerne
     auto put = [&](int n) {
         there = bits.get(mask);
         const uint64_t rows = mask ? there | (KEYS < 64 ? ~0ull << (KEYS & 63) : 0ull) : ~0ull;      // (rows behind the last are 0 already)
+        if (!all_there<KEYS>(there)) put_keys<KEYS>(keys + (n & 1) * KEYS, there, threadIdx.x);
         kx.store(tiles + (n & 1) * 2 * TILE, threadIdx.x, rows);
         vx.store(tiles + (n & 1) * 2 * TILE + TILE, threadIdx.x, rows);
     };
@@ -678,32 +689,42 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 ? 2 : 1)) void tiles_kerne
         const uint32_t tile = lds_address(tiles) + (n & 1) * 2 * TILE, kr = tile + L::rows_at(lane), vc = tile + TILE + L::columns_at(lane);
         if (n + 1 < count) fetch(n + 1);
         f32x16 s[KEYS / 32];
+        const int j0 = n * KEYS, low = j0 - (i0 + 31) - shift, high = j0 + KEYS - 1 - i0 - shift;
+        const bool near = BIAS && low < A.reach && high > -A.reach;
+        auto products = [&] {
+#pragma unroll
+            for (int c = 0; c < DC / 16; c++)
+#pragma unroll
+                for (int u = 0; u < KEYS / 32; u++) s[u] = Operand<T>::product(L::rows(kr, 32 * u, c), qf[c], s[u]);
+        };
+        if (near) {
+            const float* const at = line + (j0 + 4 * half - i - shift + A.reach + MARGIN);
+#pragma unroll
+            for (int u = 0; u < KEYS / 32; u++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) s[u][r] = at[32 * u + result_row(r)];
+            products();
+        } else {
+#pragma unroll
+            for (int u = 0; u < KEYS / 32; u++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) s[u][r] = 0.0f;
+            products();
+        }
+        const float flat = BIAS && !near ? line[low >= A.reach ? 2 * (A.reach + MARGIN) : 0] : 0.0f;
+        if (!all_there<KEYS>(there))
+#pragma unroll
+            for (int u = 0; u < KEYS / 32; u++) drop_keys(s[u], lds_address(keys + (n & 1) * KEYS + 32 * u), lane);
+        if (A.causal && high > 0)
+#pragma unroll
+            for (int u = 0; u < KEYS / 32; u++) drop_behind(s[u], i + shift - j0 - 32 * u, lane);
         float top = NONE;
 #pragma unroll
         for (int u = 0; u < KEYS / 32; u++)
 #pragma unroll
-            for (int r = 0; r < 16; r++) s[u][r] = 0.0f;
-#pragma unroll
-        for (int c = 0; c < DC / 16; c++)
-#pragma unroll
-            for (int u = 0; u < KEYS / 32; u++) s[u] = Operand<T>::product(L::rows(kr, 32 * u, c), qf[c], s[u]);
-#pragma unroll
-        for (int u = 0; u < KEYS / 32; u++) {
-            const int j0 = n * KEYS + 32 * u;
-            const int low = j0 - (i0 + 31) - shift, high = j0 + 31 - i0 - shift;
-            const bool causal = A.causal && high > 0;
-            if (!BIAS || low >= A.reach || high <= -A.reach) {
-                const float flat = BIAS ? line[low >= A.reach ? 2 * (A.reach + MARGIN) : 0] : 0.0f;
-                scores<T, BIAS>(s[u], score, (uint32_t)(there >> 32 * u), causal, i + shift - j0, lane, [&](int) { return flat; });
-            } else {
-                const float* const at = line + (j0 + 4 * half - i - shift + A.reach + MARGIN);
-                scores<T, BIAS>(s[u], score, (uint32_t)(there >> 32 * u), causal, i + shift - j0, lane, [&](int r) { return at[result_row(r)]; });
-            }
-#pragma unroll
             for (int r = 0; r < 16; r++) top = fmaxf(top, s[u][r]);
-        }
-        sum.meet(other_half_max(top), score.rate);
-        const float m = sum.base(), off = POWER_LIFT<T> - m * score.rate;
+        sum.meet(other_half_max(top) + flat, score.rate);
+        const float m = sum.base() - flat, off = POWER_LIFT<T> - m * score.rate;
 #pragma unroll
         for (int u = 0; u < KEYS / 32; u++) {
 #pragma unroll
@@ -741,12 +762,12 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 ? 2 : 1)) void tiles_kerne
 
 // ---- backward: queries' side ---------------------------------------------------------------------------------------------------------------
 // Probability of a stored row: exp2((t - m) rate) / l; 16 bits: with 1 / l in the exponent (0 for a row without keys).
-template <typename T, bool BIAS>
-__device__ __forceinline__ float row_shift(const Score<T, BIAS>& score, float m, float inverse) {
+template <typename T>
+__device__ __forceinline__ float row_shift(const Score<T>& score, float m, float inverse) {
     return sizeof(T) == 4 ? 0.0f : __builtin_amdgcn_logf(inverse) - m * score.rate;
 }
-template <typename T, bool BIAS>
-__device__ __forceinline__ float probability(const Score<T, BIAS>& score, float t, float m, float inverse, float shift) {
+template <typename T>
+__device__ __forceinline__ float probability(const Score<T>& score, float t, float m, float inverse, float shift) {
     const float p = score.power(t, m, shift);
     return sizeof(T) == 4 ? p * inverse : p;
 }
@@ -785,7 +806,8 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
     constexpr int KEYS = 32, TILE = KEYS * L::ROW;
     extern __shared__ __attribute__((aligned(512))) char lds[];
     char* const tiles = lds;
-    float* const line = reinterpret_cast<float*>(lds + 4 * TILE);
+    float* const keys = reinterpret_cast<float*>(lds + 4 * TILE);       // which are there: two times KEYS
+    float* const line = keys + 2 * KEYS;
     const int entries = 2 * (A.reach + MARGIN) + 1;
     float* const sums = line + entries;                         // (2 NW, entries), then two for each wavefront
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, column = lane & 31;
@@ -807,7 +829,7 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
     const int i0 = from + wave * 32, i = i0 + column;
     const bool mine = i < q.there;
     const int shift = shift_of(A, q, k);
-    const Score<T, BIAS> score(A.scale);
+    const Score<T> score(A.scale);
     int seen = from < q.there ? k.there : 0;
     if (A.causal) seen = min(seen, min(from + NW * 32, q.there) + shift);
     const int whole = seen > 0 ? (seen + KEYS - 1) / KEYS : 0;
@@ -842,7 +864,7 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
     const T* const v_at = row_start<T>(A.v, k, A.packed, kh);
     const uint8_t* const mask = A.mask ? A.mask + k.first : nullptr;
     if (BIAS) {
-        fill_line<T, BIAS>(A, h, line, threadIdx.x, NW * 64);
+        fill_line<T>(A, h, line, threadIdx.x, NW * 64);
         for (int n = threadIdx.x; n < 2 * NW * entries; n += NW * 64) sums[n] = 0.0f;
     }
     float* const own_sums = sums + (2 * wave + half) * entries;
@@ -865,6 +887,7 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
     auto put = [&](int n) {
         there = bits.get(mask);
         const uint64_t rows = mask ? there | (KEYS < 64 ? ~0ull << (KEYS & 63) : 0ull) : ~0ull;      // (rows behind the last are 0 already)
+        if (!all_there<KEYS>(there)) put_keys<KEYS>(keys + (n & 1) * KEYS, there, threadIdx.x);
         kx.store(tiles + (n & 1) * 2 * TILE, threadIdx.x, rows);
         vx.store(tiles + (n & 1) * 2 * TILE + TILE, threadIdx.x, rows);
     };
@@ -879,31 +902,40 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
     for (int n = first; n < end; n++) {
         const uint32_t tile = lds_address(tiles) + (n & 1) * 2 * TILE, kr = tile + L::rows_at(lane), vr = kr + TILE, kc = tile + L::columns_at(lane);
         if (n + 1 < end) fetch(n + 1);
-        const int j0 = n * KEYS;
+        const int j0 = n * KEYS, low = j0 - (i0 + 31) - shift, high = j0 + 31 - i0 - shift;
+        const bool near = BIAS && low < A.reach && high > -A.reach;
         f32x16 s, dp;
+        auto products = [&] {
 #pragma unroll
-        for (int r = 0; r < 16; r++) s[r] = dp[r] = 0.0f;
+            for (int c = 0; c < DC / 16; c++) {
+                s = Operand<T>::product(L::rows(kr, 0, c), qf[c], s);
+                dp = Operand<T>::product(L::rows(vr, 0, c), gf[c], dp);
+            }
+        };
 #pragma unroll
-        for (int c = 0; c < DC / 16; c++) s = Operand<T>::product(L::rows(kr, 0, c), qf[c], s);
+        for (int r = 0; r < 16; r++) dp[r] = 0.0f;
+        if (near) {
+            const float* const at = line + (j0 + 4 * half - i - shift + A.reach + MARGIN);
 #pragma unroll
-        for (int c = 0; c < DC / 16; c++) dp = Operand<T>::product(L::rows(vr, 0, c), gf[c], dp);
-        const int low = j0 - (i0 + 31) - shift, high = j0 + 31 - i0 - shift, r0 = j0 + 4 * half - i - shift;
-        const bool causal = A.causal && high > 0, beyond = low >= A.reach || high <= -A.reach;
-        if (!BIAS || beyond) {
-            const float flat = BIAS ? line[low >= A.reach ? 2 * (A.reach + MARGIN) : 0] : 0.0f;
-            scores<T, BIAS>(s, score, (uint32_t)there, causal, i + shift - j0, lane, [&](int) { return flat; });
+            for (int r = 0; r < 16; r++) s[r] = at[result_row(r)];
+            products();
         } else {
-            const float* const at = line + (r0 + A.reach + MARGIN);
-            scores<T, BIAS>(s, score, (uint32_t)there, causal, i + shift - j0, lane, [&](int r) { return at[result_row(r)]; });
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[r] = 0.0f;
+            products();
         }
+        const float flat = BIAS && !near ? line[low >= A.reach ? 2 * (A.reach + MARGIN) : 0] : 0.0f;
+        if (!all_there<KEYS>(there)) drop_keys(s, lds_address(keys + (n & 1) * KEYS), lane);
+        if (A.causal && high > 0) drop_behind(s, i + shift - j0, lane);
+        const float mt = m - flat, offt = off + flat * score.rate;
         if (!BIAS) {
 #pragma unroll
-            for (int r = 0; r < 16; r++) s[r] = probability(score, s[r], m, inverse, off) * (dp[r] - D);
-        } else if (beyond) {
+            for (int r = 0; r < 16; r++) s[r] = probability(score, s[r], mt, inverse, offt) * (dp[r] - D);
+        } else if (!near) {
             float ds = 0.0f, ps = 0.0f;
 #pragma unroll
             for (int r = 0; r < 16; r++) {
-                const float p = probability(score, s[r], m, inverse, off);
+                const float p = probability(score, s[r], mt, inverse, offt);
                 s[r] = p * (dp[r] - D);
                 ds += s[r];
                 ps += p;
@@ -915,7 +947,7 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
         } else {
 #pragma unroll
             for (int r = 0; r < 16; r++) {
-                s[r] = probability(score, s[r], m, inverse, off) * (dp[r] - D);
+                s[r] = probability(score, s[r], mt, inverse, offt) * (dp[r] - D);
                 all_ds += s[r];
             }
             float x[3] = {0.0f, 0.0f, 0.0f};
@@ -1013,7 +1045,7 @@ __global__ __launch_bounds__(NW * 64, (NW == 4 && values_in_lds<T, DC>() ? 2 : 1
     const int j0 = from + wave * 32, j = j0 + column;
     const bool mine = j < k.there && (!A.mask || A.mask[k.first + j]);
     const int shift = shift_of(A, q, k);
-    const Score<T, BIAS> score(A.scale);
+    const Score<T> score(A.scale);
     // the first tile of queries that sees a key of this workgroup
     int skip = 0;
     if (A.causal) skip = max(0, from - shift) / ROWS;
@@ -1082,16 +1114,25 @@ __global__ __launch_bounds__(NW * 64, (NW == 4 && values_in_lds<T, DC>() ? 2 : 1
         const int h = kh * A.share + n / each, i0 = (skip + n % each) * ROWS;
         if (BIAS && h != line_of) {
             __syncthreads();
-            fill_line<T, BIAS>(A, h, line, threadIdx.x, NW * 64);
+            fill_line<T>(A, h, line, threadIdx.x, NW * 64);
             line_of = h;
         }
         __syncthreads();
         const uint32_t tile = lds_address(tiles) + (n & 1) * 2 * TILE, qr = tile + L::rows_at(lane), gr = qr + TILE, qc = tile + L::columns_at(lane),
                        gc = qc + TILE;
         const float* const st = row_stats + (n & 1) * 3 * ROWS + 4 * half;
+        if (n + 1 < end) fetch(n + 1);
         f32x16 s, dp;
+        const int low = j0 - (i0 + 31) - shift, high = j0 + 31 - i0 - shift;
+        if (BIAS && low < A.reach && high > -A.reach) {
+            const float* const at = line + (j - i0 - 4 * half - shift + A.reach + MARGIN);
 #pragma unroll
-        for (int r = 0; r < 16; r++) s[r] = 0.0f;
+            for (int r = 0; r < 16; r++) s[r] = at[-result_row(r)];
+        } else {
+            const float flat = BIAS ? line[low >= A.reach ? 2 * (A.reach + MARGIN) : 0] : 0.0f;
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[r] = flat;
+        }
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {      // do . v - D
             const f32x4 D4 = *reinterpret_cast<const f32x4*>(st + 2 * ROWS + result_row(r));
@@ -1106,23 +1147,7 @@ __global__ __launch_bounds__(NW * 64, (NW == 4 && values_in_lds<T, DC>() ? 2 : 1
             if constexpr (values_in_lds<T, DC>()) dp = Operand<T>::product(gx8, L::rows(vr, 0, c), dp);
             else dp = Operand<T>::product(gx8, vf[c], dp);
         }
-        if (BIAS) {
-            const int low = j0 - (i0 + 31) - shift, high = j0 + 31 - i0 - shift;
-            if (low >= A.reach || high <= -A.reach) {
-                const float flat = line[low >= A.reach ? 2 * (A.reach + MARGIN) : 0];
-#pragma unroll
-                for (int r = 0; r < 16; r++) s[r] = score.t(s[r], flat);
-            } else {
-                const float* const at = line + (j - i0 - 4 * half - shift + A.reach + MARGIN);
-#pragma unroll
-                for (int r = 0; r < 16; r++) s[r] = score.t(s[r], at[-result_row(r)]);
-            }
-        }
-        if (A.causal && j0 + 31 > i0 + shift) {
-            const int least = j - shift - i0 - 4 * half;      // first row that sees the column's key
-#pragma unroll
-            for (int r = 0; r < 16; r++) s[r] = result_row(r) >= least ? s[r] : NONE;
-        }
+        if (A.causal && high > 0) drop_before(s, j - shift - i0, lane);
         f32x16 p;
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {
@@ -1137,7 +1162,6 @@ __global__ __launch_bounds__(NW * 64, (NW == 4 && values_in_lds<T, DC>() ? 2 : 1
         }
         scaled.meet(s, dk);
         const Eight<T> pf[2] = {rounded<T>(p, 0), rounded<T>(p, 1)}, ds[2] = {rounded<T>(s, 0), rounded<T>(s, 1)};
-        if (n + 1 < end) fetch(n + 1);      // (here: registers that the scores had)
 #pragma unroll
         for (int c = 0; c < 2; c++)
 #pragma unroll
@@ -1249,7 +1273,7 @@ void sequence_attention_forward(const SequenceAttention& A, const AttentionPlan&
             constexpr bool BIAS = decltype(bias)::value;
             const int64_t rows = (A.packed ? A.q_rows : A.q_rows * A.batch) * A.heads;
             if (!P.few) {
-                const size_t lds = 4 * keys_at_once<T, 4>() * Tile<T, DP>::ROW + (BIAS ? (2 * (A.reach + MARGIN) + 1) * sizeof(float) : 0);
+                const size_t lds = 4 * keys_at_once<T, 4>() * Tile<T, DP>::ROW + 2 * keys_at_once<T, 4>() * sizeof(float) + (BIAS ? (2 * (A.reach + MARGIN) + 1) * sizeof(float) : 0);
                 launch_attention(tiles_kernel<T, DC, 4, BIAS>, dim3(die_grid((int64_t)P.slots * A.heads)), 256, lds, st, A, out, stats, P.slots);
                 return;
             }
@@ -1289,8 +1313,8 @@ void sequence_attention_backward(const SequenceAttention& A, const AttentionGrad
             const size_t sums = BIAS ? (2 * P.q_waves * (2 * (A.reach + MARGIN) + 1) + 2 * P.q_waves) * sizeof(float) : 0;
             if (q_all > 0) {
                 const dim3 grid(die_grid((int64_t)P.q_slots * A.heads), P.q_splits);
-                if (P.q_waves == 1) launch_attention(queries_kernel<T, DC, 1, BIAS>, grid, 64, tiles + line + sums, st, A, G, P.q_slots, P.q_splits);
-                else launch_attention(queries_kernel<T, DC, 4, BIAS>, grid, 256, tiles + line + sums, st, A, G, P.q_slots, P.q_splits);
+                if (P.q_waves == 1) launch_attention(queries_kernel<T, DC, 1, BIAS>, grid, 64, tiles + 64 * sizeof(float) + line + sums, st, A, G, P.q_slots, P.q_splits);
+                else launch_attention(queries_kernel<T, DC, 4, BIAS>, grid, 256, tiles + 64 * sizeof(float) + line + sums, st, A, G, P.q_slots, P.q_splits);
             }
             if (k_all > 0 && G.dk) {
                 const dim3 grid(die_grid((int64_t)P.k_slots * A.kv_heads), P.k_splits);
