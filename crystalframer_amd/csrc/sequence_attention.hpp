@@ -4,11 +4,11 @@
 //   D_i = do_i . o_i,   ds_ij = P_ij (do_i . v_j - D_i)
 //   dv_j = sum_i P_ij do_i,   dq_i = scale sum_j ds_ij k_j,   dk_j = scale sum_i ds_ij q_i,   dtable[b] = sum over bucket b of ds_ij
 //
-// All products are matrix instructions of 32 x 32 results, 16 (16-bit types) or 2 (float32) terms deep.  A result has its column in
+// All products are matrix instructions of 32 x 32 results, 16 terms deep.  A result has its column in
 // the lane (l % 32) and 16 of its rows in the lane's registers: rows 8 (r / 4) + 4 (l / 32) + r % 4.  The scores are made transposed
 // where sums over keys follow (rows: keys, columns: queries), and upright where sums over queries follow: either way the probabilities
 // are, register by register, the right operand of the product that follows, whose terms may come in any order as long as the left
-// operand has them in the same one.  That operand is the transpose of a tile in LDS (16 bits: ds_read_b64_tr_b16; float32: words).
+// operand has them in the same one.  That operand is the transpose of a tile in LDS (ds_read_b64_tr_b16).
 // Statistics of a row, its largest score and its sum, then live in one lane (two: the halves of the wavefront share a column).
 #pragma once
 #include <hip/hip_runtime.h>
@@ -43,23 +43,59 @@ template <> struct Operand<f16> {
     typedef f16 Eight __attribute__((ext_vector_type(8)));
     static __device__ __forceinline__ f32x16 product(Eight a, Eight b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
+// float32: three bfloat16 parts hold a value's 24 bits (each what the ones before leave, to the nearest), and six products of parts, from the
+// small ones on, hold theirs to 2^-25: 192 cycles where float32's own instruction takes 512.  An infinity becomes NaN.
 template <> struct Operand<float> {
-    typedef f32x8 Eight;
-    static __device__ __forceinline__ f32x16 product(Eight a, Eight b, f32x16 c) {
-#pragma unroll
-        for (int e = 0; e < 8; e++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
-        return c;
+    typedef Operand<bf16>::Eight Part;
+    struct Eight { Part h, m, l; };
+    static __device__ __forceinline__ f32x16 product(const Eight& a, const Eight& b, f32x16 c) {
+        c = Operand<bf16>::product(a.l, b.h, c);
+        c = Operand<bf16>::product(a.h, b.l, c);
+        c = Operand<bf16>::product(a.m, b.m, c);
+        c = Operand<bf16>::product(a.m, b.h, c);
+        c = Operand<bf16>::product(a.h, b.m, c);
+        return Operand<bf16>::product(a.h, b.h, c);
     }
 };
 template <typename T> using Eight = typename Operand<T>::Eight;
 
+template <int N>
+__device__ __forceinline__ void split(const float (&x)[N], bf16* h, bf16* m, bf16* l) {
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+        h[n] = from_float<bf16>(x[n]);
+        const float y = x[n] - to_float(h[n]);
+        m[n] = from_float<bf16>(y);
+        l[n] = from_float<bf16>(y - to_float(m[n]));
+    }
+}
+__device__ __forceinline__ Eight<float> in_parts(const float (&x)[8]) {
+    bf16 h[8], m[8], l[8];
+    split(x, h, m, l);
+    Eight<float> y;
+#pragma unroll
+    for (int n = 0; n < 8; n++) y.h[n] = h[n], y.m[n] = m[n], y.l[n] = l[n];
+    return y;
+}
 // Registers 8 s ... 8 s + 7 of a result, rounded to T (half a unit each: 2^-9, 2^-12; float32 stays), as an operand of step s.
 template <typename T>
 __device__ __forceinline__ Eight<T> rounded(const f32x16& x, int s) {
-    Eight<T> y;
+    if constexpr (sizeof(T) == 4) {
+        float y[8];
 #pragma unroll
-    for (int e = 0; e < 8; e++) y[e] = from_float<T>(x[8 * s + e]);
-    return y;
+        for (int e = 0; e < 8; e++) y[e] = x[8 * s + e];
+        return in_parts(y);
+    } else {
+        Eight<T> y;
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[e] = from_float<T>(x[8 * s + e]);
+        return y;
+    }
+}
+template <typename T>
+__device__ __forceinline__ float value(const Eight<T>& x, int e) {
+    if constexpr (sizeof(T) == 4) return to_float(x.h[e]) + (to_float(x.m[e]) + to_float(x.l[e]));
+    else return to_float(x[e]);
 }
 // Row of register r of a result, without the lane's 4 (l / 32).
 __device__ __forceinline__ constexpr int result_row(int r) { return 8 * (r / 4) + r % 4; }
@@ -84,46 +120,43 @@ __device__ __forceinline__ V lds_read(uint32_t at) { return *reinterpret_cast<__
 constexpr int pitch(int dc) { return dc <= 32 ? 32 : dc <= 64 ? 64 : 128; }
 template <typename T, int DP>
 struct Tile {
-    static constexpr int E = 16 / sizeof(T), PIECES = DP / E, ROW = DP * sizeof(T);
+    static constexpr int E = 16 / sizeof(T), PIECES = DP / E;           // in memory
+    static constexpr int ROW = DP * 2, PLANES = sizeof(T) == 4 ? 3 : 1;  // in LDS: float32 as three tiles of parts
+    static constexpr int bytes(int rows) { return rows * ROW * PLANES; }
     static __device__ __forceinline__ constexpr int mixed(int row) {
-        if (sizeof(T) == 4) return PIECES >= 16 ? ((row >> 2 & 1) << 3 | (row & 3) << 1 | (row >> 3 & 1)) : (row >> 1 & 7);
-        if (PIECES == 16) return (row & 3) << 2 | (row >> 2 & 3);
-        if (PIECES == 8) return (row >> 1 & 1) << 2 | (row >> 2 & 3);
+        if (DP == 128) return (row & 3) << 2 | (row >> 2 & 3);
+        if (DP == 64) return (row >> 1 & 1) << 2 | (row >> 2 & 3);
         return row >> 2 & 3;
     }
     static __device__ __forceinline__ int place(int row, int piece) { return row * ROW + ((piece ^ mixed(row)) << 4); }
     // The lane's part of an address for rows() and columns().
-    static __device__ __forceinline__ uint32_t rows_at(int lane) { return place(lane & 31, (lane >> 5) * (sizeof(T) / 2)); }
+    static __device__ __forceinline__ uint32_t rows_at(int lane) { return place(lane & 31, lane >> 5); }
     static __device__ __forceinline__ uint32_t columns_at(int lane) {
-        const int half = lane >> 5;
-        if (sizeof(T) == 2) return place(4 * half + (lane & 15) / 4, 2 * (lane >> 4 & 1) + (lane & 3) / 2) + (lane & 1) * 8;
-        return place(4 * half, (lane & 31) / 4) + (lane & 3) * 4;
+        return place(4 * (lane >> 5) + (lane & 15) / 4, 2 * (lane >> 4 & 1) + (lane & 3) / 2) + (lane & 1) * 8;
     }
-    // Channels 16 step + 8 (l / 32) ... of row base + l % 32.
+    template <typename U>
+    static __device__ __forceinline__ Eight<U> transposed(uint32_t at, int base, int d) {
+        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4*>((at ^ d << 6) + base * ROW));
+        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4*>((at ^ (d << 6 | 32)) + (base + 8) * ROW));
+        typedef short s16x8 __attribute__((ext_vector_type(8)));
+        return __builtin_bit_cast(Eight<U>, s16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]});
+    }
+    // Channels 16 step + 8 (l / 32) ... of row base + l % 32 of a tile of ROWS rows.
+    template <int ROWS>
     static __device__ __forceinline__ Eight<T> rows(uint32_t at, int base, int step) {
+        const uint32_t a = (at ^ step << 5) + base * ROW;
         if constexpr (sizeof(T) == 2) {
-            return lds_read<Eight<T>>((at ^ step << 5) + base * ROW);
+            return lds_read<Eight<T>>(a);
         } else {
-            const f32x4 a = lds_read<f32x4>((at ^ step << 6) + base * ROW), b = lds_read<f32x4>((at ^ (step << 6 | 16)) + base * ROW);
-            return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+            typedef Operand<float>::Part Part;
+            return {lds_read<Part>(a), lds_read<Part>(a + ROWS * ROW), lds_read<Part>(a + 2 * ROWS * ROW)};
         }
     }
     // Channel 32 d + l % 32 of rows base + 8 (e / 4) + 4 (l / 32) + e % 4.
+    template <int ROWS>
     static __device__ __forceinline__ Eight<T> columns(uint32_t at, int base, int d) {
-        if constexpr (sizeof(T) == 2) {
-            const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4*>((at ^ d << 6) + base * ROW));
-            const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4*>((at ^ (d << 6 | 32)) + (base + 8) * ROW));
-            typedef short s16x8 __attribute__((ext_vector_type(8)));
-            return __builtin_bit_cast(Eight<T>, s16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]});
-        } else {
-            f32x8 x;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {      // (the row's part in the exchange: 4 (l / 32) is in the lane's, 8 (e / 4) + e % 4 here)
-                const int row = 8 * (e / 4) + e % 4;
-                x[e] = lds_read<float>((at ^ (d << 7 | mixed(row) << 4)) + (base + row) * ROW);
-            }
-            return x;
-        }
+        if constexpr (sizeof(T) == 2) return transposed<T>(at, base, d);
+        else return {transposed<bf16>(at, base, d), transposed<bf16>(at, base + ROWS, d), transposed<bf16>(at, base + 2 * ROWS, d)};
     }
 };
 
@@ -165,14 +198,26 @@ __device__ __forceinline__ void row_operands(Eight<T> (&y)[DC / 16], const T* ro
             }
         }
     }
-    __builtin_memcpy(y, x, sizeof(x));
+    if constexpr (sizeof(T) == 2) {
+        __builtin_memcpy(y, x, sizeof(x));
+    } else {
+#pragma unroll
+        for (int c = 0; c < DC / 16; c++) {
+            float e[8];
+            __builtin_memcpy(e, x + 2 * c, 32);
+            y[c] = in_parts(e);
+        }
+    }
 }
 
 // Waits for operands here.  (Left to their first use, in the loop, the wait would also be for the tile that was asked for last.)
 template <typename T, int N>
 __device__ __forceinline__ void settle(Eight<T> (&y)[N]) {
 #pragma unroll
-    for (int n = 0; n < N; n++) asm volatile("" : "+v"(y[n]));
+    for (int n = 0; n < N; n++) {
+        if constexpr (sizeof(T) == 2) asm volatile("" : "+v"(y[n]));
+        else asm volatile("" : "+v"(y[n].h), "+v"(y[n].m), "+v"(y[n].l));
+    }
 }
 
 // Which of the next keys are there: a bit for each, of the mask's bytes on their way (lane l: key l), or of their number.
@@ -215,7 +260,19 @@ struct Staged {
             if (ALL % THREADS != 0 && r >= ROWS) continue;
             u32x4 y = x[n];
             if (!whole) y &= (uint32_t)((int64_t)(bits << (63 - (r & 63))) >> 63);      // all bits of the row's
-            *reinterpret_cast<u32x4*>(tile + L::place(r, piece)) = y;
+            if constexpr (sizeof(T) == 2) {
+                *reinterpret_cast<u32x4*>(tile + L::place(r, piece)) = y;
+            } else {      // half a piece of each part
+                typedef bf16 Four __attribute__((ext_vector_type(4)));
+                float e[4];
+                bf16 part[3][4];
+                __builtin_memcpy(e, &y, 16);
+                split(e, part[0], part[1], part[2]);
+#pragma unroll
+                for (int a = 0; a < 3; a++)
+                    *reinterpret_cast<Four*>(tile + a * ROWS * L::ROW + L::place(r, piece / 2) + piece % 2 * 8) =
+                        Four{part[a][0], part[a][1], part[a][2], part[a][3]};
+            }
         }
     }
 };
@@ -328,9 +385,8 @@ struct Score {
     }
 };
 
-// Biases of one head by relative position in LDS, from -reach - MARGIN to reach + MARGIN: a tile that is not beyond the reach as a whole
-// needs no bounds.
-constexpr int MARGIN = 96;
+// Biases of one head by relative position in LDS, from -reach - MARGIN to reach + MARGIN.
+constexpr int MARGIN = ATTENTION_MARGIN;
 template <typename T>
 __device__ __forceinline__ float table_entry(const SequenceAttention& A, int at, int head) {
     const int b = A.bucket_of[at];
@@ -443,7 +499,7 @@ __device__ __forceinline__ int heads_at_once(int share) { return share < 32 ? sh
 
 template <typename T, int DP, int NW>
 struct FewLds {
-    static constexpr int TILE = 32 * Tile<T, DP>::ROW, SUM = 32 * (DP + 4) * 4;
+    static constexpr int TILE = Tile<T, DP>::bytes(32), SUM = 32 * (DP + 4) * 4;
     static constexpr int EACH = 2 * TILE > SUM ? 2 * TILE : SUM;
     alignas(512) char wave[NW][(EACH + 511) / 512 * 512];
     float m[NW][32], l[NW][32], there[NW][32];
@@ -451,7 +507,7 @@ struct FewLds {
 
 template <typename T, int DC, int NW, bool BIAS>
 __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && NW == 4 ? 2 : 1)) void few_kernel(SequenceAttention A, T* out, float* stats, float* part_o, float* part_ml, int splits) {
-    constexpr int DP = pitch(DC), ND = (DC + 31) / 32;
+    constexpr int DP = pitch(DC), ND = (DC + 31) / 32, KEYS = 32;
     using L = Tile<T, DP>;
     __shared__ __attribute__((aligned(16))) FewLds<T, DP, NW> S;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
@@ -523,7 +579,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && NW == 4 ? 2 : 1)) void 
             for (int r = 0; r < 16; r++) s[r] = 0.0f;
         }
 #pragma unroll
-        for (int c = 0; c < DC / 16; c++) s = Operand<T>::product(L::rows(kr, 0, c), qf[c], s);
+        for (int c = 0; c < DC / 16; c++) s = Operand<T>::product(L::template rows<KEYS>(kr, 0, c), qf[c], s);
         if (!all_there<32>(there)) drop_keys(s, lds_address(S.there[wave]), lane);
         if (A.causal && high > 0) drop_behind(s, i + shift - j0, lane);
         const float flat = BIAS && !near ? low >= A.reach ? far[1] : far[0] : 0.0f;
@@ -541,7 +597,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && NW == 4 ? 2 : 1)) void 
         for (int c = 0; c < 2; c++) {
             const Eight<T> p = rounded<T>(s, c);
 #pragma unroll
-            for (int d = 0; d < ND; d++) sum.o[d] = Operand<T>::product(L::columns(vc, 16 * c, d), p, sum.o[d]);
+            for (int d = 0; d < ND; d++) sum.o[d] = Operand<T>::product(L::template columns<KEYS>(vc, 16 * c, d), p, sum.o[d]);
         }
     }
     // the wavefronts' sums, side by side in LDS
@@ -631,7 +687,7 @@ template <typename T, int DC, int NW, bool BIAS>
 __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 ? 2 : 1)) void tiles_kernel(SequenceAttention A, T* out, float* stats, int64_t slots) {
     constexpr int DP = pitch(DC), ND = (DC + 31) / 32;
     using L = Tile<T, DP>;
-    constexpr int KEYS = keys_at_once<T, NW>(), TILE = KEYS * L::ROW;
+    constexpr int KEYS = keys_at_once<T, NW>(), TILE = L::bytes(KEYS);
     extern __shared__ __attribute__((aligned(512))) char lds[];
     char* const tiles = lds;                    // two pairs of a tile of keys and one of values
     float* const keys = reinterpret_cast<float*>(lds + 4 * TILE);       // which are there: two times KEYS
@@ -695,7 +751,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 ? 2 : 1)) void tiles_kerne
 #pragma unroll
             for (int c = 0; c < DC / 16; c++)
 #pragma unroll
-                for (int u = 0; u < KEYS / 32; u++) s[u] = Operand<T>::product(L::rows(kr, 32 * u, c), qf[c], s[u]);
+                for (int u = 0; u < KEYS / 32; u++) s[u] = Operand<T>::product(L::template rows<KEYS>(kr, 32 * u, c), qf[c], s[u]);
         };
         if (near) {
             const float* const at = line + (j0 + 4 * half - i - shift + A.reach + MARGIN);
@@ -736,7 +792,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 ? 2 : 1)) void tiles_kerne
             for (int c = 0; c < 2; c++) {
                 const Eight<T> p = rounded<T>(s[u], c);
 #pragma unroll
-                for (int d = 0; d < ND; d++) sum.o[d] = Operand<T>::product(L::columns(vc, 32 * u + 16 * c, d), p, sum.o[d]);
+                for (int d = 0; d < ND; d++) sum.o[d] = Operand<T>::product(L::template columns<KEYS>(vc, 32 * u + 16 * c, d), p, sum.o[d]);
             }
         }
         if (n + 1 < count) put(n + 1);
@@ -803,7 +859,7 @@ template <typename T, int DC, int NW, bool BIAS>
 __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, AttentionGrads G, int64_t slots, int splits) {
     constexpr int DP = pitch(DC), ND = (DC + 31) / 32;
     using L = Tile<T, DP>;
-    constexpr int KEYS = 32, TILE = KEYS * L::ROW;
+    constexpr int KEYS = 32, TILE = L::bytes(KEYS);
     extern __shared__ __attribute__((aligned(512))) char lds[];
     char* const tiles = lds;
     float* const keys = reinterpret_cast<float*>(lds + 4 * TILE);       // which are there: two times KEYS
@@ -850,7 +906,7 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
 #pragma unroll
         for (int s = 0; s < DC / 16; s++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) D = __builtin_fmaf(to_float(gf[s][e]), to_float(of[s][e]), D);
+            for (int e = 0; e < 8; e++) D = __builtin_fmaf(value<T>(gf[s], e), value<T>(of[s], e), D);
         D = other_half_sum(D);
     }
     float m = -NONE, inverse = 0.0f;
@@ -908,8 +964,8 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
         auto products = [&] {
 #pragma unroll
             for (int c = 0; c < DC / 16; c++) {
-                s = Operand<T>::product(L::rows(kr, 0, c), qf[c], s);
-                dp = Operand<T>::product(L::rows(vr, 0, c), gf[c], dp);
+                s = Operand<T>::product(L::template rows<KEYS>(kr, 0, c), qf[c], s);
+                dp = Operand<T>::product(L::template rows<KEYS>(vr, 0, c), gf[c], dp);
             }
         };
 #pragma unroll
@@ -964,7 +1020,7 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
         for (int c = 0; c < 2; c++) {
             const Eight<T> ds = rounded<T>(s, c);
 #pragma unroll
-            for (int d = 0; d < ND; d++) dq[d] = Operand<T>::product(L::columns(kc, 16 * c, d), ds, dq[d]);
+            for (int d = 0; d < ND; d++) dq[d] = Operand<T>::product(L::template columns<KEYS>(kc, 16 * c, d), ds, dq[d]);
         }
         if (n + 1 < end) put(n + 1);
         __syncthreads();
@@ -1025,7 +1081,7 @@ template <typename T, int DC, int NW, bool BIAS>
 __global__ __launch_bounds__(NW * 64, (NW == 4 && values_in_lds<T, DC>() ? 2 : 1)) void keys_kernel(SequenceAttention A, AttentionGrads G, int64_t slots, int splits) {
     constexpr int DP = pitch(DC), ND = (DC + 31) / 32;
     using L = Tile<T, DP>;
-    constexpr int ROWS = 32, TILE = ROWS * L::ROW;
+    constexpr int ROWS = 32, TILE = L::bytes(ROWS);
     extern __shared__ __attribute__((aligned(512))) char lds[];
     char* const tiles = lds;                                            // two pairs: q, do
     float* const row_stats = reinterpret_cast<float*>(lds + 4 * TILE);  // two times (3, ROWS): m or shift, 1 / l, -D
@@ -1140,11 +1196,11 @@ __global__ __launch_bounds__(NW * 64, (NW == 4 && values_in_lds<T, DC>() ? 2 : 1
             for (int e = 0; e < 4; e++) dp[r + e] = D4[e];
         }
 #pragma unroll
-        for (int c = 0; c < DC / 16; c++) s = Operand<T>::product(L::rows(qr, 0, c), kf[c], s);
+        for (int c = 0; c < DC / 16; c++) s = Operand<T>::product(L::template rows<ROWS>(qr, 0, c), kf[c], s);
 #pragma unroll
         for (int c = 0; c < DC / 16; c++) {
-            const Eight<T> gx8 = L::rows(gr, 0, c);
-            if constexpr (values_in_lds<T, DC>()) dp = Operand<T>::product(gx8, L::rows(vr, 0, c), dp);
+            const Eight<T> gx8 = L::template rows<ROWS>(gr, 0, c);
+            if constexpr (values_in_lds<T, DC>()) dp = Operand<T>::product(gx8, L::template rows<ROWS>(vr, 0, c), dp);
             else dp = Operand<T>::product(gx8, vf[c], dp);
         }
         if (A.causal && high > 0) drop_before(s, j - shift - i0, lane);
@@ -1166,8 +1222,8 @@ __global__ __launch_bounds__(NW * 64, (NW == 4 && values_in_lds<T, DC>() ? 2 : 1
         for (int c = 0; c < 2; c++)
 #pragma unroll
             for (int d = 0; d < ND; d++) {
-                dv[d] = Operand<T>::product(L::columns(gc, 16 * c, d), pf[c], dv[d]);
-                dk[d] = Operand<T>::product(L::columns(qc, 16 * c, d), ds[c], dk[d]);
+                dv[d] = Operand<T>::product(L::template columns<ROWS>(gc, 16 * c, d), pf[c], dv[d]);
+                dk[d] = Operand<T>::product(L::template columns<ROWS>(qc, 16 * c, d), ds[c], dk[d]);
             }
         if (n + 1 < end) put(n + 1);
     }
@@ -1273,7 +1329,7 @@ void sequence_attention_forward(const SequenceAttention& A, const AttentionPlan&
             constexpr bool BIAS = decltype(bias)::value;
             const int64_t rows = (A.packed ? A.q_rows : A.q_rows * A.batch) * A.heads;
             if (!P.few) {
-                const size_t lds = 4 * keys_at_once<T, 4>() * Tile<T, DP>::ROW + 2 * keys_at_once<T, 4>() * sizeof(float) + (BIAS ? (2 * (A.reach + MARGIN) + 1) * sizeof(float) : 0);
+                const size_t lds = 4 * Tile<T, DP>::bytes(keys_at_once<T, 4>()) + 2 * keys_at_once<T, 4>() * sizeof(float) + (BIAS ? (2 * (A.reach + MARGIN) + 1) * sizeof(float) : 0);
                 launch_attention(tiles_kernel<T, DC, 4, BIAS>, dim3(die_grid((int64_t)P.slots * A.heads)), 256, lds, st, A, out, stats, P.slots);
                 return;
             }
@@ -1281,7 +1337,7 @@ void sequence_attention_forward(const SequenceAttention& A, const AttentionPlan&
             float* const part_ml = scratch + P.splits * rows * DP;
             const dim3 grid(P.slots, A.kv_heads * ((A.share + 31) / 32), P.splits);
             if (P.waves == 1) launch_attention(few_kernel<T, DC, 1, BIAS>, grid, 64, 0, st, A, out, stats, part_o, part_ml, P.splits);
-            else launch_attention(few_kernel<T, DC, 4, BIAS>, grid, 256, 0, st, A, out, stats, part_o, part_ml, P.splits);
+            else launch_attention(few_kernel<T, DC, few_waves(sizeof(T) == 4, DC), BIAS>, grid, P.waves * 64, 0, st, A, out, stats, part_o, part_ml, P.splits);
             if (P.splits > 1)
                 launch_attention(combine_parts<T, DC, BIAS>, dim3((unsigned)((rows + 7) / 8)), 256, 0, st, A, part_o, part_ml, P.splits, rows, out, stats);
         });
@@ -1309,16 +1365,16 @@ void sequence_attention_backward(const SequenceAttention& A, const AttentionGrad
         with_choice(A.table != nullptr, [&](auto bias) {
             constexpr int DC = decltype(dc)::value, DP = pitch(DC);
             constexpr bool BIAS = decltype(bias)::value;
-            const size_t line = BIAS ? (2 * (A.reach + MARGIN) + 1) * sizeof(float) : 0, tiles = 4 * 32 * Tile<T, DP>::ROW;
-            const size_t sums = BIAS ? (2 * P.q_waves * (2 * (A.reach + MARGIN) + 1) + 2 * P.q_waves) * sizeof(float) : 0;
+            const size_t line = BIAS ? (2 * (A.reach + MARGIN) + 1) * sizeof(float) : 0, tiles = 4 * Tile<T, DP>::bytes(32);
+            const size_t queries = queries_lds(sizeof(T) == 4, A.dim, A.reach, BIAS, P.q_waves);
             if (q_all > 0) {
                 const dim3 grid(die_grid((int64_t)P.q_slots * A.heads), P.q_splits);
-                if (P.q_waves == 1) launch_attention(queries_kernel<T, DC, 1, BIAS>, grid, 64, tiles + 64 * sizeof(float) + line + sums, st, A, G, P.q_slots, P.q_splits);
-                else launch_attention(queries_kernel<T, DC, 4, BIAS>, grid, 256, tiles + 64 * sizeof(float) + line + sums, st, A, G, P.q_slots, P.q_splits);
+                if (P.q_waves == 1) launch_attention(queries_kernel<T, DC, 1, BIAS>, grid, 64, queries, st, A, G, P.q_slots, P.q_splits);
+                else launch_attention(queries_kernel<T, DC, 4, BIAS>, grid, 256, queries, st, A, G, P.q_slots, P.q_splits);
             }
             if (k_all > 0 && G.dk) {
                 const dim3 grid(die_grid((int64_t)P.k_slots * A.kv_heads), P.k_splits);
-                const size_t lds = tiles + 6 * 32 * sizeof(float) + line + (values_in_lds<T, DC>() ? P.k_waves * 32 * Tile<T, DP>::ROW : 0);
+                const size_t lds = tiles + 6 * 32 * sizeof(float) + line + (values_in_lds<T, DC>() ? P.k_waves * Tile<T, DP>::bytes(32) : 0);
                 if (P.k_waves == 1) launch_attention(keys_kernel<T, DC, 1, BIAS>, grid, 64, lds, st, A, G, P.k_slots, P.k_splits);
                 else launch_attention(keys_kernel<T, DC, 4, BIAS>, grid, 256, lds, st, A, G, P.k_slots, P.k_splits);
             }

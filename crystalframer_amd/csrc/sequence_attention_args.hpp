@@ -8,6 +8,9 @@ namespace cfh {
 constexpr int ATTENTION_MAX_DIM = 128;
 constexpr int ATTENTION_MAX_REACH = 1024;      // relative positions beyond this (either way) share a bucket
 constexpr int ATTENTION_CUS = 256;
+constexpr int ATTENTION_LDS = 160 * 1024;
+// Beyond the reach by this much on either side biases are kept in LDS: a tile that is not beyond it as a whole needs no bounds.
+constexpr int ATTENTION_MARGIN = 96;
 
 // Element strides of (batch, position, head); channels lie next to one another, rows at multiples of 16 bytes.
 struct AttentionRows {
@@ -22,7 +25,7 @@ struct SequenceAttention {
     const void* table;                 // (buckets, heads)
     const int32_t* bucket_of;          // (2 reach + 1): of the relative positions -reach ... reach
     int64_t q_rows, k_rows;            // packed: of all sequences; else of one
-    int32_t packed, batch, heads, kv_heads, share, dim, buckets, reach, causal, last, table_float;
+    int32_t packed, batch, heads, kv_heads, share, dim, buckets, reach, causal, last, table_float, float32;
     float scale;
 };
 
@@ -47,6 +50,13 @@ inline int split_count(int64_t wavefronts, int64_t wanted, int64_t rows, int64_t
     return (int)(n < 1 || most < 1 ? 1 : n > most ? most : n);
 }
 
+// Wavefronts of few_kernel and of the backward kernels: what the 160 KB of LDS hold.
+constexpr int few_waves(bool float32, int dim) { return float32 && dim > 64 ? 2 : 4; }
+inline int64_t queries_lds(bool float32, int dim, int reach, bool table, int waves) {
+    const int64_t pitch = dim <= 32 ? 32 : dim <= 64 ? 64 : 128, entries = 2 * (reach + ATTENTION_MARGIN) + 1;
+    return 4 * 32 * pitch * (float32 ? 6 : 2) + 64 * 4 + (table ? (entries * (2 * waves + 1) + 2 * waves) * 4 : 0);
+}
+
 struct AttentionPlan {
     bool few;              // few_kernel
     int waves, splits;
@@ -63,7 +73,7 @@ inline AttentionPlan attention_plan(const SequenceAttention& A) {
     if (!P.few) return P;
     const int at_once = A.share < 32 ? A.share : 32, groups = (A.share + at_once - 1) / at_once;
     P.slots = tile_slots(A.packed, A.q_rows, A.batch, 32 / at_once);
-    P.waves = k_each > 64 ? 4 : 1;
+    P.waves = k_each <= 64 ? 1 : few_waves(A.float32, A.dim);
     P.splits = split_count(P.slots * A.kv_heads * groups * P.waves, 16 * ATTENTION_CUS, k_each, 64 * P.waves);
     return P;
 }
@@ -75,7 +85,7 @@ struct AttentionGradPlan {
 inline AttentionGradPlan attention_grad_plan(const SequenceAttention& A) {
     AttentionGradPlan P{};
     const int64_t q_each = A.packed && A.batch > 0 ? A.q_rows / A.batch : A.q_rows, k_each = A.packed && A.batch > 0 ? A.k_rows / A.batch : A.k_rows;
-    P.q_waves = q_each > 64 ? 4 : 1;
+    P.q_waves = q_each > 64 && queries_lds(A.float32, A.dim, A.reach, A.table != nullptr, 4) <= ATTENTION_LDS ? 4 : 1;
     P.k_waves = k_each > 64 ? 4 : 1;
     P.q_slots = tile_slots(A.packed, A.q_rows, A.batch, 32 * P.q_waves);
     P.k_slots = tile_slots(A.packed, A.k_rows, A.batch, 32 * P.k_waves);

@@ -78,6 +78,7 @@ cfh::SequenceAttention device_args(const cfh_attention* a) {
     A.packed = a->packed; A.batch = a->batch; A.heads = a->heads; A.kv_heads = a->kv_heads; A.share = a->heads / a->kv_heads;
     A.dim = a->dim; A.buckets = a->buckets; A.reach = a->reach; A.causal = a->causal; A.last = a->queries_last;
     A.table_float = a->table_dtype == CFH_FLOAT32;
+    A.float32 = a->dtype == CFH_FLOAT32;
     A.scale = a->scale;
     return A;
 }
