@@ -529,7 +529,9 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && NW == 4 ? 2 : 1)) void 
     int seen = i0 < q.there ? k.there : 0;
     if (A.causal) seen = min(seen, i_last + shift + 1);
     const int tiles = seen > 0 ? (seen + 31) / 32 : 0;
-    const int first = (int)((int64_t)tiles * blockIdx.z / splits), end = (int)((int64_t)tiles * (blockIdx.z + 1) / splits);
+    // (padded sequences: parts of one length, so that long ones take more workgroups, not longer ones)
+    const int part = A.packed ? (tiles + splits - 1) / splits : (int)((A.k_rows + 32LL * splits - 1) / (32LL * splits));
+    const int first = min(tiles, (int)blockIdx.z * part), end = min(tiles, first + part);
 
     Eight<T> qf[DC / 16];
     const T* const q_row = row_start<T>(A.q, q, A.packed, mine ? h : 0) + (mine ? i : 0) * A.q.row;
@@ -637,7 +639,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && NW == 4 ? 2 : 1)) void 
         const int64_t row = (q.first + ci) * A.heads + ch;
         if (splits > 1) {
             const int64_t rows = (A.packed ? A.q_rows : A.q_rows * A.batch) * A.heads, at = blockIdx.z * rows + row;
-            *reinterpret_cast<f32x4*>(part_o + at * DP + from) = o;
+            if (m != NONE) *reinterpret_cast<f32x4*>(part_o + at * DP + from) = o;
             if (from == 0) {
                 part_ml[2 * at] = m;
                 part_ml[2 * at + 1] = l;
@@ -653,27 +655,45 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && NW == 4 ? 2 : 1)) void 
     }
 }
 
-// Joins the splits: 8 rows to a workgroup, 32 lanes to a row.
+// Joins the splits: 8 rows to a workgroup, 32 lanes to a row.  The lanes look at a part's statistics each, and then all at its sums.
 template <typename T, int DC, bool BIAS>
 __global__ __launch_bounds__(256) void combine_parts(SequenceAttention A, const float* part_o, const float* part_ml, int splits, int64_t rows, T* out,
                                                      float* stats) {
     constexpr int DP = pitch(DC);
     const int64_t row = blockIdx.x * 8LL + threadIdx.x / 32;
-    const int from = (threadIdx.x & 31) * 4;
-    if (row >= rows || from >= DP) return;
+    const int lane = threadIdx.x & 31, from = lane * 4;
+    if (row >= rows) return;
     const Score<T> score(A.scale);
     float m = NONE, l = 0.0f;
-    for (int z = 0; z < splits; z++) m = fmaxf(m, part_ml[2 * (z * rows + row)]);
     f32x4 o{0, 0, 0, 0};
-    for (int z = 0; z < splits; z++) {
-        const float mz = part_ml[2 * (z * rows + row)];
-        const float by = mz == NONE ? 0.0f : __builtin_amdgcn_exp2f((mz - m) * score.rate);
-        l += by * part_ml[2 * (z * rows + row) + 1];
-        if (from < A.dim) o += by * *reinterpret_cast<const f32x4*>(part_o + (z * rows + row) * DP + from);
+    for (int z0 = 0; z0 < splits; z0 += 32) {
+        float mz = NONE, lz = 0.0f;
+        if (z0 + lane < splits) {
+            mz = part_ml[2 * ((z0 + lane) * rows + row)];
+            lz = part_ml[2 * ((z0 + lane) * rows + row) + 1];
+        }
+        float top = mz;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 32));
+        top = fmaxf(top, m);
+        const float old = m == NONE ? 0.0f : __builtin_amdgcn_exp2f((m - top) * score.rate);
+        const float by = mz == NONE ? 0.0f : __builtin_amdgcn_exp2f((mz - top) * score.rate);
+        float sum = by * lz;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor(sum, d, 32);
+        l = l * old + sum;
+        o *= old;
+        m = top;
+        const int here = splits - z0 < 32 ? splits - z0 : 32;
+#pragma unroll 4
+        for (int z = 0; z < here; z++) {
+            const float w = __shfl(by, z, 32);
+            if (w != 0.0f && from < DP) o += w * *reinterpret_cast<const f32x4*>(part_o + ((z0 + z) * rows + row) * DP + from);
+        }
     }
     const float inverse = l > 0.0f || l != l ? 1.0f / l : 0.0f;
     if (from < A.dim) put_four<T>(out + row * A.dim, from, A.dim, o * inverse);
-    if (stats && from == 0) {
+    if (stats && lane == 0) {
         stats[2 * row] = m == NONE ? -NONE : m;
         stats[2 * row + 1] = inverse * (NARROW<T> ? 0x1p6f : 1.0f);
     }

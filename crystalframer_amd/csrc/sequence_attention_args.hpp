@@ -74,7 +74,7 @@ inline AttentionPlan attention_plan(const SequenceAttention& A) {
     const int at_once = A.share < 32 ? A.share : 32, groups = (A.share + at_once - 1) / at_once;
     P.slots = tile_slots(A.packed, A.q_rows, A.batch, 32 / at_once);
     P.waves = k_each <= 64 ? 1 : few_waves(A.float32, A.dim);
-    P.splits = split_count(P.slots * A.kv_heads * groups * P.waves, 16 * ATTENTION_CUS, k_each, 64 * P.waves);
+    P.splits = split_count(P.slots * A.kv_heads * groups * P.waves, 32 * ATTENTION_CUS, k_each, 64 * P.waves);
     return P;
 }
 
