@@ -236,7 +236,7 @@ struct KeyBits {
 
 // ROWS rows on their way into a tile through the registers of THREADS lanes.  A row that is not there is 0 in LDS: what memory holds
 // in its place, infinities and NaN among it, meets no product.
-template <typename T, int DP, int ROWS, int THREADS>
+template <typename T, int DP, int ROWS, int THREADS, int HOW = 0>
 struct Staged {
     using L = Tile<T, DP>;
     static constexpr int ALL = ROWS * L::PIECES, EACH = (ALL + THREADS - 1) / THREADS, EVERY = THREADS / L::PIECES;
@@ -248,7 +248,7 @@ struct Staged {
         const auto from = buffer(first, rows <= 0 ? 0 : (rows - 1) * step + last);
         const int at = piece * 16 < last && row < ROWS ? row * step + piece * 16 : BEYOND;
 #pragma unroll
-        for (int n = 0; n < EACH; n++) x[n] = __builtin_amdgcn_raw_buffer_load_b128(from, at + n * EVERY * step, 0, 0);
+        for (int n = 0; n < EACH; n++) x[n] = __builtin_amdgcn_raw_buffer_load_b128(from, at + n * EVERY * step, 0, HOW);
     }
     // rows whose bit is 0 are not there
     __device__ __forceinline__ void store(char* tile, int thread, uint64_t bits = ~0ull) const {
@@ -493,7 +493,9 @@ __device__ __forceinline__ bool all_there(uint64_t bits) { return COUNT == 64 ? 
 // ---- few queries: the keys in parts -----------------------------------------------------------------------------------------------------
 // 32 columns are (query, head of one key head): single tokens of shared heads fill them together.  Every wavefront goes through keys of
 // its own, in tiles of 32 that it alone puts into LDS and reads (no barrier in the loop), and the wavefronts' sums are joined at the end;
-// so are, by combine_parts, those of `splits` workgroups.  Bound by the bytes of keys and values for single tokens.
+// so are, by combine_parts, those of `splits` workgroups.  Bound by the bytes of keys and values for single tokens; PAST: these go past the
+// caches, where one workgroup reads them and they are more than the last cache keeps (0.5 GB: 129 -> 119 us; 240 MB that no call before had
+// read: 77 -> 73, that one just had: 64 -> 70).
 template <typename T>
 __device__ __forceinline__ int heads_at_once(int share) { return share < 32 ? share : 32; }
 
@@ -505,7 +507,7 @@ struct FewLds {
     float m[NW][32], l[NW][32], there[NW][32];
 };
 
-template <typename T, int DC, int NW, bool BIAS>
+template <typename T, int DC, int NW, bool BIAS, bool PAST>
 __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && NW == 4 ? 2 : 1)) void few_kernel(SequenceAttention A, T* out, float* stats, float* part_o, float* part_ml, int splits) {
     constexpr int DP = pitch(DC), ND = (DC + 31) / 32, KEYS = 32;
     using L = Tile<T, DP>;
@@ -549,7 +551,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && NW == 4 ? 2 : 1)) void 
     char* const vt = kt + FewLds<T, DP, NW>::TILE;
     const uint32_t kr = lds_address(kt) + L::rows_at(lane), vc = lds_address(vt) + L::columns_at(lane);
     Running<ND> sum;
-    Staged<T, DP, 32, 64> kx, vx;
+    Staged<T, DP, 32, 64, PAST ? 2 : 0> kx, vx;
     KeyBits bits;
     auto fetch = [&](int n) {
         const int j0 = n * 32;
@@ -1356,8 +1358,11 @@ void sequence_attention_forward(const SequenceAttention& A, const AttentionPlan&
             float* const part_o = scratch;
             float* const part_ml = scratch + P.splits * rows * DP;
             const dim3 grid(P.slots, A.kv_heads * ((A.share + 31) / 32), P.splits);
-            if (P.waves == 1) launch_attention(few_kernel<T, DC, 1, BIAS>, grid, 64, 0, st, A, out, stats, part_o, part_ml, P.splits);
-            else launch_attention(few_kernel<T, DC, few_waves(sizeof(T) == 4, DC), BIAS>, grid, P.waves * 64, 0, st, A, out, stats, part_o, part_ml, P.splits);
+            if (P.waves == 1) launch_attention(few_kernel<T, DC, 1, BIAS, false>, grid, 64, 0, st, A, out, stats, part_o, part_ml, P.splits);
+            else with_choice(P.past, [&](auto past) {
+                launch_attention(few_kernel<T, DC, few_waves(sizeof(T) == 4, DC), BIAS, decltype(past)::value>, grid, P.waves * 64, 0, st, A, out, stats,
+                                 part_o, part_ml, P.splits);
+            });
             if (P.splits > 1)
                 launch_attention(combine_parts<T, DC, BIAS>, dim3((unsigned)((rows + 7) / 8)), 256, 0, st, A, part_o, part_ml, P.splits, rows, out, stats);
         });

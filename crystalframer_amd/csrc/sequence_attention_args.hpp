@@ -58,7 +58,7 @@ inline int64_t queries_lds(bool float32, int dim, int reach, bool table, int wav
 }
 
 struct AttentionPlan {
-    bool few;              // few_kernel
+    bool few, past;        // few_kernel, and keys and values past the caches
     int waves, splits;
     int64_t slots;
 };
@@ -74,6 +74,8 @@ inline AttentionPlan attention_plan(const SequenceAttention& A) {
     const int at_once = A.share < 32 ? A.share : 32, groups = (A.share + at_once - 1) / at_once;
     P.slots = tile_slots(A.packed, A.q_rows, A.batch, 32 / at_once);
     P.waves = k_each <= 64 ? 1 : few_waves(A.float32, A.dim);
+    const int64_t keys = A.packed ? A.k_rows : A.k_rows * A.batch;
+    P.past = q_each * at_once <= 32 && groups == 1 && keys * A.kv_heads * A.dim * (A.float32 ? 8 : 4) >= 1 << 27;
     P.splits = split_count(P.slots * A.kv_heads * groups * P.waves, 32 * ATTENTION_CUS, k_each, 64 * P.waves);
     return P;
 }
