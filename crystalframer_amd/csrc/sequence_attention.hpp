@@ -294,6 +294,20 @@ __device__ __forceinline__ void put_four(T* row, int from, int dim, f32x4 x) {
     }
 }
 
+// The order of what stands before it in a block: operands are read from LDS `AHEAD` products before the one that takes them, which is
+// longer than a read takes.  (Left alone, a read is followed by the wait for it.)  EACH reads to a product.
+template <int PRODUCTS, int AHEAD, int EACH>
+__device__ __forceinline__ void reads_ahead() {
+    constexpr int first = AHEAD < PRODUCTS ? AHEAD : PRODUCTS;
+    __builtin_amdgcn_sched_group_barrier(0x100, first * EACH, 0);
+#pragma unroll
+    for (int n = 0; n < PRODUCTS - first; n++) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, EACH, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x8, first, 0);
+}
+
 // ---- which rows a workgroup has --------------------------------------------------------------------------------------------------------
 struct Span {
     int64_t first;      // row of the sequence's first position among all rows
@@ -774,6 +788,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 ? 2 : 1)) void tiles_kerne
             for (int c = 0; c < DC / 16; c++)
 #pragma unroll
                 for (int u = 0; u < KEYS / 32; u++) s[u] = Operand<T>::product(L::template rows<KEYS>(kr, 32 * u, c), qf[c], s[u]);
+            if (sizeof(T) == 2) reads_ahead<DC / 16 * KEYS / 32, 4, 1>();
         };
         if (near) {
             const float* const at = line + (j0 + 4 * half - i - shift + A.reach + MARGIN);
@@ -989,6 +1004,7 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
                 s = Operand<T>::product(L::template rows<KEYS>(kr, 0, c), qf[c], s);
                 dp = Operand<T>::product(L::template rows<KEYS>(vr, 0, c), gf[c], dp);
             }
+            if (sizeof(T) == 2) reads_ahead<DC / 16 * 2, 4, 1>();
         };
 #pragma unroll
         for (int r = 0; r < 16; r++) dp[r] = 0.0f;
