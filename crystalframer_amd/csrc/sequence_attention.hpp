@@ -401,12 +401,14 @@ struct Score {
 
 // Biases of one head by relative position in LDS, from -reach - MARGIN to reach + MARGIN.
 constexpr int MARGIN = ATTENTION_MARGIN;
+// (No branch but the one on the table's type, which is the same for all: loads of several entries are on their way together.)
 template <typename T>
 __device__ __forceinline__ float table_entry(const SequenceAttention& A, int at, int head) {
     const int b = A.bucket_of[at];
-    if ((unsigned)b >= (unsigned)A.buckets) return 0.0f;
-    const int64_t n = (int64_t)b * A.heads + head;
-    return A.table_float ? static_cast<const float*>(A.table)[n] : to_float(static_cast<const T*>(A.table)[n]);
+    const bool real = (unsigned)b < (unsigned)A.buckets;
+    const int64_t n = (int64_t)(real ? b : 0) * A.heads + head;
+    const float x = A.table_float ? static_cast<const float*>(A.table)[n] : to_float(static_cast<const T*>(A.table)[n]);
+    return real ? x : 0.0f;
 }
 __device__ __forceinline__ int clamped(int r, int reach) { return (r < -reach ? -reach : r > reach ? reach : r) + reach; }
 template <typename T>
@@ -557,9 +559,10 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && NW == 4 ? 2 : 1)) void 
     const uint8_t* const mask = A.mask ? A.mask + k.first : nullptr;
     const float by = 1.0f / A.scale;
     float far[2] = {0.0f, 0.0f};
-    if (BIAS && mine) {
-        far[0] = table_entry<T>(A, 0, h) * by;
-        far[1] = table_entry<T>(A, 2 * A.reach, h) * by;
+    if (BIAS) {
+        const int head = mine ? h : 0;
+        far[0] = table_entry<T>(A, 0, head) * by;
+        far[1] = table_entry<T>(A, 2 * A.reach, head) * by;
     }
     char* const kt = S.wave[wave];
     char* const vt = kt + FewLds<T, DP, NW>::TILE;
@@ -573,8 +576,19 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && NW == 4 ? 2 : 1)) void 
         kx.load(k_at + j0 * A.k.row, A.k.row, k.there - j0, A.dim, lane);
         vx.load(v_at + j0 * A.v.row, A.v.row, k.there - j0, A.dim, lane);
     };
-    settle<T>(qf);
     if (first + wave < end) fetch(first + wave);
+    extern __shared__ float line[];        // (heads at once, entries) where few_line() says so
+    const int entries = 2 * (A.reach + MARGIN) + 1;
+    const bool lines = BIAS && few_line(at_once, A.reach);
+    if (lines) {
+        if (first < end && first * 32 - i_last - shift < A.reach && end * 32 - 1 - i0 - shift > -A.reach)
+            for (int n = threadIdx.x; n < at_once * entries; n += NW * 64) {
+                const int g = n / entries, head = h0 + g < (kh + 1) * A.share ? h0 + g : h0;
+                line[n] = table_entry<T>(A, clamped(n - g * entries - A.reach - MARGIN, A.reach), head) * by;
+            }
+        __syncthreads();
+    }
+    settle<T>(qf);
     for (int n = first + wave; n < end; n += NW) {
         const int j0 = n * 32;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -588,7 +602,11 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && NW == 4 ? 2 : 1)) void 
         f32x16 s;
         const int low = j0 - i_last - shift, high = j0 + 31 - i0 - shift;      // relative positions of the tile
         const bool near = BIAS && low < A.reach && high > -A.reach;
-        if (near) {
+        if (near && lines) {
+            const float* const at = line + column % at_once * entries + (j0 + 4 * half - i - shift + A.reach + MARGIN);
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[r] = at[result_row(r)];
+        } else if (near) {
             const int r0 = j0 + 4 * half - i - shift;
 #pragma unroll
             for (int r = 0; r < 16; r++) s[r] = mine ? table_entry<T>(A, clamped(r0 + result_row(r), A.reach), h) * by : 0.0f;
@@ -753,7 +771,6 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 ? 2 : 1)) void tiles_kerne
     const T* const k_at = row_start<T>(A.k, k, A.packed, kh);
     const T* const v_at = row_start<T>(A.v, k, A.packed, kh);
     const uint8_t* const mask = A.mask ? A.mask + k.first : nullptr;
-    if (BIAS) fill_line<T>(A, h, line, threadIdx.x, NW * 64);
     Running<ND> sum;
     Staged<T, DP, KEYS, NW * 64> kx, vx;
     KeyBits bits;
@@ -771,11 +788,10 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 ? 2 : 1)) void tiles_kerne
         kx.store(tiles + (n & 1) * 2 * TILE, threadIdx.x, rows);
         vx.store(tiles + (n & 1) * 2 * TILE + TILE, threadIdx.x, rows);
     };
+    if (count > 0) fetch(0);
+    if (BIAS) fill_line<T>(A, h, line, threadIdx.x, NW * 64);
+    if (count > 0) put(0);
     settle<T>(qf);
-    if (count > 0) {
-        fetch(0);
-        put(0);
-    }
     __syncthreads();
     for (int n = 0; n < count; n++) {
         const uint32_t tile = lds_address(tiles) + (n & 1) * 2 * TILE, kr = tile + L::rows_at(lane), vc = tile + TILE + L::columns_at(lane);
@@ -929,35 +945,19 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
     const int first = (int)((int64_t)whole * z / splits), end = (int)((int64_t)whole * (z + 1) / splits);
 
     const int64_t row = (q.first + i) * A.heads + h;
-    Eight<T> qf[DC / 16], gf[DC / 16];
-    float D = 0.0f;
-    {
-        const T* const q_row = row_start<T>(A.q, q, A.packed, h) + (mine ? i : 0) * A.q.row;
-        const T* const g_row = row_start<T>(G.go, q, A.packed, h) + (mine ? i : 0) * G.go.row;
-        const T* const o_row = static_cast<const T*>(G.out) + (mine ? row : 0) * A.dim;
-        const bool o_whole = A.dim % L::E == 0;
-        Eight<T> of[DC / 16];
-        row_operands<T, DC>(qf, q_row, mine, A.dim, true, lane);
-        row_operands<T, DC>(gf, g_row, mine, A.dim, true, lane);
-        row_operands<T, DC>(of, o_row, mine, A.dim, o_whole, lane);
-#pragma unroll
-        for (int s = 0; s < DC / 16; s++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) D = __builtin_fmaf(value<T>(gf[s], e), value<T>(of[s], e), D);
-        D = other_half_sum(D);
-    }
+    Eight<T> qf[DC / 16], gf[DC / 16], of[DC / 16];
+    row_operands<T, DC>(qf, row_start<T>(A.q, q, A.packed, h) + (mine ? i : 0) * A.q.row, mine, A.dim, true, lane);
+    row_operands<T, DC>(gf, row_start<T>(G.go, q, A.packed, h) + (mine ? i : 0) * G.go.row, mine, A.dim, true, lane);
+    row_operands<T, DC>(of, static_cast<const T*>(G.out) + (mine ? row : 0) * A.dim, mine, A.dim, A.dim % L::E == 0, lane);
     float m = -NONE, inverse = 0.0f;
     if (mine) {
         m = G.stats[2 * row];
         inverse = G.stats[2 * row + 1];
     }
-    if (z == 0 && half == 0 && i < q.rows) G.rows[row] = D;
-    const float off = row_shift(score, m, inverse);
     const T* const k_at = row_start<T>(A.k, k, A.packed, kh);
     const T* const v_at = row_start<T>(A.v, k, A.packed, kh);
     const uint8_t* const mask = A.mask ? A.mask + k.first : nullptr;
     if (BIAS) {
-        fill_line<T>(A, h, line, threadIdx.x, NW * 64);
         for (int n = threadIdx.x; n < 2 * NW * entries; n += NW * 64) sums[n] = 0.0f;
     }
     float* const own_sums = sums + (2 * wave + half) * entries;
@@ -984,13 +984,20 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
         kx.store(tiles + (n & 1) * 2 * TILE, threadIdx.x, rows);
         vx.store(tiles + (n & 1) * 2 * TILE + TILE, threadIdx.x, rows);
     };
+    if (first < end) fetch(first);
+    if (BIAS) fill_line<T>(A, h, line, threadIdx.x, NW * 64);
+    float D = 0.0f;
+#pragma unroll
+    for (int s = 0; s < DC / 16; s++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) D = __builtin_fmaf(value<T>(gf[s], e), value<T>(of[s], e), D);
+    D = other_half_sum(D);
+    if (z == 0 && half == 0 && i < q.rows) G.rows[row] = D;
+    const float off = row_shift(score, m, inverse);
+    if (first < end) put(first);
     settle<T>(qf);
     settle<T>(gf);
     asm volatile("" : "+v"(m), "+v"(inverse));
-    if (first < end) {
-        fetch(first);
-        put(first);
-    }
     __syncthreads();
     for (int n = first; n < end; n++) {
         const uint32_t tile = lds_address(tiles) + (n & 1) * 2 * TILE, kr = tile + L::rows_at(lane), vr = kr + TILE, kc = tile + L::columns_at(lane);
@@ -1137,7 +1144,8 @@ __global__ __launch_bounds__(NW * 64, (NW == 4 && values_in_lds<T, DC>() ? 2 : 1
     Span q{0, 0, 0, 0};
     if (!A.packed || b < A.batch) q = span_of(A.q_starts, A.q_sizes, A.q_rows, A.packed, A.batch, b);
     const int j0 = from + wave * 32, j = j0 + column;
-    const bool mine = j < k.there && (!A.mask || A.mask[k.first + j]);
+    const bool inside = j < k.there;
+    const bool mine = inside && (!A.mask || A.mask[k.first + j]);
     const int shift = shift_of(A, q, k);
     const Score<T> score(A.scale);
     // the first tile of queries that sees a key of this workgroup
@@ -1146,20 +1154,15 @@ __global__ __launch_bounds__(NW * 64, (NW == 4 && values_in_lds<T, DC>() ? 2 : 1
     const int each = from < k.there ? max(0, (q.there + ROWS - 1) / ROWS - skip) : 0, whole = each * A.share;
     const int first = (int)((int64_t)whole * z / splits), end = (int)((int64_t)whole * (z + 1) / splits);
 
+    // (a masked key's column is computed like the others, and not written)
     Eight<T> kf[DC / 16], vf[values_in_lds<T, DC>() ? 1 : DC / 16];
+    [[maybe_unused]] Staged<T, DP, 32, 64> vx;
     {
-        const T* const k_row = row_start<T>(A.k, k, A.packed, kh) + (mine ? j : 0) * A.k.row;
-        const T* const v_row = row_start<T>(A.v, k, A.packed, kh) + (mine ? j : 0) * A.v.row;
-        row_operands<T, DC>(kf, k_row, mine, A.dim, true, lane);
-        if constexpr (values_in_lds<T, DC>()) {
-            Staged<T, DP, 32, 64> vx;
-            vx.load(row_start<T>(A.v, k, A.packed, kh) + j0 * A.v.row, A.v.row, k.there - j0, A.dim, lane);
-            vx.store(values, lane);      // (read by this wavefront alone)
-            (void)v_row;
-        } else {
-            row_operands<T, DC>(vf, v_row, mine, A.dim, true, lane);
-            settle<T>(vf);
-        }
+        const T* const k_row = row_start<T>(A.k, k, A.packed, kh) + (inside ? j : 0) * A.k.row;
+        [[maybe_unused]] const T* const v_row = row_start<T>(A.v, k, A.packed, kh) + (inside ? j : 0) * A.v.row;
+        row_operands<T, DC>(kf, k_row, inside, A.dim, true, lane);
+        if constexpr (values_in_lds<T, DC>()) vx.load(row_start<T>(A.v, k, A.packed, kh) + j0 * A.v.row, A.v.row, k.there - j0, A.dim, lane);
+        else row_operands<T, DC>(vf, v_row, inside, A.dim, true, lane);
     }
     f32x16 dk[ND], dv[ND];
     Scaled<T, ND> scaled;
@@ -1196,11 +1199,11 @@ __global__ __launch_bounds__(NW * 64, (NW == 4 && values_in_lds<T, DC>() ? 2 : 1
             st[2 * ROWS] = -sx[2];
         }
     };
+    if (first < end) fetch(first);
+    if constexpr (values_in_lds<T, DC>()) vx.store(values, lane);      // (read by this wavefront alone)
+    else settle<T>(vf);
     settle<T>(kf);
-    if (first < end) {
-        fetch(first);
-        put(first);
-    }
+    if (first < end) put(first);
     int line_of = -1;
     const uint32_t vr = lds_address(values) + L::rows_at(lane);
     (void)vr;
@@ -1374,9 +1377,11 @@ void sequence_attention_forward(const SequenceAttention& A, const AttentionPlan&
             float* const part_o = scratch;
             float* const part_ml = scratch + P.splits * rows * DP;
             const dim3 grid(P.slots, A.kv_heads * ((A.share + 31) / 32), P.splits);
-            if (P.waves == 1) launch_attention(few_kernel<T, DC, 1, BIAS, false>, grid, 64, 0, st, A, out, stats, part_o, part_ml, P.splits);
+            const int at_once = A.share < 32 ? A.share : 32;
+            const size_t line = BIAS && few_line(at_once, A.reach) ? (size_t)at_once * (2 * (A.reach + MARGIN) + 1) * sizeof(float) : 0;
+            if (P.waves == 1) launch_attention(few_kernel<T, DC, 1, BIAS, false>, grid, 64, line, st, A, out, stats, part_o, part_ml, P.splits);
             else with_choice(P.past, [&](auto past) {
-                launch_attention(few_kernel<T, DC, few_waves(sizeof(T) == 4, DC), BIAS, decltype(past)::value>, grid, P.waves * 64, 0, st, A, out, stats,
+                launch_attention(few_kernel<T, DC, few_waves(sizeof(T) == 4, DC), BIAS, decltype(past)::value>, grid, P.waves * 64, line, st, A, out, stats,
                                  part_o, part_ml, P.splits);
             });
             if (P.splits > 1)

@@ -57,6 +57,9 @@ inline int64_t queries_lds(bool float32, int dim, int reach, bool table, int wav
     return 4 * 32 * pitch * (float32 ? 6 : 2) + 64 * 4 + (table ? (entries * (2 * waves + 1) + 2 * waves) * 4 : 0);
 }
 
+// Whether few_kernel keeps the biases of its heads in LDS (up to 8 KB); otherwise it reads what tiles within the reach take.
+__host__ __device__ inline bool few_line(int heads, int reach) { return heads * (2 * (reach + ATTENTION_MARGIN) + 1) <= 2048; }
+
 struct AttentionPlan {
     bool few, past;        // few_kernel, and keys and values past the caches
     int waves, splits;
