@@ -323,9 +323,9 @@ def load():
             getattr(lib, name).restype = ctypes.c_size_t
             getattr(lib, name).argtypes = [_P]
         lib.cfh_attention_forward.restype = ctypes.c_int
-        lib.cfh_attention_forward.argtypes = [_P] * 4 + [ctypes.c_size_t, _P]
+        lib.cfh_attention_forward.argtypes = [_P] * 5 + [ctypes.c_size_t, _P]
         lib.cfh_attention_backward.restype = ctypes.c_int
-        lib.cfh_attention_backward.argtypes = [_P] * 10 + [ctypes.c_size_t, _P]
+        lib.cfh_attention_backward.argtypes = [_P] * 11 + [ctypes.c_size_t, _P]
         if lib.cfh_abi_version() != ABI_VERSION:
             raise RuntimeError(f"ABI version {lib.cfh_abi_version()} of {LIB_PATH} != {ABI_VERSION}")
         _lib = lib

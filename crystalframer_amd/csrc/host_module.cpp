@@ -579,9 +579,9 @@ py::object residual_norm(const at::Tensor& x, const c10::optional<at::Tensor>& b
 // ---- attention between sequences ---------------------------------------------------------------------------------------------------
 struct AttentionLibrary {
     size_t (*forward_bytes)(const cfh_attention*) = nullptr;
-    int (*forward)(const cfh_attention*, void*, float*, void*, size_t, void*) = nullptr;
+    int (*forward)(const cfh_attention*, void*, void*, float*, void*, size_t, void*) = nullptr;
     size_t (*backward_bytes)(const cfh_attention*) = nullptr;
-    int (*backward)(const cfh_attention*, const void*, const float*, const void*, const int64_t*, void*, void*, void*, void*, void*, size_t, void*) = nullptr;
+    int (*backward)(const cfh_attention*, const void*, const void*, const float*, const void*, const int64_t*, void*, void*, void*, void*, void*, size_t, void*) = nullptr;
 } g_attention;
 
 enum { QUERY, KEY, VALUE, TABLE, ATTENTION_LEAVES, BUCKETS = ATTENTION_LEAVES, QUERY_STARTS, KEY_STARTS, QUERY_SIZES, KEY_SIZES, KEY_MASK, ATTENTION_TENSORS };
@@ -705,7 +705,7 @@ struct SequenceAttentionBackward : public torch::autograd::Node {
     AttentionSpec spec;
     std::array<torch::autograd::SavedVariable, ATTENTION_TENSORS> saved;
     torch::autograd::SavedVariable out;
-    at::Tensor stats;
+    at::Tensor stats, rest;                    // rest: what rounding to 16 bits left of the output
     bool released = false;
 
     std::string name() const override { return "SequenceAttentionHIPBackward"; }
@@ -714,6 +714,7 @@ struct SequenceAttentionBackward : public torch::autograd::Node {
         for (auto& s : saved) s.reset_data();
         out.reset_data();
         stats.reset();
+        rest.reset();
     }
     torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
         TORCH_CHECK(!released, "Trying to backward through an attention a second time: make the first pass with retain_graph=True");
@@ -745,7 +746,7 @@ struct SequenceAttentionBackward : public torch::autograd::Node {
             // (scratch of its own for every call: two captured passes never share it)
             const at::Tensor scratch = bytes(g_attention.backward_bytes(&a), o.device());
             auto p = [](const at::Tensor& u) { return u.defined() ? u.data_ptr() : nullptr; };
-            check(g_attention.backward(&a, p(o), stats.data_ptr<float>(), p(go), go_stride, p(dq), p(dk), p(dv), p(dtable), scratch.data_ptr(),
+            check(g_attention.backward(&a, p(o), p(rest), stats.data_ptr<float>(), p(go), go_stride, p(dq), p(dk), p(dv), p(dtable), scratch.data_ptr(),
                                        (size_t)scratch.numel(), raw_stream(o)),
                   "cfh_attention_backward");
             if (wanted[QUERY]) result[QUERY] = dq;
@@ -781,21 +782,23 @@ at::Tensor sequence_attention(const at::Tensor& query, const at::Tensor& key, co
         for (int n = 0; n < ATTENTION_LEAVES; n++) train = train || (inputs[n].defined() && inputs[n].requires_grad());
     c10::DeviceGuard guard(query.device());
     AttentionTensors t = inputs;
-    at::Tensor out, stats;
+    at::Tensor out, stats, rest;
     {
         at::AutoDispatchBelowADInplaceOrView below;
         const cfh_attention a = attention_args(t, s);
         out = at::empty(query.sizes(), query.options().memory_format(at::MemoryFormat::Contiguous));
         if (train) stats = at::empty({query.numel() / query.size(-1), 2}, query.options().dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous));
+        if (train && query.scalar_type() != at::kFloat) rest = at::empty_like(out);
         const size_t need = g_attention.forward_bytes(&a);
         const at::Tensor scratch = need ? bytes(need, query.device()) : at::Tensor();
-        check(g_attention.forward(&a, out.data_ptr(), train ? stats.data_ptr<float>() : nullptr, need ? scratch.data_ptr() : nullptr, need, raw_stream(query)),
+        check(g_attention.forward(&a, out.data_ptr(), rest.defined() ? rest.data_ptr() : nullptr, train ? stats.data_ptr<float>() : nullptr, need ? scratch.data_ptr() : nullptr, need, raw_stream(query)),
               "cfh_attention_forward");
     }
     if (train) {
         auto node = std::shared_ptr<SequenceAttentionBackward>(new SequenceAttentionBackward(), torch::autograd::deleteNode);
         node->spec = s;
         node->stats = std::move(stats);
+        node->rest = std::move(rest);
         torch::autograd::edge_list edges;
         for (int n = 0; n < ATTENTION_LEAVES; n++)
             edges.push_back(inputs[n].defined() && inputs[n].requires_grad() ? torch::autograd::impl::gradient_edge(inputs[n]) : torch::autograd::Edge());

@@ -308,6 +308,17 @@ __device__ __forceinline__ void reads_ahead() {
     __builtin_amdgcn_sched_group_barrier(0x8, first, 0);
 }
 
+// An output and, for the backward pass, what its rounding to 16 bits left (rounded to them in turn): D, the sum of do . o, then has an
+// error of 2^-17 of its terms instead of 2^-9, which a row's ds have in common and its sums over keys would keep.
+template <typename T>
+__device__ __forceinline__ void put_output(T* out, T* rest, int64_t row, int from, int dim, f32x4 x) {
+    put_four<T>(out + row * dim, from, dim, x);
+    if constexpr (sizeof(T) == 2) {
+        if (rest) put_four<T>(rest + row * dim, from, dim, f32x4{x[0] - to_float(from_float<T>(x[0])), x[1] - to_float(from_float<T>(x[1])),
+                                                                  x[2] - to_float(from_float<T>(x[2])), x[3] - to_float(from_float<T>(x[3]))});
+    }
+}
+
 // ---- which rows a workgroup has --------------------------------------------------------------------------------------------------------
 struct Span {
     int64_t first;      // row of the sequence's first position among all rows
@@ -524,7 +535,7 @@ struct FewLds {
 };
 
 template <typename T, int DC, int NW, bool BIAS, bool PAST>
-__global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && NW == 4 ? 2 : 1)) void few_kernel(SequenceAttention A, T* out, float* stats, float* part_o, float* part_ml, int splits) {
+__global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && NW == 4 ? 2 : 1)) void few_kernel(SequenceAttention A, T* out, T* rest, float* stats, float* part_o, float* part_ml, int splits) {
     constexpr int DP = pitch(DC), ND = (DC + 31) / 32, KEYS = 32;
     using L = Tile<T, DP>;
     __shared__ __attribute__((aligned(16))) FewLds<T, DP, NW> S;
@@ -681,7 +692,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && NW == 4 ? 2 : 1)) void 
             continue;
         }
         const float inverse = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-        put_four<T>(out + row * A.dim, from, A.dim, o * inverse);
+        put_output<T>(out, rest, row, from, A.dim, o * inverse);
         if (stats && from == 0) {
             stats[2 * row] = m == NONE ? -NONE : m;
             stats[2 * row + 1] = inverse * (NARROW<T> ? 0x1p6f : 1.0f);
@@ -692,7 +703,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && NW == 4 ? 2 : 1)) void 
 // Joins the splits: 8 rows to a workgroup, 32 lanes to a row.  The lanes look at a part's statistics each, and then all at its sums.
 template <typename T, int DC, bool BIAS>
 __global__ __launch_bounds__(256) void combine_parts(SequenceAttention A, const float* part_o, const float* part_ml, int splits, int64_t rows, T* out,
-                                                     float* stats) {
+                                                     T* rest, float* stats) {
     constexpr int DP = pitch(DC);
     const int64_t row = blockIdx.x * 8LL + threadIdx.x / 32;
     const int lane = threadIdx.x & 31, from = lane * 4;
@@ -726,7 +737,7 @@ __global__ __launch_bounds__(256) void combine_parts(SequenceAttention A, const 
         }
     }
     const float inverse = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-    if (from < A.dim) put_four<T>(out + row * A.dim, from, A.dim, o * inverse);
+    if (from < A.dim) put_output<T>(out, rest, row, from, A.dim, o * inverse);
     if (stats && lane == 0) {
         stats[2 * row] = m == NONE ? -NONE : m;
         stats[2 * row + 1] = inverse * (NARROW<T> ? 0x1p6f : 1.0f);
@@ -738,7 +749,7 @@ template <typename T, int NW>
 constexpr int keys_at_once() { return sizeof(T) == 2 && NW >= 4 ? 64 : 32; }
 
 template <typename T, int DC, int NW, bool BIAS>
-__global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 ? 2 : 1)) void tiles_kernel(SequenceAttention A, T* out, float* stats, int64_t slots) {
+__global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 ? 2 : 1)) void tiles_kernel(SequenceAttention A, T* out, T* rest, float* stats, int64_t slots) {
     constexpr int DP = pitch(DC), ND = (DC + 31) / 32;
     using L = Tile<T, DP>;
     constexpr int KEYS = keys_at_once<T, NW>(), TILE = L::bytes(KEYS);
@@ -861,7 +872,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 ? 2 : 1)) void tiles_kerne
         for (int r = 0; r < 16; r += 4) {
             f32x4 x{sum.o[d][r], sum.o[d][r + 1], sum.o[d][r + 2], sum.o[d][r + 3]};
             x *= inverse;
-            put_four<T>(out + row * A.dim, 32 * d + result_row(r) + 4 * half, A.dim, mine ? x : f32x4{0, 0, 0, 0});
+            put_output<T>(out, rest, row, 32 * d + result_row(r) + 4 * half, A.dim, mine ? x : f32x4{0, 0, 0, 0});
         }
     if (stats && half == 0) {
         stats[2 * row] = mine && sum.m != NONE ? sum.m : -NONE;
@@ -945,10 +956,11 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
     const int first = (int)((int64_t)whole * z / splits), end = (int)((int64_t)whole * (z + 1) / splits);
 
     const int64_t row = (q.first + i) * A.heads + h;
-    Eight<T> qf[DC / 16], gf[DC / 16], of[DC / 16];
+    Eight<T> qf[DC / 16], gf[DC / 16], of[DC / 16], rf[sizeof(T) == 2 ? DC / 16 : 1];
     row_operands<T, DC>(qf, row_start<T>(A.q, q, A.packed, h) + (mine ? i : 0) * A.q.row, mine, A.dim, true, lane);
     row_operands<T, DC>(gf, row_start<T>(G.go, q, A.packed, h) + (mine ? i : 0) * G.go.row, mine, A.dim, true, lane);
     row_operands<T, DC>(of, static_cast<const T*>(G.out) + (mine ? row : 0) * A.dim, mine, A.dim, A.dim % L::E == 0, lane);
+    if constexpr (sizeof(T) == 2) row_operands<T, DC>(rf, static_cast<const T*>(G.rest) + (mine ? row : 0) * A.dim, mine, A.dim, A.dim % L::E == 0, lane);
     float m = -NONE, inverse = 0.0f;
     if (mine) {
         m = G.stats[2 * row];
@@ -990,7 +1002,11 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
 #pragma unroll
     for (int s = 0; s < DC / 16; s++)
 #pragma unroll
-        for (int e = 0; e < 8; e++) D = __builtin_fmaf(value<T>(gf[s], e), value<T>(of[s], e), D);
+        for (int e = 0; e < 8; e++) {
+            float o = value<T>(of[s], e);
+            if constexpr (sizeof(T) == 2) o += value<T>(rf[s], e);
+            D = __builtin_fmaf(value<T>(gf[s], e), o, D);
+        }
     D = other_half_sum(D);
     if (z == 0 && half == 0 && i < q.rows) G.rows[row] = D;
     const float off = row_shift(score, m, inverse);
@@ -1362,7 +1378,7 @@ void with_choice(bool yes, F f) {
 inline unsigned die_grid(int64_t count) { return (unsigned)((count + 7) / 8 * 8); }
 
 template <typename T>
-void sequence_attention_forward(const SequenceAttention& A, const AttentionPlan& P, T* out, float* stats, float* scratch, hipStream_t st) {
+void sequence_attention_forward(const SequenceAttention& A, const AttentionPlan& P, T* out, T* rest, float* stats, float* scratch, hipStream_t st) {
     using namespace attention;
     with_padded_dim(A.dim, [&](auto dc) {
         with_choice(A.table != nullptr, [&](auto bias) {
@@ -1371,7 +1387,7 @@ void sequence_attention_forward(const SequenceAttention& A, const AttentionPlan&
             const int64_t rows = (A.packed ? A.q_rows : A.q_rows * A.batch) * A.heads;
             if (!P.few) {
                 const size_t lds = 4 * Tile<T, DP>::bytes(keys_at_once<T, 4>()) + 2 * keys_at_once<T, 4>() * sizeof(float) + (BIAS ? (2 * (A.reach + MARGIN) + 1) * sizeof(float) : 0);
-                launch_attention(tiles_kernel<T, DC, 4, BIAS>, dim3(die_grid((int64_t)P.slots * A.heads)), 256, lds, st, A, out, stats, P.slots);
+                launch_attention(tiles_kernel<T, DC, 4, BIAS>, dim3(die_grid((int64_t)P.slots * A.heads)), 256, lds, st, A, out, rest, stats, P.slots);
                 return;
             }
             float* const part_o = scratch;
@@ -1379,13 +1395,13 @@ void sequence_attention_forward(const SequenceAttention& A, const AttentionPlan&
             const dim3 grid(P.slots, A.kv_heads * ((A.share + 31) / 32), P.splits);
             const int at_once = A.share < 32 ? A.share : 32;
             const size_t line = BIAS && few_line(at_once, A.reach) ? (size_t)at_once * (2 * (A.reach + MARGIN) + 1) * sizeof(float) : 0;
-            if (P.waves == 1) launch_attention(few_kernel<T, DC, 1, BIAS, false>, grid, 64, line, st, A, out, stats, part_o, part_ml, P.splits);
+            if (P.waves == 1) launch_attention(few_kernel<T, DC, 1, BIAS, false>, grid, 64, line, st, A, out, rest, stats, part_o, part_ml, P.splits);
             else with_choice(P.past, [&](auto past) {
-                launch_attention(few_kernel<T, DC, few_waves(sizeof(T) == 4, DC), BIAS, decltype(past)::value>, grid, P.waves * 64, line, st, A, out, stats,
+                launch_attention(few_kernel<T, DC, few_waves(sizeof(T) == 4, DC), BIAS, decltype(past)::value>, grid, P.waves * 64, line, st, A, out, rest, stats,
                                  part_o, part_ml, P.splits);
             });
             if (P.splits > 1)
-                launch_attention(combine_parts<T, DC, BIAS>, dim3((unsigned)((rows + 7) / 8)), 256, 0, st, A, part_o, part_ml, P.splits, rows, out, stats);
+                launch_attention(combine_parts<T, DC, BIAS>, dim3((unsigned)((rows + 7) / 8)), 256, 0, st, A, part_o, part_ml, P.splits, rows, out, rest, stats);
         });
     });
 }

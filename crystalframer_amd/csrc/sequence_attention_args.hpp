@@ -31,7 +31,7 @@ struct SequenceAttention {
 
 struct AttentionGrads {
     AttentionRows go;
-    const void* out;                   // (rows, heads, dim), as all that follows
+    const void *out, *rest;            // (rows, heads, dim), as all that follows; rest: what rounding left of out, in 16 bits
     const float* stats;                // (rows, heads, 2): largest score, one over the sum
     float* rows;                       // (rows, heads): D, from the queries' kernel for the keys'
     void *dq, *dk, *dv;                // (dk, dv over kv_heads)
@@ -90,17 +90,20 @@ struct AttentionGradPlan {
 inline AttentionGradPlan attention_grad_plan(const SequenceAttention& A) {
     AttentionGradPlan P{};
     const int64_t q_each = A.packed && A.batch > 0 ? A.q_rows / A.batch : A.q_rows, k_each = A.packed && A.batch > 0 ? A.k_rows / A.batch : A.k_rows;
-    P.q_waves = q_each > 64 && queries_lds(A.float32, A.dim, A.reach, A.table != nullptr, 4) <= ATTENTION_LDS ? 4 : 1;
+    // (with a table rather more workgroups of one wavefront than keys in parts: rows whose ds are there as a whole are summed more exactly)
+    const bool table = A.table != nullptr;
+    const int64_t quads = tile_slots(A.packed, A.q_rows, A.batch, 128) * A.heads;
+    P.q_waves = q_each > 64 && (!table || (quads >= 2 * ATTENTION_CUS && queries_lds(A.float32, A.dim, A.reach, true, 4) <= ATTENTION_LDS)) ? 4 : 1;
     P.k_waves = k_each > 64 ? 4 : 1;
     P.q_slots = tile_slots(A.packed, A.q_rows, A.batch, 32 * P.q_waves);
     P.k_slots = tile_slots(A.packed, A.k_rows, A.batch, 32 * P.k_waves);
-    P.q_splits = split_count(P.q_slots * A.heads * P.q_waves, 8 * ATTENTION_CUS, k_each, 128);
+    P.q_splits = split_count(P.q_slots * A.heads * P.q_waves, (table ? 2 : 8) * ATTENTION_CUS, k_each, 128);
     P.k_splits = split_count(P.k_slots * A.kv_heads * P.k_waves, 8 * ATTENTION_CUS, q_each * A.share, 128);
     return P;
 }
 
 template <typename T>
-void sequence_attention_forward(const SequenceAttention& A, const AttentionPlan& P, T* out, float* stats, float* scratch, hipStream_t st);
+void sequence_attention_forward(const SequenceAttention& A, const AttentionPlan& P, T* out, T* rest, float* stats, float* scratch, hipStream_t st);
 template <typename T>
 void sequence_attention_backward(const SequenceAttention& A, const AttentionGradPlan& P, AttentionGrads G, void* dtable, float* scratch, hipStream_t st);
 }  // namespace cfh

@@ -109,16 +109,17 @@ size_t cfh_attention_forward_workspace_bytes(const cfh_attention* a) {
     return P.splits > 1 ? (size_t)P.splits * q_all(A) * (padded_dim(A.dim) + 2) * sizeof(float) : 0;
 }
 
-int cfh_attention_forward(const cfh_attention* a, void* out, float* stats, void* workspace, size_t workspace_bytes, void* stream) {
+int cfh_attention_forward(const cfh_attention* a, void* out, void* out_rest, float* stats, void* workspace, size_t workspace_bytes, void* stream) {
     int rc = check_attention(a);
     if (rc) return rc;
     const cfh::SequenceAttention A = device_args(a);
     if (q_all(A) == 0) return CFH_OK;
-    if (!out || ((uintptr_t)out & 15)) return fail(CFH_EINVAL, "attention: out must not be NULL, and aligned to 16 bytes");
+    if (!out || (((uintptr_t)out | (uintptr_t)out_rest) & 15)) return fail(CFH_EINVAL, "attention: out must not be NULL, and aligned to 16 bytes, as out_rest");
+    if (a->dtype == CFH_FLOAT32 && out_rest) return fail(CFH_EINVAL, "attention: out_rest is of 16-bit types");
     if ((rc = check_workspace(workspace, workspace_bytes, cfh_attention_forward_workspace_bytes(a)))) return rc;
     with_type(a->dtype, [&](auto t) {
         using T = decltype(t);
-        cfh::sequence_attention_forward<T>(A, cfh::attention_plan(A), (T*)out, stats, (float*)workspace, (hipStream_t)stream);
+        cfh::sequence_attention_forward<T>(A, cfh::attention_plan(A), (T*)out, (T*)out_rest, stats, (float*)workspace, (hipStream_t)stream);
     });
     return finish_launch("attention_forward");
 }
@@ -134,22 +135,23 @@ size_t cfh_attention_backward_workspace_bytes(const cfh_attention* a) {
     return floats * sizeof(float);
 }
 
-int cfh_attention_backward(const cfh_attention* a, const void* out, const float* stats, const void* gout, const int64_t gout_stride[3],
+int cfh_attention_backward(const cfh_attention* a, const void* out, const void* out_rest, const float* stats, const void* gout, const int64_t gout_stride[3],
                            void* dq, void* dk, void* dv, void* dtable, void* workspace, size_t workspace_bytes, void* stream) {
     int rc = check_attention(a);
     if (rc) return rc;
     const cfh::SequenceAttention A = device_args(a);
     if (dtable && !a->table) return fail(CFH_EINVAL, "attention: a gradient of a table that is not there");
     if (q_all(A) > 0 && (!out || !stats || !gout || !gout_stride || !dq)) return fail(CFH_EINVAL, "attention: out, stats, gout, its strides and dq must not be NULL");
+    if (q_all(A) > 0 && !out_rest != (a->dtype == CFH_FLOAT32)) return fail(CFH_EINVAL, "attention: out_rest belongs to 16-bit types");
     if (k_all(A) > 0 && !dk != !dv) return fail(CFH_EINVAL, "attention: dk and dv go together");
-    if (((uintptr_t)out | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15) return fail(CFH_EINVAL, "attention: out, dq, dk and dv must be aligned to 16 bytes");
+    if (((uintptr_t)out | (uintptr_t)out_rest | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15) return fail(CFH_EINVAL, "attention: out, dq, dk and dv must be aligned to 16 bytes");
     const int64_t none[3] = {0, 0, 0};
     const int64_t* const gs = gout_stride ? gout_stride : none;
     if ((rc = check_rows(gout, gs, a->dtype))) return rc;
     if ((rc = check_workspace(workspace, workspace_bytes, cfh_attention_backward_workspace_bytes(a)))) return rc;
     cfh::AttentionGrads G{};
     G.go = {gout, gs[0], gs[1], gs[2]};
-    G.out = out; G.stats = stats; G.dq = dq; G.dk = dk; G.dv = dv;
+    G.out = out; G.rest = out_rest; G.stats = stats; G.dq = dq; G.dk = dk; G.dv = dv;
     with_type(a->dtype, [&](auto t) {
         cfh::sequence_attention_backward<decltype(t)>(A, cfh::attention_grad_plan(A), G, dtable, (float*)workspace, (hipStream_t)stream);
     });

@@ -809,13 +809,14 @@ typedef struct cfh_attention {
     const void* table;                    /* (buckets, heads) or NULL                                    */
     const int32_t* bucket_of;             /* (2 reach + 1)                                               */
 } cfh_attention;
-/* stats (rows, heads, 2): for the backward pass, or NULL.  workspace aligned to 16 bytes; 0 bytes may be needed. */
+/* For the backward pass, or NULL: stats (rows, heads, 2), and in 16-bit types out_rest (as out), what rounding left of the output.
+ * workspace aligned to 16 bytes; 0 bytes may be needed. */
 size_t cfh_attention_forward_workspace_bytes(const cfh_attention* a);
-int cfh_attention_forward(const cfh_attention* a, void* out, float* stats, void* workspace, size_t workspace_bytes, void* stream);
+int cfh_attention_forward(const cfh_attention* a, void* out, void* out_rest, float* stats, void* workspace, size_t workspace_bytes, void* stream);
 /* gout with strides as q_stride; dk and dv may both be NULL (states that are not trained); dtable (buckets, heads) in table_dtype, or
  * NULL.  Every sum in a fixed order. */
 size_t cfh_attention_backward_workspace_bytes(const cfh_attention* a);
-int cfh_attention_backward(const cfh_attention* a, const void* out, const float* stats, const void* gout, const int64_t gout_stride[3],
+int cfh_attention_backward(const cfh_attention* a, const void* out, const void* out_rest, const float* stats, const void* gout, const int64_t gout_stride[3],
                            void* dq, void* dk, void* dv, void* dtable, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus

@@ -5,7 +5,7 @@ Bounds.  u: half a unit of the type, e: 2^-24.  With A_i the largest of scale su
 up to (D + 24) e A_i (its products' sum, scale, bias, maximum and the change of base), and a probability relative to its sum one of
 twice that and of the sum's own additions: E_i = e (2 (D + 24) A_i + keys + 64).
     o:      u |o| + (u + E_i) sum_j P |v|                                       (P rounded to the type before its product)
-    D_i:    sum_d |do| (error of o) + e (D + 8) sum_d |do o|  =: Z_i
+    D_i:    sum_d |do| (error of o, where u |o| is u^2 |o| in 16 bits: the output is kept in two parts) + e (D + 8) sum_d |do o|  =: Z_i
     ds:     P (2 E_i (W + |D|) + Z_i), W_ij = sum_d |do v|                      (W's own sum in it: D + 8 < what E_i holds, W e each)
     dq:     u |dq| + scale sum_j (error of ds + (u + e keys) |ds|) |k|          (ds rounded to the type before its product)
     dk:     u |dk| + scale sum_i (error of ds + (u + e rows) |ds|) |q|
@@ -68,7 +68,7 @@ def attention(q, k, v, keep, bias=None, scale=None, go=None, bucket=None, bucket
         gh = go[:, h]
         dp, W = gh @ vh.T, gh.abs() @ vh.abs().T
         Di = (gh * o).sum(1, keepdim=True)
-        Z = (gh.abs() * err_o).sum(1, keepdim=True) + e * (D + 8) * (gh * o).abs().sum(1, keepdim=True)
+        Z = (gh.abs() * (err_o + ((u * u - u) * o.abs() + TINY[dtype] if dtype != torch.float32 else 0.0))).sum(1, keepdim=True) + e * (D + 8) * (gh * o).abs().sum(1, keepdim=True)
         ds = P * (dp - Di)
         err = P * (2 * E * (W + Di.abs()) + Z)
         lost = [narrow * 2.0 ** -39 * (ds.abs().amax(n, keepdim=True) if ds.numel() else 0.0) * torch.ones_like(ds) for n in (1, 0)]

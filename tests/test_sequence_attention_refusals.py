@@ -38,11 +38,11 @@ TABLE = dict(table=A, buckets=4, reach=8, bucket_of=A)
     (dict(batch=0x7fffffff, key_rows=0x7fffff00), b"grid")])
 def test_arguments(change, word):
     lib, a = _lib.load(), _args(**change)
-    assert lib.cfh_attention_forward(ctypes.byref(a), A, None, A, 1 << 30, None) < 0 and word in lib.cfh_last_error()
+    assert lib.cfh_attention_forward(ctypes.byref(a), A, None, None, A, 1 << 30, None) < 0 and word in lib.cfh_last_error()
     assert lib.cfh_attention_forward_workspace_bytes(ctypes.byref(a)) == 0
     assert lib.cfh_attention_backward_workspace_bytes(ctypes.byref(a)) == 0
     strides = (ctypes.c_int64 * 3)(320, 64, 16)
-    assert lib.cfh_attention_backward(ctypes.byref(a), A, A, A, strides, A, A, A, None, A, 1 << 30, None) < 0 and word in lib.cfh_last_error()
+    assert lib.cfh_attention_backward(ctypes.byref(a), A, None, A, A, strides, A, A, A, None, A, 1 << 30, None) < 0 and word in lib.cfh_last_error()
 
 
 def test_results_and_workspaces():
@@ -51,21 +51,22 @@ def test_results_and_workspaces():
     need = lib.cfh_attention_backward_workspace_bytes(ctypes.byref(a))
     assert need > 0
 
-    def backward(out=A, stats=A, go=A, st=strides, dq=A, dk=A, dv=A, table=None, ws=A, n=need, args=a):
-        return lib.cfh_attention_backward(ctypes.byref(args), out, stats, go, st, dq, dk, dv, table, ws, n, None)
+    def backward(out=A, stats=A, go=A, st=strides, dq=A, dk=A, dv=A, table=None, ws=A, n=need, args=a, rest=None):
+        return lib.cfh_attention_backward(ctypes.byref(args), out, rest, stats, go, st, dq, dk, dv, table, ws, n, None)
     for change, word in ((dict(out=None), b"NULL"), (dict(stats=None), b"NULL"), (dict(go=None), b"NULL"), (dict(st=None), b"NULL"),
                          (dict(dq=None), b"NULL"), (dict(dk=None), b"together"), (dict(dv=None), b"together"), (dict(dq=A + 8), b"16"),
                          (dict(out=A + 4), b"16"), (dict(table=A), b"table"), (dict(ws=None), b"workspace"), (dict(n=need - 1), b"workspace"),
-                         (dict(ws=A + 4), b"workspace"), (dict(go=A + 4), b"address"), (dict(st=(ctypes.c_int64 * 3)(4, -4, 4)), b"strides")):
+                         (dict(ws=A + 4), b"workspace"), (dict(go=A + 4), b"address"), (dict(rest=A), b"out_rest"), (dict(args=_args(dtype=1)), b"out_rest"), (dict(st=(ctypes.c_int64 * 3)(4, -4, 4)), b"strides")):
         assert backward(**change) < 0 and word in lib.cfh_last_error(), (change, lib.cfh_last_error())
-    assert lib.cfh_attention_forward(ctypes.byref(a), None, None, None, 0, None) < 0 and b"out" in lib.cfh_last_error()
-    assert lib.cfh_attention_forward(ctypes.byref(a), A + 8, None, None, 0, None) < 0 and b"out" in lib.cfh_last_error()
-    assert lib.cfh_attention_forward(None, A, None, None, 0, None) < 0
+    assert lib.cfh_attention_forward(ctypes.byref(a), None, None, None, None, 0, None) < 0 and b"out" in lib.cfh_last_error()
+    assert lib.cfh_attention_forward(ctypes.byref(a), A + 8, None, None, None, 0, None) < 0 and b"out" in lib.cfh_last_error()
+    assert lib.cfh_attention_forward(None, A, None, None, None, 0, None) < 0
+    assert lib.cfh_attention_forward(ctypes.byref(a), A, A, None, None, 0, None) < 0 and b"out_rest" in lib.cfh_last_error()
     long = _args(batch=1, query_rows=1, key_rows=1 << 16)          # keys in parts
     need = lib.cfh_attention_forward_workspace_bytes(ctypes.byref(long))
     assert need > 0
     for ws, n in ((None, need), (A, need - 1), (A + 8, need)):
-        assert lib.cfh_attention_forward(ctypes.byref(long), A, None, ws, n, None) == -2
+        assert lib.cfh_attention_forward(ctypes.byref(long), A, None, None, ws, n, None) == -2
 
 
 def test_struct_matches_the_header():
