@@ -4,8 +4,8 @@
 //   D_i = do_i . o_i,   ds_ij = P_ij (do_i . v_j - D_i)
 //   dv_j = sum_i P_ij do_i,   dq_i = scale sum_j ds_ij k_j,   dk_j = scale sum_i ds_ij q_i,   dtable[b] = sum over bucket b of ds_ij
 //
-// All products are matrix instructions of 32 x 32 results, 16 terms deep.  A result has its column in
-// the lane (l % 32) and 16 of its rows in the lane's registers: rows 8 (r / 4) + 4 (l / 32) + r % 4.  The scores are made transposed
+// All products are matrix instructions of 32 x 32 results, 16 terms deep.  A result has its column in the lane (l % 32) and 16 of its
+// rows in the lane's registers: rows 8 (r / 4) + 4 (l / 32) + r % 4.  The scores are made transposed
 // where sums over keys follow (rows: keys, columns: queries), and upright where sums over queries follow: either way the probabilities
 // are, register by register, the right operand of the product that follows, whose terms may come in any order as long as the left
 // operand has them in the same one.  That operand is the transpose of a tile in LDS (ds_read_b64_tr_b16).
@@ -25,7 +25,6 @@ namespace cfh {
 namespace attention {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
@@ -419,7 +418,9 @@ __device__ __forceinline__ float table_entry(const SequenceAttention& A, int at,
     const bool real = (unsigned)b < (unsigned)A.buckets;
     const int64_t n = (int64_t)(real ? b : 0) * A.heads + head;
     const float x = A.table_float ? static_cast<const float*>(A.table)[n] : to_float(static_cast<const T*>(A.table)[n]);
-    return real ? x : 0.0f;
+    // (beyond 2^16, where a mask's lowest value would end a float32's range with 1 / scale, all are as far away; infinities stay)
+    const float most = 65536.0f, size = fabsf(x);
+    return real ? size > most && size < -NONE ? copysignf(most, x) : x : 0.0f;
 }
 __device__ __forceinline__ int clamped(int r, int reach) { return (r < -reach ? -reach : r > reach ? reach : r) + reach; }
 template <typename T>
@@ -523,7 +524,6 @@ __device__ __forceinline__ bool all_there(uint64_t bits) { return COUNT == 64 ? 
 // so are, by combine_parts, those of `splits` workgroups.  Bound by the bytes of keys and values for single tokens; PAST: these go past the
 // caches, where one workgroup reads them and they are more than the last cache keeps (0.5 GB: 129 -> 119 us; 240 MB that no call before had
 // read: 77 -> 73, that one just had: 64 -> 70).
-template <typename T>
 __device__ __forceinline__ int heads_at_once(int share) { return share < 32 ? share : 32; }
 
 template <typename T, int DP, int NW>
@@ -540,7 +540,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && NW == 4 ? 2 : 1)) void 
     using L = Tile<T, DP>;
     __shared__ __attribute__((aligned(16))) FewLds<T, DP, NW> S;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-    const int at_once = heads_at_once<T>(A.share), groups = (A.share + at_once - 1) / at_once, tile = 32 / at_once;
+    const int at_once = heads_at_once(A.share), groups = (A.share + at_once - 1) / at_once, tile = 32 / at_once;
     int b, i0;
     if (!find_slot(A.q_starts, A.q_rows, A.packed, A.batch, tile, blockIdx.x, lane, b, i0)) return;
     const Span q = span_of(A.q_starts, A.q_sizes, A.q_rows, A.packed, A.batch, b);
@@ -894,7 +894,7 @@ __device__ __forceinline__ float probability(const Score<T>& score, float t, flo
 
 // Sums of a 32 x 32 result over its diagonals: column l of 16 and row 16 a + b meet in place (l - b) of sum a, or of sum a + 1 where that
 // is negative.  A shift within 16 lanes that fills with zeros is part of the addition (DPP): two instructions for a register, none of
-// them an LDS atomic, of which one takes 94 cycles for a wavefront (16 of them per tile: 330 us where this takes NEARUS, 32 x 512 tokens, 12 heads
+// them an LDS atomic, of which one takes 94 cycles for a wavefront (16 of them per tile: 330 us where this takes 101, 32 x 512 tokens, 12 heads
 // of 64).  Register r is row 8 (r / 4) + r % 4; the 4 of the upper half wavefront are in the place that the sums are added to.
 template <int CTRL>
 __device__ __forceinline__ float shifted(float x) {

@@ -17,7 +17,8 @@ using cfh::fail;
 using cfh::finish_launch;
 
 constexpr int64_t MAX_ROWS = 0x7fffff00LL;      // of a sequence, and of all packed ones
-constexpr int64_t MAX_GRID = 0x7fffff00LL;
+constexpr int64_t MAX_ALL = 1LL << 40;               // rows of a batch
+constexpr int64_t MAX_THREADS = 0xffffff00LL;      // of a grid's first dimension
 
 // Rows begin at multiples of 16 bytes, and a tile of them is less than 2^30 bytes.
 int check_rows(const void* at, const int64_t* stride, int dtype) {
@@ -42,6 +43,8 @@ int check_attention(const cfh_attention* a) {
     if (a->batch < 0 || a->query_rows < 0 || a->query_rows > MAX_ROWS || a->key_rows < 0 || a->key_rows > MAX_ROWS)
         return fail(CFH_EINVAL, "attention: batch = %d, query_rows = %lld, key_rows = %lld out of range", (int)a->batch, (long long)a->query_rows,
                     (long long)a->key_rows);
+    if (!a->packed && a->batch > 0 && (a->query_rows * a->batch > MAX_ALL || a->key_rows * a->batch > MAX_ALL))
+        return fail(CFH_EINVAL, "attention: %d sequences of %lld and %lld rows are too many", (int)a->batch, (long long)a->query_rows, (long long)a->key_rows);
     if (!(a->scale > 0.0f) || std::isinf(a->scale)) return fail(CFH_EINVAL, "attention: scale = %g must be positive and finite", a->scale);
     if (a->packed && (!a->query_starts || !a->key_starts)) return fail(CFH_EINVAL, "attention: packed sequences need query_starts and key_starts");
     if (a->packed && (a->query_sizes || a->key_sizes)) return fail(CFH_EINVAL, "attention: query_sizes and key_sizes are of sequences that are not packed");
@@ -60,9 +63,7 @@ int check_attention(const cfh_attention* a) {
     } else if (a->buckets || a->reach || a->bucket_of) {
         return fail(CFH_EINVAL, "attention: buckets, reach and bucket_of belong to a table");
     }
-    // (the smallest tile of either side is one row)
-    const int64_t slots = cfh::tile_slots(a->packed, a->query_rows > a->key_rows ? a->query_rows : a->key_rows, a->batch, 1);
-    if (slots > MAX_GRID / a->heads) return fail(CFH_EINVAL, "attention: %lld rows of %d heads are more than a grid holds", (long long)slots, (int)a->heads);
+    if (a->table && !(a->scale >= 0x1p-64f)) return fail(CFH_EINVAL, "attention: scale = %g: at least 2^-64 with a table", a->scale);
     return CFH_OK;
 }
 
@@ -86,6 +87,16 @@ int padded_dim(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : 128; }
 int64_t q_all(const cfh::SequenceAttention& A) { return (A.packed ? A.q_rows : A.q_rows * A.batch) * A.heads; }
 int64_t k_all(const cfh::SequenceAttention& A) { return (A.packed ? A.k_rows : A.k_rows * A.batch) * A.kv_heads; }
 
+// The launches' sizes; a row more than a grid holds is refused here.
+int check_grids(const cfh::SequenceAttention& A, bool backward) {
+    const cfh::AttentionPlan P = cfh::attention_plan(A);
+    const cfh::AttentionGradPlan B = cfh::attention_grad_plan(A);
+    const int64_t rows = A.packed ? A.q_rows : A.q_rows * A.batch;
+    const bool fits = !backward ? P.slots <= MAX_THREADS / (P.few ? 64 * P.waves : 256) / (P.few ? 1 : A.heads) && (P.splits == 1 || rows <= MAX_THREADS / 64 / A.heads)
+                                : B.q_slots <= MAX_THREADS / (64 * B.q_waves) / A.heads && B.k_slots <= MAX_THREADS / (64 * B.k_waves) / A.kv_heads;
+    if (!fits) return fail(CFH_EINVAL, "attention: %lld rows and %lld keys of %d heads are more than a grid holds", (long long)rows, (long long)A.k_rows, (int)A.heads);
+    return CFH_OK;
+}
 int check_workspace(const void* workspace, size_t have, size_t need) {
     if (need > 0 && (!workspace || ((uintptr_t)workspace & 15) || have < need))
         return fail(CFH_EWORKSPACE, "attention: workspace of %zu bytes, aligned to 16, is missing", need);
@@ -116,6 +127,7 @@ int cfh_attention_forward(const cfh_attention* a, void* out, void* out_rest, flo
     if (q_all(A) == 0) return CFH_OK;
     if (!out || (((uintptr_t)out | (uintptr_t)out_rest) & 15)) return fail(CFH_EINVAL, "attention: out must not be NULL, and aligned to 16 bytes, as out_rest");
     if (a->dtype == CFH_FLOAT32 && out_rest) return fail(CFH_EINVAL, "attention: out_rest is of 16-bit types");
+    if ((rc = check_grids(A, false))) return rc;
     if ((rc = check_workspace(workspace, workspace_bytes, cfh_attention_forward_workspace_bytes(a)))) return rc;
     with_type(a->dtype, [&](auto t) {
         using T = decltype(t);
@@ -148,6 +160,7 @@ int cfh_attention_backward(const cfh_attention* a, const void* out, const void* 
     const int64_t none[3] = {0, 0, 0};
     const int64_t* const gs = gout_stride ? gout_stride : none;
     if ((rc = check_rows(gout, gs, a->dtype))) return rc;
+    if ((rc = check_grids(A, true))) return rc;
     if ((rc = check_workspace(workspace, workspace_bytes, cfh_attention_backward_workspace_bytes(a)))) return rc;
     cfh::AttentionGrads G{};
     G.go = {gout, gs[0], gs[1], gs[2]};

@@ -785,7 +785,8 @@ int cfh_model_backward(const cfh_model* m, const cfh_model_batch* b, const float
  * packed = 1: the sequences lie behind one another, query_starts and key_starts (batch + 1, int64, beginning with 0) say where, rows
  *   behind the last are 0 in every result; query_rows, key_rows are those of all sequences.
  * packed = 0: (batch, query_rows) and (batch, key_rows); query_sizes, key_sizes (batch, int64, or NULL: whole rows).
- * Values of these arrays are cut to what is there; an entry of bucket_of outside 0 ... buckets - 1 means no bias.
+ * Values of these arrays are cut to what is there; an entry of bucket_of outside 0 ... buckets - 1 means no bias, finite entries of table
+ * beyond +-65536 count as that.
  * Strides are in elements; channels lie next to one another.  Rows of q, k, v and gout begin at multiples of 16 bytes, less than 2^24 bytes
  * apart, and where dim channels do not fill their last 16 bytes, these are filled with zeros.  out and gradients are contiguous: (rows,
  * heads or kv_heads, dim).
@@ -798,7 +799,7 @@ typedef struct cfh_attention {
     int32_t packed, causal, queries_last;
     int32_t batch, heads, kv_heads, dim;
     int32_t buckets, reach;               /* 0 without a table                                           */
-    float scale;                          /* positive                                                    */
+    float scale;                          /* positive; with a table at least 2^-64                       */
     int32_t reserved0;
     int64_t query_rows, key_rows;
     int64_t q_stride[3], k_stride[3], v_stride[3];      /* of batch (packed: unused), row, head          */

@@ -258,3 +258,30 @@ def test_many_tiles(dtype):
     _run([(1030, 1030)], 3, 3, 64, dtype, seed=2, relative=_buckets(32, 128, False), causal=True)
     _run([(1, 5000), (2, 3000)], 4, 1, 128, dtype, seed=3)
     _run([(3000, 3)], 2, 1, 32, dtype, seed=4)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("reach", [4, 200])
+def test_buckets_that_take_keys_away(reach, dtype):
+    """Minus infinity in the table takes a bucket's keys away, as a mask does, and so does the type's lowest value where a row has others;
+    a row that has only such keys stays a mean of their values."""
+    from crystalframer_amd import cuda_funcs
+    gen = torch.Generator().manual_seed(0)
+    for tq, tk in ((150, 170), (3, 300)):
+        q, k, v, go = (torch.randn(1, n, 2, 32, generator=gen).to(dtype).cuda() for n in (tq, tk, tk, tq))
+        of = torch.zeros(2 * reach + 1, dtype=torch.int32)
+        of[:reach], of[reach + 1:] = 1, 2                # behind, here, ahead
+        for low in (-float("inf"), torch.finfo(dtype).min):
+            x = [t.clone().requires_grad_() for t in (q, k, v)]
+            y = [t.clone().requires_grad_() for t in (q, k, v)]
+            table = torch.tensor([[0.5, -0.5], [0.25, 1.0], [low, low]], dtype=dtype).cuda()
+            a = cuda_funcs.relative_attention(*x, table, of.cuda())
+            b = cuda_funcs.relative_attention(*y, torch.where(table == low, 0.0, table), of.cuda(), causal=True)      # (a row's own key is always there)
+            assert torch.equal(a, b)
+            for g, w in zip(torch.autograd.grad(a, x, go), torch.autograd.grad(b, y, go)):
+                assert torch.equal(g, w)
+            only = cuda_funcs.relative_attention(q, k, v, torch.full((3, 2), low, dtype=dtype).cuda(), of.cuda())
+            if low == -float("inf"):
+                assert (only == 0).all()
+            else:
+                assert (only <= v.amax(1, keepdim=True)).all() and (only >= v.amin(1, keepdim=True)).all() and only.isfinite().all()

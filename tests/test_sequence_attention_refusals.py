@@ -34,8 +34,8 @@ TABLE = dict(table=A, buckets=4, reach=8, bucket_of=A)
     (dict(k=A + 4), b"address"), (dict(dtype=1, q=A + 2), b"address"), (dict(k_stride=(224, 30, 16)), b"16 bytes"),
     (dict(v_stride=(0, 1 << 22, 16)), b"strides"), (dict(q_stride=(1 << 62, 64, 16)), b"strides"), (dict(TABLE, dtype=1, table_dtype=2), b"table_dtype"),
     (dict(TABLE, reach=1025), b"reach"), (dict(TABLE, reach=-1), b"reach"), (dict(TABLE, buckets=0), b"buckets"), (dict(TABLE, bucket_of=None), b"bucket_of"),
-    (dict(buckets=3), b"table"), (dict(bucket_of=A), b"table"), (dict(batch=1 << 20, query_rows=1 << 20), b"grid"),
-    (dict(batch=0x7fffffff, key_rows=0x7fffff00), b"grid")])
+    (dict(buckets=3), b"table"), (dict(bucket_of=A), b"table"), (dict(TABLE, scale=2.0 ** -65), b"scale"),
+    (dict(batch=0x7fffffff, key_rows=0x7fffff00), b"too many")])
 def test_arguments(change, word):
     lib, a = _lib.load(), _args(**change)
     assert lib.cfh_attention_forward(ctypes.byref(a), A, None, None, A, 1 << 30, None) < 0 and word in lib.cfh_last_error()
@@ -43,6 +43,14 @@ def test_arguments(change, word):
     assert lib.cfh_attention_backward_workspace_bytes(ctypes.byref(a)) == 0
     strides = (ctypes.c_int64 * 3)(320, 64, 16)
     assert lib.cfh_attention_backward(ctypes.byref(a), A, None, A, A, strides, A, A, A, None, A, 1 << 30, None) < 0 and word in lib.cfh_last_error()
+
+
+@pytest.mark.parametrize("change", [dict(batch=1 << 20, query_rows=1 << 19), dict(batch=1 << 30, query_rows=1, key_rows=1)])
+def test_grids(change):
+    lib, a = _lib.load(), _args(heads=128, kv_heads=1, **change)
+    strides = (ctypes.c_int64 * 3)(320, 64, 16)
+    assert lib.cfh_attention_forward(ctypes.byref(a), A, None, None, A, 1 << 62, None) < 0 and b"grid" in lib.cfh_last_error()
+    assert lib.cfh_attention_backward(ctypes.byref(a), A, None, A, A, strides, A, A, A, None, A, 1 << 62, None) < 0 and b"grid" in lib.cfh_last_error()
 
 
 def test_results_and_workspaces():
