@@ -918,7 +918,7 @@ __device__ __forceinline__ void add_diagonals(const f32x16& s, float (&x)[3], st
 // dq, D, and the table's gradient: scores transposed as in the forward pass.  The gradients of the biases are summed in float32 by
 // relative position (for each half wavefront by itself), those of tiles beyond the reach in the lane.
 // D comes from a rounded output, so that the ds of a row add up to a small e instead of 0; what lies beyond the reach, where most of
-// a long row's probability is, gets its share of -e back.
+// a long row's probability is, gets its share of -e back (here, or, where a row's keys are in parts, from finish_kernel).
 template <typename T, int DC, int NW, bool BIAS>
 __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, AttentionGrads G, int64_t slots, int splits) {
     constexpr int DP = pitch(DC), ND = (DC + 31) / 32;
@@ -1107,7 +1107,12 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
 #pragma unroll
     for (int side = 0; side < 2; side++) {
         const float ds = other_half_sum(far_ds[side]), p = other_half_sum(far_p[side]);
-        const float x = wave_sum(mine && half == 0 ? (splits > 1 ? ds : ds - all_ds * p) : 0.0f);
+        if (G.row_parts && half == 0 && i < q.rows) {
+            float* const at = G.row_parts + ((A.packed ? A.q_rows : A.q_rows * A.batch) * A.heads * z + row) * 3;
+            at[0] = mine ? all_ds : 0.0f;
+            at[1 + side] = mine ? p : 0.0f;
+        }
+        const float x = wave_sum(mine && half == 0 ? (G.row_parts ? ds : ds - all_ds * p) : 0.0f);
         if (lane == 0) far_sums[2 * wave + side] = x;
     }
     __syncthreads();
@@ -1315,6 +1320,10 @@ struct Finish {
     const float* table_parts;
     void* dtable;
     int64_t table_count;              // workgroups' sums for a (head, bucket)
+    const float* row_parts;           // see AttentionGrads; table_splits, rows without heads
+    const int32_t* bucket_of;
+    int64_t rows;
+    int table_splits, reach;
     int buckets, heads, table_float;
 };
 template <typename T>
@@ -1348,6 +1357,20 @@ __global__ __launch_bounds__(256) void finish_kernel(Finish F) {
     const int h = (int)(at / F.buckets), n = (int)(at - (int64_t)h * F.buckets), lane = threadIdx.x & 63;
     double x = 0.0;
     for (int64_t w = lane; w < F.table_count; w += 64) x += F.table_parts[(h * F.table_count + w) * F.buckets + n];
+    if (F.row_parts)
+#pragma unroll
+        for (int side = 0; side < 2; side++) {
+            if (F.bucket_of[side * 2 * F.reach] != n) continue;
+            for (int64_t r = lane; r < F.rows; r += 64) {
+                float ds = 0.0f, p = 0.0f;
+                for (int z = 0; z < F.table_splits; z++) {
+                    const float* const at = F.row_parts + ((z * F.rows + r) * F.heads + h) * 3;
+                    ds += at[0];
+                    p += at[1 + side];
+                }
+                x -= (double)ds * p;
+            }
+        }
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d);
     if (lane) return;
@@ -1422,6 +1445,7 @@ void sequence_attention_backward(const SequenceAttention& A, const AttentionGrad
         G.dk_parts = take(P.k_splits * k_all * A.dim);
         G.dv_parts = take(P.k_splits * k_all * A.dim);
     }
+    if (dtable && P.q_splits > 1) G.row_parts = take(P.q_splits * q_all * 3);
     G.dtable = dtable ? next : nullptr;
     with_padded_dim(A.dim, [&](auto dc) {
         with_choice(A.table != nullptr, [&](auto bias) {
@@ -1455,6 +1479,8 @@ void sequence_attention_backward(const SequenceAttention& A, const AttentionGrad
     if (dtable) {
         F.table_parts = G.dtable; F.dtable = dtable;
         F.table_count = q_all > 0 ? P.q_slots * P.q_splits : 0;
+        F.row_parts = G.row_parts; F.bucket_of = A.bucket_of; F.rows = A.packed ? A.q_rows : A.q_rows * A.batch;
+        F.table_splits = P.q_splits; F.reach = A.reach;
         F.buckets = A.buckets; F.heads = A.heads; F.table_float = A.table_float;
         blocks += ((int64_t)A.heads * A.buckets + 3) / 4;
     }

@@ -37,6 +37,7 @@ struct AttentionGrads {
     void *dq, *dk, *dv;                // (dk, dv over kv_heads)
     float *dq_parts, *dk_parts, *dv_parts;      // of the splits, or NULL
     float* dtable;                     // (workgroups, buckets), or NULL
+    float* row_parts;                  // (splits, rows, heads, 3): sum of ds, of P beyond the reach on either side; NULL: one split
 };
 
 // Tiles of the grid for rows of `tile`: packed sequence b begins at tile starts[b] / tile + b, which leaves every sequence as many as it
@@ -90,14 +91,11 @@ struct AttentionGradPlan {
 inline AttentionGradPlan attention_grad_plan(const SequenceAttention& A) {
     AttentionGradPlan P{};
     const int64_t q_each = A.packed && A.batch > 0 ? A.q_rows / A.batch : A.q_rows, k_each = A.packed && A.batch > 0 ? A.k_rows / A.batch : A.k_rows;
-    // (with a table rather more workgroups of one wavefront than keys in parts: rows whose ds are there as a whole are summed more exactly)
-    const bool table = A.table != nullptr;
-    const int64_t quads = tile_slots(A.packed, A.q_rows, A.batch, 128) * A.heads;
-    P.q_waves = q_each > 64 && (!table || (quads >= 2 * ATTENTION_CUS && queries_lds(A.float32, A.dim, A.reach, true, 4) <= ATTENTION_LDS)) ? 4 : 1;
+    P.q_waves = q_each > 64 && queries_lds(A.float32, A.dim, A.reach, A.table != nullptr, 4) <= ATTENTION_LDS ? 4 : 1;
     P.k_waves = k_each > 64 ? 4 : 1;
     P.q_slots = tile_slots(A.packed, A.q_rows, A.batch, 32 * P.q_waves);
     P.k_slots = tile_slots(A.packed, A.k_rows, A.batch, 32 * P.k_waves);
-    P.q_splits = split_count(P.q_slots * A.heads * P.q_waves, (table ? 2 : 8) * ATTENTION_CUS, k_each, 128);
+    P.q_splits = split_count(P.q_slots * A.heads * P.q_waves, 8 * ATTENTION_CUS, k_each, 128);
     P.k_splits = split_count(P.k_slots * A.kv_heads * P.k_waves, 8 * ATTENTION_CUS, q_each * A.share, 128);
     return P;
 }

@@ -143,7 +143,7 @@ size_t cfh_attention_backward_workspace_bytes(const cfh_attention* a) {
     size_t floats = (size_t)q_all(A) + 32;
     if (P.q_splits > 1) floats += (size_t)P.q_splits * q_all(A) * A.dim;
     if (P.k_splits > 1) floats += 2 * (size_t)P.k_splits * k_all(A) * A.dim;
-    if (A.table) floats += (size_t)P.q_slots * P.q_splits * A.heads * A.buckets;
+    if (A.table) floats += (size_t)P.q_slots * P.q_splits * A.heads * A.buckets + (P.q_splits > 1 ? 3 * (size_t)P.q_splits * q_all(A) : 0);
     return floats * sizeof(float);
 }
 
