@@ -1010,6 +1010,12 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
     D = other_half_sum(D);
     if (z == 0 && half == 0 && i < q.rows) G.rows[row] = D;
     const float off = row_shift(score, m, inverse);
+    // 16 bits without a bias: the accumulators of do . v begin at -D, in registers that stay, a subtraction less for each score
+    // (4 x 4096, 128 channels with ragged keys, all passes: 2698 -> 2676 us)
+    constexpr bool KEPT = !BIAS && sizeof(T) == 2 && DC > 64;
+    f32x16 from_D;
+#pragma unroll
+    for (int r = 0; r < 16; r++) from_D[r] = -D;
     if (first < end) put(first);
     settle<T>(qf);
     settle<T>(gf);
@@ -1030,7 +1036,7 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
             if (sizeof(T) == 2) reads_ahead<DC / 16 * 2, 4, 1>();
         };
 #pragma unroll
-        for (int r = 0; r < 16; r++) dp[r] = 0.0f;
+        for (int r = 0; r < 16; r++) dp[r] = KEPT ? from_D[r] : 0.0f;
         if (near) {
             const float* const at = line + (j0 + 4 * half - i - shift + A.reach + MARGIN);
 #pragma unroll
@@ -1047,7 +1053,7 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
         const float mt = m - flat, offt = off + flat * score.rate;
         if (!BIAS) {
 #pragma unroll
-            for (int r = 0; r < 16; r++) s[r] = probability(score, s[r], mt, inverse, offt) * (dp[r] - D);
+            for (int r = 0; r < 16; r++) s[r] = probability(score, s[r], mt, inverse, offt) * (KEPT ? dp[r] : dp[r] - D);
         } else if (!near) {
             float ds = 0.0f, ps = 0.0f;
 #pragma unroll
