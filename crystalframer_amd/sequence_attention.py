@@ -4,7 +4,7 @@ The encoder's own attention is over the atoms of one crystal (``attention.py``; 
 models/indexed_lattice_multi_head_attention_cuda.py:737-996).  Here queries of one set of sequences read keys and values of another,
 of other lengths (``cross_attention``: a crystal's atoms read by property queries, tokens or the atoms of another structure), or
 sequences attend to themselves with a learned bias by relative position (``relative_attention``: the other attention of a layer that
-reads such states).  Both are one launch forward (two where the keys are split) and two to five backward, for float32, bfloat16
+reads such states).  Both are one launch forward (two where the keys are split) and two or three backward, for float32, bfloat16
 and float16.  Also reachable as ``cuda_funcs.cross_attention``, ``cuda_funcs.relative_attention`` and ``cuda_funcs.position_buckets``.  The
 checks, the library's calls and the autograd function are native (csrc/host_module.cpp).
 """
@@ -49,7 +49,9 @@ def cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     sums are in float32, probabilities and the scores' gradients are rounded to the type before their products.  Any strides; rows
     that do not begin at multiples of 16 bytes, or do not fill them, are laid out again first.  The values of starts and sizes are cut to the rows that are there.
 
-    All gradients are there, with sums in a fixed order; a gradient of a gradient raises."""
+    Float32 products are made of three bfloat16 parts, which hold every finite number; an infinity in them makes a NaN.  All gradients are
+    there, with sums in a fixed order; a gradient of a gradient raises.  The graph keeps the inputs, the output, two numbers for each of its rows and, in 16 bits,
+    what rounding took from the output."""
     return _call(query, key, value, None, None, query_starts, key_starts, query_sizes, key_sizes, key_mask, scale, False, False)
 
 
