@@ -49,9 +49,10 @@ def cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     sums are in float32, probabilities and the scores' gradients are rounded to the type before their products.  Any strides; rows
     that do not begin at multiples of 16 bytes, or do not fill them, are laid out again first.  The values of starts and sizes are cut to the rows that are there.
 
-    Float32 products are made of three bfloat16 parts, which hold every finite number; an infinity in them makes a NaN.  All gradients are
-    there, with sums in a fixed order; a gradient of a gradient raises.  The graph keeps the inputs, the output, two numbers for each of its rows and, in 16 bits,
-    what rounding took from the output."""
+    Float32 products are made of three bfloat16 parts, which hold 24 bits of numbers from 2^-110 to 3.38e38 in size (fewer below); what is
+    beyond, infinities included, makes a NaN.  All gradients are there, with
+    sums in a fixed order; a gradient of a gradient raises.  The graph keeps the inputs, the output, two numbers for each of its rows and,
+    in 16 bits, what rounding took from the output."""
     return _call(query, key, value, None, None, query_starts, key_starts, query_sizes, key_sizes, key_mask, scale, False, False)
 
 
