@@ -70,6 +70,9 @@ inline AttentionPlan attention_plan(const SequenceAttention& A) {
     AttentionPlan P{};
     const int64_t q_each = A.packed && A.batch > 0 ? A.q_rows / A.batch : A.q_rows, k_each = A.packed && A.batch > 0 ? A.k_rows / A.batch : A.k_rows;
     const int64_t whole = tile_slots(A.packed, A.q_rows, A.batch, 128);
+    // few_kernel where its 32 columns hold a sequence's queries, and where tiles_kernel's workgroups of 128 queries would leave compute
+    // units idle (us, few and tiles, workgroups of these: 4 x 512 queries, 2048 keys, 8 heads of 64, 128: 29, 39; 1024 x 1024, 8 heads of 128,
+    // 64: 22, 28, twice that, 128: 29, 29; odd lengths in float32, all passes: 217, 226).
     P.few = q_each * (A.share < 32 ? A.share : 32) <= 32 || whole * A.heads < 192;
     P.splits = 1;
     P.slots = whole;
@@ -77,10 +80,17 @@ inline AttentionPlan attention_plan(const SequenceAttention& A) {
     if (!P.few) return P;
     const int at_once = A.share < 32 ? A.share : 32, groups = (A.share + at_once - 1) / at_once;
     P.slots = tile_slots(A.packed, A.q_rows, A.batch, 32 / at_once);
-    P.waves = k_each <= 64 ? 1 : few_waves(A.float32, A.dim);
+    // One wavefront where there are no keys for more (256 x 16 queries, up to 60 keys, all passes: 56 us, with four 83); but biases of a call that
+    // leaves compute units idle are brought by all of them (37 tokens with a bias: 7.7 us, with one wavefront 10.7).
+    const bool idle = P.slots * A.kv_heads * groups <= ATTENTION_CUS;
+    P.waves = k_each <= 64 && !(A.table && idle) ? 1 : few_waves(A.float32, A.dim);
     const int64_t keys = A.packed ? A.k_rows : A.k_rows * A.batch;
-    P.past = q_each * at_once <= 32 && groups == 1 && keys * A.kv_heads * A.dim * (A.float32 ? 8 : 4) >= 1 << 27;
-    P.splits = split_count(P.slots * A.kv_heads * groups * P.waves, 32 * ATTENTION_CUS, k_each, 64 * P.waves);
+    // One tile of queries for each key head reads keys and values once: bytes, which many wavefronts bring fastest (16 x 1 to 8192 keys of
+    // 16 heads of 64: 80 us undivided, 71 with 32 wavefronts for each compute unit).  Several tiles read them from the caches: no more parts
+    // than fill the SIMDs, since a part costs its sums' way through memory (4 x 512 queries, 2048 keys, 8 heads of 64: 29 us, four parts 40).
+    const bool once = q_each * at_once <= 32 && groups == 1;
+    P.past = once && keys * A.kv_heads * A.dim * (A.float32 ? 8 : 4) >= 1 << 27;
+    P.splits = split_count(P.slots * A.kv_heads * groups * P.waves, (once ? 32 : 4) * ATTENTION_CUS, k_each, 64 * P.waves);
     return P;
 }
 
@@ -95,6 +105,7 @@ inline AttentionGradPlan attention_grad_plan(const SequenceAttention& A) {
     P.k_waves = k_each > 64 ? 4 : 1;
     P.q_slots = tile_slots(A.packed, A.q_rows, A.batch, 32 * P.q_waves);
     P.k_slots = tile_slots(A.packed, A.k_rows, A.batch, 32 * P.k_waves);
+    // (parts: odd lengths, 5 heads on 1 of 40 in float32, all passes 217 us, without 599; 6 heads on 3 of 80 in float16 62 and 81)
     P.q_splits = split_count(P.q_slots * A.heads * P.q_waves, 8 * ATTENTION_CUS, k_each, 128);
     P.k_splits = split_count(P.k_slots * A.kv_heads * P.k_waves, 8 * ATTENTION_CUS, q_each * A.share, 128);
     return P;
