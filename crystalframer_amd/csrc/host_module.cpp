@@ -655,7 +655,13 @@ at::Tensor aligned_rows(const at::Tensor& t) {
     for (int64_t d = 0; d + 1 < n; d++)
         if (t.size(d) > 1) all |= (uint64_t)(t.stride(d) * size);
     const bool near = t.size(n - 3) <= 1 || t.stride(n - 3) * size < 1 << 24;
-    if (D * size % 16) return at::constant_pad_nd(t, {0, (16 - D * size % 16) / size});
+    if (D * size % 16) {      // (at::constant_pad_nd would keep the order of t's dimensions in memory)
+        std::vector<int64_t> filled = t.sizes().vec();
+        filled.back() += (16 - D * size % 16) / size;
+        const at::Tensor y = at::zeros(filled, t.options().memory_format(at::MemoryFormat::Contiguous));
+        y.narrow(-1, 0, D).copy_(t);
+        return y;
+    }
     return (D == 1 || t.stride(-1) == 1) && !(all & 15) && near ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 // Strides of (batch, row, head); of a dimension that has one entry, 0.
