@@ -648,13 +648,14 @@ void check_attention(const AttentionTensors& t, const AttentionSpec& s) {
     TORCH_CHECK_VALUE(s.scale == 0.0 || (s.scale > 0.0 && std::isfinite((float)s.scale) && (float)s.scale > 0.0f), "scale ", s.scale, " must be positive and finite");
 }
 
-// t as the library reads it: rows of neighbouring channels that begin at multiples of 16 bytes and fill them; others are laid out again.
+// t as the library reads it: rows of neighbouring channels that begin at multiples of 16 bytes and fill them, and lie apart from one
+// another (not one row for all positions); others are laid out again.
 at::Tensor aligned_rows(const at::Tensor& t) {
     const int64_t size = (int64_t)t.element_size(), D = t.size(-1), n = t.dim();
     uint64_t all = (uint64_t)reinterpret_cast<uintptr_t>(t.data_ptr());
     for (int64_t d = 0; d + 1 < n; d++)
         if (t.size(d) > 1) all |= (uint64_t)(t.stride(d) * size);
-    const bool near = t.size(n - 3) <= 1 || t.stride(n - 3) * size < 1 << 24;
+    const bool fit = t.size(n - 3) <= 1 || (t.stride(n - 3) >= D && t.stride(n - 3) * size < 1 << 24);
     if (D * size % 16) {      // (at::constant_pad_nd would keep the order of t's dimensions in memory)
         std::vector<int64_t> filled = t.sizes().vec();
         filled.back() += (16 - D * size % 16) / size;
@@ -662,7 +663,7 @@ at::Tensor aligned_rows(const at::Tensor& t) {
         y.narrow(-1, 0, D).copy_(t);
         return y;
     }
-    return (D == 1 || t.stride(-1) == 1) && !(all & 15) && near ? t : t.clone(at::MemoryFormat::Contiguous);
+    return (D == 1 || t.stride(-1) == 1) && !(all & 15) && fit ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 // Strides of (batch, row, head); of a dimension that has one entry, 0.
 void strides_of(const at::Tensor& t, int64_t* out) {

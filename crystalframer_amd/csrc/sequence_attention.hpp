@@ -171,8 +171,8 @@ struct Tile {
 };
 
 // ---- rows in memory ------------------------------------------------------------------------------------------------------------------
-// Rows lie at multiples of 16 bytes and are read as pieces of a buffer that ends behind the last row that is there: what is beyond
-// comes back as 0, without a branch.  (A last piece that the row's channels do not fill is filled with zeros in memory.)
+// Rows lie at multiples of 16 bytes, apart from one another, and are read as pieces of a buffer that ends behind the last row that is
+// there: what is beyond comes back as 0, without a branch.  (A last piece that the row's channels do not fill is filled with zeros in memory.)
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr int BEYOND = 0x40000000;      // behind any buffer here
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* at, int bytes) {

@@ -67,11 +67,16 @@ int check_attention(const cfh_attention* a) {
     return CFH_OK;
 }
 
+// A single row needs no stride to the next; the kernels need one, so that what they read behind it lies behind its buffer's end, too.
+cfh::AttentionRows device_rows(const cfh_attention* a, const void* at, const int64_t* stride, int64_t rows) {
+    const int each = a->dtype == CFH_FLOAT32 ? 4 : 8;
+    return {at, stride[0], rows > 1 ? stride[1] : (a->dim + each - 1) / each * each, stride[2]};
+}
 cfh::SequenceAttention device_args(const cfh_attention* a) {
     cfh::SequenceAttention A{};
-    A.q = {a->q, a->q_stride[0], a->q_stride[1], a->q_stride[2]};
-    A.k = {a->k, a->k_stride[0], a->k_stride[1], a->k_stride[2]};
-    A.v = {a->v, a->v_stride[0], a->v_stride[1], a->v_stride[2]};
+    A.q = device_rows(a, a->q, a->q_stride, a->query_rows);
+    A.k = device_rows(a, a->k, a->k_stride, a->key_rows);
+    A.v = device_rows(a, a->v, a->v_stride, a->key_rows);
     A.mask = a->key_mask;
     A.q_starts = a->query_starts; A.k_starts = a->key_starts; A.q_sizes = a->query_sizes; A.k_sizes = a->key_sizes;
     A.table = a->table; A.bucket_of = a->bucket_of;
@@ -163,7 +168,7 @@ int cfh_attention_backward(const cfh_attention* a, const void* out, const void* 
     if ((rc = check_grids(A, true))) return rc;
     if ((rc = check_workspace(workspace, workspace_bytes, cfh_attention_backward_workspace_bytes(a)))) return rc;
     cfh::AttentionGrads G{};
-    G.go = {gout, gs[0], gs[1], gs[2]};
+    G.go = device_rows(a, gout, gs, a->query_rows);
     G.out = out; G.rest = out_rest; G.stats = stats; G.dq = dq; G.dk = dk; G.dv = dv;
     with_type(a->dtype, [&](auto t) {
         cfh::sequence_attention_backward<decltype(t)>(A, cfh::attention_grad_plan(A), G, dtable, (float*)workspace, (hipStream_t)stream);

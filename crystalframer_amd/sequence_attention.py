@@ -47,7 +47,8 @@ def cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     The heads may be a multiple of the key heads: head h reads key head h // (heads // key heads).  1 to 128 channels of a head;
     ``scale``: one over their root.  One type, float32, bfloat16 or float16, for all and for the result; sums, maxima and the gradients'
     sums are in float32, probabilities and the scores' gradients are rounded to the type before their products.  Any strides; rows
-    that do not begin at multiples of 16 bytes, or do not fill them, are laid out again first.  The values of starts and sizes are cut to the rows that are there.
+    that do not begin at multiples of 16 bytes, do not fill them, or share their memory (one row expanded over positions) are laid out
+    again first.  The values of starts and sizes are cut to the rows that are there.
 
     Float32 products are made of three bfloat16 parts, which hold 24 bits of numbers from 2^-110 to 3.38e38 in size (fewer below); what is
     beyond, infinities included, makes a NaN.  All gradients are there, with

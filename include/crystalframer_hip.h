@@ -788,8 +788,9 @@ int cfh_model_backward(const cfh_model* m, const cfh_model_batch* b, const float
  * Values of these arrays are cut to what is there; an entry of bucket_of outside 0 ... buckets - 1 means no bias, finite entries of table
  * beyond +-65536 count as that.
  * Strides are in elements; channels lie next to one another.  Rows of q, k, v and gout begin at multiples of 16 bytes, less than 2^24 bytes
- * apart, and where dim channels do not fill their last 16 bytes, these are filled with zeros.  out and gradients are contiguous: (rows,
- * heads or kv_heads, dim).
+ * apart, and where dim channels do not fill their last 16 bytes, these are filled with zeros.  Rows that share memory (a row stride of less
+ * than a row's bytes, 0 among them) have to be finite; that of a single row may be 0.  out and gradients are contiguous: (rows, heads or
+ * kv_heads, dim).
  */
 #define CFH_ATTENTION_MAX_DIM 128
 #define CFH_ATTENTION_MAX_REACH 1024
