@@ -441,6 +441,13 @@ __device__ __forceinline__ void fill_line(const SequenceAttention& A, int head, 
         line[n] = table_entry<T>(A, clamped(n - A.reach - MARGIN, A.reach), head) * by;
 }
 
+// A bias that is the same for a whole tile goes into the maximum, unless it is plus infinity or NaN: it would reach the keys of the tile
+// that are not there, or that a row does not see, so that the scores begin with it as with a near one, and these keys' are dropped.
+__device__ __forceinline__ bool far_in_scores(float far) { return !(far < -NONE); }
+__device__ __forceinline__ bool any_far_in_scores(const float* line, int reach) {
+    return __any(far_in_scores(line[0]) || far_in_scores(line[2 * (reach + MARGIN)]));
+}
+
 __device__ __forceinline__ float other_half_max(float x) { float a, b; swap32(x, a, b); return fmaxf(a, b); }
 __device__ __forceinline__ float other_half_sum(float x) { float a, b; swap32(x, a, b); return a + b; }
 
@@ -500,16 +507,19 @@ struct Scaled {
     __device__ __forceinline__ float back() const { return NARROW<T> ? 1.0f / by : 1.0f; }
 };
 
-// Without the keys (rows) that are not there: `there` holds 0 for one that is and minus infinity for others, in LDS.
-__device__ __forceinline__ void drop_keys(f32x16& s, uint32_t there, int lane) {
+// Without the keys (rows) that are not there: `gone` holds 0 for one that is and all bits for others, in LDS.  (One instruction for a
+// score, as an addition of minus infinity would be; but that leaves a bias of plus infinity or NaN a NaN.)
+__device__ __forceinline__ void drop_keys(f32x16& s, uint32_t gone, int lane) {
+    uint32_t none = __float_as_uint(NONE);
+    asm("" : "+s"(none));                  // (with a known number the choice of bits becomes two instructions)
 #pragma unroll
     for (int r = 0; r < 16; r += 4) {
-        const f32x4 x = lds_read<f32x4>(there + (result_row(r) + 4 * (lane >> 5)) * 4);
+        const u32x4 x = lds_read<u32x4>(gone + (result_row(r) + 4 * (lane >> 5)) * 4);
 #pragma unroll
-        for (int e = 0; e < 4; e++) s[r + e] += x[e];
+        for (int e = 0; e < 4; e++) s[r + e] = __uint_as_float((x[e] & none) | (~x[e] & __float_as_uint(s[r + e])));
     }
 }
-// Without the keys behind number `last` of the tile.
+// Without the rows behind number `last` of the tile.
 __device__ __forceinline__ void drop_behind(f32x16& s, int last, int lane) {
     const int mine = last - (lane >> 5) * 4;
 #pragma unroll
@@ -523,8 +533,8 @@ __device__ __forceinline__ void drop_before(f32x16& s, int first, int lane) {
 }
 // Writes what drop_keys() reads, for COUNT keys.
 template <int COUNT>
-__device__ __forceinline__ void put_keys(float* at, uint64_t bits, int thread) {
-    if (thread < COUNT) at[thread] = bits >> thread & 1 ? 0.0f : NONE;
+__device__ __forceinline__ void put_keys(uint32_t* at, uint64_t bits, int thread) {
+    if (thread < COUNT) at[thread] = bits >> thread & 1 ? 0u : ~0u;
 }
 template <int COUNT>
 __device__ __forceinline__ bool all_there(uint64_t bits) { return COUNT == 64 ? bits == ~0ull : (uint32_t)bits == ~0u; }
@@ -542,7 +552,8 @@ struct FewLds {
     static constexpr int TILE = Tile<T, DP>::bytes(32), SUM = 32 * (DP + 4) * 4;
     static constexpr int EACH = 2 * TILE > SUM ? 2 * TILE : SUM;
     alignas(512) char wave[NW][(EACH + 511) / 512 * 512];
-    float m[NW][32], l[NW][32], there[NW][32];
+    float m[NW][32], l[NW][32];
+    uint32_t gone[NW][32];
 };
 
 template <typename T, int DC, int NW, bool BIAS, bool PAST>
@@ -616,7 +627,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && NW == 4 ? 2 : 1)) void 
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         const uint32_t there = (uint32_t)bits.get(mask);
         const uint64_t rows = mask ? there | ~0xffffffffull : ~0ull;      // (rows behind the last are 0 already)
-        if (!all_there<32>(there)) put_keys<32>(S.there[wave], there, lane);
+        if (!all_there<32>(there)) put_keys<32>(S.gone[wave], there, lane);
         kx.store(kt, lane, rows);
         vx.store(vt, lane, rows);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -634,13 +645,13 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && NW == 4 ? 2 : 1)) void 
             for (int r = 0; r < 16; r++) s[r] = mine ? table_entry<T>(A, clamped(r0 + result_row(r), A.reach), h) * by : 0.0f;
         } else {
 #pragma unroll
-            for (int r = 0; r < 16; r++) s[r] = 0.0f;
+            for (int r = 0; r < 16; r++) s[r] = BIAS && far_in_scores(far[low >= A.reach]) ? far[low >= A.reach] : 0.0f;
         }
 #pragma unroll
         for (int c = 0; c < DC / 16; c++) s = Operand<T>::product(L::template rows<KEYS>(kr, 0, c), qf[c], s);
-        if (!all_there<32>(there)) drop_keys(s, lds_address(S.there[wave]), lane);
+        if (!all_there<32>(there)) drop_keys(s, lds_address(S.gone[wave]), lane);
         if (A.causal && high > 0) drop_behind(s, i + shift - j0, lane);
-        const float flat = BIAS && !near ? low >= A.reach ? far[1] : far[0] : 0.0f;
+        const float flat = BIAS && !near && !far_in_scores(far[low >= A.reach]) ? far[low >= A.reach] : 0.0f;
         float top = s[0];
 #pragma unroll
         for (int r = 1; r < 16; r++) top = fmaxf(top, s[r]);
@@ -766,8 +777,8 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 ? 2 : 1)) void tiles_kerne
     constexpr int KEYS = keys_at_once<T, NW>(), TILE = L::bytes(KEYS);
     extern __shared__ __attribute__((aligned(512))) char lds[];
     char* const tiles = lds;                    // two pairs of a tile of keys and one of values
-    float* const keys = reinterpret_cast<float*>(lds + 4 * TILE);       // which are there: two times KEYS
-    float* const line = keys + 2 * KEYS;
+    uint32_t* const keys = reinterpret_cast<uint32_t*>(lds + 4 * TILE);      // which are not there: two times KEYS
+    float* const line = reinterpret_cast<float*>(keys + 2 * KEYS);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, column = lane & 31;
     int h;
     int64_t slot;
@@ -815,6 +826,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 ? 2 : 1)) void tiles_kerne
     if (count > 0) put(0);
     settle<T>(qf);
     __syncthreads();
+    const bool odd = BIAS && any_far_in_scores(line, A.reach);
     for (int n = 0; n < count; n++) {
         const uint32_t tile = lds_address(tiles) + (n & 1) * 2 * TILE, kr = tile + L::rows_at(lane), vc = tile + TILE + L::columns_at(lane);
         if (n + 1 < count) fetch(n + 1);
@@ -828,8 +840,9 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 ? 2 : 1)) void tiles_kerne
                 for (int u = 0; u < KEYS / 32; u++) s[u] = Operand<T>::product(L::template rows<KEYS>(kr, 32 * u, c), qf[c], s[u]);
             if (sizeof(T) == 2) reads_ahead<DC / 16 * KEYS / 32, 4, 1>();
         };
-        if (near) {
-            const float* const at = line + (j0 + 4 * half - i - shift + A.reach + MARGIN);
+        const bool side = low >= A.reach, begin = near || (odd && far_in_scores(line[side ? 2 * (A.reach + MARGIN) : 0]));
+        if (begin) {
+            const float* const at = line + (near ? j0 + 4 * half - i - shift + A.reach + MARGIN : side ? 2 * A.reach + MARGIN : 0);
 #pragma unroll
             for (int u = 0; u < KEYS / 32; u++)
 #pragma unroll
@@ -842,7 +855,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 ? 2 : 1)) void tiles_kerne
                 for (int r = 0; r < 16; r++) s[u][r] = 0.0f;
             products();
         }
-        const float flat = BIAS && !near ? line[low >= A.reach ? 2 * (A.reach + MARGIN) : 0] : 0.0f;
+        const float flat = BIAS && !begin ? line[side ? 2 * (A.reach + MARGIN) : 0] : 0.0f;
         if (!all_there<KEYS>(there))
 #pragma unroll
             for (int u = 0; u < KEYS / 32; u++) drop_keys(s[u], lds_address(keys + (n & 1) * KEYS + 32 * u), lane);
@@ -937,8 +950,8 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
     constexpr int KEYS = 32, TILE = L::bytes(KEYS);
     extern __shared__ __attribute__((aligned(512))) char lds[];
     char* const tiles = lds;
-    float* const keys = reinterpret_cast<float*>(lds + 4 * TILE);       // which are there: two times KEYS
-    float* const line = keys + 2 * KEYS;
+    uint32_t* const keys = reinterpret_cast<uint32_t*>(lds + 4 * TILE);      // which are not there: two times KEYS
+    float* const line = reinterpret_cast<float*>(keys + 2 * KEYS);
     const int entries = 2 * (A.reach + MARGIN) + 1;
     float* const sums = line + entries;                         // (2 NW, entries), then two for each wavefront
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, column = lane & 31;
@@ -1032,6 +1045,7 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
     settle<T>(gf);
     asm volatile("" : "+v"(m), "+v"(inverse));
     __syncthreads();
+    const bool odd = BIAS && any_far_in_scores(line, A.reach);
     for (int n = first; n < end; n++) {
         const uint32_t tile = lds_address(tiles) + (n & 1) * 2 * TILE, kr = tile + L::rows_at(lane), vr = kr + TILE, kc = tile + L::columns_at(lane);
         if (n + 1 < end) fetch(n + 1);
@@ -1054,8 +1068,9 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
         };
 #pragma unroll
         for (int r = 0; r < 16; r++) dp[r] = KEPT ? from_D[r] : 0.0f;
-        if (near) {
-            const float* const at = line + (j0 + 4 * half - i - shift + A.reach + MARGIN);
+        const bool side = low >= A.reach, begin = near || (odd && far_in_scores(line[side ? 2 * (A.reach + MARGIN) : 0]));
+        if (begin) {
+            const float* const at = line + (near ? j0 + 4 * half - i - shift + A.reach + MARGIN : side ? 2 * A.reach + MARGIN : 0);
 #pragma unroll
             for (int r = 0; r < 16; r++) s[r] = at[result_row(r)];
             products();
@@ -1064,7 +1079,7 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
             for (int r = 0; r < 16; r++) s[r] = 0.0f;
             products();
         }
-        const float flat = BIAS && !near ? line[low >= A.reach ? 2 * (A.reach + MARGIN) : 0] : 0.0f;
+        const float flat = BIAS && !begin ? line[side ? 2 * (A.reach + MARGIN) : 0] : 0.0f;
         if (!all_there<KEYS>(there)) drop_keys(s, lds_address(keys + (n & 1) * KEYS), lane);
         if (A.causal && high > 0) drop_behind(s, i + shift - j0, lane);
         const float mt = m - flat, offt = off + flat * score.rate;
@@ -1080,7 +1095,6 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
                 ds += s[r];
                 ps += p;
             }
-            const int side = low >= A.reach;
             far_ds[0] += side ? 0.0f : ds; far_p[0] += side ? 0.0f : ps;
             far_ds[1] += side ? ds : 0.0f; far_p[1] += side ? ps : 0.0f;
             all_ds += ds;
@@ -1090,6 +1104,9 @@ __global__ __launch_bounds__(NW * 64) void queries_kernel(SequenceAttention A, A
                 s[r] = probability(score, s[r], mt, inverse, offt) * (dp[r] - D);
                 all_ds += s[r];
             }
+            if (i0 + 32 > q.there)      // (rows that are not there meet biases that no row may have)
+#pragma unroll
+                for (int r = 0; r < 16; r++) s[r] = mine ? s[r] : 0.0f;
             float x[3] = {0.0f, 0.0f, 0.0f};
             add_diagonals(s, x, std::make_integer_sequence<int, 16>());
             float* const at = own_sums + (j0 - i0 - shift + 4 * half - (lane & 31) + A.reach + MARGIN);
@@ -1295,6 +1312,7 @@ __global__ __launch_bounds__(NW * 64, (NW == 4 && values_in_lds<T, DC>() ? 2 : 1
         }
         if constexpr (sizeof(T) == 4) dp += small;
         if (A.causal && high > 0) drop_before(s, j - shift - i0, lane);
+        if (BIAS && i0 + ROWS > q.there) drop_behind(s, q.there - 1 - i0, lane);      // (their biases may be plus infinity or NaN)
         f32x16 p;
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {

@@ -68,8 +68,9 @@ def relative_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tens
 
     ``table`` (number of buckets, heads), of query's type or float32, gets a gradient.  ``buckets`` (2 reach + 1, int32): the bucket of
     each relative position from -reach to reach (``position_buckets`` makes one; positions beyond count as -reach and reach, reach up to
-    1024; a number that is no row of ``table`` means no bias).  Entries of ``table`` beyond 65536 either way count as that; minus infinity
-    takes a bucket's keys away.  shift: 0, or with ``queries_last`` how many more keys than queries the
+    1024; a number that is no row of ``table`` means no bias).  Finite entries of ``table`` beyond 65536 either way count as that; minus
+    infinity takes a bucket's keys away, plus infinity and NaN make NaN of the rows that see such a key, and of no others.
+    shift: 0, or with ``queries_last`` how many more keys than queries the
     sequence has (single tokens behind a cache, whose ``key_sizes`` include them).  ``causal``: keys j <= i + shift only.
 
     The table's gradient from 16-bit tensors is as exact as the products of these are, in float32 as well."""

@@ -786,7 +786,7 @@ int cfh_model_backward(const cfh_model* m, const cfh_model_batch* b, const float
  *   behind the last are 0 in every result; query_rows, key_rows are those of all sequences.
  * packed = 0: (batch, query_rows) and (batch, key_rows); query_sizes, key_sizes (batch, int64, or NULL: whole rows).
  * Values of these arrays are cut to what is there; an entry of bucket_of outside 0 ... buckets - 1 means no bias, finite entries of table
- * beyond +-65536 count as that.
+ * beyond +-65536 count as that.  Minus infinity takes its keys away; plus infinity and NaN make NaN of the rows that see such a key only.
  * Strides are in elements; channels lie next to one another.  Rows of q, k, v and gout begin at multiples of 16 bytes, less than 2^24 bytes
  * apart, and where dim channels do not fill their last 16 bytes, these are filled with zeros.  Rows that share memory (a row stride of less
  * than a row's bytes, 0 among them) have to be finite; that of a single row may be 0.  out and gradients are contiguous: (rows, heads or
