@@ -403,7 +403,12 @@ template <typename T>
 __device__ __forceinline__ const T* row_start(const AttentionRows& r, const Span& s, int packed, int head) {
     return static_cast<const T*>(r.at) + (packed ? s.first * r.row : s.batch * r.batch) + head * r.head;
 }
-__device__ __forceinline__ int shift_of(const SequenceAttention& A, const Span& q, const Span& k) { return A.last ? k.there - q.there : 0; }
+// What to add to a query's position for the key's that is its own.  Causal: keys behind the last query's are seen by none, and not there.
+__device__ __forceinline__ int shift_of(const SequenceAttention& A, const Span& q, Span& k) {
+    const int shift = A.last ? k.there - q.there : 0;
+    if (A.causal) k.there = max(0, min(k.there, q.there + shift));
+    return shift;
+}
 
 // ---- scores ----------------------------------------------------------------------------------------------------------------------------
 // A score t is what the product sums up to, q . k + bias / scale, and exp2((t - m) rate) its power.  The bias costs no instruction of its
@@ -1200,14 +1205,14 @@ __global__ __launch_bounds__(NW * 64, (NW == 4 && values_in_lds<T, DC>() ? 2 : 1
     const int z = blockIdx.y;
     int b, from;
     if (!find_slot(A.k_starts, A.k_rows, A.packed, A.batch, NW * 32, slot, lane, b, from)) return;
-    const Span k = span_of(A.k_starts, A.k_sizes, A.k_rows, A.packed, A.batch, b);
+    Span k = span_of(A.k_starts, A.k_sizes, A.k_rows, A.packed, A.batch, b);
     if (from >= k.rows) return;
     Span q{0, 0, 0, 0};
     if (!A.packed || b < A.batch) q = span_of(A.q_starts, A.q_sizes, A.q_rows, A.packed, A.batch, b);
     const int j0 = from + wave * 32, j = j0 + column;
+    const int shift = shift_of(A, q, k);
     const bool inside = j < k.there;
     const bool mine = inside && (!A.mask || A.mask[k.first + j]);
-    const int shift = shift_of(A, q, k);
     const Score<T> score(A.scale);
     // the first tile of queries that sees a key of this workgroup
     int skip = 0;

@@ -71,7 +71,8 @@ def relative_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tens
     1024; a number that is no row of ``table`` means no bias).  Finite entries of ``table`` beyond 65536 either way count as that; minus
     infinity takes a bucket's keys away, plus infinity and NaN make NaN of the rows that see such a key, and of no others.
     shift: 0, or with ``queries_last`` how many more keys than queries the
-    sequence has (single tokens behind a cache, whose ``key_sizes`` include them).  ``causal``: keys j <= i + shift only.
+    sequence has (single tokens behind a cache, whose ``key_sizes`` include them).  ``causal``: keys j <= i + shift only; one that no query
+    of the sequence sees is not there, one that some see has to be finite for the others' sake (it is 0 times in their sums).
 
     The table's gradient from 16-bit tensors is as exact as the products of these are, in float32 as well."""
     if table is None or buckets is None:

@@ -780,7 +780,8 @@ int cfh_model_backward(const cfh_model* m, const cfh_model_batch* b, const float
  *
  * over the keys j of the query's own sequence which key_mask keeps and, with causal, j <= i + shift; shift = keys - queries of the
  * sequence with queries_last, else 0; relative positions beyond +-reach count as +-reach.  Head h has key head h / (heads / kv_heads).
- * A row without keys is 0.  In place of a key that is not there, anything may be in memory, NaN included.
+ * A row without keys is 0.  In place of a key that is not there, or with causal seen by no query, anything may be in memory, NaN included;
+ * a key that some queries see has to be finite for the others' sake.
  *
  * packed = 1: the sequences lie behind one another, query_starts and key_starts (batch + 1, int64, beginning with 0) say where, rows
  *   behind the last are 0 in every result; query_rows, key_rows are those of all sequences.
