@@ -565,7 +565,9 @@ template <typename T, int DC, int NW, bool BIAS, bool PAST>
 __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && NW == 4 ? 2 : 1)) void few_kernel(SequenceAttention A, T* out, T* rest, float* stats, float* part_o, float* part_ml, int splits) {
     constexpr int DP = pitch(DC), ND = (DC + 31) / 32, KEYS = 32;
     using L = Tile<T, DP>;
-    __shared__ __attribute__((aligned(16))) FewLds<T, DP, NW> S;
+    __shared__ FewLds<T, DP, NW> S;
+    // (an aligned attribute of the variable's own would take the place of the type's)
+    static_assert(__alignof__(S) % L::ROW == 0 && sizeof(S.wave[0]) % L::ROW == 0 && L::bytes(32) % L::ROW == 0, "tiles begin at multiples of their rows' length");
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int at_once = heads_at_once(A.share), groups = (A.share + at_once - 1) / at_once, tile = 32 / at_once;
     int b, i0;
