@@ -730,7 +730,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && NW == 4 ? 2 : 1)) void 
 }
 
 // Joins the splits: 8 rows to a workgroup, 32 lanes to a row.  The lanes look at a part's statistics each, and then all at its sums.
-template <typename T, int DC, bool BIAS>
+template <typename T, int DC>
 __global__ __launch_bounds__(256) void combine_parts(SequenceAttention A, const float* part_o, const float* part_ml, int splits, int64_t rows, T* out,
                                                      T* rest, float* stats) {
     constexpr int DP = pitch(DC);
@@ -774,14 +774,14 @@ __global__ __launch_bounds__(256) void combine_parts(SequenceAttention A, const 
 }
 
 // ---- many queries: tiles of keys shared by the wavefronts of a workgroup ------------------------------------------------------------------
-template <typename T, int NW>
-constexpr int keys_at_once() { return sizeof(T) == 2 && NW >= 4 ? 64 : 32; }
+template <typename T>
+constexpr int keys_at_once() { return sizeof(T) == 2 ? 64 : 32; }
 
 template <typename T, int DC, int NW, bool BIAS>
 __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 ? 2 : 1)) void tiles_kernel(SequenceAttention A, T* out, T* rest, float* stats, int64_t slots) {
     constexpr int DP = pitch(DC), ND = (DC + 31) / 32;
     using L = Tile<T, DP>;
-    constexpr int KEYS = keys_at_once<T, NW>(), TILE = L::bytes(KEYS);
+    constexpr int KEYS = keys_at_once<T>(), TILE = L::bytes(KEYS);
     extern __shared__ __attribute__((aligned(512))) char lds[];
     char* const tiles = lds;                    // two pairs of a tile of keys and one of values
     uint32_t* const keys = reinterpret_cast<uint32_t*>(lds + 4 * TILE);      // which are not there: two times KEYS
@@ -1463,7 +1463,7 @@ void sequence_attention_forward(const SequenceAttention& A, const AttentionPlan&
             constexpr bool BIAS = decltype(bias)::value;
             const int64_t rows = (A.packed ? A.q_rows : A.q_rows * A.batch) * A.heads;
             if (!P.few) {
-                const size_t lds = 4 * Tile<T, DP>::bytes(keys_at_once<T, 4>()) + 2 * keys_at_once<T, 4>() * sizeof(float) + (BIAS ? (2 * (A.reach + MARGIN) + 1) * sizeof(float) : 0);
+                const size_t lds = 4 * Tile<T, DP>::bytes(keys_at_once<T>()) + 2 * keys_at_once<T>() * sizeof(float) + (BIAS ? (2 * (A.reach + MARGIN) + 1) * sizeof(float) : 0);
                 launch_attention(tiles_kernel<T, DC, 4, BIAS>, dim3(die_grid((int64_t)P.slots * A.heads)), 256, lds, st, A, out, rest, stats, P.slots);
                 return;
             }
@@ -1478,7 +1478,7 @@ void sequence_attention_forward(const SequenceAttention& A, const AttentionPlan&
                                  part_o, part_ml, P.splits);
             });
             if (P.splits > 1)
-                launch_attention(combine_parts<T, DC, BIAS>, dim3((unsigned)((rows + 7) / 8)), 256, 0, st, A, part_o, part_ml, P.splits, rows, out, rest, stats);
+                launch_attention(combine_parts<T, DC>, dim3((unsigned)((rows + 7) / 8)), 256, 0, st, A, part_o, part_ml, P.splits, rows, out, rest, stats);
         });
     });
 }
