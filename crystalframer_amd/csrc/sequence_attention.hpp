@@ -548,8 +548,7 @@ __device__ __forceinline__ bool all_there(uint64_t bits) { return COUNT == 64 ? 
 // 32 columns are (query, head of one key head): single tokens of shared heads fill them together.  Every wavefront goes through keys of
 // its own, in tiles of 32 that it alone puts into LDS and reads (no barrier in the loop), and the wavefronts' sums are joined at the end;
 // so are, by combine_parts, those of `splits` workgroups.  Bound by the bytes of keys and values for single tokens; PAST: these go past the
-// caches, where one workgroup reads them and they are more than the last cache keeps (0.5 GB: 129 -> 119 us; 240 MB that no call before had
-// read: 77 -> 73, that one just had: 64 -> 70).
+// caches (see attention_plan).
 __device__ __forceinline__ int heads_at_once(int share) { return share < 32 ? share : 32; }
 
 template <typename T, int DP, int NW>

@@ -51,16 +51,19 @@ inline int split_count(int64_t wavefronts, int64_t wanted, int64_t rows, int64_t
     return (int)(n < 1 || most < 1 ? 1 : n > most ? most : n);
 }
 
-// Wavefronts of few_kernel and of the backward kernels: what the 160 KB of LDS hold.
+// Wavefronts of few_kernel: as many as the 160 KB of LDS hold tiles for (a power of two; float32 of 128 channels: 48 KB each).
 constexpr int few_waves(bool float32, int dim) { return float32 && dim > 64 ? 2 : 4; }
 inline int64_t queries_lds(bool float32, int dim, int reach, bool table, int waves) {
     const int64_t pitch = dim <= 32 ? 32 : dim <= 64 ? 64 : 128, entries = 2 * (reach + ATTENTION_MARGIN) + 1;
     return 4 * 32 * pitch * (float32 ? 6 : 2) + 64 * 4 + (table ? (entries * (2 * waves + 1) + 2 * waves) * 4 : 0);
 }
 
-// Whether few_kernel keeps the biases of its heads in LDS (up to 8 KB); otherwise it reads what tiles within the reach take.
+// Whether few_kernel keeps the biases of its heads in LDS (up to 8 KB); otherwise it reads what tiles within the reach take.  (us, read and
+// kept: 6 x 500 tokens, 5 heads of 40 in float32, reach 77, 7 KB: 57, 50; 4 x 200, 8 heads of 64 in 16 bits, reach 128, 2 KB: 19.6, 17.8; but
+// single tokens of 64 heads on 8 of 128 to 4096 positions, 14 KB, where fewer workgroups have room: 70, 94.)
 __host__ __device__ inline bool few_line(int heads, int reach) { return heads * (2 * (reach + ATTENTION_MARGIN) + 1) <= 2048; }
 
+// (Times at the rules: us a pass, those of wavefronts, parts, lines and caches replayed from captured graphs, some 8 us with each replay.)
 struct AttentionPlan {
     bool few, past;        // few_kernel, and keys and values past the caches
     int waves, splits;
@@ -88,6 +91,12 @@ inline AttentionPlan attention_plan(const SequenceAttention& A) {
     // One tile of queries for each key head reads keys and values once: bytes, which many wavefronts bring fastest (16 x 1 to 8192 keys of
     // 16 heads of 64: 80 us undivided, 71 with 32 wavefronts for each compute unit).  Several tiles read them from the caches: no more parts
     // than fill the SIMDs, since a part costs its sums' way through memory (4 x 512 queries, 2048 keys, 8 heads of 64: 29 us, four parts 40).
+    // A wavefront has two tiles of a part at least (us with a half, one, two, four, eight: one token to 2000 keys, 8 heads of 64: 20, 18, 17, 19, 27;
+    // 4 to 4000, 32 heads on 8 of 128: 49, 39, 30, 29, 35).
+    // Such keys and values go past the caches from 128 MB on, as the tensors have, filled or not: a model's call reads caches that other layers'
+    // have been read after.  (us, through and past the caches, 16 heads of 64: of several caches in turn 96 MB 35, 32; 160 MB 47, 43; 256 MB
+    // 63, 56; 640 MB 132, 116; one that the call before read 96 MB 30, 30; 160 MB 41, 43; 256 MB 53, 56; 352 MB 79, 73.  Of 512 MB an eighth
+    // filled, in turn: 23.4, 24.9, a quarter: 40, 36.)
     const bool once = q_each * at_once <= 32 && groups == 1;
     P.past = once && keys * A.kv_heads * A.dim * (A.float32 ? 8 : 4) >= 1 << 27;
     P.splits = split_count(P.slots * A.kv_heads * groups * P.waves, (once ? 32 : 4) * ATTENTION_CUS, k_each, 64 * P.waves);
@@ -101,11 +110,19 @@ struct AttentionGradPlan {
 inline AttentionGradPlan attention_grad_plan(const SequenceAttention& A) {
     AttentionGradPlan P{};
     const int64_t q_each = A.packed && A.batch > 0 ? A.q_rows / A.batch : A.q_rows, k_each = A.packed && A.batch > 0 ? A.k_rows / A.batch : A.k_rows;
+    // A workgroup has one wavefront where a sequence has no rows for more.  us of all passes with one and four, 128 sequences, 8 heads of 64:
+    //   queries_kernel  bfloat16  33 tokens 44, 50;  48: 52, 55;  64: 60, 61;  65: 76, 76;  96: 89, 86      float32  33: 129, 122;  64: 136, 128;  96: 238, 176
+    //                   with a bias  64: 126, 88;  100: 194, 123       256 x 16 queries of 16 channels, 30 keys, float32: 50, 57
+    //   keys_kernel     bfloat16  30 tokens 38, 47;  48: 52, 60;  64: 60, 65;  65: 70, 75;  96: 85, 86      float32  30: 77, 97;  64: 136, 146;  96: 210, 175
+    // (one bound for all; below it float32 and biases lose by it in queries_kernel).  Also where four have no room in LDS: float32 of more than
+    // 64 channels with a reach beyond 809.
     P.q_waves = q_each > 64 && queries_lds(A.float32, A.dim, A.reach, A.table != nullptr, 4) <= ATTENTION_LDS ? 4 : 1;
     P.k_waves = k_each > 64 ? 4 : 1;
     P.q_slots = tile_slots(A.packed, A.q_rows, A.batch, 32 * P.q_waves);
     P.k_slots = tile_slots(A.packed, A.k_rows, A.batch, 32 * P.k_waves);
-    // (parts: odd lengths, 5 heads on 1 of 40 in float32, all passes 217 us, without 599; 6 heads on 3 of 80 in float16 62 and 81)
+    // (parts: odd lengths, 5 heads on 1 of 40 in float32, all passes 217 us, without 599; 6 heads on 3 of 80 in float16 62 and 81.  At least
+    // 128 rows of the other axis to each; with 64, 128, 256, 512: 6 x 500 tokens, 5 heads on 1 of 40 in float32 205, 206, 182, 183; 7 x 200 queries,
+    // 350 keys, 6 heads on 3 of 80 in float16 60, 58, 68, 69; 1000 tokens, 8 heads of 64 63, 65, 63, 91; 2 x 300, 2000 keys, 4 heads of 128 97, 89, 80, 89.)
     P.q_splits = split_count(P.q_slots * A.heads * P.q_waves, 8 * ATTENTION_CUS, k_each, 128);
     P.k_splits = split_count(P.k_slots * A.kv_heads * P.k_waves, 8 * ATTENTION_CUS, q_each * A.share, 128);
     return P;
