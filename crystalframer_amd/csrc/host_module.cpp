@@ -645,7 +645,8 @@ void check_attention(const AttentionTensors& t, const AttentionSpec& s) {
         TORCH_CHECK_VALUE(of.dim() == 1 && of.size(0) % 2 == 1 && of.size(0) <= 2 * CFH_ATTENTION_MAX_REACH + 1, "buckets of shape ", of.sizes(),
                           ": one for each relative position from -reach to reach, up to ", CFH_ATTENTION_MAX_REACH);
     }
-    TORCH_CHECK_VALUE(s.scale == 0.0 || (s.scale > 0.0 && std::isfinite((float)s.scale) && (float)s.scale > 0.0f), "scale ", s.scale, " must be positive and finite");
+    TORCH_CHECK_VALUE(s.scale == 0.0 || (s.scale <= CFH_ATTENTION_MAX_SCALE && (float)s.scale > 0.0f), "scale ", s.scale, " must be positive, up to ", CFH_ATTENTION_MAX_SCALE);
+    TORCH_CHECK_VALUE(s.scale == 0.0 || !t[TABLE].defined() || (s.scale >= 0x1p-64 && s.scale <= 0x1p64), "scale ", s.scale, ": from 2^-64 to 2^64 with a table");
 }
 
 // t as the library reads it: rows of neighbouring channels that begin at multiples of 16 bytes and fill them, and lie apart from one

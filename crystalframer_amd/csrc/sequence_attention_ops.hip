@@ -45,7 +45,7 @@ int check_attention(const cfh_attention* a) {
                     (long long)a->key_rows);
     if (!a->packed && a->batch > 0 && (a->query_rows * a->batch > MAX_ALL || a->key_rows * a->batch > MAX_ALL))
         return fail(CFH_EINVAL, "attention: %d sequences of %lld and %lld rows are too many", (int)a->batch, (long long)a->query_rows, (long long)a->key_rows);
-    if (!(a->scale > 0.0f) || std::isinf(a->scale)) return fail(CFH_EINVAL, "attention: scale = %g must be positive and finite", a->scale);
+    if (!(a->scale > 0.0f) || !(a->scale <= CFH_ATTENTION_MAX_SCALE)) return fail(CFH_EINVAL, "attention: scale = %g: positive, up to %g", a->scale, CFH_ATTENTION_MAX_SCALE);
     if (a->packed && (!a->query_starts || !a->key_starts)) return fail(CFH_EINVAL, "attention: packed sequences need query_starts and key_starts");
     if (a->packed && (a->query_sizes || a->key_sizes)) return fail(CFH_EINVAL, "attention: query_sizes and key_sizes are of sequences that are not packed");
     if (!a->packed && (a->query_starts || a->key_starts)) return fail(CFH_EINVAL, "attention: query_starts and key_starts are of packed sequences");
@@ -63,7 +63,7 @@ int check_attention(const cfh_attention* a) {
     } else if (a->buckets || a->reach || a->bucket_of) {
         return fail(CFH_EINVAL, "attention: buckets, reach and bucket_of belong to a table");
     }
-    if (a->table && !(a->scale >= 0x1p-64f)) return fail(CFH_EINVAL, "attention: scale = %g: at least 2^-64 with a table", a->scale);
+    if (a->table && !(a->scale >= 0x1p-64f && a->scale <= 0x1p64f)) return fail(CFH_EINVAL, "attention: scale = %g: from 2^-64 to 2^64 with a table", a->scale);
     return CFH_OK;
 }
 

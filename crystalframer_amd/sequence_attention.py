@@ -28,7 +28,7 @@ def _call(query, key, value, table, buckets, query_starts, key_starts, query_siz
     if scale is None:
         scale = 0.0                    # one over the root of the channels
     elif not scale > 0.0:
-        raise ValueError(f"scale {scale} must be positive and finite")
+        raise ValueError(f"scale {scale} must be positive")
     return _native(query, key, value, table, buckets, query_starts, key_starts, query_sizes, key_sizes, key_mask, scale, causal, queries_last)
 
 
@@ -45,8 +45,8 @@ def cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     there.  A query without keys gets 0.  What memory holds in the place of keys that are not there does not matter, NaN included.
 
     The heads may be a multiple of the key heads: head h reads key head h // (heads // key heads).  1 to 128 channels of a head;
-    ``scale``: one over their root.  One type, float32, bfloat16 or float16, for all and for the result; sums, maxima and the gradients'
-    sums are in float32, probabilities and the scores' gradients are rounded to the type before their products.  Any strides; rows
+    ``scale``: one over their root, up to 2.3e38, with a table from 2^-64 to 2^64.  One type, float32, bfloat16 or float16, for all and for
+    the result; sums, maxima and the gradients' sums are in float32, probabilities and the scores' gradients are rounded to the type before their products.  Any strides; rows
     that do not begin at multiples of 16 bytes, do not fill them, or share their memory (one row expanded over positions) are laid out
     again first.  The values of starts and sizes are cut to the rows that are there.
 

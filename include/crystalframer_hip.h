@@ -795,13 +795,14 @@ int cfh_model_backward(const cfh_model* m, const cfh_model_batch* b, const float
  */
 #define CFH_ATTENTION_MAX_DIM 128
 #define CFH_ATTENTION_MAX_REACH 1024
+#define CFH_ATTENTION_MAX_SCALE 2.3e38f    /* times log2 e it has to be finite */
 typedef struct cfh_attention {
     int32_t struct_size;                  /* = sizeof(cfh_attention)                                     */
     int32_t dtype, table_dtype;           /* table_dtype: dtype or CFH_FLOAT32                           */
     int32_t packed, causal, queries_last;
     int32_t batch, heads, kv_heads, dim;
     int32_t buckets, reach;               /* 0 without a table                                           */
-    float scale;                          /* positive; with a table at least 2^-64                       */
+    float scale;                          /* positive, up to CFH_ATTENTION_MAX_SCALE; with a table from 2^-64 to 2^64 */
     int32_t reserved0;
     int64_t query_rows, key_rows;
     int64_t q_stride[3], k_stride[3], v_stride[3];      /* of batch (packed: unused), row, head          */
