@@ -39,15 +39,15 @@ def cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     """o_i = sum_j softmax_j(scale q_i . k_j) v_j over the keys j of the query's own sequence.
 
     Packed: query (rows, heads, channels), key and value (rows, key heads, channels), the sequences of each behind one another;
-    ``query_starts``, ``key_starts`` (batch + 1, int64, from 0 on) say where each begins and the last ends.  Rows behind that are 0 in the
-    result and in all gradients.  Padded: (batch, positions, heads, channels), with ``query_sizes``, ``key_sizes`` (batch, int64) where
+    ``query_starts``, ``key_starts`` (batch + 1, int64, from 0 on, none below the one before) say where each begins and the last ends.  Rows
+    behind that are 0 in the result and in all gradients.  Padded: (batch, positions, heads, channels), with ``query_sizes``, ``key_sizes`` (batch, int64) where
     not all positions are meant; the others are 0 in the result.  ``key_mask`` (key's leading dimensions, bool): keys with False are not
     there.  A query without keys gets 0.  What memory holds in the place of keys that are not there does not matter, NaN included.
 
     The heads may be a multiple of the key heads: head h reads key head h // (heads // key heads).  1 to 128 channels of a head;
     ``scale``: one over their root, up to 2.3e38, with a table from 2^-64 to 2^64.  One type, float32, bfloat16 or float16, for all and for
-    the result; sums, maxima and the gradients' sums are in float32, probabilities and the scores' gradients are rounded to the type before their products.  Any strides; rows
-    that do not begin at multiples of 16 bytes, do not fill them, or share their memory (one row expanded over positions) are laid out
+    the result; sums, maxima and the gradients' sums are in float32, probabilities and the scores' gradients are rounded to the type before
+    their products.  Any strides; rows that do not begin at multiples of 16 bytes, do not fill them, or share their memory (one row expanded over positions) are laid out
     again first.  The values of starts and sizes are cut to the rows that are there.
 
     Float32 products are made of three bfloat16 parts, which hold 24 bits of numbers from 2^-110 to 3.38e38 in size (fewer below); what is
