@@ -40,15 +40,15 @@ def cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
 
     Packed: query (rows, heads, channels), key and value (rows, key heads, channels), the sequences of each behind one another;
     ``query_starts``, ``key_starts`` (batch + 1, int64, from 0 on, none below the one before) say where each begins and the last ends.  Rows
-    behind that are 0 in the result and in all gradients.  Padded: (batch, positions, heads, channels), with ``query_sizes``, ``key_sizes`` (batch, int64) where
-    not all positions are meant; the others are 0 in the result.  ``key_mask`` (key's leading dimensions, bool): keys with False are not
+    behind that are 0 in the result and in all gradients.  Padded: (batch, positions, heads, channels), with ``query_sizes``,
+    ``key_sizes`` (batch, int64) where not all positions are meant; the others are 0 in the result.  ``key_mask`` (key's leading dimensions, bool): keys with False are not
     there.  A query without keys gets 0.  What memory holds in the place of keys that are not there does not matter, NaN included.
 
     The heads may be a multiple of the key heads: head h reads key head h // (heads // key heads).  1 to 128 channels of a head;
     ``scale``: one over their root, up to 2.3e38, with a table from 2^-64 to 2^64.  One type, float32, bfloat16 or float16, for all and for
     the result; sums, maxima and the gradients' sums are in float32, probabilities and the scores' gradients are rounded to the type before
-    their products.  Any strides; rows that do not begin at multiples of 16 bytes, do not fill them, or share their memory (one row expanded over positions) are laid out
-    again first.  The values of starts and sizes are cut to the rows that are there.
+    their products.  Any strides; rows that do not begin at multiples of 16 bytes, do not fill them, or share their memory (one row expanded
+    over positions) are laid out again first.  The values of starts and sizes are cut to the rows that are there.
 
     Float32 products are made of three bfloat16 parts, which hold 24 bits of numbers from 2^-110 to 3.38e38 in size (fewer below); what is
     beyond, infinities included, makes a NaN.  All gradients are there, with
@@ -70,8 +70,8 @@ def relative_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tens
     each relative position from -reach to reach (``position_buckets`` makes one; positions beyond count as -reach and reach, reach up to
     1024; a number that is no row of ``table`` means no bias).  Finite entries of ``table`` beyond 65536 either way count as that; minus
     infinity takes a bucket's keys away, plus infinity and NaN make NaN of the rows that see such a key, and of no others.
-    shift: 0, or with ``queries_last`` how many more keys than queries the
-    sequence has (single tokens behind a cache, whose ``key_sizes`` include them).  ``causal``: keys j <= i + shift only; one that no query
+    shift: 0, or with ``queries_last`` how many more keys than queries the sequence has (single tokens behind a cache, whose ``key_sizes``
+    include them).  ``causal``: keys j <= i + shift only; one that no query
     of the sequence sees is not there, one that some see has to be finite for the others' sake (it is 0 times in their sums).
 
     The table's gradient from 16-bit tensors is as exact as the products of these are, in float32 as well."""
